@@ -242,11 +242,12 @@ def _own_attn(s):
     ops, case = _ops(), s["case"]
     ids = (ops.DENSE, ops.FRAME_LOCAL, ops.ANCHOR_LOCAL, ops.ANCHOR)
     patterns = [ids[p] for p in s["patterns"]]
-    out, lse = ops.frame_attn_fwd(s["q"], s["k"], s["v"], patterns, frames=case["frames"], token_mask=s["mask"])
+    args = dict(frames=case["frames"], token_mask=s["mask"])
     if not case["train"]:
+        out, lse = ops.frame_attn_fwd(s["q"], s["k"], s["v"], patterns, **args)
         return {"out": out, "lse": lse}
-    dq, dk, dv = ops.frame_attn_bwd(s["dout"], s["q"], s["k"], s["v"], out, lse, patterns, frames=case["frames"],
-                                    token_mask=s["mask"])
+    out, lse, rest = ops.frame_attn_fwd(s["q"], s["k"], s["v"], patterns, rest=True, **args)
+    dq, dk, dv = ops.frame_attn_bwd(s["dout"], s["q"], s["k"], s["v"], out, lse, patterns, rest=rest, **args)
     return {"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv}
 
 
