@@ -116,6 +116,24 @@ typedef struct saf3r_rows {
   int64_t frame_row_stride;
 } saf3r_rows;
 
+/* Element types of the row kernels (saf3r_layer_norm_*, saf3r_head_rotary_*). */
+enum saf3r_dtype {
+  SAF3R_FP32 = 0,
+  SAF3R_BF16 = 1,
+  SAF3R_FP16 = 2
+};
+
+/* Rows of several heads where another kernel left them: the row of (clip b, token t, group g, head h) starts at
+ * ptr + b*clip_stride + t*token_stride + g*group_stride + h*head_stride elements, its elements are consecutive.
+ * (saf3r_frame_attn_*: one group, group_stride is not read.) */
+typedef struct saf3r_heads {
+  const void* ptr;
+  int64_t clip_stride;
+  int64_t token_stride;
+  int64_t group_stride;
+  int64_t head_stride;
+} saf3r_heads;
+
 int saf3r_abi_version(void);
 const char* saf3r_last_error(void);
 
@@ -484,6 +502,103 @@ int64_t saf3r_token_topk_workspace_bytes(int n_q, int frames, int per_frame, int
 int saf3r_frame_topk_scores(const void* scores, int64_t score_stride, int rows, int frames, int per_frame,
                             int exclude_first, int first_stride, int per_frame_mode, int topk, int cap,
                             int32_t* idx, int64_t idx_stride, int32_t* cand_idx, uint16_t* cand_key, void* stream);
+
+/*
+ * Attention over the tokens of frames, in natural token order, with the statistics of its backward pass.
+ *   q, k, v: bf16 rows of 64 of `clips` clips of F frames x T tokens (N = F*T) and num_heads <= 64 heads;
+ *   bases 16-byte aligned, strides multiples of 8 elements.
+ *   patterns: host int32 [num_heads]: SAF3R_DENSE, SAF3R_FRAME_LOCAL, SAF3R_ANCHOR_LOCAL, SAF3R_ANCHOR or
+ *   SAF3R_SKIP (SAF3R_ERR_UNSUPPORTED for the others).
+ *   token_mask: device uint8 [clips][N] or NULL; a token whose byte is 0 is no key of any query, and its own
+ *   row comes out as zeros. Its q, k and v rows may hold anything.
+ *   out: bf16 rows, softmax_j(q.k_j * scale) v_j; zeros for a row without a key.
+ *   out_rest: bf16 rows or NULL: what the rounding of out took away (out + out_rest is the fp32 result to 16 bits),
+ *   for saf3r_frame_attn_bwd.
+ *   lse: fp32 [clips][num_heads][N], log sum_j exp(q.k_j * scale); -inf for a row without a key.
+ * ref (forward): as saf3r_sparse_attn_fwd; the reference trains nothing through these patterns.
+ */
+int saf3r_frame_attn_fwd(const saf3r_heads* q, const saf3r_heads* k, const saf3r_heads* v, int clips, int frames,
+                         int tokens_per_frame, int num_heads, const int32_t* patterns, const uint8_t* token_mask,
+                         float scale, const saf3r_heads* out, const saf3r_heads* out_rest, float* lse, void* stream);
+
+/*
+ * Gradients of saf3r_frame_attn_fwd: from dout (bf16 rows), the inputs, out and lse of that call, with the
+ * same patterns, token_mask and scale. dq, dk, dv: bf16 rows, every one of them written (zeros for masked tokens
+ * and rows without a key or a query); they must not overlap the inputs or each other. The rows of dout of
+ * masked tokens are not used.
+ *   out_rest: as written by the forward pass, or NULL: then dq and dk carry the rounding of out (a dO.O of
+ *   rounded values is subtracted from every dO.V of a row; 1.5 to 2 times the error of dq, more for rows whose
+ *   attention is nearly all on one key).
+ *   workspace: device memory of saf3r_frame_attn_bwd_workspace_bytes, 16-byte aligned, for this call alone until
+ *   it is done on its stream.
+ */
+int saf3r_frame_attn_bwd(const saf3r_heads* dout, const saf3r_heads* q, const saf3r_heads* k, const saf3r_heads* v,
+                         const saf3r_heads* out, const saf3r_heads* out_rest, const float* lse, int clips, int frames,
+                         int tokens_per_frame, int num_heads, const int32_t* patterns, const uint8_t* token_mask,
+                         float scale, const saf3r_heads* dq, const saf3r_heads* dk, const saf3r_heads* dv,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of saf3r_frame_attn_bwd (one float per row of a head), -1 for invalid sizes. */
+int64_t saf3r_frame_attn_bwd_workspace_bytes(int clips, int frames, int tokens_per_frame, int num_heads);
+
+/*
+ * Prologue of q and k of a training step: LayerNorm over the head dimension and rotary positions, in one pass over
+ * the rows where the projection left them.
+ *   x: rows of `dim` elements (even, at most 128) of type `type`, [clips][tokens][groups][heads] (q and k of a qkv
+ *   buffer are two groups); any strides, any alignment to whole elements.
+ *   norm: 1: LayerNorm with weight / bias [groups][dim] of param_type (fp32 or `type`; NULL: ones / zeros) and eps.
+ *   rope_cos / rope_sin: fp32 [positions][rotary_dim / axes / 2], or NULL for no rotation. The first rotary_dim
+ *   elements are `axes` (1 .. 8) equal sections; section a is rotated by the angles of pos[clip][token][a] (int32, or
+ *   int64 with pos_int64), pairs (j, j + half a section), or (2 j, 2 j + 1) with `interleaved`. Positions outside
+ *   the table are taken to its ends.
+ *   y: rows like x. All arithmetic is fp32, rounded once.
+ * ref: saf3r/patch/patch_vggt.py:577-583 (q / k norm, RoPE), rope.py:86-188 (two axes, half layout).
+ */
+int saf3r_head_rotary_fwd(const saf3r_heads* x, int type, int64_t clips, int tokens, int groups, int heads, int dim,
+                          const void* pos, int pos_int64, int axes, const float* rope_cos, const float* rope_sin,
+                          int positions, int rotary_dim, int interleaved, int norm, const void* weight,
+                          const void* bias, int param_type, float eps, const saf3r_heads* y, void* stream);
+
+/*
+ * Gradients of saf3r_head_rotary_fwd from dy (rows like y): dx (rows like x, every one written), and with `norm`
+ * dweight / dbias [groups][dim] of param_type (each may be NULL). x is read with `norm` only (the statistics are
+ * recomputed). The sums over rows have a fixed order.
+ *   workspace: saf3r_head_rotary_bwd_workspace_bytes when dweight or dbias is given, 16-byte aligned, for this call
+ *   alone until it is done on its stream.
+ */
+int saf3r_head_rotary_bwd(const saf3r_heads* dy, const saf3r_heads* x, int type, int64_t clips, int tokens, int groups,
+                          int heads, int dim, const void* pos, int pos_int64, int axes, const float* rope_cos,
+                          const float* rope_sin, int positions, int rotary_dim, int interleaved, int norm,
+                          const void* weight, int param_type, float eps, const saf3r_heads* dx, void* dweight,
+                          void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of saf3r_head_rotary_bwd (at most 8 * 2048 * dim), -1 for sizes that it rejects. */
+int64_t saf3r_head_rotary_bwd_workspace_bytes(int64_t clips, int tokens, int groups, int heads, int dim);
+
+/*
+ * LayerNorm over rows of `dim` elements (1 .. 8192): y = (x - mean) rstd weight + bias.
+ *   x: rows of x_type at x + r*x_stride elements; y: rows of y_type (x_type, or a 16-bit type for fp32 rows).
+ *   weight, bias: [dim] of param_type (fp32 or y_type), NULL: ones / zeros. mean, rstd: fp32 [rows], for the backward pass.
+ *   All arithmetic is fp32, y is rounded once.
+ * ref: the block norms of layers/block.py:26-105.
+ */
+int saf3r_layer_norm_fwd(const void* x, int64_t x_stride, int x_type, int64_t rows, int dim, const void* weight,
+                         const void* bias, int param_type, float eps, void* y, int64_t y_stride, int y_type,
+                         float* mean, float* rstd, void* stream);
+
+/*
+ * Gradients of saf3r_layer_norm_fwd from dy (rows of y_type): dx (rows of x_type), dweight / dbias [dim] of
+ * param_type (each may be NULL). The sums over rows have a fixed order.
+ *   workspace: saf3r_layer_norm_bwd_workspace_bytes when dweight or dbias is given, 16-byte aligned, for this call
+ *   alone until it is done on its stream.
+ */
+int saf3r_layer_norm_bwd(const void* dy, int64_t dy_stride, int y_type, const void* x, int64_t x_stride, int x_type,
+                         int64_t rows, int dim, const float* mean, const float* rstd, const void* weight,
+                         int param_type, void* dx, int64_t dx_stride, void* dweight, void* dbias, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of saf3r_layer_norm_bwd (at most 8192 * dim), -1 for sizes that it rejects. */
+int64_t saf3r_layer_norm_bwd_workspace_bytes(int64_t rows, int dim);
 
 #ifdef __cplusplus
 }

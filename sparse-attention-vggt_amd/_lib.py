@@ -22,10 +22,14 @@ EXPORTS = (
     "saf3r_gather_attn_fwd_sliced", "saf3r_gather_attn_workspace_bytes", "saf3r_pack_qkv_typed",
     "saf3r_probe_scores_host", "saf3r_keyset_build_host", "saf3r_keyset_gather_host",
     "saf3r_sparse_attn_split_heads",
+    "saf3r_frame_attn_fwd", "saf3r_frame_attn_bwd", "saf3r_frame_attn_bwd_workspace_bytes",
+    "saf3r_head_rotary_fwd", "saf3r_head_rotary_bwd", "saf3r_head_rotary_bwd_workspace_bytes",
+    "saf3r_layer_norm_fwd", "saf3r_layer_norm_bwd", "saf3r_layer_norm_bwd_workspace_bytes",
 )
 ABI_VERSION = 13
 PACK_LN_BF16, PACK_POS_INT64 = 1, 2  # enum saf3r_pack_param_flags
 GATHER_QK_FP32, GATHER_V_FP32, GATHER_OUT_FP32 = 1, 2, 4  # enum saf3r_gather_dtype
+FP32, BF16, FP16 = 0, 1, 2  # enum saf3r_dtype
 SAF3R_OK, SAF3R_ERR_INVALID, SAF3R_ERR_UNSUPPORTED, SAF3R_ERR_LAUNCH, SAF3R_ERR_INJECTED = range(5)
 
 _lib = None
@@ -40,6 +44,18 @@ class Rows(ctypes.Structure):
         ("base_row", ctypes.c_int64),
         ("rows_per_frame", ctypes.c_int64),
         ("frame_row_stride", ctypes.c_int64),
+    ]
+
+
+class Heads(ctypes.Structure):
+    """``saf3r_heads``: the row of (clip b, token t, group g, head h) at ptr + b * clip_stride + t * token_stride
+    + g * group_stride + h * head_stride elements."""
+    _fields_ = [
+        ("ptr", ctypes.c_void_p),
+        ("clip_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("group_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
     ]
 
 
@@ -58,7 +74,7 @@ def load():
         raise RuntimeError(f"HIP library not built: {LIB_PATH} is missing (run __graft_entry__.build())")
     lib = ctypes.CDLL(LIB_PATH)
     i32, i64, p, f32 = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float
-    rows = ctypes.POINTER(Rows)
+    rows, heads = ctypes.POINTER(Rows), ctypes.POINTER(Heads)
     sig = {
         "saf3r_abi_version": ([], i32),
         "saf3r_last_error": ([], ctypes.c_char_p),
@@ -88,6 +104,18 @@ def load():
         "saf3r_probe_scores_host": ([p, p, i64, i32, p, p, i32, p, i32, f32, p, p, p, i64, p], i32),
         "saf3r_keyset_build_host": ([p, i64, i32, p, p, p, p, i32, i32, i32, p, i64, p, p], i32),
         "saf3r_keyset_gather_host": ([p, i32, i32, i32, p, i32, p, i64, i64, p, i64, p, i32, p, p, i64, p], i32),
+        "saf3r_frame_attn_fwd": ([heads, heads, heads, i32, i32, i32, i32, p, p, f32, heads, heads, p, p], i32),
+        "saf3r_frame_attn_bwd": ([heads, heads, heads, heads, heads, heads, p, i32, i32, i32, i32, p, p, f32, heads,
+                                  heads, heads, p, i64, p], i32),
+        "saf3r_frame_attn_bwd_workspace_bytes": ([i32, i32, i32, i32], i64),
+        "saf3r_head_rotary_fwd": ([heads, i32, i64, i32, i32, i32, i32, p, i32, i32, p, p, i32, i32, i32, i32, p, p,
+                                   i32, f32, heads, p], i32),
+        "saf3r_head_rotary_bwd": ([heads, heads, i32, i64, i32, i32, i32, i32, p, i32, i32, p, p, i32, i32, i32, i32,
+                                   p, i32, f32, heads, p, p, p, i64, p], i32),
+        "saf3r_head_rotary_bwd_workspace_bytes": ([i64, i32, i32, i32, i32], i64),
+        "saf3r_layer_norm_fwd": ([p, i64, i32, i64, i32, p, p, i32, f32, p, i64, i32, p, p, p], i32),
+        "saf3r_layer_norm_bwd": ([p, i64, i32, p, i64, i32, i64, i32, p, p, p, i32, p, i64, p, p, p, i64, p], i32),
+        "saf3r_layer_norm_bwd_workspace_bytes": ([i64, i32], i64),
         "saf3r_frame_topk_scores": ([p, i64, i32, i32, i32, i32, i32, i32, i32, i32, p, i64, p, p, p], i32),
     }
     if lib.saf3r_abi_version() != ABI_VERSION:  # (no arguments, int result: ctypes' defaults)

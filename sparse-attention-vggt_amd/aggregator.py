@@ -21,7 +21,9 @@ checkpoints in this build.
 Frame attention (frame blocks and the DINOv2 blocks: dense attention inside each image) runs on torch's
 fused SDPA kernels (flash / memory-efficient only, never the math path), or, with
 ``frame_attention="saf3r"``, through this package's kernels as the frame-local pattern over the
-frames' tokens (identical arithmetic: every token attends to the tokens of its own frame).
+frames' tokens (identical arithmetic: every token attends to the tokens of its own frame). With
+``frame_attention="saf3r_train"`` every block's norms and the attention of unpatched blocks run through the
+differentiable kernels (``autograd``), for training steps.
 """
 from __future__ import annotations
 
@@ -31,7 +33,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import ops
+from . import autograd, ops
 from .layout import HEAD_DIM, Geometry
 from .vggt import Attention, RotaryPositionEmbedding2D
 
@@ -91,6 +93,17 @@ def frame_local_attention(attn: Attention, x: torch.Tensor, pos, num_special: in
     return attn.proj_drop(attn.proj(y))
 
 
+def trained_attention(attn: Attention, x: torch.Tensor, pos) -> torch.Tensor:
+    """``attn`` over each sequence of x [S, T, C], differentiable, through the package kernels."""
+    S, T, C = x.shape
+    if attn.head_dim != HEAD_DIM:
+        raise NotImplementedError("the kernels are built for head_dim 64")
+    y = autograd.module_attention(attn, attn.qkv(x).to(torch.bfloat16), pos, [ops.DENSE] * attn.num_heads)
+    if y.dtype != attn.proj.weight.dtype and not torch.is_autocast_enabled("cuda"):
+        y = y.to(attn.proj.weight.dtype)
+    return attn.proj_drop(attn.proj(y))
+
+
 class Block(nn.Module):
     """Pre-norm transformer block: x + ls1(attn(norm1(x))), then x + ls2(mlp(norm2(x)))."""
 
@@ -103,19 +116,29 @@ class Block(nn.Module):
         self.norm2 = nn.LayerNorm(dim)
         self.mlp = Mlp(dim, int(dim * mlp_ratio))
         self.ls2 = LayerScale(dim, init_values) if init_values else nn.Identity()
-        self.frame_attention = "sdpa"  # "saf3r": frame-local pattern of the package kernels (see module doc)
+        self.frame_attention = "sdpa"  # "saf3r", "saf3r_train": the package kernels (see module doc)
         self.num_special = 0
 
+    def _norm(self, norm: nn.LayerNorm, x):
+        if self.frame_attention != "saf3r_train":
+            return norm(x)
+        # (under autocast the products that follow take their input in the autocast type)
+        cast = torch.is_autocast_enabled("cuda") and x.dtype == torch.float32
+        return autograd.layer_norm(x, norm.weight, norm.bias, norm.eps,
+                                   torch.get_autocast_dtype("cuda") if cast else None)
+
     def forward(self, x, pos=None):
-        h = self.norm1(x)
+        h = self._norm(self.norm1, x)
         if self.frame_attention == "saf3r" and not isinstance(self.attn, Attention):
             raise RuntimeError("frame_attention='saf3r' is for unpatched frame blocks")
         if self.frame_attention == "saf3r":
             a = frame_local_attention(self.attn, h, pos, self.num_special)
+        elif self.frame_attention == "saf3r_train" and isinstance(self.attn, Attention):
+            a = trained_attention(self.attn, h, pos)
         else:
             a = self.attn(h, pos=pos)
         x = x + self.ls1(a)
-        return x + self.ls2(self.mlp(self.norm2(x)))
+        return x + self.ls2(self.mlp(self._norm(self.norm2, x)))
 
 
 class DinoPatchEmbed(nn.Module):
@@ -215,11 +238,14 @@ class Aggregator(nn.Module):
 
     def set_frame_attention(self, kind: str):
         """"sdpa" (torch's fused kernels) or "saf3r" (the frame-local pattern of the package kernels) for
-        the frame blocks and the patch embedding's blocks."""
-        if kind not in ("sdpa", "saf3r"):
+        the frame blocks and the patch embedding's blocks; "saf3r_train": the differentiable kernels for these and
+        for the norms of the global blocks (their attention too where it is not patched)."""
+        if kind not in ("sdpa", "saf3r", "saf3r_train"):
             raise ValueError(f"frame attention {kind!r}")
         for b in list(self.frame_blocks) + list(self.patch_embed.blocks):
             b.frame_attention = kind
+        for b in self.global_blocks:
+            b.frame_attention = "saf3r_train" if kind == "saf3r_train" else "sdpa"
         for b in self.frame_blocks:
             b.num_special = self.patch_start_idx
 

@@ -1,0 +1,872 @@
+// Attention over the tokens of frames with its backward pass (head_dim 64, bf16, fp32 sums): the training
+// form of the static head patterns (dense, frame-local, anchor + local, anchor, skip). It reads q, k and v
+// where the projection left them ([clip][token][head][64] with any strides) and recomputes the
+// probabilities in the backward pass from the row statistics lse of the forward pass.
+//
+//   S = scale q k^T over the keys a query may attend, L = log sum_j exp S_j, P = exp(S - L), O = P V
+//   D = sum_d dO O,  dP = dO V^T,  dS = P (dP - D),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO
+//
+// Every pattern gives a query tile (or, in the backward pass over keys, a key tile) at most two ranges of
+// consecutive tokens on the other side: all, the first frame, the own frame. A work-group of four waves owns a
+// tile of rows and walks the other side in tiles of 64 tokens that all its waves read from LDS (two buffers; the
+// next tile waits in registers while the current one is used, so any row stride and any masked row is dealt
+// with at the write). Matrix products are v_mfma_f32_32x32x16_bf16 and none of their results crosses lanes: a
+// product whose rows are summed over next (P, dS) leaves its 32x32 result with one column per lane and the rows
+// 8 (i / 4) + 4 (lane / 32) + i % 4, and the other operand of the next product is read from LDS with the
+// transposing read in that same row order (two groups of four rows per 16).
+//
+// The probabilities and dS are rounded to bf16 as operands of the second product, which is what the matrix
+// cores take; everything else (S, dP, the statistics, all sums) is fp32.
+//
+// Backward without atomics: one kernel per side. The first owns query rows, computes D and dQ; the second owns
+// key rows and computes dK and dV. Both recompute S and dP (7 products in place of 5), and the results do not
+// depend on the order in which work-groups run.
+//
+// D cancels against dP, so an O that is rounded to bf16 would leave an error of its own in every dS of a row; the
+// forward pass can store what the rounding of O took away (rest, bf16) for the sum that gives D.
+//
+// Tokens that the mask removes are no keys and their own rows come out as zeros (lse = -inf); their q, k, v and
+// dO rows are replaced by zeros where they enter a product, so that whatever they hold stays out.
+#include <algorithm>
+
+#include "common.h"
+
+namespace saf3r {
+
+constexpr int kTile = 64;          // tokens of a staged tile
+constexpr int kTileElems = kTile * kHeadDim;
+constexpr int kFaMaxSegs = 2 * kMaxHeads;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+enum Walk { kNone = 0, kAll = 1, kFirst = 2, kOwn = 3, kFirstOwn = 4 };
+
+// A run of row tiles of one head, clip-major: per frame (frames f0 ..) or over the tokens tok0 .. tok1.
+struct FaSeg {
+  int start;     // first work-group
+  int per_clip;  // tiles of a clip
+  int nt;        // tiles of a frame (per-frame runs; 0: over tokens)
+  int tok0, tok1;
+  int16_t head;
+  int16_t walk;
+};
+
+struct FaTensor {
+  __bf16* ptr;
+  int64_t clip, token, head;  // strides in elements
+};
+
+struct FaParams {
+  FaTensor q, k, v, o, rest, doo, dq, dk, dv;
+  float* lse;            // [clip][head][token]
+  float* delta;          // [clip][head][token]
+  const uint8_t* mask;   // [clip][token], 0: not there (may be null)
+  int N, T, H, n_seg;
+  float scale, c;        // softmax scale, scale * log2(e)
+  FaSeg seg[kFaMaxSegs];
+};
+
+// What a work-group owns and walks.
+struct FaItem {
+  int head, clip;
+  int row0, row_end;    // own rows: row0 .. min(row0 + tile, row_end)
+  int a0, a1, b0, b1;   // walked ranges
+};
+
+__device__ inline FaItem fa_item(const FaParams& p, int rows) {
+  const int bid = bid_x();
+  int lo = 0, hi = p.n_seg - 1;
+  while (lo < hi) {  // last segment that starts at or before bid
+    const int mid = (lo + hi + 1) >> 1;
+    if (p.seg[mid].start <= bid)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  const FaSeg s = p.seg[lo];
+  const int j = bid - s.start;
+  FaItem it;
+  it.head = s.head;
+  it.clip = j / s.per_clip;
+  const int t = j - it.clip * s.per_clip;
+  int frame0 = 0;
+  if (s.nt > 0) {
+    const int f = t / s.nt;
+    frame0 = s.tok0 + f * p.T;
+    it.row0 = frame0 + (t - f * s.nt) * rows;
+    it.row_end = frame0 + p.T;
+  } else {
+    it.row0 = s.tok0 + t * rows;
+    it.row_end = s.tok1;
+  }
+  it.a0 = it.a1 = it.b0 = it.b1 = 0;
+  switch (s.walk) {
+    case kAll: it.a1 = p.N; break;
+    case kFirst: it.a1 = p.T; break;
+    case kOwn: it.a0 = frame0; it.a1 = frame0 + p.T; break;
+    case kFirstOwn:
+      it.a1 = p.T;
+      if (frame0 > 0) { it.b0 = frame0; it.b1 = frame0 + p.T; }
+      break;
+    default: break;
+  }
+  return it;
+}
+
+__device__ inline int tiles_of(int n) { return (n + kTile - 1) / kTile; }
+
+// Position of walk tile i: tokens start .. end of it (at most 64).
+__device__ inline void walk_tile(const FaItem& it, int na, int i, int* start, int* end) {
+  if (i < na) {
+    *start = it.a0 + i * kTile;
+    *end = it.a1;
+  } else {
+    *start = it.b0 + (i - na) * kTile;
+    *end = it.b1;
+  }
+}
+
+// LDS addresses of a lane's operand fragments in a [64][64] tile whose 16-byte chunks are swizzled by row.
+struct FragAddr {
+  int row[4];     // rows operand: row lane % 32, elements 16 ks + 8 (lane / 32) .. + 7
+  int tr[2][2];   // transposed operand: [32-column half][row group 0 / 8], see tr_frag
+};
+
+__device__ inline FragAddr frag_addr(int lane) {
+  FragAddr f;
+  const int r = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) f.row[ks] = r * 64 + (((2 * ks + h) ^ swz8(r)) << 3);
+  // lane i of 16 addresses row i / 4, columns 4 (i % 4) .. + 3, and receives column i of those 4 x 16 elements
+  const int tr = 4 * h + ((lane & 15) >> 2), cc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+  for (int dh = 0; dh < 2; ++dh)
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int row = tr + 8 * g;
+      f.tr[dh][g] = row * 64 + (((4 * dh + cc) ^ swz8(row)) << 3) + 4 * (lane & 1);
+    }
+  return f;
+}
+
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// Rows operand: rows 32 half .. + 31 of the tile, k-step ks.
+__device__ __forceinline__ bf16x8 row_frag(const __bf16* tile, const FragAddr& f, int half, int ks) {
+  return *reinterpret_cast<const bf16x8*>(tile + half * 2048 + f.row[ks]);
+}
+
+// Transposed operand: columns 32 dh + lane % 32 of rows 16 step + {4 h .. 4 h + 3, 8 + 4 h ..} (h = lane / 32),
+// the order in which a 32x32 product leaves its rows in a lane.
+__device__ __forceinline__ bf16x8 tr_frag(const __bf16* tile, const FragAddr& f, int step, int dh) {
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + step * 1024 + f.tr[dh][0]));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + step * 1024 + f.tr[dh][1]));
+  const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+  return __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]});
+}
+
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// Eight accumulator elements 8 st .. 8 st + 7 as a bf16 operand.
+__device__ __forceinline__ bf16x8 pack8(const f32x16& x, int st) {
+  bf16x8 r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = (__bf16)x[8 * st + j];
+  return r;
+}
+
+__device__ __forceinline__ float pair_sum(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+__device__ __forceinline__ float pair_max(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
+// Two row tiles on their way to LDS: 32 lanes of eight 16-byte chunks each, rows r and r + 32 (r = thread / 8).
+struct Staged {
+  u32x4 x[2], y[2];
+};
+
+__device__ __forceinline__ void stage_load(Staged& s, const __bf16* x, int64_t xs, const __bf16* y, int64_t ys,
+                                           int start, int end) {
+  const int r = tid_x() >> 3, c = (tid_x() & 7) * 8;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int tok = start + r + 32 * i;
+    s.x[i] = s.y[i] = u32x4{};
+    if (tok < end) {
+      s.x[i] = *reinterpret_cast<const u32x4*>(x + tok * xs + c);
+      s.y[i] = *reinterpret_cast<const u32x4*>(y + tok * ys + c);
+    }
+  }
+}
+
+// bits: rows of the tile that are there (a row that is not is written as zeros)
+template <bool MASK>
+__device__ __forceinline__ void stage_write(const Staged& s, __bf16* xt, __bf16* yt, uint64_t bits) {
+  const int r = tid_x() >> 3, c = tid_x() & 7;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row = r + 32 * i;
+    const bool keep = !MASK || ((bits >> row) & 1);
+    const int at = row * 64 + ((c ^ swz8(row)) << 3);
+    *reinterpret_cast<u32x4*>(xt + at) = keep ? s.x[i] : u32x4{};
+    *reinterpret_cast<u32x4*>(yt + at) = keep ? s.y[i] : u32x4{};
+  }
+}
+
+// Rows of a walk tile that are there, one bit each (the same in every wave).
+template <bool MASK>
+__device__ __forceinline__ uint8_t mask_byte(const uint8_t* mask, int start, int end) {
+  const int tok = start + (tid_x() & 63);
+  if (!MASK) return tok < end;
+  return tok < end ? mask[tok] : 0;
+}
+
+// Sets the scores of keys that are not there to -inf; half: keys 32 half .. + 31 of the tile.
+__device__ __forceinline__ void mask_scores(f32x16& s, uint64_t bits, int half, int h) {
+  const uint32_t w = (uint32_t)(bits >> (32 * half)) >> (4 * h);
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (!((w >> (8 * (i / 4) + i % 4)) & 1)) s[i] = -__builtin_inff();
+}
+
+// ---------------------------------------------------------------------------------------
+// Forward: a wave owns 32 QG query rows as columns of S^T = K Q^T; O^T += V^T P^T.
+// The running reference m of a row is the maximum of its first tile; it moves only when a tile's sum of
+// exp2(S c - m) leaves [0, 2^40], so that tiles after the first take no maximum (fp32 holds the sums, and
+// bf16 the probabilities, at the same relative precision for any m at or below the row's maximum).
+// ---------------------------------------------------------------------------------------
+template <int QG, bool MASK>
+__global__ void __launch_bounds__(256, 2) frame_attn_fwd_kernel(const FaParams p) {
+  __shared__ __align__(16) __bf16 lds[2][2][kTileElems];
+  const FaItem it = fa_item(p, 128 * QG);
+  const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6), h = lane >> 5;
+  const FragAddr fa = frag_addr(lane);
+  const __bf16* kb = p.k.ptr + it.clip * p.k.clip + it.head * p.k.head;
+  const __bf16* vb = p.v.ptr + it.clip * p.v.clip + it.head * p.v.head;
+  const uint8_t* mask = MASK ? p.mask + (int64_t)it.clip * p.N : nullptr;
+  const int first = it.row0 + wave * 32 * QG;
+  const bool active = first < it.row_end;
+
+  bf16x8 qf[QG][4];
+  bool valid[QG];
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    const int r = first + 32 * g + (lane & 31);
+    valid[g] = r < it.row_end && (!MASK || mask[r]);
+    const __bf16* qp = p.q.ptr + it.clip * p.q.clip + it.head * p.q.head + r * p.q.token + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) qf[g][ks] = valid[g] ? *reinterpret_cast<const bf16x8*>(qp + 16 * ks) : bf16x8{};
+  }
+  f32x16 o[QG][2];
+  float m[QG], l[QG];
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    o[g][0] = o[g][1] = f32x16{};
+    m[g] = -__builtin_inff();
+    l[g] = 0.f;
+  }
+
+  const int na = tiles_of(it.a1 - it.a0), nw = na + tiles_of(it.b1 - it.b0);
+  Staged st;
+  int start, end;
+  uint8_t mb = 0;
+  if (nw > 0) {
+    walk_tile(it, na, 0, &start, &end);
+    stage_load(st, kb, p.k.token, vb, p.v.token, start, end);
+    mb = mask_byte<MASK>(mask, start, end);
+  }
+  for (int i = 0; i < nw; ++i) {
+    const uint64_t bits = __ballot(mb != 0);
+    __bf16* kt = lds[i & 1][0];
+    __bf16* vt = lds[i & 1][1];
+    stage_write<MASK>(st, kt, vt, bits);
+    __syncthreads();
+    if (i + 1 < nw) {
+      walk_tile(it, na, i + 1, &start, &end);
+      stage_load(st, kb, p.k.token, vb, p.v.token, start, end);
+      mb = mask_byte<MASK>(mask, start, end);
+    }
+    if (!active) continue;
+    f32x16 s[QG][2];
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh) {
+#pragma unroll
+      for (int g = 0; g < QG; ++g) s[g][kh] = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const bf16x8 a = row_frag(kt, fa, kh, ks);
+#pragma unroll
+        for (int g = 0; g < QG; ++g) s[g][kh] = mma(a, qf[g][ks], s[g][kh]);
+      }
+    }
+    if (bits != ~0ull) {
+#pragma unroll
+      for (int g = 0; g < QG; ++g) {
+        mask_scores(s[g][0], bits, 0, h);
+        mask_scores(s[g][1], bits, 1, h);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < QG; ++g) {
+      float ref = m[g];
+      f32x16 e[2];
+      float sum = 0.f;
+      bool moved = ref == -__builtin_inff();
+      if (!__any(moved)) {
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            e[kh][j] = __builtin_amdgcn_exp2f(s[g][kh][j] * p.c - ref);
+            sum += e[kh][j];
+          }
+        moved = !(sum <= 0x1p40f);
+      }
+      if (__any(moved)) {
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[g][kh][j]);
+        const float next = fmaxf(ref, pair_max(mx) * p.c);
+        const float base = next == -__builtin_inff() ? 0.f : next;  // no key yet
+        const float f = __builtin_amdgcn_exp2f(ref - base);
+        l[g] *= f;
+#pragma unroll
+        for (int dh = 0; dh < 2; ++dh)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[g][dh][j] *= f;
+        m[g] = next;
+        sum = 0.f;
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            e[kh][j] = __builtin_amdgcn_exp2f(s[g][kh][j] * p.c - base);
+            sum += e[kh][j];
+          }
+      }
+      l[g] += sum;
+      s[g][0] = e[0];
+      s[g][1] = e[1];
+    }
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        bf16x8 pf[QG];
+#pragma unroll
+        for (int g = 0; g < QG; ++g) pf[g] = pack8(s[g][kh], step);
+#pragma unroll
+        for (int dh = 0; dh < 2; ++dh) {
+          const bf16x8 a = tr_frag(vt, fa, 2 * kh + step, dh);
+#pragma unroll
+          for (int g = 0; g < QG; ++g) o[g][dh] = mma(a, pf[g], o[g][dh]);
+        }
+      }
+  }
+  if (!active) return;
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    const int r = first + 32 * g + (lane & 31);
+    const float sum = pair_sum(l[g]);
+    const bool some = valid[g] && m[g] != -__builtin_inff();
+    const float inv = some ? 1.f / sum : 0.f;
+    if (r < it.row_end) {
+      __bf16* op = p.o.ptr + it.clip * p.o.clip + it.head * p.o.head + r * p.o.token + 4 * h;
+      __bf16* rp = p.rest.ptr ? p.rest.ptr + it.clip * p.rest.clip + it.head * p.rest.head + r * p.rest.token + 4 * h
+                              : nullptr;
+#pragma unroll
+      for (int dh = 0; dh < 2; ++dh)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          __bf16 w[4], x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float y = some ? o[g][dh][4 * j + e] * inv : 0.f;
+            w[e] = (__bf16)y;
+            x[e] = (__bf16)(y - (float)w[e]);
+          }
+          *reinterpret_cast<u32x2*>(op + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(w);
+          if (rp) *reinterpret_cast<u32x2*>(rp + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(x);
+        }
+      if (h == 0)
+        p.lse[((int64_t)it.clip * p.H + it.head) * p.N + r] =
+            some ? (m[g] + __builtin_amdgcn_logf(sum)) * kLn2 : -__builtin_inff();
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Backward over queries: D and dQ. A wave owns 32 QG query rows as columns of S^T and dP^T = V dO^T;
+// dQ^T += K^T dS^T.
+// ---------------------------------------------------------------------------------------
+template <int QG, bool MASK>
+__global__ void __launch_bounds__(256, 2) frame_attn_dq_kernel(const FaParams p) {
+  __shared__ __align__(16) __bf16 lds[2][2][kTileElems];
+  const FaItem it = fa_item(p, 128 * QG);
+  const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6), h = lane >> 5;
+  const FragAddr fa = frag_addr(lane);
+  const __bf16* kb = p.k.ptr + it.clip * p.k.clip + it.head * p.k.head;
+  const __bf16* vb = p.v.ptr + it.clip * p.v.clip + it.head * p.v.head;
+  const uint8_t* mask = MASK ? p.mask + (int64_t)it.clip * p.N : nullptr;
+  const int64_t stat = ((int64_t)it.clip * p.H + it.head) * p.N;
+  const int first = it.row0 + wave * 32 * QG;
+  const bool active = first < it.row_end;
+
+  bf16x8 qf[QG][4], dof[QG][4];
+  f32x16 dq[QG][2];
+  float lse2[QG], delta[QG];
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    const int r = first + 32 * g + (lane & 31);
+    const float ls = r < it.row_end ? p.lse[stat + r] : -__builtin_inff();
+    const bool valid = ls != -__builtin_inff();  // rows without a key, or not there
+    const __bf16* qp = p.q.ptr + it.clip * p.q.clip + it.head * p.q.head + r * p.q.token + 8 * h;
+    const __bf16* dp = p.doo.ptr + it.clip * p.doo.clip + it.head * p.doo.head + r * p.doo.token + 8 * h;
+    const __bf16* op = p.o.ptr + it.clip * p.o.clip + it.head * p.o.head + r * p.o.token + 8 * h;
+    const __bf16* rp = p.rest.ptr + it.clip * p.rest.clip + it.head * p.rest.head + r * p.rest.token + 8 * h;
+    float d = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      qf[g][ks] = dof[g][ks] = bf16x8{};
+      if (valid) {
+        qf[g][ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
+        dof[g][ks] = *reinterpret_cast<const bf16x8*>(dp + 16 * ks);
+        const bf16x8 of = *reinterpret_cast<const bf16x8*>(op + 16 * ks);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d += (float)dof[g][ks][j] * (float)of[j];
+        if (p.rest.ptr) {
+          const bf16x8 rf = *reinterpret_cast<const bf16x8*>(rp + 16 * ks);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d += (float)dof[g][ks][j] * (float)rf[j];
+        }
+      }
+    }
+    d = pair_sum(d);
+    delta[g] = d;
+    lse2[g] = valid ? ls * kLog2e : __builtin_inff();
+    if (h == 0 && r < it.row_end) p.delta[stat + r] = d;
+    dq[g][0] = dq[g][1] = f32x16{};
+  }
+
+  const int na = tiles_of(it.a1 - it.a0), nw = na + tiles_of(it.b1 - it.b0);
+  Staged st;
+  int start, end;
+  uint8_t mb = 0;
+  if (nw > 0) {
+    walk_tile(it, na, 0, &start, &end);
+    stage_load(st, kb, p.k.token, vb, p.v.token, start, end);
+    mb = mask_byte<MASK>(mask, start, end);
+  }
+  for (int i = 0; i < nw; ++i) {
+    const uint64_t bits = __ballot(mb != 0);
+    __bf16* kt = lds[i & 1][0];
+    __bf16* vt = lds[i & 1][1];
+    stage_write<MASK>(st, kt, vt, bits);
+    __syncthreads();
+    if (i + 1 < nw) {
+      walk_tile(it, na, i + 1, &start, &end);
+      stage_load(st, kb, p.k.token, vb, p.v.token, start, end);
+      mb = mask_byte<MASK>(mask, start, end);
+    }
+    if (!active) continue;
+#pragma unroll
+    for (int kh = 0; kh < 2; ++kh) {
+      f32x16 s[QG], dp[QG];
+#pragma unroll
+      for (int g = 0; g < QG; ++g) s[g] = dp[g] = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const bf16x8 a = row_frag(kt, fa, kh, ks), b = row_frag(vt, fa, kh, ks);
+#pragma unroll
+        for (int g = 0; g < QG; ++g) {
+          s[g] = mma(a, qf[g][ks], s[g]);
+          dp[g] = mma(b, dof[g][ks], dp[g]);
+        }
+      }
+      if (bits != ~0ull) {
+#pragma unroll
+        for (int g = 0; g < QG; ++g) mask_scores(s[g], bits, kh, h);
+      }
+#pragma unroll
+      for (int g = 0; g < QG; ++g)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          s[g][j] = __builtin_amdgcn_exp2f(s[g][j] * p.c - lse2[g]) * (dp[g][j] - delta[g]);
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        bf16x8 ds[QG];
+#pragma unroll
+        for (int g = 0; g < QG; ++g) ds[g] = pack8(s[g], step);
+#pragma unroll
+        for (int dh = 0; dh < 2; ++dh) {
+          const bf16x8 a = tr_frag(kt, fa, 2 * kh + step, dh);
+#pragma unroll
+          for (int g = 0; g < QG; ++g) dq[g][dh] = mma(a, ds[g], dq[g][dh]);
+        }
+      }
+    }
+  }
+  if (!active) return;
+#pragma unroll
+  for (int g = 0; g < QG; ++g) {
+    const int r = first + 32 * g + (lane & 31);
+    if (r < it.row_end) {
+      __bf16* op = p.dq.ptr + it.clip * p.dq.clip + it.head * p.dq.head + r * p.dq.token + 4 * h;
+#pragma unroll
+      for (int dh = 0; dh < 2; ++dh)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          __bf16 w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = (__bf16)(dq[g][dh][4 * j + e] * p.scale);
+          *reinterpret_cast<u32x2*>(op + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(w);
+        }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Backward over keys: dK and dV. A wave owns 32 KG key rows as columns of S = Q K^T and dP = dO V^T;
+// dV^T += dO^T P, dK^T += Q^T dS. The rows' statistics come from LDS: a query that is not there has
+// lse = +inf and D = 0, so that its probabilities are zero.
+// ---------------------------------------------------------------------------------------
+template <int KG, bool MASK>
+__global__ void __launch_bounds__(256, KG == 2 ? 1 : 2) frame_attn_dkv_kernel(const FaParams p) {
+  __shared__ __align__(16) __bf16 lds[2][2][kTileElems];
+  __shared__ __align__(16) float stats[2][2][kTile];
+  const FaItem it = fa_item(p, 128 * KG);
+  const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6), h = lane >> 5;
+  const FragAddr fa = frag_addr(lane);
+  const __bf16* qb = p.q.ptr + it.clip * p.q.clip + it.head * p.q.head;
+  const __bf16* db = p.doo.ptr + it.clip * p.doo.clip + it.head * p.doo.head;
+  const uint8_t* mask = MASK ? p.mask + (int64_t)it.clip * p.N : nullptr;
+  const int64_t stat = ((int64_t)it.clip * p.H + it.head) * p.N;
+  const int first = it.row0 + wave * 32 * KG;
+  const bool active = first < it.row_end;
+
+  bf16x8 kf[KG][4], vf[KG][4];
+  f32x16 dk[KG][2], dv[KG][2];
+  bool valid[KG];
+#pragma unroll
+  for (int g = 0; g < KG; ++g) {
+    const int r = first + 32 * g + (lane & 31);
+    valid[g] = r < it.row_end && (!MASK || mask[r]);
+    const __bf16* kp = p.k.ptr + it.clip * p.k.clip + it.head * p.k.head + r * p.k.token + 8 * h;
+    const __bf16* vp = p.v.ptr + it.clip * p.v.clip + it.head * p.v.head + r * p.v.token + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      kf[g][ks] = valid[g] ? *reinterpret_cast<const bf16x8*>(kp + 16 * ks) : bf16x8{};
+      vf[g][ks] = valid[g] ? *reinterpret_cast<const bf16x8*>(vp + 16 * ks) : bf16x8{};
+    }
+    dk[g][0] = dk[g][1] = dv[g][0] = dv[g][1] = f32x16{};
+  }
+
+  const int na = tiles_of(it.a1 - it.a0), nw = na + tiles_of(it.b1 - it.b0);
+  Staged st;
+  int start, end;
+  float ls = 0.f, dl = 0.f;
+  auto load = [&](int i) {
+    walk_tile(it, na, i, &start, &end);
+    stage_load(st, qb, p.q.token, db, p.doo.token, start, end);
+    const int tok = start + lane;
+    ls = tok < end ? p.lse[stat + tok] : -__builtin_inff();
+    dl = tok < end ? p.delta[stat + tok] : 0.f;
+  };
+  if (nw > 0) load(0);
+  for (int i = 0; i < nw; ++i) {
+    // rows without a key (masked ones among them) hold whatever their buffers held: they are written as zeros
+    const bool there = ls != -__builtin_inff();
+    const uint64_t bits = __ballot(there);
+    __bf16* qt = lds[i & 1][0];
+    __bf16* dt = lds[i & 1][1];
+    stage_write<true>(st, qt, dt, bits);
+    if (wave == 0) {
+      stats[i & 1][0][lane] = there ? ls * kLog2e : __builtin_inff();
+      stats[i & 1][1][lane] = there ? dl : 0.f;
+    }
+    __syncthreads();
+    if (i + 1 < nw) load(i + 1);
+    if (!active) continue;
+#pragma unroll
+    for (int qh = 0; qh < 2; ++qh) {
+      f32x16 s[KG], dp[KG], ls2, dl2;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(&stats[i & 1][0][32 * qh + 8 * j + 4 * h]);
+        const f32x4 b = *reinterpret_cast<const f32x4*>(&stats[i & 1][1][32 * qh + 8 * j + 4 * h]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          ls2[4 * j + e] = a[e];
+          dl2[4 * j + e] = b[e];
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < KG; ++g) s[g] = dp[g] = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const bf16x8 a = row_frag(qt, fa, qh, ks), b = row_frag(dt, fa, qh, ks);
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+          s[g] = mma(a, kf[g][ks], s[g]);
+          dp[g] = mma(b, vf[g][ks], dp[g]);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < KG; ++g)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          s[g][j] = __builtin_amdgcn_exp2f(s[g][j] * p.c - ls2[j]);
+          dp[g][j] = s[g][j] * (dp[g][j] - dl2[j]);
+        }
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        bf16x8 pf[KG], ds[KG];
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+          pf[g] = pack8(s[g], step);
+          ds[g] = pack8(dp[g], step);
+        }
+#pragma unroll
+        for (int dh = 0; dh < 2; ++dh) {
+          const bf16x8 a = tr_frag(dt, fa, 2 * qh + step, dh), b = tr_frag(qt, fa, 2 * qh + step, dh);
+#pragma unroll
+          for (int g = 0; g < KG; ++g) {
+            dv[g][dh] = mma(a, pf[g], dv[g][dh]);
+            dk[g][dh] = mma(b, ds[g], dk[g][dh]);
+          }
+        }
+      }
+    }
+  }
+  if (!active) return;
+#pragma unroll
+  for (int g = 0; g < KG; ++g) {
+    const int r = first + 32 * g + (lane & 31);
+    if (r < it.row_end) {
+      __bf16* kp = p.dk.ptr + it.clip * p.dk.clip + it.head * p.dk.head + r * p.dk.token + 4 * h;
+      __bf16* vp = p.dv.ptr + it.clip * p.dv.clip + it.head * p.dv.head + r * p.dv.token + 4 * h;
+#pragma unroll
+      for (int dh = 0; dh < 2; ++dh)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          __bf16 a[4], b[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            a[e] = (__bf16)(valid[g] ? dk[g][dh][4 * j + e] * p.scale : 0.f);
+            b[e] = (__bf16)(valid[g] ? dv[g][dh][4 * j + e] : 0.f);
+          }
+          *reinterpret_cast<u32x2*>(kp + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(a);
+          *reinterpret_cast<u32x2*>(vp + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(b);
+        }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------
+struct SegList {
+  FaSeg seg[kFaMaxSegs];
+  int64_t cost[kFaMaxSegs];  // walked tokens of a tile
+  int n = 0;
+};
+
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// frames f0 .. f1 - 1, each in tiles of its own
+static void add_frames(SegList* s, int head, int T, int f0, int f1, int rows, int walk, int64_t cost) {
+  if (f1 <= f0) return;
+  FaSeg& g = s->seg[s->n];
+  g.nt = (int)ceil_div(T, rows);
+  g.per_clip = g.nt * (f1 - f0);
+  g.tok0 = f0 * T;
+  g.tok1 = f1 * T;
+  g.head = (int16_t)head;
+  g.walk = (int16_t)walk;
+  s->cost[s->n++] = cost;
+}
+
+static void add_tokens(SegList* s, int head, int tok0, int tok1, int rows, int walk, int64_t cost) {
+  if (tok1 <= tok0) return;
+  FaSeg& g = s->seg[s->n];
+  g.nt = 0;
+  g.per_clip = (int)ceil_div(tok1 - tok0, rows);
+  g.tok0 = tok0;
+  g.tok1 = tok1;
+  g.head = (int16_t)head;
+  g.walk = (int16_t)walk;
+  s->cost[s->n++] = cost;
+}
+
+// Row tiles of every head, the longest walks first. keys: the tiles are key rows and walk queries.
+static int64_t make_segs(FaParams* p, const int32_t* patterns, int clips, int frames, int rows, bool keys) {
+  SegList s;
+  const int T = p->T, N = p->N;
+  for (int h = 0; h < p->H; ++h) {
+    switch (patterns[h]) {
+      case SAF3R_DENSE: add_tokens(&s, h, 0, N, rows, kAll, N); break;
+      case SAF3R_FRAME_LOCAL: add_frames(&s, h, T, 0, frames, rows, kOwn, T); break;
+      case SAF3R_ANCHOR:
+        if (keys) {  // the first frame's keys serve every query, the others none
+          add_tokens(&s, h, 0, T, rows, kAll, N);
+          add_tokens(&s, h, T, N, rows, kNone, 0);
+        } else {
+          add_tokens(&s, h, 0, N, rows, kFirst, T);
+        }
+        break;
+      case SAF3R_ANCHOR_LOCAL:
+        if (keys) {
+          add_tokens(&s, h, 0, T, rows, kAll, N);
+          add_frames(&s, h, T, 1, frames, rows, kOwn, T);
+        } else {
+          add_frames(&s, h, T, 0, frames, rows, kFirstOwn, 2 * (int64_t)T);
+        }
+        break;
+      default: add_tokens(&s, h, 0, N, rows, kNone, 0); break;  // SAF3R_SKIP
+    }
+  }
+  int order[kFaMaxSegs];
+  for (int i = 0; i < s.n; ++i) order[i] = i;
+  std::stable_sort(order, order + s.n, [&](int a, int b) { return s.cost[a] > s.cost[b]; });
+  int64_t total = 0;
+  for (int i = 0; i < s.n; ++i) {
+    p->seg[i] = s.seg[order[i]];
+    p->seg[i].start = (int)std::min<int64_t>(total, 0x7fffffff);
+    total += (int64_t)p->seg[i].per_clip * clips;
+  }
+  p->n_seg = s.n;
+  return total;
+}
+
+static bool fa_tensor(FaTensor* t, const saf3r_heads* h) {
+  if (!h || !h->ptr) return false;
+  t->ptr = (__bf16*)const_cast<void*>(h->ptr);
+  t->clip = h->clip_stride;
+  t->token = h->token_stride;
+  t->head = h->head_stride;
+  return true;
+}
+
+static bool fa_aligned(const FaTensor& t) {
+  return (uintptr_t)t.ptr % 16 == 0 && t.clip % 8 == 0 && t.token % 8 == 0 && t.head % 8 == 0;
+}
+
+static int fa_check(const char* who, FaParams* p, int clips, int frames, int tokens_per_frame, int num_heads,
+                    const int32_t* patterns, const uint8_t* mask, float scale) {
+  if (clips < 0 || frames <= 0 || tokens_per_frame <= 0)
+    return fail(SAF3R_ERR_INVALID, "%s: invalid sizes: %d clips, %d frames x %d tokens", who, clips, frames,
+                tokens_per_frame);
+  if (num_heads <= 0) return fail(SAF3R_ERR_INVALID, "%s: bad num_heads %d", who, num_heads);
+  if (num_heads > kMaxHeads)
+    return fail(SAF3R_ERR_UNSUPPORTED, "%s: %d heads (at most %d)", who, num_heads, kMaxHeads);
+  if ((int64_t)frames * tokens_per_frame > 0x7fffff00 - 512)
+    return fail(SAF3R_ERR_UNSUPPORTED, "%s: %d frames x %d tokens pass 31 bits", who, frames, tokens_per_frame);
+  if (!patterns) return fail(SAF3R_ERR_INVALID, "%s: null patterns", who);
+  for (int h = 0; h < num_heads; ++h) {
+    const int x = patterns[h];
+    if (x != SAF3R_DENSE && x != SAF3R_FRAME_LOCAL && x != SAF3R_ANCHOR_LOCAL && x != SAF3R_ANCHOR && x != SAF3R_SKIP)
+      return fail(x < 0 || x > SAF3R_TOKEN_DYNAMIC_KEYSET ? SAF3R_ERR_INVALID : SAF3R_ERR_UNSUPPORTED,
+                  "%s: head %d: pattern %d is not one of dense, frame-local, anchor-local, anchor, skip", who, h, x);
+  }
+  if (!(scale > 0.f && scale < 3.0e38f)) return fail(SAF3R_ERR_INVALID, "%s: scale must be positive and finite", who);
+  p->N = frames * tokens_per_frame;
+  p->T = tokens_per_frame;
+  p->H = num_heads;
+  p->mask = mask;
+  p->scale = scale;
+  p->c = scale * kLog2e;
+  return SAF3R_OK;
+}
+
+static int fa_grid(const char* who, int64_t total) {
+  if (total > 0x7fffffff) return fail(SAF3R_ERR_UNSUPPORTED, "%s: too many row tiles for one launch", who);
+  return SAF3R_OK;
+}
+
+}  // namespace saf3r
+
+using namespace saf3r;
+
+extern "C" int saf3r_frame_attn_fwd(const saf3r_heads* q, const saf3r_heads* k, const saf3r_heads* v, int clips,
+                                    int frames, int tokens_per_frame, int num_heads, const int32_t* patterns,
+                                    const uint8_t* token_mask, float scale, const saf3r_heads* out,
+                                    const saf3r_heads* out_rest, float* lse, void* stream) {
+  const char* who = "saf3r_frame_attn_fwd";
+  if (int e = injected(who)) return e;
+  FaParams p{};
+  if (int e = fa_check(who, &p, clips, frames, tokens_per_frame, num_heads, patterns, token_mask, scale)) return e;
+  if (clips == 0) return SAF3R_OK;
+  if (!fa_tensor(&p.q, q) || !fa_tensor(&p.k, k) || !fa_tensor(&p.v, v) || !fa_tensor(&p.o, out) || !lse)
+    return fail(SAF3R_ERR_INVALID, "%s: null tensor pointer", who);
+  if (out_rest && !fa_tensor(&p.rest, out_rest)) return fail(SAF3R_ERR_INVALID, "%s: null out_rest", who);
+  if (!fa_aligned(p.q) || !fa_aligned(p.k) || !fa_aligned(p.v) || !fa_aligned(p.o) || !fa_aligned(p.rest) ||
+      (uintptr_t)lse % 4)
+    return fail(SAF3R_ERR_INVALID, "%s: rows must be 16-byte aligned with strides a multiple of 8", who);
+  p.lse = lse;
+  const int64_t n = make_segs(&p, patterns, clips, frames, 256, false);
+  if (int e = fa_grid(who, n)) return e;
+  if (token_mask)
+    hipLaunchKernelGGL((frame_attn_fwd_kernel<2, true>), dim3((uint32_t)n), dim3(256), 0, (hipStream_t)stream, p);
+  else
+    hipLaunchKernelGGL((frame_attn_fwd_kernel<2, false>), dim3((uint32_t)n), dim3(256), 0, (hipStream_t)stream, p);
+  return check_launch(who);
+}
+
+extern "C" int64_t saf3r_frame_attn_bwd_workspace_bytes(int clips, int frames, int tokens_per_frame, int num_heads) {
+  const char* who = "saf3r_frame_attn_bwd_workspace_bytes";
+  if (clips < 0 || frames <= 0 || tokens_per_frame <= 0 || num_heads <= 0 || num_heads > kMaxHeads ||
+      (int64_t)frames * tokens_per_frame > 0x7fffff00 - 512) {
+    fail(SAF3R_ERR_INVALID, "%s: invalid sizes", who);
+    return -1;
+  }
+  return (int64_t)clips * num_heads * frames * tokens_per_frame * 4;
+}
+
+extern "C" int saf3r_frame_attn_bwd(const saf3r_heads* dout, const saf3r_heads* q, const saf3r_heads* k,
+                                    const saf3r_heads* v, const saf3r_heads* out, const saf3r_heads* out_rest,
+                                    const float* lse, int clips, int frames, int tokens_per_frame, int num_heads,
+                                    const int32_t* patterns, const uint8_t* token_mask, float scale,
+                                    const saf3r_heads* dq, const saf3r_heads* dk, const saf3r_heads* dv,
+                                    void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "saf3r_frame_attn_bwd";
+  if (int e = injected(who)) return e;
+  FaParams p{};
+  if (int e = fa_check(who, &p, clips, frames, tokens_per_frame, num_heads, patterns, token_mask, scale)) return e;
+  if (clips == 0) return SAF3R_OK;
+  if (!fa_tensor(&p.doo, dout) || !fa_tensor(&p.q, q) || !fa_tensor(&p.k, k) || !fa_tensor(&p.v, v) ||
+      !fa_tensor(&p.o, out) || !fa_tensor(&p.dq, dq) || !fa_tensor(&p.dk, dk) || !fa_tensor(&p.dv, dv) || !lse)
+    return fail(SAF3R_ERR_INVALID, "%s: null tensor pointer", who);
+  if (out_rest && !fa_tensor(&p.rest, out_rest)) return fail(SAF3R_ERR_INVALID, "%s: null out_rest", who);
+  for (const FaTensor* t : {&p.doo, &p.q, &p.k, &p.v, &p.o, &p.rest, &p.dq, &p.dk, &p.dv})
+    if (!fa_aligned(*t))
+      return fail(SAF3R_ERR_INVALID, "%s: rows must be 16-byte aligned with strides a multiple of 8", who);
+  const int64_t need = saf3r_frame_attn_bwd_workspace_bytes(clips, frames, tokens_per_frame, num_heads);
+  if (workspace_bytes < need || !workspace || (uintptr_t)workspace % 16 || (uintptr_t)lse % 4)
+    return fail(SAF3R_ERR_INVALID, "%s: workspace of %lld bytes: %lld, 16-byte aligned, are needed", who,
+                (long long)workspace_bytes, (long long)need);
+  p.lse = const_cast<float*>(lse);
+  p.delta = (float*)workspace;
+  FaParams pk = p;
+  const int64_t nq = make_segs(&p, patterns, clips, frames, 256, false);
+  const int64_t nk = make_segs(&pk, patterns, clips, frames, 256, true);
+  if (int e = fa_grid(who, std::max(nq, nk))) return e;
+  const hipStream_t s = (hipStream_t)stream;
+  if (token_mask) {
+    hipLaunchKernelGGL((frame_attn_dq_kernel<2, true>), dim3((uint32_t)nq), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((frame_attn_dkv_kernel<2, true>), dim3((uint32_t)nk), dim3(256), 0, s, pk);
+  } else {
+    hipLaunchKernelGGL((frame_attn_dq_kernel<2, false>), dim3((uint32_t)nq), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((frame_attn_dkv_kernel<2, false>), dim3((uint32_t)nk), dim3(256), 0, s, pk);
+  }
+  return check_launch(who);
+}

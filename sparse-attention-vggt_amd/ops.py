@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
+from contextlib import nullcontext
 from dataclasses import dataclass
 from functools import lru_cache
 from typing import Sequence
@@ -899,3 +900,373 @@ def frame_topk_scores(scores: torch.Tensor, frames: int, per_frame: int, topk: i
     _mark("frame_topk", "end")
     return idx
 
+
+
+# ---- training: attention over frames with its gradients ---------------------------------------------------
+
+STATIC_PATTERNS = (DENSE, FRAME_LOCAL, ANCHOR_LOCAL, ANCHOR, SKIP)  # patterns of frame_attn_fwd / frame_attn_bwd
+
+
+def _on_device(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one (its current stream takes the launches)."""
+    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _readable(t: torch.Tensor, step: int) -> torch.Tensor:
+    """``t`` as the kernels can read it (consecutive elements in a row, 16-byte aligned rows, strides a multiple of
+    ``step``): itself, or a contiguous copy."""
+    ok = (t.shape[-1] <= 1 or t.stride(-1) == 1) and t.data_ptr() % 16 == 0 and all(
+        n <= 1 or s % step == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+    if ok:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _frame_heads(t: torch.Tensor) -> _lib.Heads:
+    """``saf3r_heads`` of a [clips, tokens, heads, 64] tensor (the stride of a size of one is not used)."""
+    b, n, h = (s if size > 1 else 0 for s, size in zip(t.stride()[:3], t.shape[:3]))
+    return _lib.Heads(t.data_ptr(), b, n, 0, h)
+
+
+def _frame_args(q, k, v, patterns, frames: int, token_mask, scale):
+    """Checks shared by the attention's two directions: (patterns as a host array, mask or None, scale)."""
+    _need_cuda(q, k, v, token_mask)
+    if q.dim() != 4 or q.shape[3] != HEAD_DIM:
+        raise ValueError(f"q must be [clips, tokens, heads, {HEAD_DIM}], got {tuple(q.shape)}")
+    for name, t in (("k", k), ("v", v)):
+        if t.shape != q.shape:
+            raise ValueError(f"{name} must have q's shape {tuple(q.shape)}, got {tuple(t.shape)}")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dtype != torch.bfloat16:
+            raise ValueError(f"{name} must be bfloat16, got {t.dtype}")
+        if t.device != q.device:
+            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
+    B, N, H, _ = q.shape
+    if frames < 1 or N < 1 or N % frames:
+        raise ValueError(f"{N} tokens are not {frames} frames of one size")
+    if len(patterns) != H:
+        raise ValueError(f"one pattern per head: got {len(patterns)} for {H} heads")
+    if token_mask is not None:
+        if token_mask.dtype not in (torch.bool, torch.uint8) or tuple(token_mask.shape) != (B, N):
+            raise ValueError(f"token_mask must be bool [{B}, {N}], got {token_mask.dtype} {tuple(token_mask.shape)}")
+        if token_mask.device != q.device:
+            raise ValueError(f"token_mask is on {token_mask.device}, q on {q.device}")
+        token_mask = token_mask.contiguous()
+    return _i32_array(patterns), token_mask, float(1.0 / math.sqrt(HEAD_DIM) if scale is None else scale)
+
+
+def frame_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, patterns: Sequence[int], frames: int = 1,
+                   token_mask: torch.Tensor | None = None, scale: float | None = None, rest: bool = False):
+    """Attention of every head over the tokens of its frames, with the statistics of the backward pass
+    (``saf3r_frame_attn_fwd``). ``q``, ``k``, ``v`` bf16 [clips, tokens, heads, 64] (views of a qkv buffer are read
+    as they are), ``tokens`` = ``frames`` frames of one size; ``patterns`` one of ``STATIC_PATTERNS`` per head.
+    ``token_mask`` [clips, tokens] (True: the token is there) removes padded tokens: they are no keys, their rows
+    come out as zeros and what their q, k and v hold is not used. Returns (out bf16 [clips, tokens, heads, 64],
+    lse fp32 [clips, heads, tokens]); a row without a key is zeros with lse -inf. With ``rest`` a third tensor like out
+    holds what its rounding took away, for the backward pass. Not differentiable by itself: see
+    ``autograd.frame_attention``."""
+    pat, mask, scale = _frame_args(q, k, v, patterns, frames, token_mask, scale)
+    lib = _lib.load()
+    B, N, H, _ = q.shape
+    q, k, v = (_readable(t, 8) for t in (q, k, v))
+    with _on_device(q):
+        out = torch.empty(B, N, H, HEAD_DIM, dtype=torch.bfloat16, device=q.device)
+        low = torch.empty_like(out) if rest else None
+        lse = torch.empty(B, H, N, dtype=torch.float32, device=q.device)
+        _mark("frame_attn_fwd", "start")
+        _lib.check(lib.saf3r_frame_attn_fwd(_frame_heads(q), _frame_heads(k), _frame_heads(v), B, frames, N // frames,
+                                            H, pat, _ptr(mask), scale, _frame_heads(out),
+                                            _frame_heads(low) if rest else None, _ptr(lse), _lib.stream_ptr()))
+        _mark("frame_attn_fwd", "end")
+    return (out, lse, low) if rest else (out, lse)
+
+
+def frame_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                   lse: torch.Tensor, patterns: Sequence[int], frames: int = 1,
+                   token_mask: torch.Tensor | None = None, scale: float | None = None, rest: torch.Tensor | None = None,
+                   grads=None):
+    """Gradients (dq, dk, dv) of ``frame_attn_fwd`` (``saf3r_frame_attn_bwd``) from the gradient ``dout`` of its
+    output; ``out``, ``lse`` and ``rest`` are its results, the other arguments those of that call (without ``rest``
+    dq and dk carry the rounding of out: 1.5 to 2 times their error). ``grads`` (optional): three
+    bf16 tensors or views of q's shape that receive them (rows 16-byte aligned, strides a multiple of 8, not
+    overlapping the inputs). The results do not depend on the order in which the GPU runs the work."""
+    pat, mask, scale = _frame_args(q, k, v, patterns, frames, token_mask, scale)
+    _need_cuda(dout, out, lse)
+    lib = _lib.load()
+    B, N, H, _ = q.shape
+    _need_cuda(rest)
+    for name, t in (("dout", dout), ("out", out)) + ((("rest", rest),) if rest is not None else ()):
+        if t.shape != q.shape or t.dtype != torch.bfloat16 or t.device != q.device:
+            raise ValueError(f"{name} must be bfloat16 {tuple(q.shape)} on {q.device}, got {t.dtype} {tuple(t.shape)}")
+    if tuple(lse.shape) != (B, H, N) or lse.dtype != torch.float32 or lse.device != q.device:
+        raise ValueError(f"lse must be float32 {(B, H, N)} on {q.device}, got {lse.dtype} {tuple(lse.shape)}")
+    dout, q, k, v, out = (_readable(t, 8) for t in (dout, q, k, v, out))
+    rest = None if rest is None else _readable(rest, 8)
+    lse = lse.contiguous()
+    with _on_device(q):
+        if grads is None:
+            grads = tuple(torch.empty(B, N, H, HEAD_DIM, dtype=torch.bfloat16, device=q.device) for _ in range(3))
+        else:
+            for t in grads:
+                if t.shape != q.shape or t.dtype != torch.bfloat16 or t.device != q.device:
+                    raise ValueError(f"grads must be bfloat16 {tuple(q.shape)} on {q.device}")
+                if _readable(t, 8) is not t:
+                    raise ValueError("grads need 16-byte aligned rows with strides a multiple of 8")
+        nbytes = lib.saf3r_frame_attn_bwd_workspace_bytes(B, frames, N // frames, H)
+        if nbytes < 0:
+            raise ValueError(f"unsupported attention: {H} heads, {frames} frames of {N // frames} tokens")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        _mark("frame_attn_bwd", "start")
+        _lib.check(lib.saf3r_frame_attn_bwd(
+            _frame_heads(dout), _frame_heads(q), _frame_heads(k), _frame_heads(v), _frame_heads(out),
+            None if rest is None else _frame_heads(rest), _ptr(lse), B, frames, N // frames, H, pat, _ptr(mask), scale,
+            *(_frame_heads(t) for t in grads), _ptr(ws), nbytes, _lib.stream_ptr()))
+        _mark("frame_attn_bwd", "end")
+    return tuple(grads)
+
+
+# ---- training: rotary positions and norms with their gradients ---------------------------------------------
+
+_DTYPES = {torch.float32: _lib.FP32, torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
+
+
+def _dtype(name: str, t: torch.Tensor) -> int:
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _norm_params(shape: tuple, rows_dtype, device, **params):
+    """(dtype of the parameters, type the kernels read them in, the contiguous tensors or None): weight and bias of one
+    type and of ``shape``. Parameters that are neither fp32 nor of the rows' 16-bit type are read as fp32 copies."""
+    given = {n: t for n, t in params.items() if t is not None}
+    for n, t in given.items():
+        _dtype(n, t)
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{n} must be {shape}, got {tuple(t.shape)}")
+        if t.device != device:
+            raise ValueError(f"{n} is on {t.device}, the rows on {device}")
+    kinds = {t.dtype for t in given.values()}
+    if len(kinds) > 1:
+        raise ValueError("weight and bias must have one dtype")
+    kind = kinds.pop() if kinds else torch.float32
+    read = kind if kind == rows_dtype else torch.float32
+    return kind, _DTYPES[read], [None if t is None else t.to(read).contiguous() for t in params.values()]
+
+
+def _param_grads(shape: tuple, kind: torch.dtype, read: int, device, needs):
+    """Buffers for the parameters' gradients, in the type that the kernels read the parameters in."""
+    dtype = kind if _DTYPES[kind] == read else torch.float32
+    return [torch.empty(shape, dtype=dtype, device=device) if need else None for need in needs]
+
+
+def _flat_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as [rows, dim] with consecutive elements in a row; a copy where its strides do not allow that view."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                   eps: float = 1e-5, out_dtype: torch.dtype | None = None):
+    """LayerNorm over the last dimension (1 .. 8192 wide, ``saf3r_layer_norm_fwd``): (y, mean, rstd), the statistics
+    fp32 of x's leading shape, for ``layer_norm_bwd``. x fp32, bf16 or fp16; y in x's type, or for fp32 x in
+    ``out_dtype`` (fp32 arithmetic, rounded once). Not differentiable by itself: see ``autograd.layer_norm``."""
+    _need_cuda(x, weight, bias)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must have a last dimension, got {tuple(x.shape)}")
+    xt = _dtype("x", x)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype != x.dtype and (x.dtype != torch.float32 or out_dtype not in _DTYPES):
+        raise ValueError(f"{x.dtype} rows give {x.dtype} rows, not {out_dtype}")
+    dim = x.shape[-1]
+    _, pt, (weight, bias) = _norm_params((dim,), out_dtype, x.device, weight=weight, bias=bias)
+    lib = _lib.load()
+    with _on_device(x):
+        rows = _flat_rows(x)
+        y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        stats = torch.empty(2, *x.shape[:-1], dtype=torch.float32, device=x.device)
+        mean, rstd = stats[0], stats[1]
+        _mark("layer_norm_fwd", "start")
+        _lib.check(lib.saf3r_layer_norm_fwd(_ptr(rows), _row_stride(rows), xt, rows.shape[0], dim, _ptr(weight),
+                                            _ptr(bias), pt, float(eps), _ptr(y), dim, _DTYPES[out_dtype], _ptr(mean),
+                                            _ptr(rstd), _lib.stream_ptr()))
+        _mark("layer_norm_fwd", "end")
+    return y, mean, rstd
+
+
+def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                   weight: torch.Tensor | None = None, need_params: tuple[bool, bool] = (True, True)):
+    """Gradients (dx, dweight, dbias) of ``layer_norm_fwd`` (``saf3r_layer_norm_bwd``) from ``dy`` (y's shape and
+    type); ``mean`` and ``rstd`` are its results. dweight / dbias are None where ``need_params`` says so, else of
+    weight's type (fp32 without a weight). Equal inputs give equal bits."""
+    _need_cuda(dy, x, mean, rstd, weight)
+    xt, yt = _dtype("x", x), _dtype("dy", dy)
+    if dy.shape != x.shape or dy.device != x.device or x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"dy must be like x {tuple(x.shape)} on {x.device}, got {tuple(dy.shape)} on {dy.device}")
+    for n, t in (("mean", mean), ("rstd", rstd)):
+        if t.shape != x.shape[:-1] or t.dtype != torch.float32 or t.device != x.device:
+            raise ValueError(f"{n} must be float32 {tuple(x.shape[:-1])}, got {t.dtype} {tuple(t.shape)}")
+    dim = x.shape[-1]
+    kind, pt, (weight,) = _norm_params((dim,), dy.dtype, x.device, weight=weight)
+    lib = _lib.load()
+    with _on_device(x):
+        rows, drows = _flat_rows(x), _flat_rows(dy)
+        mean, rstd = mean.contiguous(), rstd.contiguous()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dw, db = _param_grads((dim,), kind, pt, x.device, need_params)
+        nbytes, ws = 0, None
+        if any(need_params):
+            nbytes = lib.saf3r_layer_norm_bwd_workspace_bytes(rows.shape[0], dim)
+            if nbytes >= 0:
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _mark("layer_norm_bwd", "start")
+        _lib.check(lib.saf3r_layer_norm_bwd(_ptr(drows), _row_stride(drows), yt, _ptr(rows), _row_stride(rows), xt,
+                                            rows.shape[0], dim, _ptr(mean), _ptr(rstd), _ptr(weight), pt, _ptr(dx),
+                                            dim, _ptr(dw), _ptr(db), _ptr(ws), nbytes, _lib.stream_ptr()))
+        _mark("layer_norm_bwd", "end")
+        return (dx, *(t if t is None else t.to(kind) for t in (dw, db)))
+
+
+def rotary_tables(positions: int, section: int, base: float = 100.0, scaling: str | None = None, factor: float = 1.0,
+                  device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """cos / sin tables [positions, section / 2] fp32 of ``head_rotary_fwd`` for sections of ``section`` elements:
+    angle = position x base^(-2 j / section), computed in 64 bits (a position of 2^20 keeps 24 bits of its angle).
+    ``scaling`` for ranges longer than the trained one by ``factor``: "linear" divides the positions by it, "ntk"
+    multiplies the base by factor^(section / (section - 2)), which leaves the fastest pair as it was and divides the
+    slowest one's positions by it. Made with torch for every call: keep them as a model keeps its buffers."""
+    positions, section, base, factor = int(positions), int(section), float(base), float(factor)
+    if positions < 1 or section < 2 or section % 2:
+        raise ValueError(f"tables need a position and sections of even size, got {positions} and {section}")
+    if not (base > 0 and math.isfinite(base) and factor > 0 and math.isfinite(factor)):
+        raise ValueError(f"base {base} and factor {factor} must be positive")
+    if scaling not in (None, "linear", "ntk"):
+        raise ValueError(f"scaling {scaling!r}: None, 'linear' or 'ntk'")
+    if scaling == "ntk":
+        if section == 2:
+            raise ValueError("'ntk' scaling needs more than one pair of a section")
+        base *= factor ** (section / (section - 2))
+    inv = base ** -(torch.arange(0, section, 2, dtype=torch.float64) / section)
+    if scaling == "linear":
+        inv /= factor
+    ang = torch.arange(positions, dtype=torch.float64)[:, None] * inv
+    return ang.cos().float().to(device), ang.sin().float().to(device)
+
+
+def _rotary_args(x, pos, tables, layout: str, rotary_dim: int | None, norm: bool, weight, bias):
+    """Checks shared by both directions: (keyword values of the C entries, x's sizes)."""
+    if x.dim() != 5:
+        raise ValueError(f"x must be [clips, tokens, groups, heads, dim], got {tuple(x.shape)}")
+    B, N, G, H, D = x.shape
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"layout {layout!r}: 'half' or 'interleaved'")
+    if not norm and (weight is not None or bias is not None):
+        raise ValueError("weight and bias belong to the norm (norm=True)")
+    cos = sin = None
+    axes, positions, R = 1, 0, 0
+    if (pos is None) != (tables is None):
+        raise ValueError("rotary positions need pos and tables")
+    if tables is not None:
+        cos, sin = tables
+        _need_cuda(pos, cos, sin)
+        if pos.dim() != 3 or pos.shape[:2] != x.shape[:2] or not 1 <= pos.shape[2] <= 8:
+            raise ValueError(f"pos must be [{B}, {N}, axes] with 1 to 8 axes, got {tuple(pos.shape)}")
+        if pos.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"pos must be int32 or int64, got {pos.dtype}")
+        axes = pos.shape[2]
+        R = D if rotary_dim is None else int(rotary_dim)
+        if not 0 < R <= D or R % (2 * axes):
+            raise ValueError(f"rotary_dim {R} must be {axes} even sections of at most {D} elements")
+        for n, t in (("cos", cos), ("sin", sin)):
+            if t.dim() != 2 or t.shape != cos.shape or t.shape[1] != R // axes // 2 or t.dtype != torch.float32:
+                raise ValueError(f"{n} must be float32 [positions, {R // axes // 2}], got {t.dtype} {tuple(t.shape)}")
+        positions = cos.shape[0]
+        if positions < 1:
+            raise ValueError("the tables hold no position")
+        for n, t in (("pos", pos), ("cos", cos), ("sin", sin)):
+            if t.device != x.device:
+                raise ValueError(f"{n} is on {t.device}, x on {x.device}")
+        pos, cos, sin = pos.contiguous(), cos.contiguous(), sin.contiguous()
+    elif not norm:
+        raise ValueError("neither a norm nor rotary positions were asked for")
+    return pos, cos, sin, axes, positions, R
+
+
+def _group_heads(t: torch.Tensor) -> _lib.Heads:
+    """``saf3r_heads`` of a [clips, tokens, groups, heads, dim] tensor (the stride of a size of one is not used)."""
+    return _lib.Heads(t.data_ptr(), *(s if size > 1 else 0 for s, size in zip(t.stride()[:4], t.shape[:4])))
+
+
+def _unit_rows(t: torch.Tensor) -> torch.Tensor:
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def head_rotary_fwd(x: torch.Tensor, pos: torch.Tensor | None = None, tables=None, layout: str = "half",
+                    rotary_dim: int | None = None, norm: bool = False, weight: torch.Tensor | None = None,
+                    bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
+    """LayerNorm over the head dimension (``norm``) and rotary positions (``tables``) of q and k in one pass
+    (``saf3r_head_rotary_fwd``). ``x`` fp32, bf16 or fp16 [clips, tokens, groups, heads, dim] (dim even, at most 128),
+    for instance ``qkv.view(B, N, 3, H, 64)[:, :, :2]``, read as it lies. ``weight`` / ``bias`` [groups, dim].
+    ``tables`` (cos, sin) as of ``rotary_tables``; the first ``rotary_dim`` elements (default all) are
+    ``pos.shape[2]`` equal sections, section a rotated by position ``pos[clip, token, a]`` in pairs (j, j + half a
+    section) (``layout`` "half") or (2 j, 2 j + 1) ("interleaved"); positions outside the tables are taken to their
+    ends. Returns a contiguous tensor of x's shape and type. Not differentiable by itself: see
+    ``autograd.head_rotary``."""
+    _need_cuda(x, weight, bias)
+    xt = _dtype("x", x)
+    pos, cos, sin, axes, positions, R = _rotary_args(x, pos, tables, layout, rotary_dim, norm, weight, bias)
+    B, N, G, H, D = x.shape
+    _, pt, (weight, bias) = _norm_params((G, D), x.dtype, x.device, weight=weight, bias=bias)
+    lib = _lib.load()
+    with _on_device(x):
+        x = _unit_rows(x)
+        y = torch.empty(B, N, G, H, D, dtype=x.dtype, device=x.device)
+        _mark("head_rotary_fwd", "start")
+        _lib.check(lib.saf3r_head_rotary_fwd(
+            _group_heads(x), xt, B, N, G, H, D, _ptr(pos), int(pos is not None and pos.dtype == torch.int64), axes,
+            _ptr(cos), _ptr(sin), positions, R, int(layout == "interleaved"), int(norm), _ptr(weight), _ptr(bias), pt,
+            float(eps), _group_heads(y), _lib.stream_ptr()))
+        _mark("head_rotary_fwd", "end")
+    return y
+
+
+def head_rotary_bwd(dy: torch.Tensor, x: torch.Tensor, pos: torch.Tensor | None = None, tables=None,
+                    layout: str = "half", rotary_dim: int | None = None, norm: bool = False,
+                    weight: torch.Tensor | None = None, eps: float = 1e-5,
+                    need_params: tuple[bool, bool] = (True, True), out: torch.Tensor | None = None):
+    """Gradients (dx, dweight, dbias) of ``head_rotary_fwd`` (``saf3r_head_rotary_bwd``) from ``dy`` (x's shape and
+    type), the other arguments those of that call. dweight / dbias [groups, dim] are None without a norm or where
+    ``need_params`` says so, else of weight's type (fp32 without a weight). ``out`` (optional) receives dx: a tensor or
+    view like x with consecutive elements in a row, not overlapping the inputs. Equal inputs give equal bits."""
+    _need_cuda(dy, x, weight, out)
+    xt = _dtype("x", x)
+    pos, cos, sin, axes, positions, R = _rotary_args(x, pos, tables, layout, rotary_dim, norm, weight, None)
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError(f"dy must be like x: {x.dtype} {tuple(x.shape)}, got {dy.dtype} {tuple(dy.shape)}")
+    B, N, G, H, D = x.shape
+    kind, pt, (weight,) = _norm_params((G, D), x.dtype, x.device, weight=weight)
+    if out is not None:
+        if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or _unit_rows(out) is not out:
+            raise ValueError(f"out must be like x: {x.dtype} {tuple(x.shape)} with consecutive elements in a row")
+    lib = _lib.load()
+    with _on_device(x):
+        x, dy = _unit_rows(x), _unit_rows(dy)
+        dx = torch.empty(B, N, G, H, D, dtype=x.dtype, device=x.device) if out is None else out
+        dw, db = _param_grads((G, D), kind, pt, x.device, [need and norm for need in need_params])
+        nbytes, ws = 0, None
+        if dw is not None or db is not None:
+            nbytes = lib.saf3r_head_rotary_bwd_workspace_bytes(B, N, G, H, D)
+            if nbytes >= 0:
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _mark("head_rotary_bwd", "start")
+        _lib.check(lib.saf3r_head_rotary_bwd(
+            _group_heads(dy), _group_heads(x), xt, B, N, G, H, D, _ptr(pos),
+            int(pos is not None and pos.dtype == torch.int64), axes, _ptr(cos), _ptr(sin), positions, R,
+            int(layout == "interleaved"), int(norm), _ptr(weight), pt, float(eps), _group_heads(dx), _ptr(dw),
+            _ptr(db), _ptr(ws), nbytes, _lib.stream_ptr()))
+        _mark("head_rotary_bwd", "end")
+        return (dx, *(t if t is None else t.to(kind) for t in (dw, db)))

@@ -17,6 +17,9 @@ Configuration (plain dict or attribute object, as the reference's addict ``model
     patch_module.topk                      per-frame token top-k of dino_topk heads
     patch_module.block_topk                per-frame block top-k of block_topk heads (default 4)
     patch_module.topk_scope                "frame" (default) or "global" for block_topk heads
+    patch_module.trainable                 True: forwards that need gradients run through the differentiable
+                                           kernels (heads of the modes full / dense, global_to_frame /
+                                           frame_local, all_to_first, anchor_local and skip; others raise)
 The lazy indices are shared through one ``SelectionState`` per model instead of rebinding the
 aggregator forward: every dino_topk layer after the one holding the first correspondence head
 reads them, exactly the layers the reference copies them to. The non-lazy indices (and the DINO
@@ -78,7 +81,8 @@ def patch_model(model, model_cfg):
         orig = blocks[i].attn
         blocks[i].attn = HeadwiseSparseAttentionWrapper(
             orig, layer_idx=i, dino_topk=_get(pm, "topk", 4), lazy_dino_topk=lazy, config=layer_config,
-            block_topk=_get(pm, "block_topk", 4), topk_scope=_get(pm, "topk_scope", "frame"), shared=state)
+            block_topk=_get(pm, "block_topk", 4), topk_scope=_get(pm, "topk_scope", "frame"), shared=state,
+            trainable=_get(pm, "trainable", False))
     model.saf3r_selection_state = state
     if has_dino and not lazy:
         install_feature_topk(model, model_cfg)
@@ -170,7 +174,9 @@ class HeadwiseSparseAttentionWrapper(BaseHeadwiseSparseAttentionWrapper):
         if qkv.dtype != torch.bfloat16:
             qkv = qkv.to(torch.bfloat16)
         qkv = qkv.contiguous()
-        out = self.compute_multihead_attention_packed(qkv, None if pos is None else pos[0], geom)
+        p = None if pos is None else pos[0]
+        out = (self.compute_multihead_attention_trainable(qkv, p, geom) if self.needs_grad(qkv)
+               else self.compute_multihead_attention_packed(qkv, p, geom))
         y = out.reshape(B, N, C)
         if not torch.is_autocast_enabled("cuda") and y.dtype != om.proj.weight.dtype:
             y = y.to(om.proj.weight.dtype)

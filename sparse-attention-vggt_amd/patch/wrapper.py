@@ -20,7 +20,7 @@ from functools import lru_cache
 import torch
 from torch import nn
 
-from .. import ops
+from .. import autograd, ops
 from ..layout import HEAD_DIM, Geometry
 from .sparse_attention import keyset_spec, pattern_of
 
@@ -108,6 +108,12 @@ class BaseHeadwiseSparseAttentionWrapper(nn.Module):
         probe = {h for h in self.keyset_heads if self.head_cfg[h]["mode"] == "q_probe_topk"}
         self.fp32_heads = sorted(probe | set(self.dino_heads))
         self.fp32_slot = {h: i for i, h in enumerate(self.fp32_heads)}
+        # trainable: a forward that needs gradients runs through the differentiable kernels (static patterns)
+        self.trainable = bool(kwargs.get("trainable", False))
+        if self.trainable:
+            other = sorted({c["mode"] for c, p in zip(self.head_cfg, self.patterns) if p not in ops.STATIC_PATTERNS})
+            if other:
+                raise NotImplementedError(f"trainable: no gradients through heads of mode {', '.join(other)}")
         # pack Q with the softmax scale folded in (one bf16 rounding of the fp32 q * scale * log2 e), so
         # that the attention walks skip the running maximum; off for tests that compare the plain layout
         self.prescale_q = True
@@ -200,6 +206,22 @@ class BaseHeadwiseSparseAttentionWrapper(nn.Module):
                 orr = ops.rows(out, C, ns, P, T, offset=h * HEAD_DIM)
                 ops.gather_attn_rows(qr, kr, vr, est, W, geom.frames * P, W, geom.frames * P, None, orr, qk_fp32=True)
         kept["last_attention"] = out if self.keep_attention else None
+        return out
+
+    def needs_grad(self, qkv: torch.Tensor) -> bool:
+        """Whether this forward runs through the differentiable kernels."""
+        if not (self.trainable and torch.is_grad_enabled()):
+            return False
+        om = self.orig_module
+        return qkv.requires_grad or any(p.requires_grad for m in (om.q_norm, om.k_norm) for p in m.parameters())
+
+    def compute_multihead_attention_trainable(self, qkv: torch.Tensor, pos, geom: Geometry) -> torch.Tensor:
+        """As ``compute_multihead_attention_packed``, differentiable (``autograd.module_attention``); the same patterns
+        in natural token order, no packing."""
+        npos = max(self.patch_height, self.patch_width) + 1 if self.patch_height else None
+        out = autograd.module_attention(self.orig_module, qkv[None], None if pos is None else pos.reshape(1, -1, 2),
+                                        self.patterns, geom.frames, npos)[0]
+        self.__dict__["last_attention"] = out.detach() if self.keep_attention else None
         return out
 
     def _keysets(self, qk32, kp, qkv, geom: Geometry, C: int):
