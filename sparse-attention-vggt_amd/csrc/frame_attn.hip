@@ -8,9 +8,8 @@
 //
 // Every pattern gives a query tile (or, in the backward pass over keys, a key tile) at most two ranges of
 // consecutive tokens on the other side: all, the first frame, the own frame. A work-group of four waves owns a
-// tile of rows and walks the other side in tiles of 64 tokens that all its waves read from LDS (two buffers; the
-// next tile waits in registers while the current one is used, so any row stride and any masked row is dealt
-// with at the write). Matrix products are v_mfma_f32_32x32x16_bf16 and none of their results crosses lanes: a
+// tile of rows and walks the other side in tiles of 64 tokens that all its waves read from LDS (two buffers, the
+// next tile copied by LDS-DMA while the current one is used). Matrix products are v_mfma_f32_32x32x16_bf16 and none of their results crosses lanes: a
 // product whose rows are summed over next (P, dS) leaves its 32x32 result with one column per lane and the rows
 // 8 (i / 4) + 4 (lane / 32) + i % 4, and the other operand of the next product is read from LDS with the
 // transposing read in that same row order (two groups of four rows per 16).
@@ -28,10 +27,14 @@
 // Tokens that the mask removes are no keys and their own rows come out as zeros (lse = -inf); their q, k, v and
 // dO rows are replaced by zeros where they enter a product, so that whatever they hold stays out.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
 namespace saf3r {
+
+template <int N>
+using Int = std::integral_constant<int, N>;
 
 constexpr int kTile = 64;          // tokens of a staged tile
 constexpr int kTileElems = kTile * kHeadDim;
@@ -188,36 +191,35 @@ __device__ __forceinline__ float pair_max(float x) {
   return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
 }
 
-// Two row tiles on their way to LDS: 32 lanes of eight 16-byte chunks each, rows r and r + 32 (r = thread / 8).
-struct Staged {
-  u32x4 x[2], y[2];
-};
-
-__device__ __forceinline__ void stage_load(Staged& s, const __bf16* x, int64_t xs, const __bf16* y, int64_t ys,
-                                           int start, int end) {
-  const int r = tid_x() >> 3, c = (tid_x() & 7) * 8;
+// Copies the rows of a walk tile of two tensors to LDS (LDS-DMA, no registers): a wave takes 16 rows of each, a lane
+// 16 bytes, swizzled by the choice of its source. Rows behind the range are copies of its last row: finite where the
+// range is, and given probability zero by the caller.
+__device__ __forceinline__ void stage(const __bf16* x, int64_t xs, const __bf16* y, int64_t ys, int start, int end,
+                                      const __bf16* xt, const __bf16* yt, int wave, int lane) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int tok = start + r + 32 * i;
-    s.x[i] = s.y[i] = u32x4{};
-    if (tok < end) {
-      s.x[i] = *reinterpret_cast<const u32x4*>(x + tok * xs + c);
-      s.y[i] = *reinterpret_cast<const u32x4*>(y + tok * ys + c);
-    }
+    const int row0 = wave * 16 + i * 8, row = row0 + (lane >> 3);
+    const int tok = min(start + row, end - 1);
+    const int c = ((lane & 7) ^ swz8(row)) << 3;
+    dma16(x + tok * xs + c, lds_addr(xt) + row0 * 128);
+    dma16(y + tok * ys + c, lds_addr(yt) + row0 * 128);
   }
 }
 
-// bits: rows of the tile that are there (a row that is not is written as zeros)
+// Waits for the wave's own copies; rows that are not there (bits) become zeros, so that what they hold stays out of
+// every product. The work-group's barrier follows.
 template <bool MASK>
-__device__ __forceinline__ void stage_write(const Staged& s, __bf16* xt, __bf16* yt, uint64_t bits) {
-  const int r = tid_x() >> 3, c = tid_x() & 7;
+__device__ __forceinline__ void staged(__bf16* xt, __bf16* yt, uint64_t bits, int wave, int lane) {
+  wait_vm<0>();
+  if (MASK && bits != ~0ull) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = r + 32 * i;
-    const bool keep = !MASK || ((bits >> row) & 1);
-    const int at = row * 64 + ((c ^ swz8(row)) << 3);
-    *reinterpret_cast<u32x4*>(xt + at) = keep ? s.x[i] : u32x4{};
-    *reinterpret_cast<u32x4*>(yt + at) = keep ? s.y[i] : u32x4{};
+    for (int i = 0; i < 2; ++i) {
+      const int row = wave * 16 + i * 8 + (lane >> 3);
+      if (!((bits >> row) & 1)) {
+        *reinterpret_cast<u32x4*>(xt + row * 64 + (lane & 7) * 8) = u32x4{};
+        *reinterpret_cast<u32x4*>(yt + row * 64 + (lane & 7) * 8) = u32x4{};
+      }
+    }
   }
 }
 
@@ -275,25 +277,21 @@ __global__ void __launch_bounds__(256, 2) frame_attn_fwd_kernel(const FaParams p
   }
 
   const int na = tiles_of(it.a1 - it.a0), nw = na + tiles_of(it.b1 - it.b0);
-  Staged st;
-  int start, end;
   uint8_t mb = 0;
-  if (nw > 0) {
-    walk_tile(it, na, 0, &start, &end);
-    stage_load(st, kb, p.k.token, vb, p.v.token, start, end);
+  auto load = [&](int i) {
+    int start, end;
+    walk_tile(it, na, i, &start, &end);
     mb = mask_byte<MASK>(mask, start, end);
-  }
+    stage(kb, p.k.token, vb, p.v.token, start, end, lds[i & 1][0], lds[i & 1][1], wave, lane);
+  };
+  if (nw > 0) load(0);
   for (int i = 0; i < nw; ++i) {
     const uint64_t bits = __ballot(mb != 0);
     __bf16* kt = lds[i & 1][0];
     __bf16* vt = lds[i & 1][1];
-    stage_write<MASK>(st, kt, vt, bits);
+    staged<MASK>(kt, vt, bits, wave, lane);
     __syncthreads();
-    if (i + 1 < nw) {
-      walk_tile(it, na, i + 1, &start, &end);
-      stage_load(st, kb, p.k.token, vb, p.v.token, start, end);
-      mb = mask_byte<MASK>(mask, start, end);
-    }
+    if (i + 1 < nw) load(i + 1);
     if (!active) continue;
     f32x16 s[QG][2];
 #pragma unroll
@@ -459,38 +457,32 @@ __global__ void __launch_bounds__(256, 2) frame_attn_dq_kernel(const FaParams p)
   }
 
   const int na = tiles_of(it.a1 - it.a0), nw = na + tiles_of(it.b1 - it.b0);
-  Staged st;
-  int start, end;
   uint8_t mb = 0;
-  if (nw > 0) {
-    walk_tile(it, na, 0, &start, &end);
-    stage_load(st, kb, p.k.token, vb, p.v.token, start, end);
+  auto load = [&](int i) {
+    int start, end;
+    walk_tile(it, na, i, &start, &end);
     mb = mask_byte<MASK>(mask, start, end);
-  }
+    stage(kb, p.k.token, vb, p.v.token, start, end, lds[i & 1][0], lds[i & 1][1], wave, lane);
+  };
+  if (nw > 0) load(0);
   for (int i = 0; i < nw; ++i) {
     const uint64_t bits = __ballot(mb != 0);
     __bf16* kt = lds[i & 1][0];
     __bf16* vt = lds[i & 1][1];
-    stage_write<MASK>(st, kt, vt, bits);
+    staged<MASK>(kt, vt, bits, wave, lane);
     __syncthreads();
-    if (i + 1 < nw) {
-      walk_tile(it, na, i + 1, &start, &end);
-      stage_load(st, kb, p.k.token, vb, p.v.token, start, end);
-      mb = mask_byte<MASK>(mask, start, end);
-    }
+    if (i + 1 < nw) load(i + 1);
     if (!active) continue;
 #pragma unroll
     for (int kh = 0; kh < 2; ++kh) {
       f32x16 s[QG], dp[QG];
 #pragma unroll
-      for (int g = 0; g < QG; ++g) s[g] = dp[g] = f32x16{};
-#pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         const bf16x8 a = row_frag(kt, fa, kh, ks), b = row_frag(vt, fa, kh, ks);
 #pragma unroll
         for (int g = 0; g < QG; ++g) {
-          s[g] = mma(a, qf[g][ks], s[g]);
-          dp[g] = mma(b, dof[g][ks], dp[g]);
+          s[g] = mma(a, qf[g][ks], ks ? s[g] : f32x16{});
+          dp[g] = mma(b, dof[g][ks], ks ? dp[g] : f32x16{});
         }
       }
       if (bits != ~0ull) {
@@ -536,121 +528,249 @@ __global__ void __launch_bounds__(256, 2) frame_attn_dq_kernel(const FaParams p)
 }
 
 // ---------------------------------------------------------------------------------------
-// Backward over keys: dK and dV. A wave owns 32 KG key rows as columns of S = Q K^T and dP = dO V^T;
-// dV^T += dO^T P, dK^T += Q^T dS. The rows' statistics come from LDS: a query that is not there has
-// lse = +inf and D = 0, so that its probabilities are zero.
+// Backward over keys: dK and dV. A wave owns 64 key rows (two groups of 32) as columns of S = Q K^T and dP = dO V^T;
+// dV^T += dO^T P, dK^T += Q^T dS. The rows' statistics come from LDS: a query that is not there has lse = +inf and
+// D = 0, so that its probabilities are zero; the sums of dP start at -D.
+//
+// Two groups share every operand read from LDS (16 KB a wave for 32 queries: with one group LDS would be as busy as
+// the matrix cores). Their sums, keys and values fill 192 registers, so one wave runs on a SIMD and has to overlap
+// its own matrix products and vector work: a half tile (32 queries) is 32 products in a fixed order, with the
+// exponentials and roundings of one group placed behind the products of the other (32 cycles each, room for seven
+// vector instructions) and the LDS reads a phase ahead. (Compiler's order, two-phase loop: 686 TFLOP/s over 12 frames
+// of 1374 tokens, 16 heads.)
 // ---------------------------------------------------------------------------------------
-template <int KG, bool MASK>
-__global__ void __launch_bounds__(256, KG == 2 ? 1 : 2) frame_attn_dkv_kernel(const FaParams p) {
+struct DkvRows {
+  bf16x8 q[4], d[4];  // row operands of Q and dO
+  f32x4 ls[4], dl[4]; // lse * log2(e) and -D of the lane's rows
+};
+
+// One of the 16 reads of a half tile's row operands and statistics.
+template <int I>
+__device__ __forceinline__ void dkv_read(DkvRows& r, const __bf16* qt, const __bf16* dt, const float* stats,
+                                         const FragAddr& fa, int qh, int h) {
+  if constexpr (I < 4) r.q[I] = row_frag(qt, fa, qh, I);
+  else if constexpr (I < 8) r.ls[I - 4] = *reinterpret_cast<const f32x4*>(stats + 32 * qh + 8 * (I - 4) + 4 * h);
+  else if constexpr (I < 12) r.d[I - 8] = row_frag(dt, fa, qh, I - 8);
+  else r.dl[I - 12] = *reinterpret_cast<const f32x4*>(stats + kTile + 32 * qh + 8 * (I - 12) + 4 * h);
+}
+
+struct DkvAcc {
+  bf16x8 k[2][4], v[2][4];
+  f32x16 dk[2][2], dv[2][2];
+};
+
+// Products with a fixed register class: results that vector instructions read stay in VGPRs, the running sums and the
+// stationary operands in AGPRs. (With the builtin and more than 256 registers the compiler takes every result in
+// AGPRs and copies: 728 copies beside 64 products in this kernel's loop.) The hazard rules are the caller's: a result is
+// read by vector instructions three products later at the earliest, an operand is written by them at least two
+// instructions ahead (kNop where the order alone does not give that), and a separate third operand stays live for
+// two more products.
+template <bool NOP = false>
+__device__ __forceinline__ void mma_sum(f32x16& d, const bf16x8& a, const bf16x8& b) {
+  if constexpr (NOP)
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(d) : "v"(a), "v"(b));
+  else
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(d) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mma_zero(f32x16& d, const bf16x8& a, const bf16x8& b) {
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "a"(b));
+}
+__device__ __forceinline__ void mma_from(f32x16& d, const bf16x8& a, const bf16x8& b, const f32x16& c) {
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %3" : "=&v"(d) : "v"(a), "a"(b), "v"(c));
+}
+__device__ __forceinline__ void mma_more(f32x16& d, const bf16x8& a, const bf16x8& b) {
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "a"(b));
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+}
+__device__ __forceinline__ bf16x8 frag4(const uint32_t (&w)[8], int st) {
+  return __builtin_bit_cast(bf16x8, u32x4{w[4 * st], w[4 * st + 1], w[4 * st + 2], w[4 * st + 3]});
+}
+
+__device__ __forceinline__ f32x16 join16(const f32x4 (&x)[4]) {
+  f32x16 r;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = x[i / 4][i % 4];
+  return r;
+}
+
+// Keeps values where they are computed: the compiler may not move their computation behind this point.
+__device__ __forceinline__ void pin(uint32_t (&w)[8]) {
+  asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]), "+v"(w[4]), "+v"(w[5]), "+v"(w[6]), "+v"(w[7]));
+}
+
+// One half tile. `mid` runs when every read of this half is done; `ahead(Int<i>)` issues read i of the next half's 16.
+template <typename Mid, typename Ahead>
+__device__ __forceinline__ void dkv_half(DkvAcc& A, DkvRows& r, const __bf16* qt, const __bf16* dt, const FragAddr& fa,
+                                         int qh, float c, Mid mid, Ahead ahead) {
+  f32x16 s[2], dp[2];
+  uint32_t pw[2][8], dw[2][8];
+  bf16x8 td[2][2], tq[2][2];  // transposed operands [step][dh]
+  f32x16 dl = join16(r.dl);
+  // vector work of one pair of elements
+  auto expo = [&](int g, int t) {
+    s[g][2 * t] = __builtin_amdgcn_exp2f(s[g][2 * t] * c - r.ls[t / 2][2 * (t % 2)]);
+    s[g][2 * t + 1] = __builtin_amdgcn_exp2f(s[g][2 * t + 1] * c - r.ls[t / 2][2 * (t % 2) + 1]);
+    pw[g][t] = pack2(s[g][2 * t], s[g][2 * t + 1]);
+  };
+  auto prod = [&](int g, int t) {
+    dw[g][t] = pack2(s[g][2 * t] * dp[g][2 * t], s[g][2 * t + 1] * dp[g][2 * t + 1]);
+  };
+#define FENCE __builtin_amdgcn_sched_barrier(0)
+#define S0(g) mma_zero(s[g], r.q[0], A.k[g][0])
+#define S_(g, ks) mma_more(s[g], r.q[ks], A.k[g][ks])
+#define P0(g) mma_from(dp[g], r.d[0], A.v[g][0], dl)
+#define P_(g, ks) mma_more(dp[g], r.d[ks], A.v[g][ks])
+#define V_(g, st, dh) mma_sum(A.dv[g][dh], td[st][dh], frag4(pw[g], st))
+#define VN(g, st, dh) mma_sum<true>(A.dv[g][dh], td[st][dh], frag4(pw[g], st))
+#define K_(g, st, dh) mma_sum(A.dk[g][dh], tq[st][dh], frag4(dw[g], st))
+#define KN(g, st, dh) mma_sum<true>(A.dk[g][dh], tq[st][dh], frag4(dw[g], st))
+#define TD(st, dh) td[st][dh] = tr_frag(dt, fa, 2 * qh + st, dh)
+#define TQ(st, dh) tq[st][dh] = tr_frag(qt, fa, 2 * qh + st, dh)
+#define NEXT(i) ahead(Int<i>())
+  FENCE;
+  S0(0); TD(0, 0); FENCE;
+  S_(0, 1); TD(0, 1); FENCE;
+  S_(0, 2); TD(1, 0); FENCE;
+  S_(0, 3); TD(1, 1); FENCE;
+  S0(1); TQ(0, 0); FENCE;
+  S_(1, 1); TQ(0, 1); FENCE;
+  S_(1, 2); TQ(1, 0); expo(0, 0); FENCE;
+  S_(1, 3); TQ(1, 1); expo(0, 1); FENCE;
+  P0(0); expo(0, 2); FENCE;
+  P_(0, 1); expo(0, 3); FENCE;
+  P_(0, 2); expo(0, 4); FENCE;
+  P_(0, 3); expo(0, 5); FENCE;
+  P0(1); expo(0, 6); FENCE;
+  P_(1, 1); expo(0, 7); FENCE;
+  P_(1, 2); prod(0, 0); prod(0, 1); FENCE;
+  asm volatile("" ::"v"(dl));  // (third operand of P0: live until here)
+  P_(1, 3); prod(0, 2); prod(0, 3); FENCE;
+  pin(pw[0]);
+  V_(0, 0, 0); prod(0, 4); prod(0, 5); FENCE;
+  V_(0, 0, 1); prod(0, 6); prod(0, 7); FENCE;
+  pin(dw[0]);
+  mid();
+  FENCE;
+  V_(0, 1, 0); NEXT(0); expo(1, 0); FENCE;
+  V_(0, 1, 1); NEXT(1); expo(1, 1); FENCE;
+  KN(0, 0, 0); NEXT(2); expo(1, 2); FENCE;
+  K_(0, 0, 1); NEXT(3); expo(1, 3); FENCE;
+  K_(0, 1, 0); NEXT(8); expo(1, 4); FENCE;
+  K_(0, 1, 1); NEXT(9); expo(1, 5); FENCE;
+  VN(1, 0, 0); NEXT(10); expo(1, 6); FENCE;
+  V_(1, 0, 1); NEXT(11); expo(1, 7); FENCE;
+  VN(1, 1, 0); NEXT(4); NEXT(5); prod(1, 0); prod(1, 1); FENCE;
+  V_(1, 1, 1); NEXT(6); NEXT(7); prod(1, 2); prod(1, 3); FENCE;
+  KN(1, 0, 0); NEXT(12); NEXT(13); prod(1, 4); prod(1, 5); FENCE;
+  K_(1, 0, 1); NEXT(14); NEXT(15); prod(1, 6); prod(1, 7); FENCE;
+  KN(1, 1, 0); FENCE;
+  K_(1, 1, 1); FENCE;
+#undef FENCE
+#undef S0
+#undef S_
+#undef P0
+#undef P_
+#undef V_
+#undef VN
+#undef K_
+#undef KN
+#undef TD
+#undef TQ
+#undef NEXT
+}
+
+template <bool MASK>
+__global__ void __launch_bounds__(256, 1) frame_attn_dkv_kernel(const FaParams p) {
   __shared__ __align__(16) __bf16 lds[2][2][kTileElems];
-  __shared__ __align__(16) float stats[2][2][kTile];
-  const FaItem it = fa_item(p, 128 * KG);
+  __shared__ __align__(16) float stats[2][2 * kTile];
+  const FaItem it = fa_item(p, 256);
   const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6), h = lane >> 5;
   const FragAddr fa = frag_addr(lane);
   const __bf16* qb = p.q.ptr + it.clip * p.q.clip + it.head * p.q.head;
   const __bf16* db = p.doo.ptr + it.clip * p.doo.clip + it.head * p.doo.head;
   const uint8_t* mask = MASK ? p.mask + (int64_t)it.clip * p.N : nullptr;
   const int64_t stat = ((int64_t)it.clip * p.H + it.head) * p.N;
-  const int first = it.row0 + wave * 32 * KG;
+  const int first = it.row0 + wave * 64;
   const bool active = first < it.row_end;
 
-  bf16x8 kf[KG][4], vf[KG][4];
-  f32x16 dk[KG][2], dv[KG][2];
-  bool valid[KG];
+  const int na = tiles_of(it.a1 - it.a0), nw = na + tiles_of(it.b1 - it.b0);
+  float ls = 0.f, dl = 0.f;
+  auto load = [&](int i) {
+    int start, end;
+    walk_tile(it, na, i, &start, &end);
+    const int tok = start + lane;
+    ls = tok < end ? p.lse[stat + tok] : -__builtin_inff();
+    dl = tok < end ? p.delta[stat + tok] : 0.f;
+    stage(qb, p.q.token, db, p.doo.token, start, end, lds[i & 1][0], lds[i & 1][1], wave, lane);
+  };
+  // tile i, loaded before, becomes readable; the other buffer is free from here on
+  auto ready = [&](int i) {
+    // rows without a key (masked ones among them) hold whatever their buffers held: they become zeros
+    const bool there = ls != -__builtin_inff();
+    staged<MASK>(lds[i & 1][0], lds[i & 1][1], __ballot(there), wave, lane);
+    if (wave == 0) {
+      stats[i & 1][lane] = there ? ls * kLog2e : __builtin_inff();
+      stats[i & 1][kTile + lane] = there ? -dl : 0.f;
+    }
+    __syncthreads();
+    if (i + 1 < nw) load(i + 1);
+  };
+
+  if (nw > 0) load(0);
+  DkvAcc A;
+  bool valid[2];
 #pragma unroll
-  for (int g = 0; g < KG; ++g) {
+  for (int g = 0; g < 2; ++g) {
     const int r = first + 32 * g + (lane & 31);
     valid[g] = r < it.row_end && (!MASK || mask[r]);
     const __bf16* kp = p.k.ptr + it.clip * p.k.clip + it.head * p.k.head + r * p.k.token + 8 * h;
     const __bf16* vp = p.v.ptr + it.clip * p.v.clip + it.head * p.v.head + r * p.v.token + 8 * h;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      kf[g][ks] = valid[g] ? *reinterpret_cast<const bf16x8*>(kp + 16 * ks) : bf16x8{};
-      vf[g][ks] = valid[g] ? *reinterpret_cast<const bf16x8*>(vp + 16 * ks) : bf16x8{};
+      A.k[g][ks] = valid[g] ? *reinterpret_cast<const bf16x8*>(kp + 16 * ks) : bf16x8{};
+      A.v[g][ks] = valid[g] ? *reinterpret_cast<const bf16x8*>(vp + 16 * ks) : bf16x8{};
     }
-    dk[g][0] = dk[g][1] = dv[g][0] = dv[g][1] = f32x16{};
+    A.dk[g][0] = A.dk[g][1] = A.dv[g][0] = A.dv[g][1] = f32x16{};
   }
 
-  const int na = tiles_of(it.a1 - it.a0), nw = na + tiles_of(it.b1 - it.b0);
-  Staged st;
-  int start, end;
-  float ls = 0.f, dl = 0.f;
-  auto load = [&](int i) {
-    walk_tile(it, na, i, &start, &end);
-    stage_load(st, qb, p.q.token, db, p.doo.token, start, end);
-    const int tok = start + lane;
-    ls = tok < end ? p.lse[stat + tok] : -__builtin_inff();
-    dl = tok < end ? p.delta[stat + tok] : 0.f;
-  };
-  if (nw > 0) load(0);
-  for (int i = 0; i < nw; ++i) {
-    // rows without a key (masked ones among them) hold whatever their buffers held: they are written as zeros
-    const bool there = ls != -__builtin_inff();
-    const uint64_t bits = __ballot(there);
-    __bf16* qt = lds[i & 1][0];
-    __bf16* dt = lds[i & 1][1];
-    stage_write<true>(st, qt, dt, bits);
-    if (wave == 0) {
-      stats[i & 1][0][lane] = there ? ls * kLog2e : __builtin_inff();
-      stats[i & 1][1][lane] = there ? dl : 0.f;
-    }
-    __syncthreads();
-    if (i + 1 < nw) load(i + 1);
-    if (!active) continue;
-#pragma unroll
-    for (int qh = 0; qh < 2; ++qh) {
-      f32x16 s[KG], dp[KG], ls2, dl2;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(&stats[i & 1][0][32 * qh + 8 * j + 4 * h]);
-        const f32x4 b = *reinterpret_cast<const f32x4*>(&stats[i & 1][1][32 * qh + 8 * j + 4 * h]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          ls2[4 * j + e] = a[e];
-          dl2[4 * j + e] = b[e];
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < KG; ++g) s[g] = dp[g] = f32x16{};
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const bf16x8 a = row_frag(qt, fa, qh, ks), b = row_frag(dt, fa, qh, ks);
-#pragma unroll
-        for (int g = 0; g < KG; ++g) {
-          s[g] = mma(a, kf[g][ks], s[g]);
-          dp[g] = mma(b, vf[g][ks], dp[g]);
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < KG; ++g)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          s[g][j] = __builtin_amdgcn_exp2f(s[g][j] * p.c - ls2[j]);
-          dp[g][j] = s[g][j] * (dp[g][j] - dl2[j]);
-        }
-#pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        bf16x8 pf[KG], ds[KG];
-#pragma unroll
-        for (int g = 0; g < KG; ++g) {
-          pf[g] = pack8(s[g], step);
-          ds[g] = pack8(dp[g], step);
-        }
-#pragma unroll
-        for (int dh = 0; dh < 2; ++dh) {
-          const bf16x8 a = tr_frag(dt, fa, 2 * qh + step, dh), b = tr_frag(qt, fa, 2 * qh + step, dh);
-#pragma unroll
-          for (int g = 0; g < KG; ++g) {
-            dv[g][dh] = mma(a, pf[g], dv[g][dh]);
-            dk[g][dh] = mma(b, ds[g], dk[g][dh]);
-          }
-        }
-      }
-    }
+  if (nw > 0) ready(0);
+  if (!active) {
+    for (int i = 1; i < nw; ++i) ready(i);
+    return;
   }
-  if (!active) return;
+  DkvRows r;
+  // the 16 reads of half tile qh of tile i
+  auto reader = [&](int i, int qh) {
+    return [&, i, qh](auto n) {
+      dkv_read<decltype(n)::value>(r, lds[i & 1][0], lds[i & 1][1], stats[i & 1], fa, qh, h);
+    };
+  };
+  if (nw > 0) {
+    const auto read = reader(0, 0);
+    read(Int<0>()), read(Int<1>()), read(Int<2>()), read(Int<3>()), read(Int<4>()), read(Int<5>()), read(Int<6>());
+    read(Int<7>()), read(Int<8>()), read(Int<9>()), read(Int<10>()), read(Int<11>()), read(Int<12>());
+    read(Int<13>()), read(Int<14>()), read(Int<15>());
+  }
+  for (int i = 0; i < nw; ++i) {
+    const __bf16* qt = lds[i & 1][0];
+    const __bf16* dt = lds[i & 1][1];
+    dkv_half(A, r, qt, dt, fa, 0, p.c, [] {}, reader(i, 1));
+    // every read of this tile is done at `mid` of its second half
+    dkv_half(A, r, qt, dt, fa, 1, p.c,
+             [&] {
+               if (i + 1 < nw) ready(i + 1);
+             },
+             reader(i + 1, 0));
+  }
+  // the last products are done before the sums are read
+  asm volatile("s_nop 15\n\ts_nop 15"
+               : "+a"(A.dk[0][0]), "+a"(A.dk[0][1]), "+a"(A.dk[1][0]), "+a"(A.dk[1][1]), "+a"(A.dv[0][0]),
+                 "+a"(A.dv[0][1]), "+a"(A.dv[1][0]), "+a"(A.dv[1][1]));
 #pragma unroll
-  for (int g = 0; g < KG; ++g) {
+  for (int g = 0; g < 2; ++g) {
     const int r = first + 32 * g + (lane & 31);
     if (r < it.row_end) {
       __bf16* kp = p.dk.ptr + it.clip * p.dk.clip + it.head * p.dk.head + r * p.dk.token + 4 * h;
@@ -662,8 +782,8 @@ __global__ void __launch_bounds__(256, KG == 2 ? 1 : 2) frame_attn_dkv_kernel(co
           __bf16 a[4], b[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            a[e] = (__bf16)(valid[g] ? dk[g][dh][4 * j + e] * p.scale : 0.f);
-            b[e] = (__bf16)(valid[g] ? dv[g][dh][4 * j + e] : 0.f);
+            a[e] = (__bf16)(valid[g] ? A.dk[g][dh][4 * j + e] * p.scale : 0.f);
+            b[e] = (__bf16)(valid[g] ? A.dv[g][dh][4 * j + e] : 0.f);
           }
           *reinterpret_cast<u32x2*>(kp + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(a);
           *reinterpret_cast<u32x2*>(vp + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(b);
@@ -863,10 +983,10 @@ extern "C" int saf3r_frame_attn_bwd(const saf3r_heads* dout, const saf3r_heads* 
   const hipStream_t s = (hipStream_t)stream;
   if (token_mask) {
     hipLaunchKernelGGL((frame_attn_dq_kernel<2, true>), dim3((uint32_t)nq), dim3(256), 0, s, p);
-    hipLaunchKernelGGL((frame_attn_dkv_kernel<2, true>), dim3((uint32_t)nk), dim3(256), 0, s, pk);
+    hipLaunchKernelGGL((frame_attn_dkv_kernel<true>), dim3((uint32_t)nk), dim3(256), 0, s, pk);
   } else {
     hipLaunchKernelGGL((frame_attn_dq_kernel<2, false>), dim3((uint32_t)nq), dim3(256), 0, s, p);
-    hipLaunchKernelGGL((frame_attn_dkv_kernel<2, false>), dim3((uint32_t)nk), dim3(256), 0, s, pk);
+    hipLaunchKernelGGL((frame_attn_dkv_kernel<false>), dim3((uint32_t)nk), dim3(256), 0, s, pk);
   }
   return check_launch(who);
 }

@@ -22,6 +22,7 @@ struct LnParams {
   float* part;  // backward: [work-groups][2][dim]
   int64_t x_stride, dy_stride, y_stride;
   int64_t rows;
+  int64_t step;  // backward: rows of all work-groups' steps (the grid's size comes from host memory in a kernel: slow)
   int dim;
   float eps;
 };
@@ -118,8 +119,7 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_kernel(const LnParams p) {
       for (int e = 0; e < VE; ++e) dw[j][e] = db[j][e] = 0.f;
   }
   const float inv_n = 1.f / (float)p.dim;
-  const int64_t step = (int64_t)grid_x() * kRows;
-  for (int64_t row0 = (int64_t)bid_x() * kRows; row0 < p.rows; row0 += step) {
+  for (int64_t row0 = (int64_t)bid_x() * kRows; row0 < p.rows; row0 += p.step) {
     const int64_t row = row0 + slot;
     const bool there = row < p.rows;  // (a wave's rows end together with the loop: sums cross its lanes)
     const TX* xp = (const TX*)p.x + (there ? row : 0) * p.x_stride;
@@ -327,6 +327,7 @@ extern "C" int saf3r_layer_norm_bwd(const void* dy, int64_t dy_stride, int y_typ
       return ln_types(x_type, y_type, param_type, [&](auto tx, auto ty, auto tp) {
         constexpr int kTpr = decltype(tpr)::value;
         parts = ln_parts(rows, 256 / kTpr);
+        p.step = parts * (256 / kTpr);
         if (params)
           hipLaunchKernelGGL((layer_norm_bwd_kernel<decltype(tx), decltype(ty), decltype(tp), decltype(ve)::value,
                                                     decltype(nv)::value, kTpr, true>),

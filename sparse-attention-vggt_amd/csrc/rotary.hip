@@ -30,6 +30,7 @@ struct RotParams {
   const void* b;
   float* part;       // [parts][2][groups * dim]
   int64_t rows;      // clips * tokens * heads: rows of a group
+  int parts;         // work-groups of a group (the grid's size comes from host memory in a kernel: slow)
   int tokens, heads, groups, dim;
   int rot, axes, positions, pos_step, interleaved, norm;
   float eps;
@@ -138,7 +139,7 @@ template <typename T, typename TP, int VE, int TPR, bool BWD>
 __global__ void __launch_bounds__(256) head_rotary_kernel(const RotParams p) {
   constexpr int kRows = 256 / TPR;
   __shared__ float sums[BWD ? 256 * VE : 1];
-  const int group = bid_x() % p.groups, part = bid_x() / p.groups, parts = grid_x() / p.groups;
+  const int group = bid_x() % p.groups, part = bid_x() / p.groups;
   const int lane = tid_x() % TPR, slot = tid_x() / TPR;
   const RotLane l = rot_lane<VE>(p, lane);
   float wa[VE], wb[VE], ba[VE], bb[VE];
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(256) head_rotary_kernel(const RotParams p) {
     }
   }
   const float inv_n = 1.f / (float)p.dim;
-  for (int64_t row0 = (int64_t)part * kRows; row0 < p.rows; row0 += (int64_t)parts * kRows) {
+  for (int64_t row0 = (int64_t)part * kRows; row0 < p.rows; row0 += (int64_t)p.parts * kRows) {
     const int64_t row = row0 + slot;
     const bool there = row < p.rows && l.on;
     const RotRow r = rot_row(p, there ? row : 0);
@@ -385,8 +386,8 @@ extern "C" int saf3r_head_rotary_fwd(const saf3r_heads* x, int type, int64_t cli
   }
   return rot_dispatch(type, param_type, rot_vec(p, type, {&p.x, &p.y}), dim, [&](auto t, auto tp, auto ve, auto tpr) {
     constexpr int kTpr = decltype(tpr)::value;
-    const int64_t grid = rot_parts(p.rows, 256 / kTpr, groups, false) * groups;
-    hipLaunchKernelGGL((head_rotary_kernel<decltype(t), decltype(tp), decltype(ve)::value, kTpr, false>), dim3((uint32_t)grid),
+    p.parts = (int)rot_parts(p.rows, 256 / kTpr, groups, false);
+    hipLaunchKernelGGL((head_rotary_kernel<decltype(t), decltype(tp), decltype(ve)::value, kTpr, false>), dim3((uint32_t)(p.parts * groups)),
                        dim3(256), 0, (hipStream_t)stream, p);
     return check_launch(who);
   });
@@ -434,6 +435,7 @@ extern "C" int saf3r_head_rotary_bwd(const saf3r_heads* dy, const saf3r_heads* x
                       [&](auto t, auto tp, auto ve, auto tpr) {
       constexpr int kTpr = decltype(tpr)::value;
       parts = rot_parts(p.rows, 256 / kTpr, groups, true);
+      p.parts = (int)parts;
       hipLaunchKernelGGL((head_rotary_kernel<decltype(t), decltype(tp), decltype(ve)::value, kTpr, true>),
                          dim3((uint32_t)(parts * groups)), dim3(256), 0, (hipStream_t)stream, p);
       return check_launch(who);

@@ -12,8 +12,6 @@ namespace saf3r {
 template <int N>
 using Int = std::integral_constant<int, N>;
 
-__device__ __forceinline__ int grid_x() { return (int)__builtin_amdgcn_grid_size_x() / (int)__builtin_amdgcn_workgroup_size_x(); }
-
 // VE elements of T at p (16-byte aligned for VE > 1) as floats.
 template <int VE, typename T>
 __device__ __forceinline__ void load_vec(const T* p, float (&x)[VE]) {
