@@ -65,6 +65,7 @@ struct FaParams {
   float* delta;          // [clip][head][token]
   const uint8_t* mask;   // [clip][token], 0: not there (may be null)
   int N, T, H, n_seg;
+  int wide;              // rows of a walk tile need 64-bit offsets
   float scale, c;        // softmax scale, scale * log2(e)
   FaSeg seg[kFaMaxSegs];
 };
@@ -129,6 +130,12 @@ __device__ inline void walk_tile(const FaItem& it, int na, int i, int* start, in
   }
 }
 
+// Chunk swizzle of the tiles (16-byte chunks of 128-byte rows, XOR with a function of the row). LDS serves 256 bytes a
+// cycle: 16 lanes of a rows operand (16 rows, one chunk) and 32 lanes of a transposed one (4 rows, 4 chunks) fall on
+// 64 different banks when the eight rows of one parity take eight values and rows two apart differ in bit 2. (With
+// swz8, whose rows two apart stay in one half row, the transposed reads took twice their cycles.)
+__device__ inline int swz_tile(int r) { return ((r & 2) << 1) | ((r >> 2) & 3); }
+
 // LDS addresses of a lane's operand fragments in a [64][64] tile whose 16-byte chunks are swizzled by row.
 struct FragAddr {
   int row[4];     // rows operand: row lane % 32, elements 16 ks + 8 (lane / 32) .. + 7
@@ -139,7 +146,7 @@ __device__ inline FragAddr frag_addr(int lane) {
   FragAddr f;
   const int r = lane & 31, h = lane >> 5;
 #pragma unroll
-  for (int ks = 0; ks < 4; ++ks) f.row[ks] = r * 64 + (((2 * ks + h) ^ swz8(r)) << 3);
+  for (int ks = 0; ks < 4; ++ks) f.row[ks] = r * 64 + (((2 * ks + h) ^ swz_tile(r)) << 3);
   // lane i of 16 addresses row i / 4, columns 4 (i % 4) .. + 3, and receives column i of those 4 x 16 elements
   const int tr = 4 * h + ((lane & 15) >> 2), cc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
 #pragma unroll
@@ -147,7 +154,7 @@ __device__ inline FragAddr frag_addr(int lane) {
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const int row = tr + 8 * g;
-      f.tr[dh][g] = row * 64 + (((4 * dh + cc) ^ swz8(row)) << 3) + 4 * (lane & 1);
+      f.tr[dh][g] = row * 64 + (((4 * dh + cc) ^ swz_tile(row)) << 3) + 4 * (lane & 1);
     }
   return f;
 }
@@ -193,16 +200,51 @@ __device__ __forceinline__ float pair_max(float x) {
 
 // Copies the rows of a walk tile of two tensors to LDS (LDS-DMA, no registers): a wave takes 16 rows of each, a lane
 // 16 bytes, swizzled by the choice of its source. Rows behind the range are copies of its last row: finite where the
-// range is, and given probability zero by the caller.
-__device__ __forceinline__ void stage(const __bf16* x, int64_t xs, const __bf16* y, int64_t ys, int start, int end,
-                                      const __bf16* xt, const __bf16* yt, int wave, int lane) {
+// range is, and given probability zero by the caller. Whole tiles take a scalar base and the lane's own offsets, which
+// fit 32 bits (`wide` where they do not); the last tile of a range takes an address a lane.
+struct Stager {
+  const __bf16 *x, *y;
+  int64_t xs, ys;
+  uint32_t xo[2], yo[2];  // byte offsets of the lane's two rows in a tile
+  int row[2], c[2], wave;
+  bool wide;
+};
+
+__device__ __forceinline__ Stager stager(const __bf16* x, int64_t xs, const __bf16* y, int64_t ys, bool wide, int wave,
+                                         int lane) {
+  Stager s;
+  s.wide = wide;
+  s.x = x;
+  s.y = y;
+  s.xs = xs;
+  s.ys = ys;
+  s.wave = wave;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int row0 = wave * 16 + i * 8, row = row0 + (lane >> 3);
-    const int tok = min(start + row, end - 1);
-    const int c = ((lane & 7) ^ swz8(row)) << 3;
-    dma16(x + tok * xs + c, lds_addr(xt) + row0 * 128);
-    dma16(y + tok * ys + c, lds_addr(yt) + row0 * 128);
+    s.row[i] = wave * 16 + i * 8 + (lane >> 3);
+    s.c[i] = ((lane & 7) ^ swz_tile(s.row[i])) << 3;
+    s.xo[i] = (uint32_t)((s.row[i] * xs + s.c[i]) * 2);
+    s.yo[i] = (uint32_t)((s.row[i] * ys + s.c[i]) * 2);
+  }
+  return s;
+}
+
+__device__ __forceinline__ void stage(const Stager& s, int start, int end, const __bf16* xt, const __bf16* yt) {
+  const uint32_t xl = lds_addr(xt) + s.wave * 2048, yl = lds_addr(yt) + s.wave * 2048;
+  if (start + kTile <= end && !s.wide) {
+    const __bf16 *xb = s.x + start * s.xs, *yb = s.y + start * s.ys;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      dma16s(xb, s.xo[i], xl + i * 1024);
+      dma16s(yb, s.yo[i], yl + i * 1024);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int tok = min(start + s.row[i], end - 1);
+      dma16(s.x + tok * s.xs + s.c[i], xl + i * 1024);
+      dma16(s.y + tok * s.ys + s.c[i], yl + i * 1024);
+    }
   }
 }
 
@@ -277,12 +319,13 @@ __global__ void __launch_bounds__(256, 2) frame_attn_fwd_kernel(const FaParams p
   }
 
   const int na = tiles_of(it.a1 - it.a0), nw = na + tiles_of(it.b1 - it.b0);
+  const Stager st = stager(kb, p.k.token, vb, p.v.token, p.wide, wave, lane);
   uint8_t mb = 0;
   auto load = [&](int i) {
     int start, end;
     walk_tile(it, na, i, &start, &end);
     mb = mask_byte<MASK>(mask, start, end);
-    stage(kb, p.k.token, vb, p.v.token, start, end, lds[i & 1][0], lds[i & 1][1], wave, lane);
+    stage(st, start, end, lds[i & 1][0], lds[i & 1][1]);
   };
   if (nw > 0) load(0);
   for (int i = 0; i < nw; ++i) {
@@ -457,12 +500,13 @@ __global__ void __launch_bounds__(256, 2) frame_attn_dq_kernel(const FaParams p)
   }
 
   const int na = tiles_of(it.a1 - it.a0), nw = na + tiles_of(it.b1 - it.b0);
+  const Stager st = stager(kb, p.k.token, vb, p.v.token, p.wide, wave, lane);
   uint8_t mb = 0;
   auto load = [&](int i) {
     int start, end;
     walk_tile(it, na, i, &start, &end);
     mb = mask_byte<MASK>(mask, start, end);
-    stage(kb, p.k.token, vb, p.v.token, start, end, lds[i & 1][0], lds[i & 1][1], wave, lane);
+    stage(st, start, end, lds[i & 1][0], lds[i & 1][1]);
   };
   if (nw > 0) load(0);
   for (int i = 0; i < nw; ++i) {
@@ -529,8 +573,8 @@ __global__ void __launch_bounds__(256, 2) frame_attn_dq_kernel(const FaParams p)
 
 // ---------------------------------------------------------------------------------------
 // Backward over keys: dK and dV. A wave owns 64 key rows (two groups of 32) as columns of S = Q K^T and dP = dO V^T;
-// dV^T += dO^T P, dK^T += Q^T dS. The rows' statistics come from LDS: a query that is not there has lse = +inf and
-// D = 0, so that its probabilities are zero; the sums of dP start at -D.
+// dV^T += dO^T P, dK^T += Q^T dS. The sums of S start at -lse / scale and those of dP at -D of their rows; a query that
+// is not there starts at -inf, so that its probabilities are zero.
 //
 // Two groups share every operand read from LDS (16 KB a wave for 32 queries: with one group LDS would be as busy as
 // the matrix cores). Their sums, keys and values fill 192 registers, so one wave runs on a SIMD and has to overlap
@@ -541,17 +585,23 @@ __global__ void __launch_bounds__(256, 2) frame_attn_dq_kernel(const FaParams p)
 // ---------------------------------------------------------------------------------------
 struct DkvRows {
   bf16x8 q[4], d[4];  // row operands of Q and dO
-  f32x4 ls[4], dl[4]; // lse * log2(e) and -D of the lane's rows
+  f32x16 ls, dl;      // where the sums of S and dP start: -lse / scale and -D of the rows
 };
 
 // One of the 16 reads of a half tile's row operands and statistics.
 template <int I>
 __device__ __forceinline__ void dkv_read(DkvRows& r, const __bf16* qt, const __bf16* dt, const float* stats,
                                          const FragAddr& fa, int qh, int h) {
-  if constexpr (I < 4) r.q[I] = row_frag(qt, fa, qh, I);
-  else if constexpr (I < 8) r.ls[I - 4] = *reinterpret_cast<const f32x4*>(stats + 32 * qh + 8 * (I - 4) + 4 * h);
-  else if constexpr (I < 12) r.d[I - 8] = row_frag(dt, fa, qh, I - 8);
-  else r.dl[I - 12] = *reinterpret_cast<const f32x4*>(stats + kTile + 32 * qh + 8 * (I - 12) + 4 * h);
+  if constexpr (I < 4) {
+    r.q[I] = row_frag(qt, fa, qh, I);
+  } else if constexpr (I < 8) {
+    r.d[I - 4] = row_frag(dt, fa, qh, I - 4);
+  } else {
+    constexpr int j = I % 4;
+    const f32x4 x = *reinterpret_cast<const f32x4*>(stats + (I < 12 ? 0 : kTile) + 32 * qh + 8 * j + 4 * h);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) (I < 12 ? r.ls : r.dl)[4 * j + e] = x[e];
+  }
 }
 
 struct DkvAcc {
@@ -562,18 +612,10 @@ struct DkvAcc {
 // Products with a fixed register class: results that vector instructions read stay in VGPRs, the running sums and the
 // stationary operands in AGPRs. (With the builtin and more than 256 registers the compiler takes every result in
 // AGPRs and copies: 728 copies beside 64 products in this kernel's loop.) The hazard rules are the caller's: a result is
-// read by vector instructions three products later at the earliest, an operand is written by them at least two
-// instructions ahead (kNop where the order alone does not give that), and a separate third operand stays live for
-// two more products.
-template <bool NOP = false>
+// read by vector instructions three products later at the earliest, an operand is written by them a product ahead, and
+// a separate third operand stays live for two more products.
 __device__ __forceinline__ void mma_sum(f32x16& d, const bf16x8& a, const bf16x8& b) {
-  if constexpr (NOP)
-    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(d) : "v"(a), "v"(b));
-  else
-    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(d) : "v"(a), "v"(b));
-}
-__device__ __forceinline__ void mma_zero(f32x16& d, const bf16x8& a, const bf16x8& b) {
-  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "a"(b));
+  asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(d) : "v"(a), "v"(b));
 }
 __device__ __forceinline__ void mma_from(f32x16& d, const bf16x8& a, const bf16x8& b, const f32x16& c) {
   asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %3" : "=&v"(d) : "v"(a), "a"(b), "v"(c));
@@ -589,44 +631,50 @@ __device__ __forceinline__ bf16x8 frag4(const uint32_t (&w)[8], int st) {
   return __builtin_bit_cast(bf16x8, u32x4{w[4 * st], w[4 * st + 1], w[4 * st + 2], w[4 * st + 3]});
 }
 
-__device__ __forceinline__ f32x16 join16(const f32x4 (&x)[4]) {
-  f32x16 r;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) r[i] = x[i / 4][i % 4];
-  return r;
-}
-
 // Keeps values where they are computed: the compiler may not move their computation behind this point.
-__device__ __forceinline__ void pin(uint32_t (&w)[8]) {
-  asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]), "+v"(w[4]), "+v"(w[5]), "+v"(w[6]), "+v"(w[7]));
+__device__ __forceinline__ void pin(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+}
+template <int FIRST, int N>
+__device__ __forceinline__ void pin_elems(f32x16& x) {
+#pragma unroll
+  for (int i = FIRST; i < FIRST + N; ++i) {
+    float e = x[i];
+    asm volatile("" : "+v"(e));
+    x[i] = e;
+  }
 }
 
-// One half tile. `mid` runs when every read of this half is done; `ahead(Int<i>)` issues read i of the next half's 16.
+// One half tile. `mid` runs when every read of this half is issued (its barrier waits for them); `ahead(Int<i>)` issues
+// read i of the next half's 16.
 template <typename Mid, typename Ahead>
-__device__ __forceinline__ void dkv_half(DkvAcc& A, DkvRows& r, const __bf16* qt, const __bf16* dt, const FragAddr& fa,
-                                         int qh, float c, Mid mid, Ahead ahead) {
+__device__ __forceinline__ void dkv_half(DkvAcc& A, const DkvRows& r, const __bf16* qt, const __bf16* dt,
+                                         const FragAddr& fa, int qh, float c, Mid mid, Ahead ahead) {
   f32x16 s[2], dp[2];
   uint32_t pw[2][8], dw[2][8];
   bf16x8 td[2][2], tq[2][2];  // transposed operands [step][dh]
-  f32x16 dl = join16(r.dl);
-  // vector work of one pair of elements
-  auto expo = [&](int g, int t) {
-    s[g][2 * t] = __builtin_amdgcn_exp2f(s[g][2 * t] * c - r.ls[t / 2][2 * (t % 2)]);
-    s[g][2 * t + 1] = __builtin_amdgcn_exp2f(s[g][2 * t + 1] * c - r.ls[t / 2][2 * (t % 2) + 1]);
-    pw[g][t] = pack2(s[g][2 * t], s[g][2 * t + 1]);
+  // vector work of one pair of elements, in steps that are a product apart (a lone wave waits for each result)
+  auto fm = [&](int g, int t) {
+    s[g][2 * t] *= c;
+    s[g][2 * t + 1] *= c;
   };
-  auto prod = [&](int g, int t) {
-    dw[g][t] = pack2(s[g][2 * t] * dp[g][2 * t], s[g][2 * t + 1] * dp[g][2 * t + 1]);
+  auto ex = [&](int g, int t) {
+    s[g][2 * t] = __builtin_amdgcn_exp2f(s[g][2 * t]);
+    s[g][2 * t + 1] = __builtin_amdgcn_exp2f(s[g][2 * t + 1]);
   };
+  auto cv = [&](int g, int t) { pw[g][t] = pack2(s[g][2 * t], s[g][2 * t + 1]); };
+  auto ml = [&](int g, int t) {
+    dp[g][2 * t] *= s[g][2 * t];
+    dp[g][2 * t + 1] *= s[g][2 * t + 1];
+  };
+  auto cw = [&](int g, int t) { dw[g][t] = pack2(dp[g][2 * t], dp[g][2 * t + 1]); };
 #define FENCE __builtin_amdgcn_sched_barrier(0)
-#define S0(g) mma_zero(s[g], r.q[0], A.k[g][0])
+#define S0(g) mma_from(s[g], r.q[0], A.k[g][0], r.ls)
 #define S_(g, ks) mma_more(s[g], r.q[ks], A.k[g][ks])
-#define P0(g) mma_from(dp[g], r.d[0], A.v[g][0], dl)
+#define P0(g) mma_from(dp[g], r.d[0], A.v[g][0], r.dl)
 #define P_(g, ks) mma_more(dp[g], r.d[ks], A.v[g][ks])
 #define V_(g, st, dh) mma_sum(A.dv[g][dh], td[st][dh], frag4(pw[g], st))
-#define VN(g, st, dh) mma_sum<true>(A.dv[g][dh], td[st][dh], frag4(pw[g], st))
 #define K_(g, st, dh) mma_sum(A.dk[g][dh], tq[st][dh], frag4(dw[g], st))
-#define KN(g, st, dh) mma_sum<true>(A.dk[g][dh], tq[st][dh], frag4(dw[g], st))
 #define TD(st, dh) td[st][dh] = tr_frag(dt, fa, 2 * qh + st, dh)
 #define TQ(st, dh) tq[st][dh] = tr_frag(qt, fa, 2 * qh + st, dh)
 #define NEXT(i) ahead(Int<i>())
@@ -637,36 +685,37 @@ __device__ __forceinline__ void dkv_half(DkvAcc& A, DkvRows& r, const __bf16* qt
   S_(0, 3); TD(1, 1); FENCE;
   S0(1); TQ(0, 0); FENCE;
   S_(1, 1); TQ(0, 1); FENCE;
-  S_(1, 2); TQ(1, 0); expo(0, 0); FENCE;
-  S_(1, 3); TQ(1, 1); expo(0, 1); FENCE;
-  P0(0); expo(0, 2); FENCE;
-  P_(0, 1); expo(0, 3); FENCE;
-  P_(0, 2); expo(0, 4); FENCE;
-  P_(0, 3); expo(0, 5); FENCE;
-  P0(1); expo(0, 6); FENCE;
-  P_(1, 1); expo(0, 7); FENCE;
-  P_(1, 2); prod(0, 0); prod(0, 1); FENCE;
-  asm volatile("" ::"v"(dl));  // (third operand of P0: live until here)
-  P_(1, 3); prod(0, 2); prod(0, 3); FENCE;
-  pin(pw[0]);
-  V_(0, 0, 0); prod(0, 4); prod(0, 5); FENCE;
-  V_(0, 0, 1); prod(0, 6); prod(0, 7); FENCE;
-  pin(dw[0]);
+  S_(1, 2); TQ(1, 0); fm(0, 0); FENCE;
+  asm volatile("" ::"v"(r.ls));  // (third operand of S0: live until here)
+  S_(1, 3); TQ(1, 1); fm(0, 1); ex(0, 0); FENCE;
+  P0(0); fm(0, 2); ex(0, 1); cv(0, 0); FENCE;
+  P_(0, 1); fm(0, 3); ex(0, 2); cv(0, 1); FENCE;
+  pin_elems<0, 8>(s[0]);
+  pin(pw[0][0], pw[0][1], pw[0][0], pw[0][1]);
   mid();
   FENCE;
-  V_(0, 1, 0); NEXT(0); expo(1, 0); FENCE;
-  V_(0, 1, 1); NEXT(1); expo(1, 1); FENCE;
-  KN(0, 0, 0); NEXT(2); expo(1, 2); FENCE;
-  K_(0, 0, 1); NEXT(3); expo(1, 3); FENCE;
-  K_(0, 1, 0); NEXT(8); expo(1, 4); FENCE;
-  K_(0, 1, 1); NEXT(9); expo(1, 5); FENCE;
-  VN(1, 0, 0); NEXT(10); expo(1, 6); FENCE;
-  V_(1, 0, 1); NEXT(11); expo(1, 7); FENCE;
-  VN(1, 1, 0); NEXT(4); NEXT(5); prod(1, 0); prod(1, 1); FENCE;
-  V_(1, 1, 1); NEXT(6); NEXT(7); prod(1, 2); prod(1, 3); FENCE;
-  KN(1, 0, 0); NEXT(12); NEXT(13); prod(1, 4); prod(1, 5); FENCE;
-  K_(1, 0, 1); NEXT(14); NEXT(15); prod(1, 6); prod(1, 7); FENCE;
-  KN(1, 1, 0); FENCE;
+  P_(0, 2); NEXT(0); fm(0, 4); ex(0, 3); cv(0, 2); FENCE;
+  P_(0, 3); NEXT(1); fm(0, 5); ex(0, 4); cv(0, 3); fm(1, 0); FENCE;
+  P0(1); NEXT(2); fm(0, 6); ex(0, 5); cv(0, 4); ex(1, 0); FENCE;
+  P_(1, 1); NEXT(3); fm(0, 7); ex(0, 6); cv(0, 5); fm(1, 1); FENCE;
+  P_(1, 2); NEXT(8); ex(0, 7); cv(0, 6); ml(0, 0); ex(1, 1); FENCE;
+  asm volatile("" ::"v"(r.dl));  // (third operand of P0: live until here)
+  P_(1, 3); NEXT(9); cv(0, 7); ml(0, 1); ml(0, 2); cv(1, 0); cw(0, 0); FENCE;
+  V_(0, 0, 0); NEXT(10); ml(0, 3); cw(0, 1); cw(0, 2); fm(1, 2); cv(1, 1); FENCE;
+  V_(0, 0, 1); NEXT(11); ml(0, 4); cw(0, 3); fm(1, 3); ex(1, 2); FENCE;
+  V_(0, 1, 0); NEXT(4); ml(0, 5); cw(0, 4); ex(1, 3); cv(1, 2); FENCE;
+  V_(0, 1, 1); NEXT(5); ml(0, 6); cw(0, 5); fm(1, 4); cv(1, 3); FENCE;
+  K_(0, 0, 0); NEXT(6); ml(0, 7); cw(0, 6); fm(1, 5); ex(1, 4); FENCE;
+  K_(0, 0, 1); NEXT(7); cw(0, 7); fm(1, 6); ex(1, 5); cv(1, 4); FENCE;
+  V_(1, 0, 0); NEXT(12); fm(1, 7); ex(1, 6); cv(1, 5); FENCE;
+  V_(1, 0, 1); NEXT(13); ex(1, 7); cv(1, 6); ml(1, 0); FENCE;
+  K_(0, 1, 0); NEXT(14); cv(1, 7); ml(1, 1); ml(1, 2); cw(1, 0); FENCE;
+  K_(0, 1, 1); NEXT(15); ml(1, 3); ml(1, 4); cw(1, 1); cw(1, 2); FENCE;
+  V_(1, 1, 0); ml(1, 5); cw(1, 3); cw(1, 4); FENCE;
+  V_(1, 1, 1); ml(1, 6); ml(1, 7); cw(1, 5); FENCE;
+  K_(1, 0, 0); cw(1, 6); cw(1, 7); FENCE;
+  K_(1, 0, 1); FENCE;
+  K_(1, 1, 0); FENCE;
   K_(1, 1, 1); FENCE;
 #undef FENCE
 #undef S0
@@ -674,9 +723,7 @@ __device__ __forceinline__ void dkv_half(DkvAcc& A, DkvRows& r, const __bf16* qt
 #undef P0
 #undef P_
 #undef V_
-#undef VN
 #undef K_
-#undef KN
 #undef TD
 #undef TQ
 #undef NEXT
@@ -697,6 +744,8 @@ __global__ void __launch_bounds__(256, 1) frame_attn_dkv_kernel(const FaParams p
   const bool active = first < it.row_end;
 
   const int na = tiles_of(it.a1 - it.a0), nw = na + tiles_of(it.b1 - it.b0);
+  const float inv_scale = 1.f / p.scale;
+  const Stager st = stager(qb, p.q.token, db, p.doo.token, p.wide, wave, lane);
   float ls = 0.f, dl = 0.f;
   auto load = [&](int i) {
     int start, end;
@@ -704,7 +753,7 @@ __global__ void __launch_bounds__(256, 1) frame_attn_dkv_kernel(const FaParams p
     const int tok = start + lane;
     ls = tok < end ? p.lse[stat + tok] : -__builtin_inff();
     dl = tok < end ? p.delta[stat + tok] : 0.f;
-    stage(qb, p.q.token, db, p.doo.token, start, end, lds[i & 1][0], lds[i & 1][1], wave, lane);
+    stage(st, start, end, lds[i & 1][0], lds[i & 1][1]);
   };
   // tile i, loaded before, becomes readable; the other buffer is free from here on
   auto ready = [&](int i) {
@@ -712,7 +761,7 @@ __global__ void __launch_bounds__(256, 1) frame_attn_dkv_kernel(const FaParams p
     const bool there = ls != -__builtin_inff();
     staged<MASK>(lds[i & 1][0], lds[i & 1][1], __ballot(there), wave, lane);
     if (wave == 0) {
-      stats[i & 1][lane] = there ? ls * kLog2e : __builtin_inff();
+      stats[i & 1][lane] = there ? -ls * inv_scale : -__builtin_inff();
       stats[i & 1][kTile + lane] = there ? -dl : 0.f;
     }
     __syncthreads();
@@ -741,15 +790,20 @@ __global__ void __launch_bounds__(256, 1) frame_attn_dkv_kernel(const FaParams p
     for (int i = 1; i < nw; ++i) ready(i);
     return;
   }
-  DkvRows r;
-  // the 16 reads of half tile qh of tile i
-  auto reader = [&](int i, int qh) {
-    return [&, i, qh](auto n) {
-      dkv_read<decltype(n)::value>(r, lds[i & 1][0], lds[i & 1][1], stats[i & 1], fa, qh, h);
+  DkvRows r0, r1;  // first and second half tiles
+  // the reads of a half tile of tile i
+  auto first_half = [&](int i) {
+    return [&, i](auto n) {
+      dkv_read<decltype(n)::value>(r0, lds[i & 1][0], lds[i & 1][1], stats[i & 1], fa, 0, h);
+    };
+  };
+  auto second_half = [&](int i) {
+    return [&, i](auto n) {
+      dkv_read<decltype(n)::value>(r1, lds[i & 1][0], lds[i & 1][1], stats[i & 1], fa, 1, h);
     };
   };
   if (nw > 0) {
-    const auto read = reader(0, 0);
+    const auto read = first_half(0);
     read(Int<0>()), read(Int<1>()), read(Int<2>()), read(Int<3>()), read(Int<4>()), read(Int<5>()), read(Int<6>());
     read(Int<7>()), read(Int<8>()), read(Int<9>()), read(Int<10>()), read(Int<11>()), read(Int<12>());
     read(Int<13>()), read(Int<14>()), read(Int<15>());
@@ -757,13 +811,13 @@ __global__ void __launch_bounds__(256, 1) frame_attn_dkv_kernel(const FaParams p
   for (int i = 0; i < nw; ++i) {
     const __bf16* qt = lds[i & 1][0];
     const __bf16* dt = lds[i & 1][1];
-    dkv_half(A, r, qt, dt, fa, 0, p.c, [] {}, reader(i, 1));
+    dkv_half(A, r0, qt, dt, fa, 0, p.c, [] {}, second_half(i));
     // every read of this tile is done at `mid` of its second half
-    dkv_half(A, r, qt, dt, fa, 1, p.c,
+    dkv_half(A, r1, qt, dt, fa, 1, p.c,
              [&] {
                if (i + 1 < nw) ready(i + 1);
              },
-             reader(i + 1, 0));
+             first_half(i + 1));
   }
   // the last products are done before the sums are read
   asm volatile("s_nop 15\n\ts_nop 15"
@@ -881,6 +935,9 @@ static bool fa_aligned(const FaTensor& t) {
   return (uintptr_t)t.ptr % 16 == 0 && t.clip % 8 == 0 && t.token % 8 == 0 && t.head % 8 == 0;
 }
 
+// Whether the rows of a walk tile are so far apart (or in descending order) that their byte offsets need 64 bits.
+static bool fa_wide(const FaTensor& t) { return t.token < 0 || t.token >= ((int64_t)1 << 31) / 2 / kTile; }
+
 static int fa_check(const char* who, FaParams* p, int clips, int frames, int tokens_per_frame, int num_heads,
                     const int32_t* patterns, const uint8_t* mask, float scale) {
   if (clips < 0 || frames <= 0 || tokens_per_frame <= 0)
@@ -933,6 +990,7 @@ extern "C" int saf3r_frame_attn_fwd(const saf3r_heads* q, const saf3r_heads* k, 
       (uintptr_t)lse % 4)
     return fail(SAF3R_ERR_INVALID, "%s: rows must be 16-byte aligned with strides a multiple of 8", who);
   p.lse = lse;
+  p.wide = fa_wide(p.k) || fa_wide(p.v);
   const int64_t n = make_segs(&p, patterns, clips, frames, 256, false);
   if (int e = fa_grid(who, n)) return e;
   if (token_mask)
@@ -976,6 +1034,7 @@ extern "C" int saf3r_frame_attn_bwd(const saf3r_heads* dout, const saf3r_heads* 
                 (long long)workspace_bytes, (long long)need);
   p.lse = const_cast<float*>(lse);
   p.delta = (float*)workspace;
+  p.wide = fa_wide(p.q) || fa_wide(p.k) || fa_wide(p.v) || fa_wide(p.doo);
   FaParams pk = p;
   const int64_t nq = make_segs(&p, patterns, clips, frames, 256, false);
   const int64_t nk = make_segs(&pk, patterns, clips, frames, 256, true);
