@@ -36,22 +36,27 @@ namespace saf3r {
 template <int N>
 using Int = std::integral_constant<int, N>;
 
-constexpr int kTile = 64;          // tokens of a staged tile
+// Tokens of a staged tile: 64, or 32 for waves that walk alone (two buffers each: 64 KB a work-group, two of them on a
+// compute unit).
+constexpr int kTile = 64;
 constexpr int kTileElems = kTile * kHeadDim;
-constexpr int kFaMaxSegs = 2 * kMaxHeads;
+template <bool ALONE>
+constexpr int kTokens = ALONE ? 32 : kTile;
+constexpr int kFaClasses = 7;      // kinds of row tiles of a launch, see make_classes
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 enum Walk { kNone = 0, kAll = 1, kFirst = 2, kOwn = 3, kFirstOwn = 4 };
 
-// A run of row tiles of one head, clip-major: per frame (frames f0 ..) or over the tokens tok0 .. tok1.
-struct FaSeg {
+// Row tiles that walk alike: of the heads of a mask, head by head and clip by clip; per frame (from token tok0 on) or
+// over the tokens tok0 .. tok1.
+struct FaClass {
   int start;     // first work-group
-  int per_clip;  // tiles of a clip
+  int per_clip;  // tiles of a clip of a head
   int nt;        // tiles of a frame (per-frame runs; 0: over tokens)
   int tok0, tok1;
-  int16_t head;
-  int16_t walk;
+  int walk;
+  uint64_t heads;
 };
 
 struct FaTensor {
@@ -64,10 +69,10 @@ struct FaParams {
   float* lse;            // [clip][head][token]
   float* delta;          // [clip][head][token]
   const uint8_t* mask;   // [clip][token], 0: not there (may be null)
-  int N, T, H, n_seg;
+  int N, T, H, clips;
   int wide;              // rows of a walk tile need 64-bit offsets
   float scale, c;        // softmax scale, scale * log2(e)
-  FaSeg seg[kFaMaxSegs];
+  FaClass cls[kFaClasses];
 };
 
 // What a work-group owns and walks.
@@ -77,22 +82,30 @@ struct FaItem {
   int a0, a1, b0, b1;   // walked ranges
 };
 
+// (The kernel's arguments lie in host memory, where a load that depends on another costs microseconds: all classes are
+// read at once and chosen from in registers.)
 __device__ inline FaItem fa_item(const FaParams& p, int rows) {
   const int bid = bid_x();
-  int lo = 0, hi = p.n_seg - 1;
-  while (lo < hi) {  // last segment that starts at or before bid
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.seg[mid].start <= bid)
-      lo = mid;
-    else
-      hi = mid - 1;
+  FaClass s = p.cls[0];
+#pragma unroll
+  for (int i = 1; i < kFaClasses; ++i) {
+    const FaClass x = p.cls[i];
+    const bool in = x.start <= bid;  // (classes without tiles start behind every work-group)
+    s.start = in ? x.start : s.start;
+    s.per_clip = in ? x.per_clip : s.per_clip;
+    s.nt = in ? x.nt : s.nt;
+    s.tok0 = in ? x.tok0 : s.tok0;
+    s.tok1 = in ? x.tok1 : s.tok1;
+    s.walk = in ? x.walk : s.walk;
+    s.heads = in ? x.heads : s.heads;
   }
-  const FaSeg s = p.seg[lo];
-  const int j = bid - s.start;
+  const int j = bid - s.start, run = j / s.per_clip, t = j - run * s.per_clip;
   FaItem it;
-  it.head = s.head;
-  it.clip = j / s.per_clip;
-  const int t = j - it.clip * s.per_clip;
+  const int nth = run / p.clips;
+  it.clip = run - nth * p.clips;
+  uint64_t left = s.heads;  // the nth head of the mask
+  for (int i = 0; i < nth; ++i) left &= left - 1;
+  it.head = __builtin_ctzll(left);
   int frame0 = 0;
   if (s.nt > 0) {
     const int f = t / s.nt;
@@ -117,15 +130,19 @@ __device__ inline FaItem fa_item(const FaParams& p, int rows) {
   return it;
 }
 
-__device__ inline int tiles_of(int n) { return (n + kTile - 1) / kTile; }
+template <int TOKENS>
+__device__ inline int tiles_of(int n) {
+  return (n + TOKENS - 1) / TOKENS;
+}
 
-// Position of walk tile i: tokens start .. end of it (at most 64).
+// Position of walk tile i: tokens start .. end of it (at most TOKENS).
+template <int TOKENS>
 __device__ inline void walk_tile(const FaItem& it, int na, int i, int* start, int* end) {
   if (i < na) {
-    *start = it.a0 + i * kTile;
+    *start = it.a0 + i * TOKENS;
     *end = it.a1;
   } else {
-    *start = it.b0 + (i - na) * kTile;
+    *start = it.b0 + (i - na) * TOKENS;
     *end = it.b1;
   }
 }
@@ -198,18 +215,20 @@ __device__ __forceinline__ float pair_max(float x) {
   return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
 }
 
-// Copies the rows of a walk tile of two tensors to LDS (LDS-DMA, no registers): a wave takes 16 rows of each, a lane
-// 16 bytes, swizzled by the choice of its source. Rows behind the range are copies of its last row: finite where the
-// range is, and given probability zero by the caller. Whole tiles take a scalar base and the lane's own offsets, which
-// fit 32 bits (`wide` where they do not); the last tile of a range takes an address a lane.
+// Copies the rows of a walk tile of two tensors to LDS (LDS-DMA, no registers): a lane takes 16 bytes, swizzled by the
+// choice of its source; a wave takes 16 rows of each tensor, or all 32 where it walks alone. Rows behind the range are
+// copies of its last row: finite where the range is, and given probability zero by the caller. Whole tiles take a
+// scalar base and the lane's own offsets, which fit 32 bits (`wide` where they do not); the last tile of a range takes an
+// address a lane.
 struct Stager {
   const __bf16 *x, *y;
   int64_t xs, ys;
-  uint32_t xo[2], yo[2];  // byte offsets of the lane's two rows in a tile
-  int row[2], c[2], wave;
+  uint32_t xo[2], yo[2];  // byte offsets of the lane's two rows in 16
+  int lane, row0;
   bool wide;
 };
 
+template <bool ALONE>
 __device__ __forceinline__ Stager stager(const __bf16* x, int64_t xs, const __bf16* y, int64_t ys, bool wide, int wave,
                                          int lane) {
   Stager s;
@@ -218,54 +237,134 @@ __device__ __forceinline__ Stager stager(const __bf16* x, int64_t xs, const __bf
   s.y = y;
   s.xs = xs;
   s.ys = ys;
-  s.wave = wave;
+  s.lane = lane;
+  s.row0 = ALONE ? 0 : wave * 16;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    s.row[i] = wave * 16 + i * 8 + (lane >> 3);
-    s.c[i] = ((lane & 7) ^ swz_tile(s.row[i])) << 3;
-    s.xo[i] = (uint32_t)((s.row[i] * xs + s.c[i]) * 2);
-    s.yo[i] = (uint32_t)((s.row[i] * ys + s.c[i]) * 2);
+    const int row = 8 * i + (lane >> 3), c = ((lane & 7) ^ swz_tile(row)) << 3;
+    s.xo[i] = (uint32_t)(((s.row0 + row) * xs + c) * 2);
+    s.yo[i] = (uint32_t)(((s.row0 + row) * ys + c) * 2);
   }
   return s;
 }
 
+template <bool ALONE>
 __device__ __forceinline__ void stage(const Stager& s, int start, int end, const __bf16* xt, const __bf16* yt) {
-  const uint32_t xl = lds_addr(xt) + s.wave * 2048, yl = lds_addr(yt) + s.wave * 2048;
-  if (start + kTile <= end && !s.wide) {
-    const __bf16 *xb = s.x + start * s.xs, *yb = s.y + start * s.ys;
+  const uint32_t xl = lds_addr(xt) + s.row0 * 128, yl = lds_addr(yt) + s.row0 * 128;
+  const bool whole = start + kTokens<ALONE> <= end && !s.wide;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      dma16s(xb, s.xo[i], xl + i * 1024);
-      dma16s(yb, s.yo[i], yl + i * 1024);
-    }
-  } else {
+  for (int k = 0; k < (ALONE ? 2 : 1); ++k) {
+    if (whole) {
+      const __bf16 *xb = s.x + (start + 16 * k) * s.xs, *yb = s.y + (start + 16 * k) * s.ys;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int tok = min(start + s.row[i], end - 1);
-      dma16(s.x + tok * s.xs + s.c[i], xl + i * 1024);
-      dma16(s.y + tok * s.ys + s.c[i], yl + i * 1024);
-    }
-  }
-}
-
-// Waits for the wave's own copies; rows that are not there (bits) become zeros, so that what they hold stays out of
-// every product. The work-group's barrier follows.
-template <bool MASK>
-__device__ __forceinline__ void staged(__bf16* xt, __bf16* yt, uint64_t bits, int wave, int lane) {
-  wait_vm<0>();
-  if (MASK && bits != ~0ull) {
+      for (int i = 0; i < 2; ++i) {
+        dma16s(xb, s.xo[i], xl + k * 2048 + i * 1024);
+        dma16s(yb, s.yo[i], yl + k * 2048 + i * 1024);
+      }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = wave * 16 + i * 8 + (lane >> 3);
-      if (!((bits >> row) & 1)) {
-        *reinterpret_cast<u32x4*>(xt + row * 64 + (lane & 7) * 8) = u32x4{};
-        *reinterpret_cast<u32x4*>(yt + row * 64 + (lane & 7) * 8) = u32x4{};
+      for (int i = 0; i < 2; ++i) {
+        const int row = 8 * i + (s.lane >> 3), c = ((s.lane & 7) ^ swz_tile(row)) << 3;
+        const int tok = min(start + s.row0 + 16 * k + row, end - 1);
+        dma16(s.x + tok * s.xs + c, xl + k * 2048 + i * 1024);
+        dma16(s.y + tok * s.ys + c, yl + k * 2048 + i * 1024);
       }
     }
   }
 }
 
-// Rows of a walk tile that are there, one bit each (the same in every wave).
+// Bits of a whole tile.
+template <bool ALONE>
+constexpr uint64_t kAllRows = ALONE ? 0xFFFFFFFFull : ~0ull;
+
+// Rows that are not there (bits) become zeros, so that what they hold stays out of every product. A wave clears what it
+// copied itself.
+template <bool ALONE>
+__device__ __forceinline__ void clear_rows(const Stager& s, __bf16* xt, __bf16* yt, uint64_t bits) {
+  if (bits == kAllRows<ALONE>) return;
+#pragma unroll
+  for (int i = 0; i < (ALONE ? 4 : 2); ++i) {
+    const int row = s.row0 + i * 8 + (s.lane >> 3);
+    if (!((bits >> row) & 1)) {
+      *reinterpret_cast<u32x4*>(xt + row * 64 + (s.lane & 7) * 8) = u32x4{};
+      *reinterpret_cast<u32x4*>(yt + row * 64 + (s.lane & 7) * 8) = u32x4{};
+    }
+  }
+}
+
+// The walk of a work-group over its ranges. Together (ALONE false): all waves use every tile, staged in two buffers with
+// one barrier a tile. Alone: wave w takes tiles w, w + 4, ... of 32 tokens in two buffers of its own, without barriers; the
+// callers add up what the four waves found. load(start, end) -> the lane's share of what belongs to a tile,
+// bits(share) -> the rows that are there, publish(share, buffer) before and tile(buffer, bits) with the rows in LDS.
+template <bool MASK, bool ALONE, typename Load, typename Bits, typename Publish, typename Tile>
+__device__ __forceinline__ void walk(const FaItem& it, const Stager& st, __bf16 (*lds)[2][kTokens<ALONE> * kHeadDim],
+                                     int wave, bool active, Load load, Bits bits, Publish publish, Tile tile) {
+  constexpr int kN = kTokens<ALONE>;
+  const int na = tiles_of<kN>(it.a1 - it.a0), nw = na + tiles_of<kN>(it.b1 - it.b0);
+  auto fetch = [&](int i, int buf) {
+    int start, end;
+    walk_tile<kN>(it, na, i, &start, &end);
+    end = min(end, start + kN);
+    const auto share = load(start, end);
+    stage<ALONE>(st, start, end, lds[buf][0], lds[buf][1]);
+    return share;
+  };
+  if constexpr (MASK)
+    if (!__syncthreads_or(active)) return;  // no row of its own: nothing to walk for
+  if constexpr (ALONE) {
+    if (!active || wave >= nw) return;
+    auto now = fetch(wave, 2 * wave), next = now;
+    if (wave + 4 < nw) next = fetch(wave + 4, 2 * wave + 1);
+    int buf = 2 * wave;
+    for (int i = wave; i < nw; i += 4) {
+      if (i + 4 < nw)
+        wait_vm<8>();  // all but the next tile's copies
+      else
+        wait_vm<0>();
+      const uint64_t there = bits(now);
+      if constexpr (MASK) clear_rows<true>(st, lds[buf][0], lds[buf][1], there);
+      publish(now, buf);
+      if (there) tile(buf, there);
+      now = next;
+      if (i + 8 < nw) next = fetch(i + 8, buf);
+      buf ^= 1;
+    }
+  } else {
+    if (nw == 0) return;
+    auto now = fetch(0, 0);
+    for (int i = 0; i < nw; ++i) {
+      const int buf = i & 1;
+      const uint64_t there = bits(now);
+      wait_vm<0>();
+      if constexpr (MASK) clear_rows<false>(st, lds[buf][0], lds[buf][1], there);
+      if (wave == 0) publish(now, buf);
+      __syncthreads();
+      if (i + 1 < nw) now = fetch(i + 1, buf ^ 1);
+      if (active && there) tile(buf, there);  // (a tile without a row changes nothing)
+    }
+  }
+}
+
+// What the waves of a work-group that walked alone have to add up: a 64 x 32 result (rows 32 dh + 8 (j / 4) + 4 h + j % 4
+// of lane % 32's column) a wave, in LDS rows of 33.
+constexpr int kPart = 64 * 33;
+static_assert(4 * (kPart + 64) * 4 <= 8 * 2 * kTokens<true> * kHeadDim * 2, "the parts of four waves in their buffers");
+__device__ __forceinline__ void put_part(float* part, const f32x16 (&x)[2], int lane) {
+#pragma unroll
+  for (int dh = 0; dh < 2; ++dh)
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      part[(32 * dh + 8 * (j / 4) + 4 * (lane >> 5) + j % 4) * 33 + (lane & 31)] = x[dh][j];
+}
+
+__device__ __forceinline__ void store8(__bf16* at, const float (&x)[8]) {
+  bf16x8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (__bf16)x[e];
+  *reinterpret_cast<bf16x8*>(at) = v;
+}
+
+// A token of the mask (1 where there is none), or whether it lies in the range at all.
 template <bool MASK>
 __device__ __forceinline__ uint8_t mask_byte(const uint8_t* mask, int start, int end) {
   const int tok = start + (tid_x() & 63);
@@ -282,186 +381,175 @@ __device__ __forceinline__ void mask_scores(f32x16& s, uint64_t bits, int half, 
 }
 
 // ---------------------------------------------------------------------------------------
-// Forward: a wave owns 32 QG query rows as columns of S^T = K Q^T; O^T += V^T P^T.
+// Forward: a wave owns 32 query rows as columns of S^T = K Q^T; O^T += V^T P^T.
 // The running reference m of a row is the maximum of its first tile; it moves only when a tile's sum of
 // exp2(S c - m) leaves [0, 2^40], so that tiles after the first take no maximum (fp32 holds the sums, and
 // bf16 the probabilities, at the same relative precision for any m at or below the row's maximum).
+//
+// A wave owns 32 rows and three waves share a SIMD. (64 rows a wave, two waves: the same rate over long walks, 1.4
+// times the time over 522 tokens.) ALONE: the work-group's four waves own the same 32 rows and split the walk; their
+// sums are joined at the end.
 // ---------------------------------------------------------------------------------------
-template <int QG, bool MASK>
-__global__ void __launch_bounds__(256, 2) frame_attn_fwd_kernel(const FaParams p) {
-  __shared__ __align__(16) __bf16 lds[2][2][kTileElems];
-  const FaItem it = fa_item(p, 128 * QG);
+template <bool MASK, bool ALONE>
+__global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_fwd_kernel(const FaParams p) {
+  __shared__ __align__(16) __bf16 lds[ALONE ? 8 : 2][2][kTokens<ALONE> * kHeadDim];
+  constexpr int kH = kTokens<ALONE> / 32;
+  const FaItem it = fa_item(p, ALONE ? 32 : 128);
   const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6), h = lane >> 5;
   const FragAddr fa = frag_addr(lane);
-  const __bf16* kb = p.k.ptr + it.clip * p.k.clip + it.head * p.k.head;
-  const __bf16* vb = p.v.ptr + it.clip * p.v.clip + it.head * p.v.head;
   const uint8_t* mask = MASK ? p.mask + (int64_t)it.clip * p.N : nullptr;
-  const int first = it.row0 + wave * 32 * QG;
-  const bool active = first < it.row_end;
+  const int first = it.row0 + (ALONE ? 0 : wave * 32), r = first + (lane & 31);
+  const bool valid = r < it.row_end && (!MASK || mask[r]), active = __any(valid);
 
-  bf16x8 qf[QG][4];
-  bool valid[QG];
+  bf16x8 qf[4];
+  const __bf16* qp = p.q.ptr + it.clip * p.q.clip + it.head * p.q.head + r * p.q.token + 8 * h;
 #pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    const int r = first + 32 * g + (lane & 31);
-    valid[g] = r < it.row_end && (!MASK || mask[r]);
-    const __bf16* qp = p.q.ptr + it.clip * p.q.clip + it.head * p.q.head + r * p.q.token + 8 * h;
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) qf[g][ks] = valid[g] ? *reinterpret_cast<const bf16x8*>(qp + 16 * ks) : bf16x8{};
-  }
-  f32x16 o[QG][2];
-  float m[QG], l[QG];
-#pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    o[g][0] = o[g][1] = f32x16{};
-    m[g] = -__builtin_inff();
-    l[g] = 0.f;
-  }
+  for (int ks = 0; ks < 4; ++ks) qf[ks] = valid ? *reinterpret_cast<const bf16x8*>(qp + 16 * ks) : bf16x8{};
+  f32x16 o[2] = {};
+  float m = -__builtin_inff(), l = 0.f;
 
-  const int na = tiles_of(it.a1 - it.a0), nw = na + tiles_of(it.b1 - it.b0);
-  const Stager st = stager(kb, p.k.token, vb, p.v.token, p.wide, wave, lane);
-  uint8_t mb = 0;
-  auto load = [&](int i) {
-    int start, end;
-    walk_tile(it, na, i, &start, &end);
-    mb = mask_byte<MASK>(mask, start, end);
-    stage(st, start, end, lds[i & 1][0], lds[i & 1][1]);
-  };
-  if (nw > 0) load(0);
-  for (int i = 0; i < nw; ++i) {
-    const uint64_t bits = __ballot(mb != 0);
-    __bf16* kt = lds[i & 1][0];
-    __bf16* vt = lds[i & 1][1];
-    staged<MASK>(kt, vt, bits, wave, lane);
+  const Stager st = stager<ALONE>(p.k.ptr + it.clip * p.k.clip + it.head * p.k.head, p.k.token,
+                                  p.v.ptr + it.clip * p.v.clip + it.head * p.v.head, p.v.token, p.wide, wave, lane);
+  walk<MASK, ALONE>(
+      it, st, lds, wave, active, [&](int start, int end) { return mask_byte<MASK>(mask, start, end); },
+      [](uint8_t b) { return __ballot(b != 0); }, [](uint8_t, int) {},
+      [&](int buf, uint64_t bits) {
+        const __bf16 *kt = lds[buf][0], *vt = lds[buf][1];
+        f32x16 s[kH], e[kH];
+#pragma unroll
+        for (int kh = 0; kh < kH; ++kh)
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) s[kh] = mma(row_frag(kt, fa, kh, ks), qf[ks], ks ? s[kh] : f32x16{});
+        if (bits != kAllRows<ALONE>) {
+#pragma unroll
+          for (int kh = 0; kh < kH; ++kh) mask_scores(s[kh], bits, kh, h);
+        }
+        float sum = 0.f;
+        bool moved = m == -__builtin_inff();
+        if (!__any(moved)) {
+#pragma unroll
+          for (int kh = 0; kh < kH; ++kh)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              e[kh][j] = __builtin_amdgcn_exp2f(s[kh][j] * p.c - m);
+              sum += e[kh][j];
+            }
+          moved = !(sum <= 0x1p40f);
+        }
+        if (__any(moved)) {
+          float mx = -__builtin_inff();
+#pragma unroll
+          for (int kh = 0; kh < kH; ++kh)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[kh][j]);
+          const float next = fmaxf(m, pair_max(mx) * p.c);
+          const float base = next == -__builtin_inff() ? 0.f : next;  // no key yet
+          const float f = __builtin_amdgcn_exp2f(m - base);
+          l *= f;
+#pragma unroll
+          for (int dh = 0; dh < 2; ++dh)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[dh][j] *= f;
+          m = next;
+          sum = 0.f;
+#pragma unroll
+          for (int kh = 0; kh < kH; ++kh)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              e[kh][j] = __builtin_amdgcn_exp2f(s[kh][j] * p.c - base);
+              sum += e[kh][j];
+            }
+        }
+        l += sum;
+#pragma unroll
+        for (int step = 0; step < 2 * kH; ++step) {
+          const bf16x8 pf = pack8(e[step / 2], step % 2);
+#pragma unroll
+          for (int dh = 0; dh < 2; ++dh) o[dh] = mma(tr_frag(vt, fa, step, dh), pf, o[dh]);
+        }
+      });
+
+  const float sum = pair_sum(l);
+  const int64_t stat = ((int64_t)it.clip * p.H + it.head) * p.N;
+  __bf16* op = p.o.ptr + it.clip * p.o.clip + it.head * p.o.head;
+  __bf16* rp = p.rest.ptr + it.clip * p.rest.clip + it.head * p.rest.head;
+  if constexpr (ALONE) {
+    // joined: the largest reference, every wave's sums on its scale
+    float* part = reinterpret_cast<float*>(lds);
     __syncthreads();
-    if (i + 1 < nw) load(i + 1);
-    if (!active) continue;
-    f32x16 s[QG][2];
-#pragma unroll
-    for (int kh = 0; kh < 2; ++kh) {
-#pragma unroll
-      for (int g = 0; g < QG; ++g) s[g][kh] = f32x16{};
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const bf16x8 a = row_frag(kt, fa, kh, ks);
-#pragma unroll
-        for (int g = 0; g < QG; ++g) s[g][kh] = mma(a, qf[g][ks], s[g][kh]);
-      }
+    put_part(part + wave * (kPart + 64), o, lane);
+    if (h == 0) {
+      part[wave * (kPart + 64) + kPart + lane] = m;
+      part[wave * (kPart + 64) + kPart + 32 + lane] = sum;
     }
-    if (bits != ~0ull) {
+    __syncthreads();
+    const int col = tid_x() & 31, d0 = (tid_x() >> 5) * 8, row = it.row0 + col;
+    if (row >= it.row_end) return;
+    float mw[4], top = -__builtin_inff(), total = 0.f;
 #pragma unroll
-      for (int g = 0; g < QG; ++g) {
-        mask_scores(s[g][0], bits, 0, h);
-        mask_scores(s[g][1], bits, 1, h);
-      }
+    for (int w = 0; w < 4; ++w) {
+      mw[w] = part[w * (kPart + 64) + kPart + col];
+      top = fmaxf(top, mw[w]);
     }
+    const bool some = (!MASK || mask[row]) && top != -__builtin_inff();
+    float y[8] = {}, x[8];
 #pragma unroll
-    for (int g = 0; g < QG; ++g) {
-      float ref = m[g];
-      f32x16 e[2];
-      float sum = 0.f;
-      bool moved = ref == -__builtin_inff();
-      if (!__any(moved)) {
+    for (int w = 0; w < 4; ++w) {
+      const float f = some ? __builtin_amdgcn_exp2f(mw[w] - top) : 0.f;
+      total += f * part[w * (kPart + 64) + kPart + 32 + col];
 #pragma unroll
-        for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            e[kh][j] = __builtin_amdgcn_exp2f(s[g][kh][j] * p.c - ref);
-            sum += e[kh][j];
-          }
-        moved = !(sum <= 0x1p40f);
-      }
-      if (__any(moved)) {
-        float mx = -__builtin_inff();
-#pragma unroll
-        for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[g][kh][j]);
-        const float next = fmaxf(ref, pair_max(mx) * p.c);
-        const float base = next == -__builtin_inff() ? 0.f : next;  // no key yet
-        const float f = __builtin_amdgcn_exp2f(ref - base);
-        l[g] *= f;
-#pragma unroll
-        for (int dh = 0; dh < 2; ++dh)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) o[g][dh][j] *= f;
-        m[g] = next;
-        sum = 0.f;
-#pragma unroll
-        for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            e[kh][j] = __builtin_amdgcn_exp2f(s[g][kh][j] * p.c - base);
-            sum += e[kh][j];
-          }
-      }
-      l[g] += sum;
-      s[g][0] = e[0];
-      s[g][1] = e[1];
+      for (int e = 0; e < 8; ++e) y[e] += f * part[w * (kPart + 64) + (d0 + e) * 33 + col];
     }
+    const float inv = some ? 1.f / total : 0.f;
 #pragma unroll
-    for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        bf16x8 pf[QG];
-#pragma unroll
-        for (int g = 0; g < QG; ++g) pf[g] = pack8(s[g][kh], step);
-#pragma unroll
-        for (int dh = 0; dh < 2; ++dh) {
-          const bf16x8 a = tr_frag(vt, fa, 2 * kh + step, dh);
-#pragma unroll
-          for (int g = 0; g < QG; ++g) o[g][dh] = mma(a, pf[g], o[g][dh]);
-        }
-      }
-  }
-  if (!active) return;
-#pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    const int r = first + 32 * g + (lane & 31);
-    const float sum = pair_sum(l[g]);
-    const bool some = valid[g] && m[g] != -__builtin_inff();
+    for (int e = 0; e < 8; ++e) {
+      y[e] = some ? y[e] * inv : 0.f;
+      x[e] = y[e] - (float)(__bf16)y[e];
+    }
+    store8(op + row * p.o.token + d0, y);
+    if (p.rest.ptr) store8(rp + row * p.rest.token + d0, x);
+    if (d0 == 0) p.lse[stat + row] = some ? (top + __builtin_amdgcn_logf(total)) * kLn2 : -__builtin_inff();
+  } else {
+    if (r >= it.row_end) return;
+    const bool some = valid && m != -__builtin_inff();
     const float inv = some ? 1.f / sum : 0.f;
-    if (r < it.row_end) {
-      __bf16* op = p.o.ptr + it.clip * p.o.clip + it.head * p.o.head + r * p.o.token + 4 * h;
-      __bf16* rp = p.rest.ptr ? p.rest.ptr + it.clip * p.rest.clip + it.head * p.rest.head + r * p.rest.token + 4 * h
-                              : nullptr;
+    op += r * p.o.token + 4 * h;
+    rp += r * p.rest.token + 4 * h;
 #pragma unroll
-      for (int dh = 0; dh < 2; ++dh)
+    for (int dh = 0; dh < 2; ++dh)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          __bf16 w[4], x[4];
+      for (int j = 0; j < 4; ++j) {
+        __bf16 w[4], x[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float y = some ? o[g][dh][4 * j + e] * inv : 0.f;
-            w[e] = (__bf16)y;
-            x[e] = (__bf16)(y - (float)w[e]);
-          }
-          *reinterpret_cast<u32x2*>(op + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(w);
-          if (rp) *reinterpret_cast<u32x2*>(rp + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(x);
+        for (int e = 0; e < 4; ++e) {
+          const float y = some ? o[dh][4 * j + e] * inv : 0.f;
+          w[e] = (__bf16)y;
+          x[e] = (__bf16)(y - (float)w[e]);
         }
-      if (h == 0)
-        p.lse[((int64_t)it.clip * p.H + it.head) * p.N + r] =
-            some ? (m[g] + __builtin_amdgcn_logf(sum)) * kLn2 : -__builtin_inff();
-    }
+        *reinterpret_cast<u32x2*>(op + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(w);
+        if (p.rest.ptr) *reinterpret_cast<u32x2*>(rp + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(x);
+      }
+    if (h == 0) p.lse[stat + r] = some ? (m + __builtin_amdgcn_logf(sum)) * kLn2 : -__builtin_inff();
   }
 }
 
 // ---------------------------------------------------------------------------------------
 // Backward over queries: D and dQ. A wave owns 32 QG query rows as columns of S^T and dP^T = V dO^T;
 // dQ^T += K^T dS^T.
+//
+// QG 2, two waves a SIMD: long launches (12 frames of 1374, dense-heavy: 1147 us against 1200). QG 1, three waves: short
+// ones. ALONE: as in the forward pass.
 // ---------------------------------------------------------------------------------------
-template <int QG, bool MASK>
-__global__ void __launch_bounds__(256, 2) frame_attn_dq_kernel(const FaParams p) {
-  __shared__ __align__(16) __bf16 lds[2][2][kTileElems];
-  const FaItem it = fa_item(p, 128 * QG);
+template <int QG, bool MASK, bool ALONE>
+__global__ void __launch_bounds__(256, ALONE || QG == 2 ? 2 : 3) frame_attn_dq_kernel(const FaParams p) {
+  __shared__ __align__(16) __bf16 lds[ALONE ? 8 : 2][2][kTokens<ALONE> * kHeadDim];
+  const FaItem it = fa_item(p, ALONE ? 32 : 128 * QG);
   const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6), h = lane >> 5;
   const FragAddr fa = frag_addr(lane);
-  const __bf16* kb = p.k.ptr + it.clip * p.k.clip + it.head * p.k.head;
-  const __bf16* vb = p.v.ptr + it.clip * p.v.clip + it.head * p.v.head;
   const uint8_t* mask = MASK ? p.mask + (int64_t)it.clip * p.N : nullptr;
   const int64_t stat = ((int64_t)it.clip * p.H + it.head) * p.N;
-  const int first = it.row0 + wave * 32 * QG;
-  const bool active = first < it.row_end;
+  const int first = it.row0 + (ALONE ? 0 : wave * 32 * QG);
+  bool active = false;
 
   bf16x8 qf[QG][4], dof[QG][4];
   f32x16 dq[QG][2];
@@ -470,7 +558,8 @@ __global__ void __launch_bounds__(256, 2) frame_attn_dq_kernel(const FaParams p)
   for (int g = 0; g < QG; ++g) {
     const int r = first + 32 * g + (lane & 31);
     const float ls = r < it.row_end ? p.lse[stat + r] : -__builtin_inff();
-    const bool valid = ls != -__builtin_inff();  // rows without a key, or not there
+    const bool valid = ls != -__builtin_inff();  // not: rows without a key, or not there
+    active = active || __any(valid);
     const __bf16* qp = p.q.ptr + it.clip * p.q.clip + it.head * p.q.head + r * p.q.token + 8 * h;
     const __bf16* dp = p.doo.ptr + it.clip * p.doo.clip + it.head * p.doo.head + r * p.doo.token + 8 * h;
     const __bf16* op = p.o.ptr + it.clip * p.o.clip + it.head * p.o.head + r * p.o.token + 8 * h;
@@ -495,86 +584,227 @@ __global__ void __launch_bounds__(256, 2) frame_attn_dq_kernel(const FaParams p)
     d = pair_sum(d);
     delta[g] = d;
     lse2[g] = valid ? ls * kLog2e : __builtin_inff();
-    if (h == 0 && r < it.row_end) p.delta[stat + r] = d;
+    if (h == 0 && r < it.row_end && (!ALONE || wave == 0)) p.delta[stat + r] = d;
     dq[g][0] = dq[g][1] = f32x16{};
   }
 
-  const int na = tiles_of(it.a1 - it.a0), nw = na + tiles_of(it.b1 - it.b0);
-  const Stager st = stager(kb, p.k.token, vb, p.v.token, p.wide, wave, lane);
-  uint8_t mb = 0;
-  auto load = [&](int i) {
-    int start, end;
-    walk_tile(it, na, i, &start, &end);
-    mb = mask_byte<MASK>(mask, start, end);
-    stage(st, start, end, lds[i & 1][0], lds[i & 1][1]);
-  };
-  if (nw > 0) load(0);
-  for (int i = 0; i < nw; ++i) {
-    const uint64_t bits = __ballot(mb != 0);
-    __bf16* kt = lds[i & 1][0];
-    __bf16* vt = lds[i & 1][1];
-    staged<MASK>(kt, vt, bits, wave, lane);
+  const Stager st = stager<ALONE>(p.k.ptr + it.clip * p.k.clip + it.head * p.k.head, p.k.token,
+                                  p.v.ptr + it.clip * p.v.clip + it.head * p.v.head, p.v.token, p.wide, wave, lane);
+  walk<MASK, ALONE>(
+      it, st, lds, wave, active, [&](int start, int end) { return mask_byte<MASK>(mask, start, end); },
+      [](uint8_t b) { return __ballot(b != 0); }, [](uint8_t, int) {},
+      [&](int buf, uint64_t bits) {
+        const __bf16 *kt = lds[buf][0], *vt = lds[buf][1];
+#pragma unroll
+        for (int kh = 0; kh < kTokens<ALONE> / 32; ++kh) {
+          if (!(uint32_t)(bits >> (32 * kh))) continue;
+          f32x16 s[QG], dp[QG];
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            const bf16x8 a = row_frag(kt, fa, kh, ks), b = row_frag(vt, fa, kh, ks);
+#pragma unroll
+            for (int g = 0; g < QG; ++g) {
+              s[g] = mma(a, qf[g][ks], ks ? s[g] : f32x16{});
+              dp[g] = mma(b, dof[g][ks], ks ? dp[g] : f32x16{});
+            }
+          }
+          if (bits != kAllRows<ALONE>) {
+#pragma unroll
+            for (int g = 0; g < QG; ++g) mask_scores(s[g], bits, kh, h);
+          }
+#pragma unroll
+          for (int g = 0; g < QG; ++g)
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              s[g][j] = __builtin_amdgcn_exp2f(s[g][j] * p.c - lse2[g]) * (dp[g][j] - delta[g]);
+#pragma unroll
+          for (int step = 0; step < 2; ++step) {
+            bf16x8 ds[QG];
+#pragma unroll
+            for (int g = 0; g < QG; ++g) ds[g] = pack8(s[g], step);
+#pragma unroll
+            for (int dh = 0; dh < 2; ++dh) {
+              const bf16x8 a = tr_frag(kt, fa, 2 * kh + step, dh);
+#pragma unroll
+              for (int g = 0; g < QG; ++g) dq[g][dh] = mma(a, ds[g], dq[g][dh]);
+            }
+          }
+        }
+      });
+
+  __bf16* base = p.dq.ptr + it.clip * p.dq.clip + it.head * p.dq.head;
+  if constexpr (ALONE) {
+    float* part = reinterpret_cast<float*>(lds);
     __syncthreads();
-    if (i + 1 < nw) load(i + 1);
-    if (!active) continue;
+    put_part(part + wave * kPart, dq[0], lane);
+    __syncthreads();
+    const int col = tid_x() & 31, d0 = (tid_x() >> 5) * 8, row = it.row0 + col;
+    if (row >= it.row_end) return;
+    float y[8];
 #pragma unroll
-    for (int kh = 0; kh < 2; ++kh) {
-      f32x16 s[QG], dp[QG];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const bf16x8 a = row_frag(kt, fa, kh, ks), b = row_frag(vt, fa, kh, ks);
-#pragma unroll
-        for (int g = 0; g < QG; ++g) {
-          s[g] = mma(a, qf[g][ks], ks ? s[g] : f32x16{});
-          dp[g] = mma(b, dof[g][ks], ks ? dp[g] : f32x16{});
-        }
-      }
-      if (bits != ~0ull) {
-#pragma unroll
-        for (int g = 0; g < QG; ++g) mask_scores(s[g], bits, kh, h);
-      }
-#pragma unroll
-      for (int g = 0; g < QG; ++g)
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          s[g][j] = __builtin_amdgcn_exp2f(s[g][j] * p.c - lse2[g]) * (dp[g][j] - delta[g]);
-#pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        bf16x8 ds[QG];
-#pragma unroll
-        for (int g = 0; g < QG; ++g) ds[g] = pack8(s[g], step);
-#pragma unroll
-        for (int dh = 0; dh < 2; ++dh) {
-          const bf16x8 a = tr_frag(kt, fa, 2 * kh + step, dh);
-#pragma unroll
-          for (int g = 0; g < QG; ++g) dq[g][dh] = mma(a, ds[g], dq[g][dh]);
-        }
-      }
+    for (int e = 0; e < 8; ++e) {
+      const float* x = part + (d0 + e) * 33 + col;
+      y[e] = ((x[0] + x[kPart]) + (x[2 * kPart] + x[3 * kPart])) * p.scale;
     }
-  }
-  if (!active) return;
+    store8(base + row * p.dq.token + d0, y);
+  } else {
 #pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    const int r = first + 32 * g + (lane & 31);
-    if (r < it.row_end) {
-      __bf16* op = p.dq.ptr + it.clip * p.dq.clip + it.head * p.dq.head + r * p.dq.token + 4 * h;
+    for (int g = 0; g < QG; ++g) {
+      const int r = first + 32 * g + (lane & 31);
+      if (r < it.row_end) {
+        __bf16* at = base + r * p.dq.token + 4 * h;
 #pragma unroll
-      for (int dh = 0; dh < 2; ++dh)
+        for (int dh = 0; dh < 2; ++dh)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          __bf16 w[4];
+          for (int j = 0; j < 4; ++j) {
+            __bf16 w[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = (__bf16)(dq[g][dh][4 * j + e] * p.scale);
-          *reinterpret_cast<u32x2*>(op + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(w);
-        }
+            for (int e = 0; e < 4; ++e) w[e] = (__bf16)(dq[g][dh][4 * j + e] * p.scale);
+            *reinterpret_cast<u32x2*>(at + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(w);
+          }
+      }
     }
   }
 }
 
 // ---------------------------------------------------------------------------------------
-// Backward over keys: dK and dV. A wave owns 64 key rows (two groups of 32) as columns of S = Q K^T and dP = dO V^T;
-// dV^T += dO^T P, dK^T += Q^T dS. The sums of S start at -lse / scale and those of dP at -D of their rows; a query that
-// is not there starts at -inf, so that its probabilities are zero.
+// Backward over keys, short launches: dK and dV. A wave owns 32 key rows as columns of S = Q K^T and dP = dO V^T;
+// dV^T += dO^T P, dK^T += Q^T dS. The sums of S start at -lse / scale and those of dP at -D of their rows (from LDS); a
+// query that is not there starts at -inf, so that its probabilities are zero. ALONE: as in the forward pass.
+// ---------------------------------------------------------------------------------------
+struct RowStats {
+  float ls, dl;
+};
+
+template <bool MASK, bool ALONE>
+__global__ void __launch_bounds__(256, 2) frame_attn_dkv_short_kernel(const FaParams p) {
+  __shared__ __align__(16) __bf16 lds[ALONE ? 8 : 2][2][kTokens<ALONE> * kHeadDim];
+  __shared__ __align__(16) float stats[ALONE ? 8 : 2][2 * kTile];
+  const FaItem it = fa_item(p, ALONE ? 32 : 128);
+  const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6), h = lane >> 5;
+  const FragAddr fa = frag_addr(lane);
+  const uint8_t* mask = MASK ? p.mask + (int64_t)it.clip * p.N : nullptr;
+  const int64_t stat = ((int64_t)it.clip * p.H + it.head) * p.N;
+  const int first = it.row0 + (ALONE ? 0 : wave * 32), r = first + (lane & 31);
+  const bool valid = r < it.row_end && (!MASK || mask[r]), active = __any(valid);
+
+  bf16x8 kf[4], vf[4];
+  const __bf16* kp = p.k.ptr + it.clip * p.k.clip + it.head * p.k.head + r * p.k.token + 8 * h;
+  const __bf16* vp = p.v.ptr + it.clip * p.v.clip + it.head * p.v.head + r * p.v.token + 8 * h;
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    kf[ks] = valid ? *reinterpret_cast<const bf16x8*>(kp + 16 * ks) : bf16x8{};
+    vf[ks] = valid ? *reinterpret_cast<const bf16x8*>(vp + 16 * ks) : bf16x8{};
+  }
+  f32x16 dk[2] = {}, dv[2] = {};
+
+  const float inv_scale = 1.f / p.scale;
+  const Stager st = stager<ALONE>(p.q.ptr + it.clip * p.q.clip + it.head * p.q.head, p.q.token,
+                                  p.doo.ptr + it.clip * p.doo.clip + it.head * p.doo.head, p.doo.token, p.wide, wave,
+                                  lane);
+  walk<MASK, ALONE>(
+      it, st, lds, wave, active,
+      [&](int start, int end) {
+        const int tok = start + lane;  // (end: at most the tile's)
+        RowStats x;
+        x.ls = tok < end ? p.lse[stat + tok] : -__builtin_inff();
+        x.dl = tok < end ? p.delta[stat + tok] : 0.f;
+        return x;
+      },
+      [](const RowStats& x) { return __ballot(x.ls != -__builtin_inff()); },
+      [&](const RowStats& x, int buf) {
+        const bool there = x.ls != -__builtin_inff();
+        stats[buf][lane] = there ? -x.ls * inv_scale : -__builtin_inff();
+        stats[buf][kTile + lane] = there ? -x.dl : 0.f;
+      },
+      [&](int buf, uint64_t bits) {
+        const __bf16 *qt = lds[buf][0], *dt = lds[buf][1];
+#pragma unroll
+        for (int qh = 0; qh < kTokens<ALONE> / 32; ++qh) {
+          if (!(uint32_t)(bits >> (32 * qh))) continue;
+          f32x16 s, dp;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(&stats[buf][32 * qh + 8 * j + 4 * h]);
+            const f32x4 b = *reinterpret_cast<const f32x4*>(&stats[buf][kTile + 32 * qh + 8 * j + 4 * h]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              s[4 * j + e] = a[e];
+              dp[4 * j + e] = b[e];
+            }
+          }
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            s = mma(row_frag(qt, fa, qh, ks), kf[ks], s);
+            dp = mma(row_frag(dt, fa, qh, ks), vf[ks], dp);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            s[j] = __builtin_amdgcn_exp2f(s[j] * p.c);
+            dp[j] *= s[j];
+          }
+#pragma unroll
+          for (int step = 0; step < 2; ++step) {
+            const bf16x8 pf = pack8(s, step), ds = pack8(dp, step);
+#pragma unroll
+            for (int dh = 0; dh < 2; ++dh) {
+              dv[dh] = mma(tr_frag(dt, fa, 2 * qh + step, dh), pf, dv[dh]);
+              dk[dh] = mma(tr_frag(qt, fa, 2 * qh + step, dh), ds, dk[dh]);
+            }
+          }
+        }
+      });
+
+  __bf16* dkp = p.dk.ptr + it.clip * p.dk.clip + it.head * p.dk.head;
+  __bf16* dvp = p.dv.ptr + it.clip * p.dv.clip + it.head * p.dv.head;
+  if constexpr (ALONE) {
+    float* part = reinterpret_cast<float*>(lds);
+    __syncthreads();
+    const int col = tid_x() & 31, d0 = (tid_x() >> 5) * 8, row = it.row0 + col;
+    auto total = [&](const f32x16(&x)[2], float (&y)[8]) {  // (one result at a time: 34 KB of the 64)
+      put_part(part + wave * kPart, x, lane);
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float* at = part + (d0 + e) * 33 + col;
+        y[e] = (at[0] + at[kPart]) + (at[2 * kPart] + at[3 * kPart]);
+      }
+      __syncthreads();
+    };
+    float a[8], b[8];
+    total(dk, a);
+    total(dv, b);
+    if (row >= it.row_end) return;
+    const bool there = !MASK || mask[row];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      a[e] = there ? a[e] * p.scale : 0.f;
+      b[e] = there ? b[e] : 0.f;
+    }
+    store8(dkp + row * p.dk.token + d0, a);
+    store8(dvp + row * p.dv.token + d0, b);
+  } else {
+    if (r >= it.row_end) return;
+    dkp += r * p.dk.token + 4 * h;
+    dvp += r * p.dv.token + 4 * h;
+#pragma unroll
+    for (int dh = 0; dh < 2; ++dh)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        __bf16 a[4], b[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          a[e] = (__bf16)(valid ? dk[dh][4 * j + e] * p.scale : 0.f);
+          b[e] = (__bf16)(valid ? dv[dh][4 * j + e] : 0.f);
+        }
+        *reinterpret_cast<u32x2*>(dkp + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(a);
+        *reinterpret_cast<u32x2*>(dvp + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(b);
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Backward over keys, long launches without a mask: the same with 64 key rows a wave (two groups of 32).
 //
 // Two groups share every operand read from LDS (16 KB a wave for 32 queries: with one group LDS would be as busy as
 // the matrix cores). Their sums, keys and values fill 192 registers, so one wave runs on a SIMD and has to overlap
@@ -729,8 +959,7 @@ __device__ __forceinline__ void dkv_half(DkvAcc& A, const DkvRows& r, const __bf
 #undef NEXT
 }
 
-template <bool MASK>
-__global__ void __launch_bounds__(256, 1) frame_attn_dkv_kernel(const FaParams p) {
+__global__ void __launch_bounds__(256, 1) frame_attn_dkv_long_kernel(const FaParams p) {
   __shared__ __align__(16) __bf16 lds[2][2][kTileElems];
   __shared__ __align__(16) float stats[2][2 * kTile];
   const FaItem it = fa_item(p, 256);
@@ -738,28 +967,26 @@ __global__ void __launch_bounds__(256, 1) frame_attn_dkv_kernel(const FaParams p
   const FragAddr fa = frag_addr(lane);
   const __bf16* qb = p.q.ptr + it.clip * p.q.clip + it.head * p.q.head;
   const __bf16* db = p.doo.ptr + it.clip * p.doo.clip + it.head * p.doo.head;
-  const uint8_t* mask = MASK ? p.mask + (int64_t)it.clip * p.N : nullptr;
   const int64_t stat = ((int64_t)it.clip * p.H + it.head) * p.N;
   const int first = it.row0 + wave * 64;
   const bool active = first < it.row_end;
 
-  const int na = tiles_of(it.a1 - it.a0), nw = na + tiles_of(it.b1 - it.b0);
+  const int na = tiles_of<kTile>(it.a1 - it.a0), nw = na + tiles_of<kTile>(it.b1 - it.b0);
   const float inv_scale = 1.f / p.scale;
-  const Stager st = stager(qb, p.q.token, db, p.doo.token, p.wide, wave, lane);
+  const Stager st = stager<false>(qb, p.q.token, db, p.doo.token, p.wide, wave, lane);
   float ls = 0.f, dl = 0.f;
   auto load = [&](int i) {
     int start, end;
-    walk_tile(it, na, i, &start, &end);
+    walk_tile<kTile>(it, na, i, &start, &end);
     const int tok = start + lane;
     ls = tok < end ? p.lse[stat + tok] : -__builtin_inff();
     dl = tok < end ? p.delta[stat + tok] : 0.f;
-    stage(st, start, end, lds[i & 1][0], lds[i & 1][1]);
+    stage<false>(st, start, end, lds[i & 1][0], lds[i & 1][1]);
   };
   // tile i, loaded before, becomes readable; the other buffer is free from here on
   auto ready = [&](int i) {
-    // rows without a key (masked ones among them) hold whatever their buffers held: they become zeros
     const bool there = ls != -__builtin_inff();
-    staged<MASK>(lds[i & 1][0], lds[i & 1][1], __ballot(there), wave, lane);
+    wait_vm<0>();
     if (wave == 0) {
       stats[i & 1][lane] = there ? -ls * inv_scale : -__builtin_inff();
       stats[i & 1][kTile + lane] = there ? -dl : 0.f;
@@ -770,17 +997,16 @@ __global__ void __launch_bounds__(256, 1) frame_attn_dkv_kernel(const FaParams p
 
   if (nw > 0) load(0);
   DkvAcc A;
-  bool valid[2];
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     const int r = first + 32 * g + (lane & 31);
-    valid[g] = r < it.row_end && (!MASK || mask[r]);
+    const bool valid = r < it.row_end;
     const __bf16* kp = p.k.ptr + it.clip * p.k.clip + it.head * p.k.head + r * p.k.token + 8 * h;
     const __bf16* vp = p.v.ptr + it.clip * p.v.clip + it.head * p.v.head + r * p.v.token + 8 * h;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      A.k[g][ks] = valid[g] ? *reinterpret_cast<const bf16x8*>(kp + 16 * ks) : bf16x8{};
-      A.v[g][ks] = valid[g] ? *reinterpret_cast<const bf16x8*>(vp + 16 * ks) : bf16x8{};
+      A.k[g][ks] = valid ? *reinterpret_cast<const bf16x8*>(kp + 16 * ks) : bf16x8{};
+      A.v[g][ks] = valid ? *reinterpret_cast<const bf16x8*>(vp + 16 * ks) : bf16x8{};
     }
     A.dk[g][0] = A.dk[g][1] = A.dv[g][0] = A.dv[g][1] = f32x16{};
   }
@@ -836,8 +1062,8 @@ __global__ void __launch_bounds__(256, 1) frame_attn_dkv_kernel(const FaParams p
           __bf16 a[4], b[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            a[e] = (__bf16)(valid[g] ? A.dk[g][dh][4 * j + e] * p.scale : 0.f);
-            b[e] = (__bf16)(valid[g] ? A.dv[g][dh][4 * j + e] : 0.f);
+            a[e] = (__bf16)(A.dk[g][dh][4 * j + e] * p.scale);
+            b[e] = (__bf16)A.dv[g][dh][4 * j + e];
           }
           *reinterpret_cast<u32x2*>(kp + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(a);
           *reinterpret_cast<u32x2*>(vp + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(b);
@@ -849,76 +1075,48 @@ __global__ void __launch_bounds__(256, 1) frame_attn_dkv_kernel(const FaParams p
 // ---------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------
-struct SegList {
-  FaSeg seg[kFaMaxSegs];
-  int64_t cost[kFaMaxSegs];  // walked tokens of a tile
-  int n = 0;
-};
-
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// frames f0 .. f1 - 1, each in tiles of its own
-static void add_frames(SegList* s, int head, int T, int f0, int f1, int rows, int walk, int64_t cost) {
-  if (f1 <= f0) return;
-  FaSeg& g = s->seg[s->n];
-  g.nt = (int)ceil_div(T, rows);
-  g.per_clip = g.nt * (f1 - f0);
-  g.tok0 = f0 * T;
-  g.tok1 = f1 * T;
-  g.head = (int16_t)head;
-  g.walk = (int16_t)walk;
-  s->cost[s->n++] = cost;
-}
-
-static void add_tokens(SegList* s, int head, int tok0, int tok1, int rows, int walk, int64_t cost) {
-  if (tok1 <= tok0) return;
-  FaSeg& g = s->seg[s->n];
-  g.nt = 0;
-  g.per_clip = (int)ceil_div(tok1 - tok0, rows);
-  g.tok0 = tok0;
-  g.tok1 = tok1;
-  g.head = (int16_t)head;
-  g.walk = (int16_t)walk;
-  s->cost[s->n++] = cost;
-}
-
-// Row tiles of every head, the longest walks first. keys: the tiles are key rows and walk queries.
-static int64_t make_segs(FaParams* p, const int32_t* patterns, int clips, int frames, int rows, bool keys) {
-  SegList s;
+// Row tiles of every head, the longest walks first, at most one class of each kind. keys: the tiles are key rows and
+// walk queries. Returns the number of work-groups.
+static int64_t make_classes(FaParams* p, const int32_t* patterns, int frames, int rows, bool keys) {
   const int T = p->T, N = p->N;
-  for (int h = 0; h < p->H; ++h) {
-    switch (patterns[h]) {
-      case SAF3R_DENSE: add_tokens(&s, h, 0, N, rows, kAll, N); break;
-      case SAF3R_FRAME_LOCAL: add_frames(&s, h, T, 0, frames, rows, kOwn, T); break;
-      case SAF3R_ANCHOR:
-        if (keys) {  // the first frame's keys serve every query, the others none
-          add_tokens(&s, h, 0, T, rows, kAll, N);
-          add_tokens(&s, h, T, N, rows, kNone, 0);
-        } else {
-          add_tokens(&s, h, 0, N, rows, kFirst, T);
-        }
-        break;
-      case SAF3R_ANCHOR_LOCAL:
-        if (keys) {
-          add_tokens(&s, h, 0, T, rows, kAll, N);
-          add_frames(&s, h, T, 1, frames, rows, kOwn, T);
-        } else {
-          add_frames(&s, h, T, 0, frames, rows, kFirstOwn, 2 * (int64_t)T);
-        }
-        break;
-      default: add_tokens(&s, h, 0, N, rows, kNone, 0); break;  // SAF3R_SKIP
-    }
-  }
-  int order[kFaMaxSegs];
-  for (int i = 0; i < s.n; ++i) order[i] = i;
-  std::stable_sort(order, order + s.n, [&](int a, int b) { return s.cost[a] > s.cost[b]; });
+  uint64_t of[SAF3R_SKIP + 1] = {};
+  for (int h = 0; h < p->H; ++h) of[patterns[h]] |= 1ull << h;
   int64_t total = 0;
-  for (int i = 0; i < s.n; ++i) {
-    p->seg[i] = s.seg[order[i]];
-    p->seg[i].start = (int)std::min<int64_t>(total, 0x7fffffff);
-    total += (int64_t)p->seg[i].per_clip * clips;
+  int n = 0;
+  auto add = [&](uint64_t heads, int tok0, int tok1, bool per_frame, int walk) {
+    if (!heads || tok1 <= tok0) return;
+    FaClass& c = p->cls[n++];
+    c.start = (int)std::min<int64_t>(total, 0x7fffffff);
+    c.nt = per_frame ? (int)ceil_div(T, rows) : 0;
+    const int64_t per_clip = per_frame ? (int64_t)c.nt * ((tok1 - tok0) / T) : ceil_div(tok1 - tok0, rows);
+    c.per_clip = (int)per_clip;
+    c.tok0 = tok0;
+    c.tok1 = tok1;
+    c.walk = walk;
+    c.heads = heads;
+    total += per_clip * __builtin_popcountll(heads) * p->clips;
+  };
+  const uint64_t anchor = of[SAF3R_ANCHOR], both = of[SAF3R_ANCHOR_LOCAL], local = of[SAF3R_FRAME_LOCAL];
+  add(of[SAF3R_DENSE], 0, N, false, kAll);
+  if (keys) {  // the first frame's keys serve every query, those of the others their own frame or none
+    add(anchor | both, 0, T, false, kAll);
+    add(local, 0, N, true, kOwn);
+    add(both, T, N, true, kOwn);
+    add(anchor, T, N, false, kNone);
+  } else {
+    add(both, 0, N, true, kFirstOwn);
+    add(local, 0, N, true, kOwn);
+    add(anchor, 0, N, false, kFirst);
   }
-  p->n_seg = s.n;
+  add(of[SAF3R_SKIP], 0, N, false, kNone);
+  for (; n < kFaClasses; ++n) {
+    p->cls[n] = FaClass{};
+    p->cls[n].start = 0x7fffffff;
+    p->cls[n].per_clip = 1;
+    p->cls[n].heads = 1;
+  }
   return total;
 }
 
@@ -959,10 +1157,28 @@ static int fa_check(const char* who, FaParams* p, int clips, int frames, int tok
   p->N = frames * tokens_per_frame;
   p->T = tokens_per_frame;
   p->H = num_heads;
+  p->clips = clips;
   p->mask = mask;
   p->scale = scale;
   p->c = scale * kLog2e;
   return SAF3R_OK;
+}
+
+// Rows of a work-group, by the number of work-groups of 128 rows that a launch would have. Below half a one a compute
+// unit the four waves of a work-group share 32 rows and split the walk (16 dense heads, forward / dQ / dK and dV: 522
+// tokens, 80 work-groups, 10.6 / 13.9 / 12.9 us against 13.9 / 17.6 / 16.4; 1041 tokens, 144 work-groups, 21.8 / 29.0 /
+// 30.0 against 20.4 / 27.4 / 27.6).
+constexpr int64_t kAloneBelow = 128;
+// Launches of several rounds take 64 rows a wave.
+constexpr int64_t kWideFrom = 1792;
+
+// f(whether there is a mask, whether the waves walk alone)
+template <typename F>
+static void fa_launch(bool mask, bool alone, F f) {
+  if (mask)
+    alone ? f(std::true_type(), std::true_type()) : f(std::true_type(), std::false_type());
+  else
+    alone ? f(std::false_type(), std::true_type()) : f(std::false_type(), std::false_type());
 }
 
 static int fa_grid(const char* who, int64_t total) {
@@ -991,12 +1207,14 @@ extern "C" int saf3r_frame_attn_fwd(const saf3r_heads* q, const saf3r_heads* k, 
     return fail(SAF3R_ERR_INVALID, "%s: rows must be 16-byte aligned with strides a multiple of 8", who);
   p.lse = lse;
   p.wide = fa_wide(p.k) || fa_wide(p.v);
-  const int64_t n = make_segs(&p, patterns, clips, frames, 256, false);
+  int64_t n = make_classes(&p, patterns, frames, 128, false);
+  const bool alone = n < kAloneBelow;
+  if (alone) n = make_classes(&p, patterns, frames, 32, false);
   if (int e = fa_grid(who, n)) return e;
-  if (token_mask)
-    hipLaunchKernelGGL((frame_attn_fwd_kernel<2, true>), dim3((uint32_t)n), dim3(256), 0, (hipStream_t)stream, p);
-  else
-    hipLaunchKernelGGL((frame_attn_fwd_kernel<2, false>), dim3((uint32_t)n), dim3(256), 0, (hipStream_t)stream, p);
+  fa_launch(token_mask != nullptr, alone, [&](auto m, auto a) {
+    hipLaunchKernelGGL((frame_attn_fwd_kernel<decltype(m)::value, decltype(a)::value>), dim3((uint32_t)n), dim3(256), 0,
+                       (hipStream_t)stream, p);
+  });
   return check_launch(who);
 }
 
@@ -1036,16 +1254,27 @@ extern "C" int saf3r_frame_attn_bwd(const saf3r_heads* dout, const saf3r_heads* 
   p.delta = (float*)workspace;
   p.wide = fa_wide(p.q) || fa_wide(p.k) || fa_wide(p.v) || fa_wide(p.doo);
   FaParams pk = p;
-  const int64_t nq = make_segs(&p, patterns, clips, frames, 256, false);
-  const int64_t nk = make_segs(&pk, patterns, clips, frames, 256, true);
-  if (int e = fa_grid(who, std::max(nq, nk))) return e;
+  // the query side: see kAloneBelow, kWideFrom
+  int64_t n = make_classes(&p, patterns, frames, 128, false);
+  const bool masked = token_mask != nullptr, alone = n < kAloneBelow, wide = n >= kWideFrom;
+  if (alone || wide) n = make_classes(&p, patterns, frames, alone ? 32 : 256, false);
+  int64_t nk = make_classes(&pk, patterns, frames, 128, true);
+  const bool alone_k = nk < kAloneBelow, wide_k = !masked && nk >= kWideFrom;
+  if (alone_k || wide_k) nk = make_classes(&pk, patterns, frames, alone_k ? 32 : 256, true);
+  if (int e = fa_grid(who, std::max(n, nk))) return e;
   const hipStream_t s = (hipStream_t)stream;
-  if (token_mask) {
-    hipLaunchKernelGGL((frame_attn_dq_kernel<2, true>), dim3((uint32_t)nq), dim3(256), 0, s, p);
-    hipLaunchKernelGGL((frame_attn_dkv_kernel<true>), dim3((uint32_t)nk), dim3(256), 0, s, pk);
-  } else {
-    hipLaunchKernelGGL((frame_attn_dq_kernel<2, false>), dim3((uint32_t)nq), dim3(256), 0, s, p);
-    hipLaunchKernelGGL((frame_attn_dkv_kernel<false>), dim3((uint32_t)nk), dim3(256), 0, s, pk);
-  }
+  const dim3 gq((uint32_t)n), gk((uint32_t)nk), block(256);
+  fa_launch(masked, alone, [&](auto m, auto a) {
+    if (wide)
+      hipLaunchKernelGGL((frame_attn_dq_kernel<2, decltype(m)::value, false>), gq, block, 0, s, p);
+    else
+      hipLaunchKernelGGL((frame_attn_dq_kernel<1, decltype(m)::value, decltype(a)::value>), gq, block, 0, s, p);
+  });
+  fa_launch(masked, alone_k, [&](auto m, auto a) {
+    if (wide_k)
+      hipLaunchKernelGGL(frame_attn_dkv_long_kernel, gk, block, 0, s, pk);
+    else
+      hipLaunchKernelGGL((frame_attn_dkv_short_kernel<decltype(m)::value, decltype(a)::value>), gk, block, 0, s, pk);
+  });
   return check_launch(who);
 }

@@ -305,3 +305,27 @@ def test_long_walk_sample(ops):
         rel = float((t[0, :, 1].double() - w).norm() / w.norm())
         # a result's rounding and its operands' (P, dS, D), each at most U of magnitudes that add in quadrature
         assert rel < 2 * R.U, (name, rel)
+
+
+@pytest.mark.parametrize("pattern,B,F,T,H", [("dense", 30, 1, 520, 12), ("mix", 26, 3, 190, 15), ("anchor_local", 120, 2, 65, 16),
+                                             ("dense", 3, 1, 4999, 16)])
+def test_launches_of_many_rows(ops, pattern, B, F, T, H):
+    """Launches that take 64 rows a wave (1792 work-groups of 128 rows and more): the first and the last clip against
+    64 bits, and equal bits for a clip by itself where its own launch takes fewer rows a wave."""
+    N = F * T
+    q, k, v, do = inputs(B, N, H, T)
+    pat = patterns_of(ops, pattern, H)
+    gq, gk, gv, gdo = (t.to(DEV) for t in (q, k, v, do))
+    out, lse, rest = ops.frame_attn_fwd(gq, gk, gv, pat, frames=F, rest=True)
+    dq, dk, dv = ops.frame_attn_bwd(gdo, gq, gk, gv, out, lse, pat, frames=F, rest=rest)
+    heads = range(H) if N < 1000 else (0, H - 1)
+    for b in (0, B - 1):
+        for h in heads:
+            sl = (slice(b, b + 1), slice(None), slice(h, h + 1))
+            ref = R.frame_attention(*(t[sl] for t in (q, k, v, do)), [pat[h]], F)
+            for name, t in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+                want, tol = ref[name]
+                err = (t[sl].double().cpu() - want).abs()
+                assert (err <= tol).all(), (name, b, h, float((err / tol).max()))
+            want, tol = ref["lse"]
+            assert ((lse[b:b + 1, h:h + 1].double().cpu() - want).abs() <= tol)[torch.isfinite(want)].all()
