@@ -534,59 +534,55 @@ __global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_fwd_kernel(cons
 }
 
 // ---------------------------------------------------------------------------------------
-// Backward over queries: D and dQ. A wave owns 32 QG query rows as columns of S^T and dP^T = V dO^T;
+// Backward over queries: D and dQ. A wave owns 32 query rows as columns of S^T and dP^T = V dO^T;
 // dQ^T += K^T dS^T.
-//
-// QG 2, two waves a SIMD: long launches (12 frames of 1374, dense-heavy: 1147 us against 1200). QG 1, three waves: short
-// ones. ALONE: as in the forward pass.
+// The sums of dP start at -D. Three waves a SIMD (64 rows a wave and two waves: the same rate). ALONE: as in the forward
+// pass.
 // ---------------------------------------------------------------------------------------
-template <int QG, bool MASK, bool ALONE>
-__global__ void __launch_bounds__(256, ALONE || QG == 2 ? 2 : 3) frame_attn_dq_kernel(const FaParams p) {
+template <bool MASK, bool ALONE>
+__global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_dq_kernel(const FaParams p) {
   __shared__ __align__(16) __bf16 lds[ALONE ? 8 : 2][2][kTokens<ALONE> * kHeadDim];
-  const FaItem it = fa_item(p, ALONE ? 32 : 128 * QG);
+  const FaItem it = fa_item(p, ALONE ? 32 : 128);
   const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6), h = lane >> 5;
   const FragAddr fa = frag_addr(lane);
   const uint8_t* mask = MASK ? p.mask + (int64_t)it.clip * p.N : nullptr;
   const int64_t stat = ((int64_t)it.clip * p.H + it.head) * p.N;
-  const int first = it.row0 + (ALONE ? 0 : wave * 32 * QG);
-  bool active = false;
+  const int first = it.row0 + (ALONE ? 0 : wave * 32), r = first + (lane & 31);
+  const float ls = r < it.row_end ? p.lse[stat + r] : -__builtin_inff();
+  const bool valid = ls != -__builtin_inff(), active = __any(valid);  // not: rows without a key, or not there
 
-  bf16x8 qf[QG][4], dof[QG][4];
-  f32x16 dq[QG][2];
-  float lse2[QG], delta[QG];
-#pragma unroll
-  for (int g = 0; g < QG; ++g) {
-    const int r = first + 32 * g + (lane & 31);
-    const float ls = r < it.row_end ? p.lse[stat + r] : -__builtin_inff();
-    const bool valid = ls != -__builtin_inff();  // not: rows without a key, or not there
-    active = active || __any(valid);
+  bf16x8 qf[4] = {}, dof[4] = {};
+  float d = 0.f;
+  if (valid) {
     const __bf16* qp = p.q.ptr + it.clip * p.q.clip + it.head * p.q.head + r * p.q.token + 8 * h;
     const __bf16* dp = p.doo.ptr + it.clip * p.doo.clip + it.head * p.doo.head + r * p.doo.token + 8 * h;
     const __bf16* op = p.o.ptr + it.clip * p.o.clip + it.head * p.o.head + r * p.o.token + 8 * h;
-    const __bf16* rp = p.rest.ptr + it.clip * p.rest.clip + it.head * p.rest.head + r * p.rest.token + 8 * h;
-    float d = 0.f;
+    bf16x8 of[4], rf[4] = {};
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      qf[g][ks] = dof[g][ks] = bf16x8{};
-      if (valid) {
-        qf[g][ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
-        dof[g][ks] = *reinterpret_cast<const bf16x8*>(dp + 16 * ks);
-        const bf16x8 of = *reinterpret_cast<const bf16x8*>(op + 16 * ks);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) d += (float)dof[g][ks][j] * (float)of[j];
-        if (p.rest.ptr) {
-          const bf16x8 rf = *reinterpret_cast<const bf16x8*>(rp + 16 * ks);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) d += (float)dof[g][ks][j] * (float)rf[j];
-        }
-      }
+      qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
+      dof[ks] = *reinterpret_cast<const bf16x8*>(dp + 16 * ks);
+      of[ks] = *reinterpret_cast<const bf16x8*>(op + 16 * ks);
     }
-    d = pair_sum(d);
-    delta[g] = d;
-    lse2[g] = valid ? ls * kLog2e : __builtin_inff();
-    if (h == 0 && r < it.row_end && (!ALONE || wave == 0)) p.delta[stat + r] = d;
-    dq[g][0] = dq[g][1] = f32x16{};
+    if (p.rest.ptr) {
+      const __bf16* rp = p.rest.ptr + it.clip * p.rest.clip + it.head * p.rest.head + r * p.rest.token + 8 * h;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) rf[ks] = *reinterpret_cast<const bf16x8*>(rp + 16 * ks);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        d += (float)dof[ks][j] * (float)of[ks][j];
+        d += (float)dof[ks][j] * (float)rf[ks][j];
+      }
   }
+  d = pair_sum(d);
+  if (h == 0 && r < it.row_end && (!ALONE || wave == 0)) p.delta[stat + r] = d;
+  const float lse2 = valid ? ls * kLog2e : __builtin_inff();
+  f32x16 dq[2] = {}, from;  // from: where the sums of dP start
+#pragma unroll
+  for (int j = 0; j < 16; ++j) from[j] = -d;
 
   const Stager st = stager<ALONE>(p.k.ptr + it.clip * p.k.clip + it.head * p.k.head, p.k.token,
                                   p.v.ptr + it.clip * p.v.clip + it.head * p.v.head, p.v.token, p.wide, wave, lane);
@@ -598,36 +594,20 @@ __global__ void __launch_bounds__(256, ALONE || QG == 2 ? 2 : 3) frame_attn_dq_k
 #pragma unroll
         for (int kh = 0; kh < kTokens<ALONE> / 32; ++kh) {
           if (!(uint32_t)(bits >> (32 * kh))) continue;
-          f32x16 s[QG], dp[QG];
+          f32x16 s, dp;
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
-            const bf16x8 a = row_frag(kt, fa, kh, ks), b = row_frag(vt, fa, kh, ks);
-#pragma unroll
-            for (int g = 0; g < QG; ++g) {
-              s[g] = mma(a, qf[g][ks], ks ? s[g] : f32x16{});
-              dp[g] = mma(b, dof[g][ks], ks ? dp[g] : f32x16{});
-            }
+            s = mma(row_frag(kt, fa, kh, ks), qf[ks], ks ? s : f32x16{});
+            dp = mma(row_frag(vt, fa, kh, ks), dof[ks], ks ? dp : from);
           }
-          if (bits != kAllRows<ALONE>) {
+          if (bits != kAllRows<ALONE>) mask_scores(s, bits, kh, h);
 #pragma unroll
-            for (int g = 0; g < QG; ++g) mask_scores(s[g], bits, kh, h);
-          }
-#pragma unroll
-          for (int g = 0; g < QG; ++g)
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              s[g][j] = __builtin_amdgcn_exp2f(s[g][j] * p.c - lse2[g]) * (dp[g][j] - delta[g]);
+          for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(s[j] * p.c - lse2) * dp[j];
 #pragma unroll
           for (int step = 0; step < 2; ++step) {
-            bf16x8 ds[QG];
+            const bf16x8 ds = pack8(s, step);
 #pragma unroll
-            for (int g = 0; g < QG; ++g) ds[g] = pack8(s[g], step);
-#pragma unroll
-            for (int dh = 0; dh < 2; ++dh) {
-              const bf16x8 a = tr_frag(kt, fa, 2 * kh + step, dh);
-#pragma unroll
-              for (int g = 0; g < QG; ++g) dq[g][dh] = mma(a, ds[g], dq[g][dh]);
-            }
+            for (int dh = 0; dh < 2; ++dh) dq[dh] = mma(tr_frag(kt, fa, 2 * kh + step, dh), ds, dq[dh]);
           }
         }
       });
@@ -636,7 +616,7 @@ __global__ void __launch_bounds__(256, ALONE || QG == 2 ? 2 : 3) frame_attn_dq_k
   if constexpr (ALONE) {
     float* part = reinterpret_cast<float*>(lds);
     __syncthreads();
-    put_part(part + wave * kPart, dq[0], lane);
+    put_part(part + wave * kPart, dq, lane);
     __syncthreads();
     const int col = tid_x() & 31, d0 = (tid_x() >> 5) * 8, row = it.row0 + col;
     if (row >= it.row_end) return;
@@ -648,22 +628,17 @@ __global__ void __launch_bounds__(256, ALONE || QG == 2 ? 2 : 3) frame_attn_dq_k
     }
     store8(base + row * p.dq.token + d0, y);
   } else {
+    if (r >= it.row_end) return;
+    base += r * p.dq.token + 4 * h;
 #pragma unroll
-    for (int g = 0; g < QG; ++g) {
-      const int r = first + 32 * g + (lane & 31);
-      if (r < it.row_end) {
-        __bf16* at = base + r * p.dq.token + 4 * h;
+    for (int dh = 0; dh < 2; ++dh)
 #pragma unroll
-        for (int dh = 0; dh < 2; ++dh)
+      for (int j = 0; j < 4; ++j) {
+        __bf16 w[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            __bf16 w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = (__bf16)(dq[g][dh][4 * j + e] * p.scale);
-            *reinterpret_cast<u32x2*>(at + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(w);
-          }
+        for (int e = 0; e < 4; ++e) w[e] = (__bf16)(dq[dh][4 * j + e] * p.scale);
+        *reinterpret_cast<u32x2*>(base + 32 * dh + 8 * j) = *reinterpret_cast<u32x2*>(w);
       }
-    }
   }
 }
 
@@ -1169,8 +1144,8 @@ static int fa_check(const char* who, FaParams* p, int clips, int frames, int tok
 // tokens, 80 work-groups, 10.6 / 13.9 / 12.9 us against 13.9 / 17.6 / 16.4; 1041 tokens, 144 work-groups, 21.8 / 29.0 /
 // 30.0 against 20.4 / 27.4 / 27.6).
 constexpr int64_t kAloneBelow = 128;
-// Launches of several rounds take 64 rows a wave.
-constexpr int64_t kWideFrom = 1792;
+// From here on the backward pass over keys takes 64 rows a wave (without a mask).
+constexpr int64_t kLongFrom = 1792;
 
 // f(whether there is a mask, whether the waves walk alone)
 template <typename F>
@@ -1254,24 +1229,21 @@ extern "C" int saf3r_frame_attn_bwd(const saf3r_heads* dout, const saf3r_heads* 
   p.delta = (float*)workspace;
   p.wide = fa_wide(p.q) || fa_wide(p.k) || fa_wide(p.v) || fa_wide(p.doo);
   FaParams pk = p;
-  // the query side: see kAloneBelow, kWideFrom
+  const bool masked = token_mask != nullptr;
   int64_t n = make_classes(&p, patterns, frames, 128, false);
-  const bool masked = token_mask != nullptr, alone = n < kAloneBelow, wide = n >= kWideFrom;
-  if (alone || wide) n = make_classes(&p, patterns, frames, alone ? 32 : 256, false);
+  const bool alone = n < kAloneBelow;
+  if (alone) n = make_classes(&p, patterns, frames, 32, false);
   int64_t nk = make_classes(&pk, patterns, frames, 128, true);
-  const bool alone_k = nk < kAloneBelow, wide_k = !masked && nk >= kWideFrom;
-  if (alone_k || wide_k) nk = make_classes(&pk, patterns, frames, alone_k ? 32 : 256, true);
+  const bool alone_k = nk < kAloneBelow, long_k = !masked && nk >= kLongFrom;
+  if (alone_k || long_k) nk = make_classes(&pk, patterns, frames, alone_k ? 32 : 256, true);
   if (int e = fa_grid(who, std::max(n, nk))) return e;
   const hipStream_t s = (hipStream_t)stream;
-  const dim3 gq((uint32_t)n), gk((uint32_t)nk), block(256);
+  const dim3 gk((uint32_t)nk), block(256);
   fa_launch(masked, alone, [&](auto m, auto a) {
-    if (wide)
-      hipLaunchKernelGGL((frame_attn_dq_kernel<2, decltype(m)::value, false>), gq, block, 0, s, p);
-    else
-      hipLaunchKernelGGL((frame_attn_dq_kernel<1, decltype(m)::value, decltype(a)::value>), gq, block, 0, s, p);
+    hipLaunchKernelGGL((frame_attn_dq_kernel<decltype(m)::value, decltype(a)::value>), dim3((uint32_t)n), block, 0, s, p);
   });
   fa_launch(masked, alone_k, [&](auto m, auto a) {
-    if (wide_k)
+    if (long_k)
       hipLaunchKernelGGL(frame_attn_dkv_long_kernel, gk, block, 0, s, pk);
     else
       hipLaunchKernelGGL((frame_attn_dkv_short_kernel<decltype(m)::value, decltype(a)::value>), gk, block, 0, s, pk);
