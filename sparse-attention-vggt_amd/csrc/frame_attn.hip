@@ -645,14 +645,16 @@ __global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_dq_kernel(const
 // ---------------------------------------------------------------------------------------
 // Backward over keys, short launches: dK and dV. A wave owns 32 key rows as columns of S = Q K^T and dP = dO V^T;
 // dV^T += dO^T P, dK^T += Q^T dS. The sums of S start at -lse / scale and those of dP at -D of their rows (from LDS); a
-// query that is not there starts at -inf, so that its probabilities are zero. ALONE: as in the forward pass.
+// query that is not there starts at -inf, so that its probabilities are zero. Three waves a SIMD without a mask (four
+// registers spilled to hold them: 8 x 1374 frames 161 us against 174); with one, three spill too much (254 us against
+// 200 on the masked mix). ALONE: as in the forward pass.
 // ---------------------------------------------------------------------------------------
 struct RowStats {
   float ls, dl;
 };
 
 template <bool MASK, bool ALONE>
-__global__ void __launch_bounds__(256, 2) frame_attn_dkv_short_kernel(const FaParams p) {
+__global__ void __launch_bounds__(256, MASK || ALONE ? 2 : 3) frame_attn_dkv_short_kernel(const FaParams p) {
   __shared__ __align__(16) __bf16 lds[ALONE ? 8 : 2][2][kTokens<ALONE> * kHeadDim];
   __shared__ __align__(16) float stats[ALONE ? 8 : 2][2 * kTile];
   const FaItem it = fa_item(p, ALONE ? 32 : 128);

@@ -8,7 +8,6 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
-from contextlib import nullcontext
 from dataclasses import dataclass
 from functools import lru_cache
 from typing import Sequence
@@ -907,9 +906,9 @@ def frame_topk_scores(scores: torch.Tensor, frames: int, per_frame: int, topk: i
 STATIC_PATTERNS = (DENSE, FRAME_LOCAL, ANCHOR_LOCAL, ANCHOR, SKIP)  # patterns of frame_attn_fwd / frame_attn_bwd
 
 
-def _on_device(t: torch.Tensor):
-    """Context in which ``t``'s device is the current one (its current stream takes the launches)."""
-    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _elsewhere(t: torch.Tensor) -> bool:
+    """Whether ``t`` lies on another device than the current one (whose current stream takes the launches)."""
+    return t.device.index != torch.cuda.current_device()
 
 
 def _readable(t: torch.Tensor, step: int) -> torch.Tensor:
@@ -923,26 +922,42 @@ def _readable(t: torch.Tensor, step: int) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _frame_heads(t: torch.Tensor) -> _lib.Heads:
-    """``saf3r_heads`` of a [clips, tokens, heads, 64] tensor (the stride of a size of one is not used)."""
-    b, n, h = (s if size > 1 else 0 for s, size in zip(t.stride()[:3], t.shape[:3]))
-    return _lib.Heads(t.data_ptr(), b, n, 0, h)
+def _frame_heads(t: torch.Tensor, copy: bool = True) -> _lib.Heads | None:
+    """``saf3r_heads`` of a [clips, tokens, heads, 64] tensor, or of a copy that the kernels can read (held by the
+    result), or None where it would have to be one and ``copy`` says no."""
+    b, n, h, d = t.stride()
+    ptr = t.data_ptr()
+    if d != 1 or ptr & 15 or (b | n | h) & 7:
+        r = _readable(t, 8)
+        if r is not t and not copy:
+            return None
+        b, n, h = (s if size > 1 else 0 for s, size in zip(r.stride()[:3], r.shape[:3]))
+        res = _lib.Heads(r.data_ptr(), b, n, 0, h)
+        res.held = r
+        return res
+    return _lib.Heads(ptr, b, n, 0, h)
+
+
+def _frame_like(name: str, t: torch.Tensor, q: torch.Tensor) -> None:
+    if t.shape != q.shape or t.dtype != torch.bfloat16 or t.device != q.device:
+        raise ValueError(f"{name} must be bfloat16 {tuple(q.shape)} on {q.device}, got {t.dtype} {tuple(t.shape)} on "
+                         f"{t.device}")
 
 
 def _frame_args(q, k, v, patterns, frames: int, token_mask, scale):
     """Checks shared by the attention's two directions: (patterns as a host array, mask or None, scale)."""
-    _need_cuda(q, k, v, token_mask)
-    if q.dim() != 4 or q.shape[3] != HEAD_DIM:
-        raise ValueError(f"q must be [clips, tokens, heads, {HEAD_DIM}], got {tuple(q.shape)}")
-    for name, t in (("k", k), ("v", v)):
-        if t.shape != q.shape:
-            raise ValueError(f"{name} must have q's shape {tuple(q.shape)}, got {tuple(t.shape)}")
+    if not (q.is_cuda and k.is_cuda and v.is_cuda and (token_mask is None or token_mask.is_cuda)):
+        raise ValueError("saf3r kernels take GPU tensors")
+    shape = q.shape
+    if len(shape) != 4 or shape[3] != HEAD_DIM:
+        raise ValueError(f"q must be [clips, tokens, heads, {HEAD_DIM}], got {tuple(shape)}")
+    if k.shape != shape or v.shape != shape:
+        name, t = ("k", k) if k.shape != shape else ("v", v)
+        raise ValueError(f"{name} must have q's shape {tuple(shape)}, got {tuple(t.shape)}")
     for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dtype != torch.bfloat16:
-            raise ValueError(f"{name} must be bfloat16, got {t.dtype}")
-        if t.device != q.device:
-            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
-    B, N, H, _ = q.shape
+        if t.dtype != torch.bfloat16 or t.device != q.device:
+            raise ValueError(f"{name} must be bfloat16 on {q.device}, got {t.dtype} on {t.device}")
+    B, N, H, _ = shape
     if frames < 1 or N < 1 or N % frames:
         raise ValueError(f"{N} tokens are not {frames} frames of one size")
     if len(patterns) != H:
@@ -953,7 +968,10 @@ def _frame_args(q, k, v, patterns, frames: int, token_mask, scale):
         if token_mask.device != q.device:
             raise ValueError(f"token_mask is on {token_mask.device}, q on {q.device}")
         token_mask = token_mask.contiguous()
-    return _i32_array(patterns), token_mask, float(1.0 / math.sqrt(HEAD_DIM) if scale is None else scale)
+    return _i32_array(patterns), token_mask, _FRAME_SCALE if scale is None else float(scale)
+
+
+_FRAME_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 
 def frame_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, patterns: Sequence[int], frames: int = 1,
@@ -966,19 +984,20 @@ def frame_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, patterns: 
     lse fp32 [clips, heads, tokens]); a row without a key is zeros with lse -inf. With ``rest`` a third tensor like out
     holds what its rounding took away, for the backward pass. Not differentiable by itself: see
     ``autograd.frame_attention``."""
-    pat, mask, scale = _frame_args(q, k, v, patterns, frames, token_mask, scale)
-    lib = _lib.load()
+    pat, mask, fscale = _frame_args(q, k, v, patterns, frames, token_mask, scale)
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return frame_attn_fwd(q, k, v, patterns, frames, token_mask, scale, rest)
     B, N, H, _ = q.shape
-    q, k, v = (_readable(t, 8) for t in (q, k, v))
-    with _on_device(q):
-        out = torch.empty(B, N, H, HEAD_DIM, dtype=torch.bfloat16, device=q.device)
-        low = torch.empty_like(out) if rest else None
-        lse = torch.empty(B, H, N, dtype=torch.float32, device=q.device)
-        _mark("frame_attn_fwd", "start")
-        _lib.check(lib.saf3r_frame_attn_fwd(_frame_heads(q), _frame_heads(k), _frame_heads(v), B, frames, N // frames,
-                                            H, pat, _ptr(mask), scale, _frame_heads(out),
-                                            _frame_heads(low) if rest else None, _ptr(lse), _lib.stream_ptr()))
-        _mark("frame_attn_fwd", "end")
+    out = q.new_empty(q.shape)
+    low = q.new_empty(q.shape) if rest else None
+    lse = q.new_empty((B, H, N), dtype=torch.float32)
+    hq, hk, hv, ho = _frame_heads(q), _frame_heads(k), _frame_heads(v), _frame_heads(out)
+    _mark("frame_attn_fwd", "start")
+    _lib.check(_lib.load().saf3r_frame_attn_fwd(hq, hk, hv, B, frames, N // frames, H, pat, _ptr(mask), fscale, ho,
+                                                _frame_heads(low) if rest else None, lse.data_ptr(),
+                                                _lib.stream_ptr()))
+    _mark("frame_attn_fwd", "end")
     return (out, lse, low) if rest else (out, lse)
 
 
@@ -991,39 +1010,37 @@ def frame_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
     dq and dk carry the rounding of out: 1.5 to 2 times their error). ``grads`` (optional): three
     bf16 tensors or views of q's shape that receive them (rows 16-byte aligned, strides a multiple of 8, not
     overlapping the inputs). The results do not depend on the order in which the GPU runs the work."""
-    pat, mask, scale = _frame_args(q, k, v, patterns, frames, token_mask, scale)
-    _need_cuda(dout, out, lse)
-    lib = _lib.load()
+    pat, mask, fscale = _frame_args(q, k, v, patterns, frames, token_mask, scale)
     B, N, H, _ = q.shape
-    _need_cuda(rest)
-    for name, t in (("dout", dout), ("out", out)) + ((("rest", rest),) if rest is not None else ()):
-        if t.shape != q.shape or t.dtype != torch.bfloat16 or t.device != q.device:
-            raise ValueError(f"{name} must be bfloat16 {tuple(q.shape)} on {q.device}, got {t.dtype} {tuple(t.shape)}")
+    _frame_like("dout", dout, q)
+    _frame_like("out", out, q)
+    if rest is not None:
+        _frame_like("rest", rest, q)
     if tuple(lse.shape) != (B, H, N) or lse.dtype != torch.float32 or lse.device != q.device:
         raise ValueError(f"lse must be float32 {(B, H, N)} on {q.device}, got {lse.dtype} {tuple(lse.shape)}")
-    dout, q, k, v, out = (_readable(t, 8) for t in (dout, q, k, v, out))
-    rest = None if rest is None else _readable(rest, 8)
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return frame_attn_bwd(dout, q, k, v, out, lse, patterns, frames, token_mask, scale, rest, grads)
     lse = lse.contiguous()
-    with _on_device(q):
-        if grads is None:
-            grads = tuple(torch.empty(B, N, H, HEAD_DIM, dtype=torch.bfloat16, device=q.device) for _ in range(3))
-        else:
-            for t in grads:
-                if t.shape != q.shape or t.dtype != torch.bfloat16 or t.device != q.device:
-                    raise ValueError(f"grads must be bfloat16 {tuple(q.shape)} on {q.device}")
-                if _readable(t, 8) is not t:
-                    raise ValueError("grads need 16-byte aligned rows with strides a multiple of 8")
-        nbytes = lib.saf3r_frame_attn_bwd_workspace_bytes(B, frames, N // frames, H)
-        if nbytes < 0:
-            raise ValueError(f"unsupported attention: {H} heads, {frames} frames of {N // frames} tokens")
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        _mark("frame_attn_bwd", "start")
-        _lib.check(lib.saf3r_frame_attn_bwd(
-            _frame_heads(dout), _frame_heads(q), _frame_heads(k), _frame_heads(v), _frame_heads(out),
-            None if rest is None else _frame_heads(rest), _ptr(lse), B, frames, N // frames, H, pat, _ptr(mask), scale,
-            *(_frame_heads(t) for t in grads), _ptr(ws), nbytes, _lib.stream_ptr()))
-        _mark("frame_attn_bwd", "end")
-    return tuple(grads)
+    if grads is None:
+        grads = (q.new_empty(q.shape), q.new_empty(q.shape), q.new_empty(q.shape))
+    else:
+        grads = tuple(grads)
+        if len(grads) != 3:
+            raise ValueError("grads must be three tensors")
+        for t in grads:
+            _frame_like("grads", t, q)
+    into = [_frame_heads(t, copy=False) for t in grads]
+    if None in into:
+        raise ValueError("grads need 16-byte aligned rows with strides a multiple of 8")
+    ws = q.new_empty((B, H, N), dtype=torch.float32)  # (saf3r_frame_attn_bwd_workspace_bytes)
+    held = (_frame_heads(dout), _frame_heads(q), _frame_heads(k), _frame_heads(v), _frame_heads(out),
+            None if rest is None else _frame_heads(rest))
+    _mark("frame_attn_bwd", "start")
+    _lib.check(_lib.load().saf3r_frame_attn_bwd(*held, lse.data_ptr(), B, frames, N // frames, H, pat, _ptr(mask), fscale,
+                                                *into, ws.data_ptr(), ws.numel() * 4, _lib.stream_ptr()))
+    _mark("frame_attn_bwd", "end")
+    return grads
 
 
 # ---- training: rotary positions and norms with their gradients ---------------------------------------------
@@ -1037,38 +1054,44 @@ def _dtype(name: str, t: torch.Tensor) -> int:
     return _DTYPES[t.dtype]
 
 
-def _norm_params(shape: tuple, rows_dtype, device, **params):
-    """(dtype of the parameters, type the kernels read them in, the contiguous tensors or None): weight and bias of one
-    type and of ``shape``. Parameters that are neither fp32 nor of the rows' 16-bit type are read as fp32 copies."""
-    given = {n: t for n, t in params.items() if t is not None}
-    for n, t in given.items():
+def _norm_params(shape: tuple, rows: torch.Tensor, rows_dtype, weight, bias=None):
+    """(dtype of the parameters, type the kernels read them in, weight, bias): weight and bias of one type and of
+    ``shape``, contiguous. Parameters that are neither fp32 nor of the rows' 16-bit type are read as fp32 copies."""
+    kind = None
+    for n, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.shape != shape:
+            raise ValueError(f"{n} must be {tuple(shape)}, got {tuple(t.shape)}")
+        if t.device != rows.device:
+            raise ValueError(f"{n} is on {t.device}, the rows on {rows.device}")
         _dtype(n, t)
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{n} must be {shape}, got {tuple(t.shape)}")
-        if t.device != device:
-            raise ValueError(f"{n} is on {t.device}, the rows on {device}")
-    kinds = {t.dtype for t in given.values()}
-    if len(kinds) > 1:
-        raise ValueError("weight and bias must have one dtype")
-    kind = kinds.pop() if kinds else torch.float32
-    read = kind if kind == rows_dtype else torch.float32
-    return kind, _DTYPES[read], [None if t is None else t.to(read).contiguous() for t in params.values()]
+        if kind is not None and t.dtype != kind:
+            raise ValueError("weight and bias must have one dtype")
+        kind = t.dtype
+    kind = torch.float32 if kind is None else kind
+    read = torch.float32
+    if kind != torch.float32:
+        if kind == rows_dtype:
+            read = kind
+        else:
+            weight, bias = (None if t is None else t.float() for t in (weight, bias))
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    return kind, read, weight, bias
 
 
-def _param_grads(shape: tuple, kind: torch.dtype, read: int, device, needs):
-    """Buffers for the parameters' gradients, in the type that the kernels read the parameters in."""
-    dtype = kind if _DTYPES[kind] == read else torch.float32
-    return [torch.empty(shape, dtype=dtype, device=device) if need else None for need in needs]
-
-
-def _flat_rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as [rows, dim] with consecutive elements in a row; a copy where its strides do not allow that view."""
-    t = t.reshape(-1, t.shape[-1])
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _flat_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t`` as rows with consecutive elements (a copy where its strides do not allow that view), and the row stride."""
+    dim = t.shape[-1]
+    if t.is_contiguous():
+        return t, dim
+    t = t.reshape(-1, dim)
+    if dim > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else dim
 
 
 def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
@@ -1077,25 +1100,26 @@ def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     fp32 of x's leading shape, for ``layer_norm_bwd``. x fp32, bf16 or fp16; y in x's type, or for fp32 x in
     ``out_dtype`` (fp32 arithmetic, rounded once). Not differentiable by itself: see ``autograd.layer_norm``."""
     _need_cuda(x, weight, bias)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x must have a last dimension, got {tuple(x.shape)}")
+    shape, dt = x.shape, x.dtype
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"x must have a last dimension, got {tuple(shape)}")
     xt = _dtype("x", x)
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype != x.dtype and (x.dtype != torch.float32 or out_dtype not in _DTYPES):
-        raise ValueError(f"{x.dtype} rows give {x.dtype} rows, not {out_dtype}")
-    dim = x.shape[-1]
-    _, pt, (weight, bias) = _norm_params((dim,), out_dtype, x.device, weight=weight, bias=bias)
-    lib = _lib.load()
-    with _on_device(x):
-        rows = _flat_rows(x)
-        y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-        stats = torch.empty(2, *x.shape[:-1], dtype=torch.float32, device=x.device)
-        mean, rstd = stats[0], stats[1]
-        _mark("layer_norm_fwd", "start")
-        _lib.check(lib.saf3r_layer_norm_fwd(_ptr(rows), _row_stride(rows), xt, rows.shape[0], dim, _ptr(weight),
-                                            _ptr(bias), pt, float(eps), _ptr(y), dim, _DTYPES[out_dtype], _ptr(mean),
-                                            _ptr(rstd), _lib.stream_ptr()))
-        _mark("layer_norm_fwd", "end")
+    out_dtype = dt if out_dtype is None else out_dtype
+    if out_dtype != dt and (dt != torch.float32 or out_dtype not in _DTYPES):
+        raise ValueError(f"{dt} rows give {dt} rows, not {out_dtype}")
+    _, read, w, b = _norm_params(shape[-1:], x, out_dtype, weight, bias)
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return layer_norm_fwd(x, weight, bias, eps, out_dtype)
+    dim = shape[-1]
+    rows, stride = _flat_rows(x)
+    y = x.new_empty(shape, dtype=out_dtype)
+    mean, rstd = x.new_empty(shape[:-1], dtype=torch.float32), x.new_empty(shape[:-1], dtype=torch.float32)
+    _mark("layer_norm_fwd", "start")
+    _lib.check(_lib.load().saf3r_layer_norm_fwd(rows.data_ptr(), stride, xt, mean.numel(), dim, _ptr(w), _ptr(b),
+                                                _DTYPES[read], eps, y.data_ptr(), dim, _DTYPES[out_dtype],
+                                                mean.data_ptr(), rstd.data_ptr(), _lib.stream_ptr()))
+    _mark("layer_norm_fwd", "end")
     return y, mean, rstd
 
 
@@ -1106,30 +1130,35 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: 
     weight's type (fp32 without a weight). Equal inputs give equal bits."""
     _need_cuda(dy, x, mean, rstd, weight)
     xt, yt = _dtype("x", x), _dtype("dy", dy)
-    if dy.shape != x.shape or dy.device != x.device or x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"dy must be like x {tuple(x.shape)} on {x.device}, got {tuple(dy.shape)} on {dy.device}")
+    shape = x.shape
+    if dy.shape != shape or dy.device != x.device or len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"dy must be like x {tuple(shape)} on {x.device}, got {tuple(dy.shape)} on {dy.device}")
     for n, t in (("mean", mean), ("rstd", rstd)):
-        if t.shape != x.shape[:-1] or t.dtype != torch.float32 or t.device != x.device:
-            raise ValueError(f"{n} must be float32 {tuple(x.shape[:-1])}, got {t.dtype} {tuple(t.shape)}")
-    dim = x.shape[-1]
-    kind, pt, (weight,) = _norm_params((dim,), dy.dtype, x.device, weight=weight)
+        if t.shape != shape[:-1] or t.dtype != torch.float32 or t.device != x.device:
+            raise ValueError(f"{n} must be float32 {tuple(shape[:-1])}, got {t.dtype} {tuple(t.shape)}")
+    kind, read, w, _ = _norm_params(shape[-1:], x, dy.dtype, weight)
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return layer_norm_bwd(dy, x, mean, rstd, weight, need_params)
+    dim = shape[-1]
     lib = _lib.load()
-    with _on_device(x):
-        rows, drows = _flat_rows(x), _flat_rows(dy)
-        mean, rstd = mean.contiguous(), rstd.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dw, db = _param_grads((dim,), kind, pt, x.device, need_params)
-        nbytes, ws = 0, None
-        if any(need_params):
-            nbytes = lib.saf3r_layer_norm_bwd_workspace_bytes(rows.shape[0], dim)
-            if nbytes >= 0:
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        _mark("layer_norm_bwd", "start")
-        _lib.check(lib.saf3r_layer_norm_bwd(_ptr(drows), _row_stride(drows), yt, _ptr(rows), _row_stride(rows), xt,
-                                            rows.shape[0], dim, _ptr(mean), _ptr(rstd), _ptr(weight), pt, _ptr(dx),
-                                            dim, _ptr(dw), _ptr(db), _ptr(ws), nbytes, _lib.stream_ptr()))
-        _mark("layer_norm_bwd", "end")
-        return (dx, *(t if t is None else t.to(kind) for t in (dw, db)))
+    rows, stride = _flat_rows(x)
+    drows, dstride = _flat_rows(dy)
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    dx = x.new_empty(shape)
+    dw, db = (x.new_empty(shape[-1:], dtype=read) if need else None for need in need_params)
+    nbytes, ws = 0, None
+    if dw is not None or db is not None:
+        nbytes = lib.saf3r_layer_norm_bwd_workspace_bytes(mean.numel(), dim)
+        ws = x.new_empty(max(nbytes, 0), dtype=torch.uint8)
+    _mark("layer_norm_bwd", "start")
+    _lib.check(lib.saf3r_layer_norm_bwd(drows.data_ptr(), dstride, yt, rows.data_ptr(), stride, xt, mean.numel(), dim,
+                                        mean.data_ptr(), rstd.data_ptr(), _ptr(w), _DTYPES[read], dx.data_ptr(), dim,
+                                        _ptr(dw), _ptr(db), _ptr(ws), nbytes, _lib.stream_ptr()))
+    _mark("layer_norm_bwd", "end")
+    if kind != read:
+        dw, db = (None if t is None else t.to(kind) for t in (dw, db))
+    return dx, dw, db
 
 
 def rotary_tables(positions: int, section: int, base: float = 100.0, scaling: str | None = None, factor: float = 1.0,
@@ -1158,51 +1187,52 @@ def rotary_tables(positions: int, section: int, base: float = 100.0, scaling: st
 
 
 def _rotary_args(x, pos, tables, layout: str, rotary_dim: int | None, norm: bool, weight, bias):
-    """Checks shared by both directions: (keyword values of the C entries, x's sizes)."""
+    """Checks shared by both directions: the positions, tables and sizes as the C entries take them."""
     if x.dim() != 5:
         raise ValueError(f"x must be [clips, tokens, groups, heads, dim], got {tuple(x.shape)}")
-    B, N, G, H, D = x.shape
     if layout not in ("half", "interleaved"):
         raise ValueError(f"layout {layout!r}: 'half' or 'interleaved'")
     if not norm and (weight is not None or bias is not None):
         raise ValueError("weight and bias belong to the norm (norm=True)")
-    cos = sin = None
-    axes, positions, R = 1, 0, 0
     if (pos is None) != (tables is None):
         raise ValueError("rotary positions need pos and tables")
-    if tables is not None:
-        cos, sin = tables
-        _need_cuda(pos, cos, sin)
-        if pos.dim() != 3 or pos.shape[:2] != x.shape[:2] or not 1 <= pos.shape[2] <= 8:
-            raise ValueError(f"pos must be [{B}, {N}, axes] with 1 to 8 axes, got {tuple(pos.shape)}")
-        if pos.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"pos must be int32 or int64, got {pos.dtype}")
-        axes = pos.shape[2]
-        R = D if rotary_dim is None else int(rotary_dim)
-        if not 0 < R <= D or R % (2 * axes):
-            raise ValueError(f"rotary_dim {R} must be {axes} even sections of at most {D} elements")
-        for n, t in (("cos", cos), ("sin", sin)):
-            if t.dim() != 2 or t.shape != cos.shape or t.shape[1] != R // axes // 2 or t.dtype != torch.float32:
-                raise ValueError(f"{n} must be float32 [positions, {R // axes // 2}], got {t.dtype} {tuple(t.shape)}")
-        positions = cos.shape[0]
-        if positions < 1:
-            raise ValueError("the tables hold no position")
-        for n, t in (("pos", pos), ("cos", cos), ("sin", sin)):
-            if t.device != x.device:
-                raise ValueError(f"{n} is on {t.device}, x on {x.device}")
-        pos, cos, sin = pos.contiguous(), cos.contiguous(), sin.contiguous()
-    elif not norm:
-        raise ValueError("neither a norm nor rotary positions were asked for")
-    return pos, cos, sin, axes, positions, R
+    if tables is None:
+        if not norm:
+            raise ValueError("neither a norm nor rotary positions were asked for")
+        return None, 0, 1, None, None, 0, 0
+    B, N, _, _, D = x.shape
+    cos, sin = tables
+    _need_cuda(pos, cos, sin)
+    if pos.dim() != 3 or pos.shape[:2] != x.shape[:2] or not 1 <= pos.shape[2] <= 8:
+        raise ValueError(f"pos must be [{B}, {N}, axes] with 1 to 8 axes, got {tuple(pos.shape)}")
+    if pos.dtype != torch.int64 and pos.dtype != torch.int32:
+        raise ValueError(f"pos must be int32 or int64, got {pos.dtype}")
+    axes = pos.shape[2]
+    R = D if rotary_dim is None else int(rotary_dim)
+    if not 0 < R <= D or R % (2 * axes):
+        raise ValueError(f"rotary_dim {R} must be {axes} even sections of at most {D} elements")
+    for n, t in (("cos", cos), ("sin", sin)):
+        if t.dim() != 2 or t.shape != cos.shape or t.shape[1] != R // axes // 2 or t.dtype != torch.float32:
+            raise ValueError(f"{n} must be float32 [positions, {R // axes // 2}], got {t.dtype} {tuple(t.shape)}")
+    positions = cos.shape[0]
+    if positions < 1:
+        raise ValueError("the tables hold no position")
+    dev = x.device
+    if pos.device != dev or cos.device != dev or sin.device != dev:
+        raise ValueError(f"pos and the tables must be on {dev}, got {pos.device}, {cos.device} and {sin.device}")
+    return pos.contiguous(), int(pos.dtype == torch.int64), axes, cos.contiguous(), sin.contiguous(), positions, R
 
 
 def _group_heads(t: torch.Tensor) -> _lib.Heads:
-    """``saf3r_heads`` of a [clips, tokens, groups, heads, dim] tensor (the stride of a size of one is not used)."""
-    return _lib.Heads(t.data_ptr(), *(s if size > 1 else 0 for s, size in zip(t.stride()[:4], t.shape[:4])))
-
-
-def _unit_rows(t: torch.Tensor) -> torch.Tensor:
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    """``saf3r_heads`` of a [clips, tokens, groups, heads, dim] tensor with consecutive elements in a row (or of a
+    contiguous copy, held by the result)."""
+    b, n, g, h, d = t.stride()
+    if d != 1 and t.shape[4] > 1:
+        r = t.contiguous()
+        res = _lib.Heads(r.data_ptr(), *r.stride()[:4])
+        res.held = r
+        return res
+    return _lib.Heads(t.data_ptr(), b, n, g, h)
 
 
 def head_rotary_fwd(x: torch.Tensor, pos: torch.Tensor | None = None, tables=None, layout: str = "half",
@@ -1218,19 +1248,19 @@ def head_rotary_fwd(x: torch.Tensor, pos: torch.Tensor | None = None, tables=Non
     ``autograd.head_rotary``."""
     _need_cuda(x, weight, bias)
     xt = _dtype("x", x)
-    pos, cos, sin, axes, positions, R = _rotary_args(x, pos, tables, layout, rotary_dim, norm, weight, bias)
+    p, pos64, axes, cos, sin, positions, R = _rotary_args(x, pos, tables, layout, rotary_dim, norm, weight, bias)
     B, N, G, H, D = x.shape
-    _, pt, (weight, bias) = _norm_params((G, D), x.dtype, x.device, weight=weight, bias=bias)
-    lib = _lib.load()
-    with _on_device(x):
-        x = _unit_rows(x)
-        y = torch.empty(B, N, G, H, D, dtype=x.dtype, device=x.device)
-        _mark("head_rotary_fwd", "start")
-        _lib.check(lib.saf3r_head_rotary_fwd(
-            _group_heads(x), xt, B, N, G, H, D, _ptr(pos), int(pos is not None and pos.dtype == torch.int64), axes,
-            _ptr(cos), _ptr(sin), positions, R, int(layout == "interleaved"), int(norm), _ptr(weight), _ptr(bias), pt,
-            float(eps), _group_heads(y), _lib.stream_ptr()))
-        _mark("head_rotary_fwd", "end")
+    _, read, w, b = _norm_params((G, D), x, x.dtype, weight, bias)
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return head_rotary_fwd(x, pos, tables, layout, rotary_dim, norm, weight, bias, eps)
+    y = x.new_empty(x.shape)
+    hx, hy = _group_heads(x), _group_heads(y)
+    _mark("head_rotary_fwd", "start")
+    _lib.check(_lib.load().saf3r_head_rotary_fwd(
+        hx, xt, B, N, G, H, D, _ptr(p), pos64, axes, _ptr(cos), _ptr(sin), positions, R, layout == "interleaved",
+        bool(norm), _ptr(w), _ptr(b), _DTYPES[read], eps, hy, _lib.stream_ptr()))
+    _mark("head_rotary_fwd", "end")
     return y
 
 
@@ -1244,29 +1274,30 @@ def head_rotary_bwd(dy: torch.Tensor, x: torch.Tensor, pos: torch.Tensor | None 
     view like x with consecutive elements in a row, not overlapping the inputs. Equal inputs give equal bits."""
     _need_cuda(dy, x, weight, out)
     xt = _dtype("x", x)
-    pos, cos, sin, axes, positions, R = _rotary_args(x, pos, tables, layout, rotary_dim, norm, weight, None)
+    p, pos64, axes, cos, sin, positions, R = _rotary_args(x, pos, tables, layout, rotary_dim, norm, weight, None)
     if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
         raise ValueError(f"dy must be like x: {x.dtype} {tuple(x.shape)}, got {dy.dtype} {tuple(dy.shape)}")
     B, N, G, H, D = x.shape
-    kind, pt, (weight,) = _norm_params((G, D), x.dtype, x.device, weight=weight)
-    if out is not None:
-        if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or _unit_rows(out) is not out:
-            raise ValueError(f"out must be like x: {x.dtype} {tuple(x.shape)} with consecutive elements in a row")
+    kind, read, w, _ = _norm_params((G, D), x, x.dtype, weight)
+    if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != x.device
+                            or (D > 1 and out.stride(4) != 1)):
+        raise ValueError(f"out must be like x: {x.dtype} {tuple(x.shape)} with consecutive elements in a row")
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return head_rotary_bwd(dy, x, pos, tables, layout, rotary_dim, norm, weight, eps, need_params, out)
     lib = _lib.load()
-    with _on_device(x):
-        x, dy = _unit_rows(x), _unit_rows(dy)
-        dx = torch.empty(B, N, G, H, D, dtype=x.dtype, device=x.device) if out is None else out
-        dw, db = _param_grads((G, D), kind, pt, x.device, [need and norm for need in need_params])
-        nbytes, ws = 0, None
-        if dw is not None or db is not None:
-            nbytes = lib.saf3r_head_rotary_bwd_workspace_bytes(B, N, G, H, D)
-            if nbytes >= 0:
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        _mark("head_rotary_bwd", "start")
-        _lib.check(lib.saf3r_head_rotary_bwd(
-            _group_heads(dy), _group_heads(x), xt, B, N, G, H, D, _ptr(pos),
-            int(pos is not None and pos.dtype == torch.int64), axes, _ptr(cos), _ptr(sin), positions, R,
-            int(layout == "interleaved"), int(norm), _ptr(weight), pt, float(eps), _group_heads(dx), _ptr(dw),
-            _ptr(db), _ptr(ws), nbytes, _lib.stream_ptr()))
-        _mark("head_rotary_bwd", "end")
-        return (dx, *(t if t is None else t.to(kind) for t in (dw, db)))
+    dx = x.new_empty(x.shape) if out is None else out
+    dw, db = (x.new_empty((G, D), dtype=read) if need and norm else None for need in need_params)
+    nbytes, ws = 0, None
+    if dw is not None or db is not None:
+        nbytes = lib.saf3r_head_rotary_bwd_workspace_bytes(B, N, G, H, D)
+        ws = x.new_empty(max(nbytes, 0), dtype=torch.uint8)
+    hdy, hx, hdx = _group_heads(dy), _group_heads(x), _group_heads(dx)
+    _mark("head_rotary_bwd", "start")
+    _lib.check(lib.saf3r_head_rotary_bwd(
+        hdy, hx, xt, B, N, G, H, D, _ptr(p), pos64, axes, _ptr(cos), _ptr(sin), positions, R, layout == "interleaved",
+        bool(norm), _ptr(w), _DTYPES[read], eps, hdx, _ptr(dw), _ptr(db), _ptr(ws), nbytes, _lib.stream_ptr()))
+    _mark("head_rotary_bwd", "end")
+    if kind != read:
+        dw, db = (None if t is None else t.to(kind) for t in (dw, db))
+    return dx, dw, db
