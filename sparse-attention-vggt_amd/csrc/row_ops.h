@@ -38,6 +38,38 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[VE]) {
   }
 }
 
+// The first `n` of VE elements at p, which is aligned to its elements only; zeros behind them. A whole vector is one load
+// (global memory takes any dword, and here any element, alignment).
+template <int VE, typename T>
+__device__ __forceinline__ void load_some(const T* p, int n, float (&x)[VE]) {
+  typedef T vec __attribute__((ext_vector_type(VE)));
+  typedef vec any __attribute__((aligned(sizeof(T))));
+  if (n >= VE) {
+    const vec v = *reinterpret_cast<const any*>(p);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) x[e] = (float)v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) x[e] = e < n ? (float)p[e] : 0.f;
+  }
+}
+
+template <int VE, typename T>
+__device__ __forceinline__ void store_some(T* p, int n, const float (&x)[VE]) {
+  typedef T vec __attribute__((ext_vector_type(VE)));
+  typedef vec any __attribute__((aligned(sizeof(T))));
+  if (n >= VE) {
+    vec v;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v[e] = (T)x[e];
+    *reinterpret_cast<any*>(p) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+      if (e < n) p[e] = (T)x[e];
+  }
+}
+
 // VE parameters from element c of a tensor, or `none` where there is no tensor. (The element type is a template
 // argument: a branch on a run-time type around these loads was compiled so that one arm left the column of the
 // store behind it unset.)
@@ -79,22 +111,46 @@ __device__ __forceinline__ float inv_sqrt(float x) {
   return x > 1e-37f && x < 1e37f ? n : r;
 }
 
-// Adds the VE values of every lane over the 256 / W groups of W lanes of a work-group; the sums end in the first
-// group. lds: 256 * VE floats (not used where there is one group).
+// Sum over the lanes of a wave that have the same place in their group of W lanes, in each of them: rotations within
+// rows of 16 lanes, then row pairs and halves.
+template <int W>
+__device__ __forceinline__ float groups_sum(float x) {
+  if constexpr (W <= 2) x += dpp_mov<0x122>(x);  // row_ror:2
+  if constexpr (W <= 4) x += dpp_mov<0x124>(x);  // row_ror:4
+  if constexpr (W <= 8) x += dpp_mov<0x128>(x);  // row_ror:8
+  if constexpr (W <= 16) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+  }
+  if constexpr (W <= 32) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    x = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+  }
+  return x;
+}
+
+// Adds the VE values of every lane over the groups of W lanes of a work-group of 256 (waves first, then four waves
+// through LDS); the sums end in the first group. lds: 4 * 64 * VE floats (not used where there is one group).
 template <int VE, int W>
 __device__ __forceinline__ void add_slots(float (&x)[VE], float* lds) {
-  constexpr int kSlots = 256 / W;
-  if constexpr (kSlots > 1) {
-    __syncthreads();
+  if constexpr (W < 256) {
+    constexpr int kLanes = W < 64 ? W : 64;
+    const int lane = tid_x() & 63, wave = tid_x() >> 6;
 #pragma unroll
-    for (int e = 0; e < VE; ++e) lds[e * 256 + tid_x()] = x[e];
+    for (int e = 0; e < VE; ++e) x[e] = groups_sum<kLanes>(x[e]);
     __syncthreads();
-    if (tid_x() < W) {
+    if (lane < kLanes) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) lds[(e * 4 + wave) * kLanes + lane] = x[e];
+    }
+    __syncthreads();
+    if (tid_x() < kLanes) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        float s = 0.f;
-        for (int k = 0; k < kSlots; ++k) s += lds[e * 256 + k * W + tid_x()];
-        x[e] = s;
+        const float* at = lds + e * 4 * kLanes + lane;
+        x[e] = (at[0] + at[kLanes]) + (at[2 * kLanes] + at[3 * kLanes]);
       }
     }
   }

@@ -254,6 +254,12 @@ def test_rotary_parameter_types(ops, pdt):
     check_rotary(ops, *rotary_inputs(1, 40, 2, 4, 64, 2, 30, 64, BF, 4, pdt=pdt), "half", 64, True)
 
 
+def test_rotary_without_eps(ops):
+    """No eps, and rows that fill no step: the lanes without a row add nothing to the parameters' gradients."""
+    for N in (1, 2, 43):
+        check_rotary(ops, *rotary_inputs(1, N, 2, 3, 64, 2, 30, 64, BF, 8 + N), "half", 64, True, eps=0.0)
+
+
 def test_rotary_many_rows(ops):
     """More rows than one step of every work-group."""
     check_rotary(ops, *rotary_inputs(2, 4100, 2, 3, 32, 2, 40, 32, BF, 6), "half", 32, True)
