@@ -511,7 +511,9 @@ int saf3r_frame_topk_scores(const void* scores, int64_t score_stride, int rows, 
  *   SAF3R_SKIP (SAF3R_ERR_UNSUPPORTED for the others).
  *   token_mask: device uint8 [clips][N] or NULL; a token whose byte is 0 is no key of any query, and its own
  *   row comes out as zeros. Its q, k and v rows may hold anything.
- *   out: bf16 rows, softmax_j(q.k_j * scale) v_j; zeros for a row without a key.
+ *   scale: 1e-30 .. 1e30.
+ *   out: bf16 rows, softmax_j(q.k_j * scale) v_j; zeros for a row without a key. Rows that a call writes have places
+ *   of their own (a stride of zero over more than one of them is refused).
  *   out_rest: bf16 rows or NULL: what the rounding of out took away (out + out_rest is the fp32 result to 16 bits),
  *   for saf3r_frame_attn_bwd.
  *   lse: fp32 [clips][num_heads][N], log sum_j exp(q.k_j * scale); -inf for a row without a key.

@@ -273,6 +273,9 @@ __device__ __forceinline__ void stage(const Stager& s, int start, int end, const
   }
 }
 
+// Every LDS access of the wave is done.
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // Bits of a whole tile.
 template <bool ALONE>
 constexpr uint64_t kAllRows = ALONE ? 0xFFFFFFFFull : ~0ull;
@@ -326,6 +329,7 @@ __device__ __forceinline__ void walk(const FaItem& it, const Stager& st, __bf16 
       publish(now, buf);
       if (there) tile(buf, there);
       now = next;
+      wait_lds();  // this tile's reads, before its buffer is filled again
       if (i + 8 < nw) next = fetch(i + 8, buf);
       buf ^= 1;
     }
@@ -1110,6 +1114,11 @@ static bool fa_aligned(const FaTensor& t) {
   return (uintptr_t)t.ptr % 16 == 0 && t.clip % 8 == 0 && t.token % 8 == 0 && t.head % 8 == 0;
 }
 
+// Whether rows that are written would lie on each other (a stride of zero).
+static bool fa_overlaps(const FaTensor& t, const FaParams& p) {
+  return t.ptr && ((t.clip == 0 && p.clips > 1) || (t.token == 0 && p.N > 1) || (t.head == 0 && p.H > 1));
+}
+
 // Whether the rows of a walk tile are so far apart (or in descending order) that their byte offsets need 64 bits.
 static bool fa_wide(const FaTensor& t) { return t.token < 0 || t.token >= ((int64_t)1 << 31) / 2 / kTile; }
 
@@ -1130,7 +1139,8 @@ static int fa_check(const char* who, FaParams* p, int clips, int frames, int tok
       return fail(x < 0 || x > SAF3R_TOKEN_DYNAMIC_KEYSET ? SAF3R_ERR_INVALID : SAF3R_ERR_UNSUPPORTED,
                   "%s: head %d: pattern %d is not one of dense, frame-local, anchor-local, anchor, skip", who, h, x);
   }
-  if (!(scale > 0.f && scale < 3.0e38f)) return fail(SAF3R_ERR_INVALID, "%s: scale must be positive and finite", who);
+  // (the backward pass starts its sums at lse / scale, in fp32)
+  if (!(scale >= 1e-30f && scale <= 1e30f)) return fail(SAF3R_ERR_INVALID, "%s: scale %g (1e-30 to 1e30)", who, scale);
   p->N = frames * tokens_per_frame;
   p->T = tokens_per_frame;
   p->H = num_heads;
@@ -1182,6 +1192,8 @@ extern "C" int saf3r_frame_attn_fwd(const saf3r_heads* q, const saf3r_heads* k, 
   if (!fa_aligned(p.q) || !fa_aligned(p.k) || !fa_aligned(p.v) || !fa_aligned(p.o) || !fa_aligned(p.rest) ||
       (uintptr_t)lse % 4)
     return fail(SAF3R_ERR_INVALID, "%s: rows must be 16-byte aligned with strides a multiple of 8", who);
+  if (fa_overlaps(p.o, p) || fa_overlaps(p.rest, p))
+    return fail(SAF3R_ERR_INVALID, "%s: written rows overlap (a stride of zero)", who);
   p.lse = lse;
   p.wide = fa_wide(p.k) || fa_wide(p.v);
   int64_t n = make_classes(&p, patterns, frames, 128, false);
@@ -1223,6 +1235,8 @@ extern "C" int saf3r_frame_attn_bwd(const saf3r_heads* dout, const saf3r_heads* 
   for (const FaTensor* t : {&p.doo, &p.q, &p.k, &p.v, &p.o, &p.rest, &p.dq, &p.dk, &p.dv})
     if (!fa_aligned(*t))
       return fail(SAF3R_ERR_INVALID, "%s: rows must be 16-byte aligned with strides a multiple of 8", who);
+  if (fa_overlaps(p.dq, p) || fa_overlaps(p.dk, p) || fa_overlaps(p.dv, p))
+    return fail(SAF3R_ERR_INVALID, "%s: written rows overlap (a stride of zero)", who);
   const int64_t need = saf3r_frame_attn_bwd_workspace_bytes(clips, frames, tokens_per_frame, num_heads);
   if (workspace_bytes < need || !workspace || (uintptr_t)workspace % 16 || (uintptr_t)lse % 4)
     return fail(SAF3R_ERR_INVALID, "%s: workspace of %lld bytes: %lld, 16-byte aligned, are needed", who,

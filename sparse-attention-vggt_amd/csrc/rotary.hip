@@ -381,6 +381,12 @@ static RotTensor rot_tensor(const saf3r_heads* h) {
   return {(char*)const_cast<void*>(h->ptr), h->clip_stride, h->token_stride, h->group_stride, h->head_stride};
 }
 
+// Whether rows that are written would lie on each other (a stride of zero).
+static bool rot_overlaps(const RotTensor& t, const RotParams& p, int64_t clips) {
+  return (t.clip == 0 && clips > 1) || (t.token == 0 && p.tokens > 1) || (t.group == 0 && p.groups > 1) ||
+         (t.head == 0 && p.heads > 1);
+}
+
 // Whether a tensor's clips follow each other as its tokens do.
 static bool rot_flat(const RotTensor& t, int clips, int tokens) {
   return !t.ptr || clips <= 1 || t.clip == t.token * tokens;
@@ -441,6 +447,7 @@ extern "C" int saf3r_head_rotary_fwd(const saf3r_heads* x, int type, int64_t cli
   const int size = type == SAF3R_FP32 ? 4 : 2;
   if (((uintptr_t)p.x.ptr | (uintptr_t)p.y.ptr) % size)
     return fail(SAF3R_ERR_INVALID, "%s: rows must be aligned to their elements", who);
+  if (rot_overlaps(p.y, p, clips)) return fail(SAF3R_ERR_INVALID, "%s: written rows overlap (a stride of zero)", who);
   if (norm) {
     p.w = weight;
     p.b = bias;
@@ -486,6 +493,7 @@ extern "C" int saf3r_head_rotary_bwd(const saf3r_heads* dy, const saf3r_heads* x
     const int size = type == SAF3R_FP32 ? 4 : 2;
     if (((uintptr_t)p.x.ptr | (uintptr_t)p.y.ptr | (uintptr_t)p.dy.ptr) % size)
       return fail(SAF3R_ERR_INVALID, "%s: rows must be aligned to their elements", who);
+    if (rot_overlaps(p.y, p, clips)) return fail(SAF3R_ERR_INVALID, "%s: written rows overlap (a stride of zero)", who);
     if (!norm) {  // the inverse rotation is all there is
       p.x = p.dy;
       p.dy = RotTensor{};

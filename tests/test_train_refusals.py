@@ -84,6 +84,33 @@ def test_attention_tensors(L):
     refused(L, attn_bwd(L, ws=264), INVALID, "16-byte")
 
 
+@pytest.mark.parametrize("call", [attn_fwd, attn_bwd])
+def test_attention_scale_range(L, call):
+    for s in (1e-31, 1e31, -0.125):
+        refused(L, call(L, scale=s), INVALID, "scale")
+
+
+def test_attention_results_on_each_other(L):
+    """Rows that are written have places of their own; rows that are read may be broadcast (not refused here: the call
+    goes on to the next check)."""
+    sizes = dict(clips=2, n=2, patterns=(0, 0))
+    for stride in ("clip", "token", "head"):
+        h = heads(L, **{stride: 0})
+        refused(L, attn_fwd(L, out=h, **sizes), INVALID, "overlap")
+        refused(L, attn_fwd(L, rest=h, **sizes), INVALID, "overlap")
+        for name in ("dq", "dk", "dv"):
+            refused(L, attn_bwd(L, **{name: h}, **sizes), INVALID, "overlap")
+        for name in ("dout", "q", "k", "v", "out"):
+            refused(L, attn_bwd(L, nbytes=0, **{name: h}, **sizes), INVALID, "workspace")
+
+
+@pytest.mark.parametrize("bwd", [False, True])
+def test_rotary_results_on_each_other(L, bwd):
+    for stride in ("clip", "token", "group", "head"):
+        for norm in (0, 1):
+            refused(L, rotary(L, bwd, y=heads(L, **{stride: 0}), clips=2, norm=norm), INVALID, "overlap")
+
+
 def rotary(L, bwd=False, x=None, y=None, dy=None, type=BF16, clips=1, tokens=3, groups=2, n=2, dim=64, pos=256, pos64=1,
            axes=2, cos=256, sin=256, positions=9, rot=64, inter=0, norm=1, w=256, b=256, pt=FP32, eps=1e-5, ws=256,
            nbytes=1 << 20):
