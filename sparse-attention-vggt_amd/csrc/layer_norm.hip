@@ -8,8 +8,8 @@
 // sums of its columns in registers while its work-group walks its rows, one work-group writes one partial row, and a
 // second kernel adds the partial rows in a fixed order (no atomics: equal inputs give equal bits). A lane reads eight
 // elements at a time, also where a row is not aligned to that or ends inside them.
-// Measured: 87936 rows of 1024, fp32 to bf16: forward 95 us for 540 MB (5.7 TB/s), backward 167 us for 900 MB (5.4
-// TB/s) and 5 us for the sums, what a copy of this size reaches; 4097 rows of 1027, fp32: 10 and 14 us (16 and 28 with
+// Measured: 87936 rows of 1024, fp32 to bf16: forward 95 us for 540 MB (5.7 TB/s), backward 156 us for 900 MB (5.8
+// TB/s) and 5 us for the sums, which a copy does not surpass; 4097 rows of 1027, fp32: 10 and 14 us (16 and 28 with
 // single elements).
 #include "row_ops.h"
 
@@ -261,10 +261,11 @@ static int ln_types(int x_type, int y_type, int param_type, F f) {
   return f(float(), float(), float());
 }
 
-// Work-groups of the backward pass: enough to fill the chip (1024: four a compute unit), few enough that the partial
-// rows they write are a small part of the rows they read (at least eight rows each).
+// Work-groups of the backward pass: two a compute unit, which all run at once at any width, with at least eight rows each,
+// so that the partial rows they write are a small part of the rows they read. (Backward and sums, 87936 rows of 1024 and
+// 10408 of 1536: 161 and 29 us; with one a compute unit 189 and 41, with three 167 and 28, with four 169 and 32.)
 static int64_t ln_parts(int64_t rows, int rows_per_step) {
-  return std::max<int64_t>(1, std::min<int64_t>(1024, rows / (rows_per_step > 8 ? rows_per_step : 8)));
+  return std::max<int64_t>(1, std::min<int64_t>(512, rows / (rows_per_step > 8 ? rows_per_step : 8)));
 }
 
 }  // namespace saf3r
