@@ -574,7 +574,7 @@ int saf3r_head_rotary_bwd(const saf3r_heads* dy, const saf3r_heads* x, int type,
                           const void* weight, int param_type, float eps, const saf3r_heads* dx, void* dweight,
                           void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Workspace bytes of saf3r_head_rotary_bwd (at most 8 * 2048 * dim), -1 for sizes that it rejects. */
+/* Workspace bytes of saf3r_head_rotary_bwd (at most 8 * 768 * dim), -1 for sizes that it rejects. */
 int64_t saf3r_head_rotary_bwd_workspace_bytes(int64_t clips, int tokens, int groups, int heads, int dim);
 
 /*

@@ -15,8 +15,8 @@
 // the table lines, and the next tokens' rows are on their way while the current ones are used. The partial sums of
 // the work-groups are added by a second kernel in a fixed order. Without the norm the backward pass is the inverse
 // rotation, the forward kernel's.
-// Measured, bf16, q and k of 21984 tokens of 16 heads of 64: forward 38 us for 180 MB (4.8 TB/s), backward 67 us for
-// 270 MB (4.0 TB/s) and 5 us for the sums; with one row at a time and no read ahead the backward took 113 us. 1041
+// Measured, bf16, q and k of 21984 tokens of 16 heads of 64: forward 31 us for 180 MB (5.8 TB/s), backward 54 us for
+// 270 MB (5.0 TB/s) and 5 us for the sums; with one row at a time and no read ahead the backward took 113 us. 1041
 // tokens: 6 us.
 #include "row_ops.h"
 
@@ -84,18 +84,13 @@ __device__ inline RotLane rot_lane(const RotParams& p, int t) {
   return r;
 }
 
-// Rotates the lane's pairs by the table row at `at`; sign -1: the inverse.
+// Rotates the lane's pairs by the cosines c and sines s of their angles.
 template <int VE>
-__device__ __forceinline__ void rotate(const RotParams& p, int64_t at, float sign, float (&u)[VE], float (&v)[VE]) {
+__device__ __forceinline__ void rotate(const RotParams& p, const float (&c)[VE], const float (&s)[VE], float (&u)[VE],
+                                       float (&v)[VE]) {
   if (p.interleaved) {
     if constexpr (VE > 1) {
       // pairs lie side by side: VE / 2 of them in each vector, their angles consecutive over both
-      float c[VE], s[VE];
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        c[e] = p.cosine[at + e];
-        s[e] = sign * p.sine[at + e];
-      }
 #pragma unroll
       for (int e = 0; e < VE / 2; ++e) {
         const float a0 = u[2 * e], a1 = u[2 * e + 1], b0 = v[2 * e], b1 = v[2 * e + 1];
@@ -109,10 +104,9 @@ __device__ __forceinline__ void rotate(const RotParams& p, int64_t at, float sig
   }
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
-    const float c = p.cosine[at + e], s = sign * p.sine[at + e];
     const float a = u[e], b = v[e];
-    u[e] = a * c - b * s;
-    v[e] = b * c + a * s;
+    u[e] = a * c[e] - b * s[e];
+    v[e] = b * c[e] + a * s[e];
   }
 }
 
@@ -203,7 +197,15 @@ __global__ void __launch_bounds__(256) head_rotary_kernel(const RotParams p) {
     const RotRow<T, VE> r = next;
     if (unit + p.parts < p.units) next = fetch(unit + p.parts);
     const bool there = r.out != nullptr, turn = there && l.axis >= 0;
-    const int64_t at = turn ? rot_table(p, l, r.low, r.high) : 0;
+    float c[VE], sn[VE];  // read before they are needed: the row's statistics come first
+    if (turn) {
+      const int64_t at = rot_table(p, l, r.low, r.high);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        c[e] = p.cosine[at + e];
+        sn[e] = (BWD ? -1.f : p.sign) * p.sine[at + e];
+      }
+    }
     float u[VE], v[VE], du[VE], dv[VE];
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
@@ -236,13 +238,13 @@ __global__ void __launch_bounds__(256) head_rotary_kernel(const RotParams p) {
           v[e] = v[e] * rstd * wb[e] + bb[e];
         }
       }
-      if (turn) rotate<VE>(p, at, p.sign, u, v);
+      if (turn) rotate<VE>(p, c, sn, u, v);
       if (there) {
         store_vec<VE>(r.out + l.a, u);
         store_vec<VE>(r.out + l.b, v);
       }
     } else {
-      if (turn) rotate<VE>(p, at, -1.f, du, dv);
+      if (turn) rotate<VE>(p, c, sn, du, dv);
       float s1 = 0.f, s2 = 0.f;
 #pragma unroll
       for (int e = 0; e < VE; ++e) {  // (lanes without a row hold zeros in du, dv)
@@ -399,10 +401,11 @@ static int rot_units(const RotParams& p, int rows, int* per, int* blocks) {
   return (int)(*blocks > 1 ? (int64_t)p.n * *blocks : ceil_div(p.n, *per));
 }
 
-// Work-groups of a group: up to sixteen a compute unit. With partial sums at least four steps each (the sums are small
-// then next to the rows), up to eight a compute unit.
+// Work-groups of a group: as many as run at once, four a compute unit, or three in the backward pass with its sums, and
+// there at least four steps each (the sums are small then next to the rows). 21984 tokens, bf16, forward / backward: 31
+// and 54 us; with two to three a unit 32 and 57, with six 33 and 58, with sixteen and eight 36 and 62.
 static int64_t rot_parts(int64_t units, int groups, bool sums) {
-  const int64_t most = std::max<int64_t>(1, (sums ? 2048 : 4096) / groups);
+  const int64_t most = std::max<int64_t>(1, (sums ? 768 : 1024) / groups);
   return std::max<int64_t>(1, std::min<int64_t>(most, sums ? (units + 3) / 4 : units));
 }
 
