@@ -36,12 +36,25 @@ namespace saf3r {
 template <int N>
 using Int = std::integral_constant<int, N>;
 
-// Tokens of a staged tile: 64, or 32 for waves that walk alone (two buffers each: 64 KB a work-group, two of them on a
-// compute unit).
+// How the waves of a work-group share its rows and its walk (MODE):
+//   kTogether: four waves, 32 rows each, walk together; a tile is 64 tokens, staged for all of them in two buffers;
+//   kPairs:    two such groups of four waves own the same 128 rows, each walks every other tile (64 KB of buffers);
+//   4 or 8:    so many waves own the same 32 rows, and each walks its share of tiles of 32 tokens in two buffers of its own
+//              (64 or 128 KB).
+// What the groups or waves found is joined at the end.
 constexpr int kTile = 64;
 constexpr int kTileElems = kTile * kHeadDim;
-template <bool ALONE>
-constexpr int kTokens = ALONE ? 32 : kTile;
+constexpr int kTogether = 0, kPairs = 2;
+template <int MODE>
+constexpr bool kAlone = MODE > kPairs;
+template <int MODE>
+constexpr int kTokens = kAlone<MODE> ? 32 : kTile;
+template <int MODE>
+constexpr int kThreads = kAlone<MODE> ? 64 * MODE : MODE == kPairs ? 512 : 256;
+template <int MODE>
+constexpr int kRows = kAlone<MODE> ? 32 : 128;  // of a work-group
+template <int MODE>
+constexpr int kBuffers = kAlone<MODE> ? 2 * MODE : MODE == kPairs ? 4 : 2;
 constexpr int kFaClasses = 7;      // kinds of row tiles of a launch, see make_classes
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -228,7 +241,7 @@ struct Stager {
   bool wide;
 };
 
-template <bool ALONE>
+template <int MODE>
 __device__ __forceinline__ Stager stager(const __bf16* x, int64_t xs, const __bf16* y, int64_t ys, bool wide, int wave,
                                          int lane) {
   Stager s;
@@ -238,7 +251,7 @@ __device__ __forceinline__ Stager stager(const __bf16* x, int64_t xs, const __bf
   s.xs = xs;
   s.ys = ys;
   s.lane = lane;
-  s.row0 = ALONE ? 0 : wave * 16;
+  s.row0 = kAlone<MODE> ? 0 : (wave & 3) * 16;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int row = 8 * i + (lane >> 3), c = ((lane & 7) ^ swz_tile(row)) << 3;
@@ -248,12 +261,12 @@ __device__ __forceinline__ Stager stager(const __bf16* x, int64_t xs, const __bf
   return s;
 }
 
-template <bool ALONE>
+template <int MODE>
 __device__ __forceinline__ void stage(const Stager& s, int start, int end, const __bf16* xt, const __bf16* yt) {
   const uint32_t xl = lds_addr(xt) + s.row0 * 128, yl = lds_addr(yt) + s.row0 * 128;
-  const bool whole = start + kTokens<ALONE> <= end && !s.wide;
+  const bool whole = start + kTokens<MODE> <= end && !s.wide;
 #pragma unroll
-  for (int k = 0; k < (ALONE ? 2 : 1); ++k) {
+  for (int k = 0; k < (kAlone<MODE> ? 2 : 1); ++k) {
     if (whole) {
       const __bf16 *xb = s.x + (start + 16 * k) * s.xs, *yb = s.y + (start + 16 * k) * s.ys;
 #pragma unroll
@@ -277,16 +290,16 @@ __device__ __forceinline__ void stage(const Stager& s, int start, int end, const
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // Bits of a whole tile.
-template <bool ALONE>
-constexpr uint64_t kAllRows = ALONE ? 0xFFFFFFFFull : ~0ull;
+template <int MODE>
+constexpr uint64_t kAllRows = kAlone<MODE> ? 0xFFFFFFFFull : ~0ull;
 
 // Rows that are not there (bits) become zeros, so that what they hold stays out of every product. A wave clears what it
 // copied itself.
-template <bool ALONE>
+template <int MODE>
 __device__ __forceinline__ void clear_rows(const Stager& s, __bf16* xt, __bf16* yt, uint64_t bits) {
-  if (bits == kAllRows<ALONE>) return;
+  if (bits == kAllRows<MODE>) return;
 #pragma unroll
-  for (int i = 0; i < (ALONE ? 4 : 2); ++i) {
+  for (int i = 0; i < (kAlone<MODE> ? 4 : 2); ++i) {
     const int row = s.row0 + i * 8 + (s.lane >> 3);
     if (!((bits >> row) & 1)) {
       *reinterpret_cast<u32x4*>(xt + row * 64 + (s.lane & 7) * 8) = u32x4{};
@@ -295,64 +308,80 @@ __device__ __forceinline__ void clear_rows(const Stager& s, __bf16* xt, __bf16* 
   }
 }
 
-// The walk of a work-group over its ranges. Together (ALONE false): all waves use every tile, staged in two buffers with
-// one barrier a tile. Alone: wave w takes tiles w, w + 4, ... of 32 tokens in two buffers of its own, without barriers; the
-// callers add up what the four waves found. load(start, end) -> the lane's share of what belongs to a tile,
+// The walk of a work-group over its ranges. Together: the four waves of a group use each of its tiles, staged in two buffers with
+// one barrier a tile. Alone: wave w of n takes tiles w, w + n, ... of 32 tokens in two buffers of its own, without barriers; the
+// callers add up what the waves found. load(start, end) -> the lane's share of what belongs to a tile,
 // bits(share) -> the rows that are there, publish(share, buffer) before and tile(buffer, bits) with the rows in LDS.
-template <bool MASK, bool ALONE, typename Load, typename Bits, typename Publish, typename Tile>
-__device__ __forceinline__ void walk(const FaItem& it, const Stager& st, __bf16 (*lds)[2][kTokens<ALONE> * kHeadDim],
+template <bool MASK, int MODE, typename Load, typename Bits, typename Publish, typename Tile>
+__device__ __forceinline__ void walk(const FaItem& it, const Stager& st, __bf16 (*lds)[2][kTokens<MODE> * kHeadDim],
                                      int wave, bool active, Load load, Bits bits, Publish publish, Tile tile) {
-  constexpr int kN = kTokens<ALONE>;
+  constexpr int kN = kTokens<MODE>;
   const int na = tiles_of<kN>(it.a1 - it.a0), nw = na + tiles_of<kN>(it.b1 - it.b0);
   auto fetch = [&](int i, int buf) {
     int start, end;
     walk_tile<kN>(it, na, i, &start, &end);
     end = min(end, start + kN);
     const auto share = load(start, end);
-    stage<ALONE>(st, start, end, lds[buf][0], lds[buf][1]);
+    stage<MODE>(st, start, end, lds[buf][0], lds[buf][1]);
     return share;
   };
   if constexpr (MASK)
     if (!__syncthreads_or(active)) return;  // no row of its own: nothing to walk for
-  if constexpr (ALONE) {
+  if constexpr (kAlone<MODE>) {
     if (!active || wave >= nw) return;
     auto now = fetch(wave, 2 * wave), next = now;
-    if (wave + 4 < nw) next = fetch(wave + 4, 2 * wave + 1);
+    if (wave + MODE < nw) next = fetch(wave + MODE, 2 * wave + 1);
     int buf = 2 * wave;
-    for (int i = wave; i < nw; i += 4) {
-      if (i + 4 < nw)
+    for (int i = wave; i < nw; i += MODE) {
+      if (i + MODE < nw)
         wait_vm<8>();  // all but the next tile's copies
       else
         wait_vm<0>();
       const uint64_t there = bits(now);
-      if constexpr (MASK) clear_rows<true>(st, lds[buf][0], lds[buf][1], there);
+      if constexpr (MASK) clear_rows<MODE>(st, lds[buf][0], lds[buf][1], there);
       publish(now, buf);
       if (there) tile(buf, there);
       now = next;
       wait_lds();  // this tile's reads, before its buffer is filled again
-      if (i + 8 < nw) next = fetch(i + 8, buf);
+      if (i + 2 * MODE < nw) next = fetch(i + 2 * MODE, buf);
       buf ^= 1;
     }
   } else {
     if (nw == 0) return;
-    auto now = fetch(0, 0);
-    for (int i = 0; i < nw; ++i) {
-      const int buf = i & 1;
+    constexpr int kGroups = MODE == kPairs ? 2 : 1;
+    const int group = wave >> 2, buf0 = 2 * group;
+    auto now = fetch(min(group, nw - 1), buf0);
+    for (int i = group, step = 0; step * kGroups < nw; i += kGroups, ++step) {  // (groups step alike, to the last barrier)
+      const int buf = buf0 + (step & 1);
       const uint64_t there = bits(now);
       wait_vm<0>();
-      if constexpr (MASK) clear_rows<false>(st, lds[buf][0], lds[buf][1], there);
-      if (wave == 0) publish(now, buf);
+      if constexpr (MASK) clear_rows<MODE>(st, lds[buf][0], lds[buf][1], there);
+      if ((wave & 3) == 0) publish(now, buf);
       __syncthreads();
-      if (i + 1 < nw) now = fetch(i + 1, buf ^ 1);
-      if (active && there) tile(buf, there);  // (a tile without a row changes nothing)
+      if (i + kGroups < nw) now = fetch(i + kGroups, buf ^ 1);
+      if (active && there && i < nw) tile(buf, there);  // (a tile without a row changes nothing)
     }
   }
+}
+
+// kPairs: the second group leaves what it found for the first, which adds it up: N values a lane, at x + 64 n.
+__device__ __forceinline__ float* pair_slot(void* lds, int wave, int lane, int n) {
+  return reinterpret_cast<float*>(lds) + (wave & 3) * n * 64 + lane;
+}
+__device__ __forceinline__ void put_sums(float* at, const f32x16& x) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) at[64 * j] = x[j];
+}
+__device__ __forceinline__ void add_sums(const float* at, f32x16& x, float own = 1.f, float other = 1.f) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) x[j] = x[j] * own + at[64 * j] * other;
 }
 
 // What the waves of a work-group that walked alone have to add up: a 64 x 32 result (rows 32 dh + 8 (j / 4) + 4 h + j % 4
 // of lane % 32's column) a wave, in LDS rows of 33.
 constexpr int kPart = 64 * 33;
-static_assert(4 * (kPart + 64) * 4 <= 8 * 2 * kTokens<true> * kHeadDim * 2, "the parts of four waves in their buffers");
+static_assert(4 * 64 * 64 * 4 <= kBuffers<kPairs> * 2 * kTileElems * 2, "the second group's sums in the buffers");
+static_assert((kPart + 64) * 4 <= 2 * 2 * kTokens<4> * kHeadDim * 2, "a wave's part in its buffers");
 __device__ __forceinline__ void put_part(float* part, const f32x16 (&x)[2], int lane) {
 #pragma unroll
   for (int dh = 0; dh < 2; ++dh)
@@ -361,11 +390,25 @@ __device__ __forceinline__ void put_part(float* part, const f32x16 (&x)[2], int 
       part[(32 * dh + 8 * (j / 4) + 4 * (lane >> 5) + j % 4) * 33 + (lane & 31)] = x[dh][j];
 }
 
-__device__ __forceinline__ void store8(__bf16* at, const float (&x)[8]) {
-  bf16x8 v;
+// Joining: a thread of a work-group takes column tid % 32 and this many consecutive rows.
+template <int MODE>
+constexpr int kJoin = 64 * 32 / kThreads<MODE>;
+
+// The sum of a part's element over the waves, pairs first.
+template <int MODE>
+__device__ __forceinline__ float sum_waves(const float* x) {
+  float y = (x[0] + x[kPart]) + (x[2 * kPart] + x[3 * kPart]);
+  if constexpr (MODE == 8) y += (x[4 * kPart] + x[5 * kPart]) + (x[6 * kPart] + x[7 * kPart]);
+  return y;
+}
+
+template <int N>
+__device__ __forceinline__ void store_row(__bf16* at, const float (&x)[N]) {
+  typedef __bf16 vec __attribute__((ext_vector_type(N)));
+  vec v;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (__bf16)x[e];
-  *reinterpret_cast<bf16x8*>(at) = v;
+  for (int e = 0; e < N; ++e) v[e] = (__bf16)x[e];
+  *reinterpret_cast<vec*>(at) = v;
 }
 
 // A token of the mask (1 where there is none), or whether it lies in the range at all.
@@ -391,18 +434,17 @@ __device__ __forceinline__ void mask_scores(f32x16& s, uint64_t bits, int half, 
 // bf16 the probabilities, at the same relative precision for any m at or below the row's maximum).
 //
 // A wave owns 32 rows and three waves share a SIMD. (64 rows a wave, two waves: the same rate over long walks, 1.4
-// times the time over 522 tokens.) ALONE: the work-group's four waves own the same 32 rows and split the walk; their
-// sums are joined at the end.
+// times the time over 522 tokens.) The other modes join their sums at the end.
 // ---------------------------------------------------------------------------------------
-template <bool MASK, bool ALONE>
-__global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_fwd_kernel(const FaParams p) {
-  __shared__ __align__(16) __bf16 lds[ALONE ? 8 : 2][2][kTokens<ALONE> * kHeadDim];
-  constexpr int kH = kTokens<ALONE> / 32;
-  const FaItem it = fa_item(p, ALONE ? 32 : 128);
+template <bool MASK, int MODE>
+__global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether ? 3 : 2) frame_attn_fwd_kernel(const FaParams p) {
+  __shared__ __align__(16) __bf16 lds[kBuffers<MODE>][2][kTokens<MODE> * kHeadDim];
+  constexpr int kH = kTokens<MODE> / 32;
+  const FaItem it = fa_item(p, kRows<MODE>);
   const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6), h = lane >> 5;
   const FragAddr fa = frag_addr(lane);
   const uint8_t* mask = MASK ? p.mask + (int64_t)it.clip * p.N : nullptr;
-  const int first = it.row0 + (ALONE ? 0 : wave * 32), r = first + (lane & 31);
+  const int first = it.row0 + (kAlone<MODE> ? 0 : (wave & 3) * 32), r = first + (lane & 31);
   const bool valid = r < it.row_end && (!MASK || mask[r]), active = __any(valid);
 
   bf16x8 qf[4];
@@ -412,9 +454,9 @@ __global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_fwd_kernel(cons
   f32x16 o[2] = {};
   float m = -__builtin_inff(), l = 0.f;
 
-  const Stager st = stager<ALONE>(p.k.ptr + it.clip * p.k.clip + it.head * p.k.head, p.k.token,
+  const Stager st = stager<MODE>(p.k.ptr + it.clip * p.k.clip + it.head * p.k.head, p.k.token,
                                   p.v.ptr + it.clip * p.v.clip + it.head * p.v.head, p.v.token, p.wide, wave, lane);
-  walk<MASK, ALONE>(
+  walk<MASK, MODE>(
       it, st, lds, wave, active, [&](int start, int end) { return mask_byte<MASK>(mask, start, end); },
       [](uint8_t b) { return __ballot(b != 0); }, [](uint8_t, int) {},
       [&](int buf, uint64_t bits) {
@@ -424,7 +466,7 @@ __global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_fwd_kernel(cons
         for (int kh = 0; kh < kH; ++kh)
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) s[kh] = mma(row_frag(kt, fa, kh, ks), qf[ks], ks ? s[kh] : f32x16{});
-        if (bits != kAllRows<ALONE>) {
+        if (bits != kAllRows<MODE>) {
 #pragma unroll
           for (int kh = 0; kh < kH; ++kh) mask_scores(s[kh], bits, kh, h);
         }
@@ -473,11 +515,29 @@ __global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_fwd_kernel(cons
         }
       });
 
+  if constexpr (MODE == kPairs) {
+    float* at = pair_slot(lds, wave, lane, 34);
+    __syncthreads();
+    if (wave >= 4) {
+      put_sums(at, o[0]);
+      put_sums(at + 64 * 16, o[1]);
+      at[64 * 32] = m;
+      at[64 * 33] = l;
+    }
+    __syncthreads();
+    if (wave >= 4) return;
+    const float other = at[64 * 32], top = fmaxf(m, other), base = top == -__builtin_inff() ? 0.f : top;
+    const float fm = __builtin_amdgcn_exp2f(m - base), fo = __builtin_amdgcn_exp2f(other - base);
+    add_sums(at, o[0], fm, fo);
+    add_sums(at + 64 * 16, o[1], fm, fo);
+    l = l * fm + at[64 * 33] * fo;
+    m = top;
+  }
   const float sum = pair_sum(l);
   const int64_t stat = ((int64_t)it.clip * p.H + it.head) * p.N;
   __bf16* op = p.o.ptr + it.clip * p.o.clip + it.head * p.o.head;
   __bf16* rp = p.rest.ptr + it.clip * p.rest.clip + it.head * p.rest.head;
-  if constexpr (ALONE) {
+  if constexpr (kAlone<MODE>) {
     // joined: the largest reference, every wave's sums on its scale
     float* part = reinterpret_cast<float*>(lds);
     __syncthreads();
@@ -487,31 +547,32 @@ __global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_fwd_kernel(cons
       part[wave * (kPart + 64) + kPart + 32 + lane] = sum;
     }
     __syncthreads();
-    const int col = tid_x() & 31, d0 = (tid_x() >> 5) * 8, row = it.row0 + col;
+    constexpr int kN = kJoin<MODE>;
+    const int col = tid_x() & 31, d0 = (tid_x() >> 5) * kN, row = it.row0 + col;
     if (row >= it.row_end) return;
-    float mw[4], top = -__builtin_inff(), total = 0.f;
+    float mw[MODE], top = -__builtin_inff(), total = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < MODE; ++w) {
       mw[w] = part[w * (kPart + 64) + kPart + col];
       top = fmaxf(top, mw[w]);
     }
     const bool some = (!MASK || mask[row]) && top != -__builtin_inff();
-    float y[8] = {}, x[8];
+    float y[kN] = {}, x[kN];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < MODE; ++w) {
       const float f = some ? __builtin_amdgcn_exp2f(mw[w] - top) : 0.f;
       total += f * part[w * (kPart + 64) + kPart + 32 + col];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] += f * part[w * (kPart + 64) + (d0 + e) * 33 + col];
+      for (int e = 0; e < kN; ++e) y[e] += f * part[w * (kPart + 64) + (d0 + e) * 33 + col];
     }
     const float inv = some ? 1.f / total : 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < kN; ++e) {
       y[e] = some ? y[e] * inv : 0.f;
       x[e] = y[e] - (float)(__bf16)y[e];
     }
-    store8(op + row * p.o.token + d0, y);
-    if (p.rest.ptr) store8(rp + row * p.rest.token + d0, x);
+    store_row(op + row * p.o.token + d0, y);
+    if (p.rest.ptr) store_row(rp + row * p.rest.token + d0, x);
     if (d0 == 0) p.lse[stat + row] = some ? (top + __builtin_amdgcn_logf(total)) * kLn2 : -__builtin_inff();
   } else {
     if (r >= it.row_end) return;
@@ -540,18 +601,17 @@ __global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_fwd_kernel(cons
 // ---------------------------------------------------------------------------------------
 // Backward over queries: D and dQ. A wave owns 32 query rows as columns of S^T and dP^T = V dO^T;
 // dQ^T += K^T dS^T.
-// The sums of dP start at -D. Three waves a SIMD (64 rows a wave and two waves: the same rate). ALONE: as in the forward
-// pass.
+// The sums of dP start at -D. Three waves a SIMD (64 rows a wave and two waves: the same rate). 
 // ---------------------------------------------------------------------------------------
-template <bool MASK, bool ALONE>
-__global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_dq_kernel(const FaParams p) {
-  __shared__ __align__(16) __bf16 lds[ALONE ? 8 : 2][2][kTokens<ALONE> * kHeadDim];
-  const FaItem it = fa_item(p, ALONE ? 32 : 128);
+template <bool MASK, int MODE>
+__global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether ? 3 : 2) frame_attn_dq_kernel(const FaParams p) {
+  __shared__ __align__(16) __bf16 lds[kBuffers<MODE>][2][kTokens<MODE> * kHeadDim];
+  const FaItem it = fa_item(p, kRows<MODE>);
   const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6), h = lane >> 5;
   const FragAddr fa = frag_addr(lane);
   const uint8_t* mask = MASK ? p.mask + (int64_t)it.clip * p.N : nullptr;
   const int64_t stat = ((int64_t)it.clip * p.H + it.head) * p.N;
-  const int first = it.row0 + (ALONE ? 0 : wave * 32), r = first + (lane & 31);
+  const int first = it.row0 + (kAlone<MODE> ? 0 : (wave & 3) * 32), r = first + (lane & 31);
   const float ls = r < it.row_end ? p.lse[stat + r] : -__builtin_inff();
   const bool valid = ls != -__builtin_inff(), active = __any(valid);  // not: rows without a key, or not there
 
@@ -582,21 +642,21 @@ __global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_dq_kernel(const
       }
   }
   d = pair_sum(d);
-  if (h == 0 && r < it.row_end && (!ALONE || wave == 0)) p.delta[stat + r] = d;
+  if (h == 0 && r < it.row_end && wave < kRows<MODE> / 32) p.delta[stat + r] = d;
   const float lse2 = valid ? ls * kLog2e : __builtin_inff();
   f32x16 dq[2] = {}, from;  // from: where the sums of dP start
 #pragma unroll
   for (int j = 0; j < 16; ++j) from[j] = -d;
 
-  const Stager st = stager<ALONE>(p.k.ptr + it.clip * p.k.clip + it.head * p.k.head, p.k.token,
+  const Stager st = stager<MODE>(p.k.ptr + it.clip * p.k.clip + it.head * p.k.head, p.k.token,
                                   p.v.ptr + it.clip * p.v.clip + it.head * p.v.head, p.v.token, p.wide, wave, lane);
-  walk<MASK, ALONE>(
+  walk<MASK, MODE>(
       it, st, lds, wave, active, [&](int start, int end) { return mask_byte<MASK>(mask, start, end); },
       [](uint8_t b) { return __ballot(b != 0); }, [](uint8_t, int) {},
       [&](int buf, uint64_t bits) {
         const __bf16 *kt = lds[buf][0], *vt = lds[buf][1];
 #pragma unroll
-        for (int kh = 0; kh < kTokens<ALONE> / 32; ++kh) {
+        for (int kh = 0; kh < kTokens<MODE> / 32; ++kh) {
           if (!(uint32_t)(bits >> (32 * kh))) continue;
           f32x16 s, dp;
 #pragma unroll
@@ -604,7 +664,7 @@ __global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_dq_kernel(const
             s = mma(row_frag(kt, fa, kh, ks), qf[ks], ks ? s : f32x16{});
             dp = mma(row_frag(vt, fa, kh, ks), dof[ks], ks ? dp : from);
           }
-          if (bits != kAllRows<ALONE>) mask_scores(s, bits, kh, h);
+          if (bits != kAllRows<MODE>) mask_scores(s, bits, kh, h);
 #pragma unroll
           for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(s[j] * p.c - lse2) * dp[j];
 #pragma unroll
@@ -616,21 +676,31 @@ __global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_dq_kernel(const
         }
       });
 
+  if constexpr (MODE == kPairs) {
+    float* at = pair_slot(lds, wave, lane, 32);
+    __syncthreads();
+    if (wave >= 4) {
+      put_sums(at, dq[0]);
+      put_sums(at + 64 * 16, dq[1]);
+    }
+    __syncthreads();
+    if (wave >= 4) return;
+    add_sums(at, dq[0]);
+    add_sums(at + 64 * 16, dq[1]);
+  }
   __bf16* base = p.dq.ptr + it.clip * p.dq.clip + it.head * p.dq.head;
-  if constexpr (ALONE) {
+  if constexpr (kAlone<MODE>) {
     float* part = reinterpret_cast<float*>(lds);
     __syncthreads();
     put_part(part + wave * kPart, dq, lane);
     __syncthreads();
-    const int col = tid_x() & 31, d0 = (tid_x() >> 5) * 8, row = it.row0 + col;
+    constexpr int kN = kJoin<MODE>;
+    const int col = tid_x() & 31, d0 = (tid_x() >> 5) * kN, row = it.row0 + col;
     if (row >= it.row_end) return;
-    float y[8];
+    float y[kN];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float* x = part + (d0 + e) * 33 + col;
-      y[e] = ((x[0] + x[kPart]) + (x[2 * kPart] + x[3 * kPart])) * p.scale;
-    }
-    store8(base + row * p.dq.token + d0, y);
+    for (int e = 0; e < kN; ++e) y[e] = sum_waves<MODE>(part + (d0 + e) * 33 + col) * p.scale;
+    store_row(base + row * p.dq.token + d0, y);
   } else {
     if (r >= it.row_end) return;
     base += r * p.dq.token + 4 * h;
@@ -651,22 +721,22 @@ __global__ void __launch_bounds__(256, ALONE ? 2 : 3) frame_attn_dq_kernel(const
 // dV^T += dO^T P, dK^T += Q^T dS. The sums of S start at -lse / scale and those of dP at -D of their rows (from LDS); a
 // query that is not there starts at -inf, so that its probabilities are zero. Three waves a SIMD without a mask (four
 // registers spilled to hold them: 8 x 1374 frames 161 us against 174); with one, three spill too much (254 us against
-// 200 on the masked mix). ALONE: as in the forward pass.
+// 200 on the masked mix).
 // ---------------------------------------------------------------------------------------
 struct RowStats {
   float ls, dl;
 };
 
-template <bool MASK, bool ALONE>
-__global__ void __launch_bounds__(256, MASK || ALONE ? 2 : 3) frame_attn_dkv_short_kernel(const FaParams p) {
-  __shared__ __align__(16) __bf16 lds[ALONE ? 8 : 2][2][kTokens<ALONE> * kHeadDim];
-  __shared__ __align__(16) float stats[ALONE ? 8 : 2][2 * kTile];
-  const FaItem it = fa_item(p, ALONE ? 32 : 128);
+template <bool MASK, int MODE>
+__global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether && !MASK ? 3 : 2) frame_attn_dkv_short_kernel(const FaParams p) {
+  __shared__ __align__(16) __bf16 lds[kBuffers<MODE>][2][kTokens<MODE> * kHeadDim];
+  __shared__ __align__(16) float stats[kBuffers<MODE>][2 * kTile];
+  const FaItem it = fa_item(p, kRows<MODE>);
   const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6), h = lane >> 5;
   const FragAddr fa = frag_addr(lane);
   const uint8_t* mask = MASK ? p.mask + (int64_t)it.clip * p.N : nullptr;
   const int64_t stat = ((int64_t)it.clip * p.H + it.head) * p.N;
-  const int first = it.row0 + (ALONE ? 0 : wave * 32), r = first + (lane & 31);
+  const int first = it.row0 + (kAlone<MODE> ? 0 : (wave & 3) * 32), r = first + (lane & 31);
   const bool valid = r < it.row_end && (!MASK || mask[r]), active = __any(valid);
 
   bf16x8 kf[4], vf[4];
@@ -680,10 +750,10 @@ __global__ void __launch_bounds__(256, MASK || ALONE ? 2 : 3) frame_attn_dkv_sho
   f32x16 dk[2] = {}, dv[2] = {};
 
   const float inv_scale = 1.f / p.scale;
-  const Stager st = stager<ALONE>(p.q.ptr + it.clip * p.q.clip + it.head * p.q.head, p.q.token,
+  const Stager st = stager<MODE>(p.q.ptr + it.clip * p.q.clip + it.head * p.q.head, p.q.token,
                                   p.doo.ptr + it.clip * p.doo.clip + it.head * p.doo.head, p.doo.token, p.wide, wave,
                                   lane);
-  walk<MASK, ALONE>(
+  walk<MASK, MODE>(
       it, st, lds, wave, active,
       [&](int start, int end) {
         const int tok = start + lane;  // (end: at most the tile's)
@@ -701,7 +771,7 @@ __global__ void __launch_bounds__(256, MASK || ALONE ? 2 : 3) frame_attn_dkv_sho
       [&](int buf, uint64_t bits) {
         const __bf16 *qt = lds[buf][0], *dt = lds[buf][1];
 #pragma unroll
-        for (int qh = 0; qh < kTokens<ALONE> / 32; ++qh) {
+        for (int qh = 0; qh < kTokens<MODE> / 32; ++qh) {
           if (!(uint32_t)(bits >> (32 * qh))) continue;
           f32x16 s, dp;
 #pragma unroll
@@ -736,34 +806,50 @@ __global__ void __launch_bounds__(256, MASK || ALONE ? 2 : 3) frame_attn_dkv_sho
         }
       });
 
+  if constexpr (MODE == kPairs) {
+    float* at = pair_slot(lds, wave, lane, 64);
+    __syncthreads();
+    if (wave >= 4) {
+#pragma unroll
+      for (int dh = 0; dh < 2; ++dh) {
+        put_sums(at + 64 * 16 * dh, dk[dh]);
+        put_sums(at + 64 * 16 * (2 + dh), dv[dh]);
+      }
+    }
+    __syncthreads();
+    if (wave >= 4) return;
+#pragma unroll
+    for (int dh = 0; dh < 2; ++dh) {
+      add_sums(at + 64 * 16 * dh, dk[dh]);
+      add_sums(at + 64 * 16 * (2 + dh), dv[dh]);
+    }
+  }
   __bf16* dkp = p.dk.ptr + it.clip * p.dk.clip + it.head * p.dk.head;
   __bf16* dvp = p.dv.ptr + it.clip * p.dv.clip + it.head * p.dv.head;
-  if constexpr (ALONE) {
+  if constexpr (kAlone<MODE>) {
     float* part = reinterpret_cast<float*>(lds);
     __syncthreads();
-    const int col = tid_x() & 31, d0 = (tid_x() >> 5) * 8, row = it.row0 + col;
-    auto total = [&](const f32x16(&x)[2], float (&y)[8]) {  // (one result at a time: 34 KB of the 64)
+    constexpr int kN = kJoin<MODE>;
+    const int col = tid_x() & 31, d0 = (tid_x() >> 5) * kN, row = it.row0 + col;
+    auto total = [&](const f32x16(&x)[2], float (&y)[kN]) {  // (one result at a time: half the buffers hold it)
       put_part(part + wave * kPart, x, lane);
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float* at = part + (d0 + e) * 33 + col;
-        y[e] = (at[0] + at[kPart]) + (at[2 * kPart] + at[3 * kPart]);
-      }
+      for (int e = 0; e < kN; ++e) y[e] = sum_waves<MODE>(part + (d0 + e) * 33 + col);
       __syncthreads();
     };
-    float a[8], b[8];
+    float a[kN], b[kN];
     total(dk, a);
     total(dv, b);
     if (row >= it.row_end) return;
     const bool there = !MASK || mask[row];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < kN; ++e) {
       a[e] = there ? a[e] * p.scale : 0.f;
       b[e] = there ? b[e] : 0.f;
     }
-    store8(dkp + row * p.dk.token + d0, a);
-    store8(dvp + row * p.dv.token + d0, b);
+    store_row(dkp + row * p.dk.token + d0, a);
+    store_row(dvp + row * p.dv.token + d0, b);
   } else {
     if (r >= it.row_end) return;
     dkp += r * p.dk.token + 4 * h;
@@ -954,7 +1040,7 @@ __global__ void __launch_bounds__(256, 1) frame_attn_dkv_long_kernel(const FaPar
 
   const int na = tiles_of<kTile>(it.a1 - it.a0), nw = na + tiles_of<kTile>(it.b1 - it.b0);
   const float inv_scale = 1.f / p.scale;
-  const Stager st = stager<false>(qb, p.q.token, db, p.doo.token, p.wide, wave, lane);
+  const Stager st = stager<0>(qb, p.q.token, db, p.doo.token, p.wide, wave, lane);
   float ls = 0.f, dl = 0.f;
   auto load = [&](int i) {
     int start, end;
@@ -962,7 +1048,7 @@ __global__ void __launch_bounds__(256, 1) frame_attn_dkv_long_kernel(const FaPar
     const int tok = start + lane;
     ls = tok < end ? p.lse[stat + tok] : -__builtin_inff();
     dl = tok < end ? p.delta[stat + tok] : 0.f;
-    stage<false>(st, start, end, lds[i & 1][0], lds[i & 1][1]);
+    stage<0>(st, start, end, lds[i & 1][0], lds[i & 1][1]);
   };
   // tile i, loaded before, becomes readable; the other buffer is free from here on
   auto ready = [&](int i) {
@@ -1151,21 +1237,57 @@ static int fa_check(const char* who, FaParams* p, int clips, int frames, int tok
   return SAF3R_OK;
 }
 
-// Rows of a work-group, by the number of work-groups of 128 rows that a launch would have. Below half a one a compute
-// unit the four waves of a work-group share 32 rows and split the walk (16 dense heads, forward / dQ / dK and dV: 522
-// tokens, 80 work-groups, 10.6 / 13.9 / 12.9 us against 13.9 / 17.6 / 16.4; 1041 tokens, 144 work-groups, 21.8 / 29.0 /
-// 30.0 against 20.4 / 27.4 / 27.6).
+// The mode of a launch, by its work-groups of 128 rows and its longest walk; the figures are forward / dQ / dK and dV in
+// us, dense heads.
+// Below half a work-group a compute unit the waves walk alone (16 heads of 522 tokens, 80 work-groups: 10.6 / 13.9 / 12.9,
+// together 13.9 / 17.6 / 16.4; 16 of 800, 112: 13 / 17 / 17, in pairs 15 / 20 / 21; one of 16000, 125: 130 / 140 / 189, in
+// pairs 153 / 181 / 238; 16 of 1041, 144: 23 / 27 / 30, in pairs 18 / 24 / 26),
 constexpr int64_t kAloneBelow = 128;
+// eight of them where the work-groups of 32 rows all run at once like that, on long walks (8 heads of 1000 tokens: 10.8 /
+// 14.4 / 13.0, four waves 11.7 / 13.9 / 15.0; one of 4096: 19 / 24 / 28 and 26 / 29 / 38; 8 of 512: 7.9 / 11.7 / 9.4 and
+// 7.6 / 10.6 / 9.6).
+constexpr int64_t kEightUpTo = 256;
+constexpr int kEightFrom = 768;
+// Up to one work-group a compute unit, pairs of groups, on long walks (3 heads of 8192 tokens, 192 work-groups: 82 / 99 /
+// 127, together 109 / 133 / 200; 16 of 2048, 256: 29 / 36 / 42 and 34 / 42 / 58; 4 clips of 16 of 512: 13.9 / 18.3 / 19.1
+// and 14.7 / 18.1 / 21.0; 10 of 8 of 256: 10.0 / 13.2 / 11.7 and 9.8 / 12.4 / 12.7).
+constexpr int64_t kPairsUpTo = 256;
+constexpr int kPairsFrom = 512;
 // From here on the backward pass over keys takes 64 rows a wave (without a mask).
 constexpr int64_t kLongFrom = 1792;
 
-// f(whether there is a mask, whether the waves walk alone)
+// Tokens of the longest walk of a launch.
+static int fa_longest(const FaParams& p) {
+  int longest = 0;
+  for (const FaClass& c : p.cls)
+    longest = std::max(longest, c.walk == kAll ? p.N : c.walk == kFirstOwn ? 2 * p.T : c.walk == kNone ? 0 : p.T);
+  return longest;
+}
+
+// The mode of a launch and its classes; n: its work-groups.
+static int fa_mode(FaParams* p, const int32_t* patterns, int frames, bool keys, int64_t* n) {
+  *n = make_classes(p, patterns, frames, kRows<kTogether>, keys);
+  if (*n > kPairsUpTo) return kTogether;
+  if (*n >= kAloneBelow) return fa_longest(*p) >= kPairsFrom ? kPairs : kTogether;
+  *n = make_classes(p, patterns, frames, kRows<4>, keys);
+  return *n <= kEightUpTo && fa_longest(*p) >= kEightFrom ? 8 : 4;
+}
+
+// f(whether there is a mask, mode)
 template <typename F>
-static void fa_launch(bool mask, bool alone, F f) {
+static void fa_launch(bool mask, int mode, F f) {
+  auto with = [&](auto m) {
+    switch (mode) {
+      case 8: return f(m, Int<8>());
+      case 4: return f(m, Int<4>());
+      case kPairs: return f(m, Int<kPairs>());
+      default: return f(m, Int<kTogether>());
+    }
+  };
   if (mask)
-    alone ? f(std::true_type(), std::true_type()) : f(std::true_type(), std::false_type());
+    with(std::true_type());
   else
-    alone ? f(std::false_type(), std::true_type()) : f(std::false_type(), std::false_type());
+    with(std::false_type());
 }
 
 static int fa_grid(const char* who, int64_t total) {
@@ -1196,12 +1318,12 @@ extern "C" int saf3r_frame_attn_fwd(const saf3r_heads* q, const saf3r_heads* k, 
     return fail(SAF3R_ERR_INVALID, "%s: written rows overlap (a stride of zero)", who);
   p.lse = lse;
   p.wide = fa_wide(p.k) || fa_wide(p.v);
-  int64_t n = make_classes(&p, patterns, frames, 128, false);
-  const bool alone = n < kAloneBelow;
-  if (alone) n = make_classes(&p, patterns, frames, 32, false);
+  int64_t n;
+  const int mode = fa_mode(&p, patterns, frames, false, &n);
   if (int e = fa_grid(who, n)) return e;
-  fa_launch(token_mask != nullptr, alone, [&](auto m, auto a) {
-    hipLaunchKernelGGL((frame_attn_fwd_kernel<decltype(m)::value, decltype(a)::value>), dim3((uint32_t)n), dim3(256), 0,
+  fa_launch(token_mask != nullptr, mode, [&](auto m, auto d) {
+    constexpr int kMode = decltype(d)::value;
+    hipLaunchKernelGGL((frame_attn_fwd_kernel<decltype(m)::value, kMode>), dim3((uint32_t)n), dim3(kThreads<kMode>), 0,
                        (hipStream_t)stream, p);
   });
   return check_launch(who);
@@ -1246,23 +1368,23 @@ extern "C" int saf3r_frame_attn_bwd(const saf3r_heads* dout, const saf3r_heads* 
   p.wide = fa_wide(p.q) || fa_wide(p.k) || fa_wide(p.v) || fa_wide(p.doo);
   FaParams pk = p;
   const bool masked = token_mask != nullptr;
-  int64_t n = make_classes(&p, patterns, frames, 128, false);
-  const bool alone = n < kAloneBelow;
-  if (alone) n = make_classes(&p, patterns, frames, 32, false);
-  int64_t nk = make_classes(&pk, patterns, frames, 128, true);
-  const bool alone_k = nk < kAloneBelow, long_k = !masked && nk >= kLongFrom;
-  if (alone_k || long_k) nk = make_classes(&pk, patterns, frames, alone_k ? 32 : 256, true);
+  int64_t n, nk;
+  const int mode = fa_mode(&p, patterns, frames, false, &n), mode_k = fa_mode(&pk, patterns, frames, true, &nk);
+  const bool long_k = !masked && nk >= kLongFrom;
+  if (long_k) nk = make_classes(&pk, patterns, frames, 256, true);
   if (int e = fa_grid(who, std::max(n, nk))) return e;
   const hipStream_t s = (hipStream_t)stream;
-  const dim3 gk((uint32_t)nk), block(256);
-  fa_launch(masked, alone, [&](auto m, auto a) {
-    hipLaunchKernelGGL((frame_attn_dq_kernel<decltype(m)::value, decltype(a)::value>), dim3((uint32_t)n), block, 0, s, p);
+  const dim3 gk((uint32_t)nk);
+  fa_launch(masked, mode, [&](auto m, auto d) {
+    constexpr int kMode = decltype(d)::value;
+    hipLaunchKernelGGL((frame_attn_dq_kernel<decltype(m)::value, kMode>), dim3((uint32_t)n), dim3(kThreads<kMode>), 0, s, p);
   });
-  fa_launch(masked, alone_k, [&](auto m, auto a) {
-    if (long_k)
-      hipLaunchKernelGGL(frame_attn_dkv_long_kernel, gk, block, 0, s, pk);
-    else
-      hipLaunchKernelGGL((frame_attn_dkv_short_kernel<decltype(m)::value, decltype(a)::value>), gk, block, 0, s, pk);
-  });
+  if (long_k)
+    hipLaunchKernelGGL(frame_attn_dkv_long_kernel, gk, dim3(256), 0, s, pk);
+  else
+    fa_launch(masked, mode_k, [&](auto m, auto d) {
+      constexpr int kMode = decltype(d)::value;
+      hipLaunchKernelGGL((frame_attn_dkv_short_kernel<decltype(m)::value, kMode>), gk, dim3(kThreads<kMode>), 0, s, pk);
+    });
   return check_launch(who);
 }

@@ -329,3 +329,31 @@ def test_launches_of_many_rows(ops, pattern, B, F, T, H):
                 assert (err <= tol).all(), (name, b, h, float((err / tol).max()))
             want, tol = ref["lse"]
             assert ((lse[b:b + 1, h:h + 1].double().cpu() - want).abs() <= tol)[torch.isfinite(want)].all()
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("pattern,B,F,T,H", [
+    # eight waves share 32 rows and walk alone
+    ("dense", 1, 1, 769, 1), ("mix", 1, 2, 500, 5), ("anchor_local", 1, 3, 600, 2), ("dense", 2, 1, 1031, 3),
+    # two groups of four waves share 128 rows
+    ("dense", 1, 1, 1050, 15), ("mix", 2, 3, 450, 10), ("anchor_local", 3, 2, 270, 11), ("dense", 8, 1, 513, 4)])
+def test_shared_walks(ops, pattern, B, F, T, H, masked):
+    """Launches of few rows and long walks, which waves or groups of waves share: odd numbers of tiles, second ranges, tiles
+    that a mask empties, and a group that finds nothing."""
+    N = F * T
+    q, k, v, do = inputs(B, N, H, T + H, 3.0)
+    mask = None
+    if masked:
+        g = torch.Generator().manual_seed(T)
+        mask = torch.rand(B, N, generator=g) < 0.7
+        mask[0, 64:256] = False
+        mask[-1, N // 2:] = False
+        if B > 1:
+            mask[1] = False
+            mask[1, 70] = True  # (one key: every other share of the walk is empty)
+        for i, t in enumerate((q, k, v, do)):
+            t[~mask] = (math.nan, math.inf, -math.inf, math.nan)[i]
+    got = check(ops, q, k, v, do, patterns_of(ops, pattern, H), F, mask)
+    if masked:
+        for n in ("out", "dq", "dk", "dv"):
+            assert (got[n].cpu()[~mask] == 0).all(), n
