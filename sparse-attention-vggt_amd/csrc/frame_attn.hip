@@ -144,7 +144,7 @@ __device__ inline FaItem fa_item(const FaParams& p, int rows) {
 }
 
 template <int TOKENS>
-__device__ inline int tiles_of(int n) {
+__host__ __device__ inline int tiles_of(int n) {
   return (n + TOKENS - 1) / TOKENS;
 }
 
@@ -1253,8 +1253,6 @@ constexpr int kEightFrom = 768;
 // and 14.7 / 18.1 / 21.0; 10 of 8 of 256: 10.0 / 13.2 / 11.7 and 9.8 / 12.4 / 12.7).
 constexpr int64_t kPairsUpTo = 256;
 constexpr int kPairsFrom = 512;
-// From here on the backward pass over keys takes 64 rows a wave (without a mask).
-constexpr int64_t kLongFrom = 1792;
 
 // Tokens of the longest walk of a launch.
 static int fa_longest(const FaParams& p) {
@@ -1262,6 +1260,17 @@ static int fa_longest(const FaParams& p) {
   for (const FaClass& c : p.cls)
     longest = std::max(longest, c.walk == kAll ? p.N : c.walk == kFirstOwn ? 2 * p.T : c.walk == kNone ? 0 : p.T);
   return longest;
+}
+
+// Whether the backward pass over keys takes 64 rows a wave (without a mask, for launches of more than kPairsUpTo
+// work-groups n of 128 rows; n256: work-groups of 256). Those run one a compute unit, in rounds of 256 that take 7 units of
+// time a walked tile where 256 work-groups of 128 rows take 4, and start and end without another to fill the time, about
+// five tiles. (16 dense heads, long and short in us: 2050 tokens, 1 round against 2, 64 and 75; 4096, 1 and 2, 133 and 155;
+// 6144, 2 and 3, 330 and 307; 7168, 2 and 4, 386 and 473; 10240, 3 and 5, 810 and 816; 12288, 3 and 6, 1021 and 1145;
+// 20 frames of 1374, 8 and 14, 411 and 365; 8 of them, 3 and 6, 151 and 147; 60 of 250, 4 and 8, 72 and 61.)
+static bool fa_takes_long(int64_t n, int64_t n256, int longest) {
+  const int64_t tiles = tiles_of<kTile>(longest);
+  return 7 * ceil_div(n256, 256) * (tiles + 5) <= 4 * ceil_div(n, 256) * (tiles + 1);
 }
 
 // The mode of a launch and its classes; n: its work-groups.
@@ -1370,8 +1379,16 @@ extern "C" int saf3r_frame_attn_bwd(const saf3r_heads* dout, const saf3r_heads* 
   const bool masked = token_mask != nullptr;
   int64_t n, nk;
   const int mode = fa_mode(&p, patterns, frames, false, &n), mode_k = fa_mode(&pk, patterns, frames, true, &nk);
-  const bool long_k = !masked && nk >= kLongFrom;
-  if (long_k) nk = make_classes(&pk, patterns, frames, 256, true);
+  bool long_k = false;
+  if (!masked && nk > kPairsUpTo) {
+    FaParams wide = pk;
+    const int64_t n256 = make_classes(&wide, patterns, frames, 256, true);
+    long_k = fa_takes_long(nk, n256, fa_longest(wide));
+    if (long_k) {
+      pk = wide;
+      nk = n256;
+    }
+  }
   if (int e = fa_grid(who, std::max(n, nk))) return e;
   const hipStream_t s = (hipStream_t)stream;
   const dim3 gk((uint32_t)nk);
