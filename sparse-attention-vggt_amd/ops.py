@@ -906,9 +906,10 @@ def frame_topk_scores(scores: torch.Tensor, frames: int, per_frame: int, topk: i
 STATIC_PATTERNS = (DENSE, FRAME_LOCAL, ANCHOR_LOCAL, ANCHOR, SKIP)  # patterns of frame_attn_fwd / frame_attn_bwd
 
 
-def _elsewhere(t: torch.Tensor) -> bool:
-    """Whether ``t`` lies on another device than the current one (whose current stream takes the launches)."""
-    return t.device.index != torch.cuda.current_device()
+# The calls below are short: of a launch of one small layer, most is spent here and not on the GPU. So each fact is looked up
+# once, and results like one that is there are made like it.
+_here = torch._C._cuda_getDevice  # index of the current device
+_stream = torch._C._cuda_getCurrentRawStream  # of a device index
 
 
 def _readable(t: torch.Tensor, step: int) -> torch.Tensor:
@@ -939,7 +940,7 @@ def _frame_heads(t: torch.Tensor, copy: bool = True) -> _lib.Heads | None:
 
 
 def _frame_like(name: str, t: torch.Tensor, q: torch.Tensor) -> None:
-    if t.shape != q.shape or t.dtype != torch.bfloat16 or t.device != q.device:
+    if t.shape != q.shape or t.dtype != torch.bfloat16 or t.get_device() != q.get_device():
         raise ValueError(f"{name} must be bfloat16 {tuple(q.shape)} on {q.device}, got {t.dtype} {tuple(t.shape)} on "
                          f"{t.device}")
 
@@ -948,14 +949,14 @@ def _frame_args(q, k, v, patterns, frames: int, token_mask, scale):
     """Checks shared by the attention's two directions: (patterns as a host array, mask or None, scale)."""
     if not (q.is_cuda and k.is_cuda and v.is_cuda and (token_mask is None or token_mask.is_cuda)):
         raise ValueError("saf3r kernels take GPU tensors")
-    shape = q.shape
+    shape, dev = q.shape, q.get_device()
     if len(shape) != 4 or shape[3] != HEAD_DIM:
         raise ValueError(f"q must be [clips, tokens, heads, {HEAD_DIM}], got {tuple(shape)}")
     if k.shape != shape or v.shape != shape:
         name, t = ("k", k) if k.shape != shape else ("v", v)
         raise ValueError(f"{name} must have q's shape {tuple(shape)}, got {tuple(t.shape)}")
     for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dtype != torch.bfloat16 or t.device != q.device:
+        if t.dtype != torch.bfloat16 or t.get_device() != dev:
             raise ValueError(f"{name} must be bfloat16 on {q.device}, got {t.dtype} on {t.device}")
     B, N, H, _ = shape
     if frames < 1 or N < 1 or N % frames:
@@ -965,7 +966,7 @@ def _frame_args(q, k, v, patterns, frames: int, token_mask, scale):
     if token_mask is not None:
         if token_mask.dtype not in (torch.bool, torch.uint8) or tuple(token_mask.shape) != (B, N):
             raise ValueError(f"token_mask must be bool [{B}, {N}], got {token_mask.dtype} {tuple(token_mask.shape)}")
-        if token_mask.device != q.device:
+        if token_mask.get_device() != dev:
             raise ValueError(f"token_mask is on {token_mask.device}, q on {q.device}")
         token_mask = token_mask.contiguous()
     return _i32_array(patterns), token_mask, _FRAME_SCALE if scale is None else float(scale)
@@ -985,18 +986,18 @@ def frame_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, patterns: 
     holds what its rounding took away, for the backward pass. Not differentiable by itself: see
     ``autograd.frame_attention``."""
     pat, mask, fscale = _frame_args(q, k, v, patterns, frames, token_mask, scale)
-    if _elsewhere(q):
+    dev = q.get_device()
+    if dev != _here():
         with torch.cuda.device(q.device):
             return frame_attn_fwd(q, k, v, patterns, frames, token_mask, scale, rest)
     B, N, H, _ = q.shape
     out = q.new_empty(q.shape)
-    low = q.new_empty(q.shape) if rest else None
+    low = torch.empty_like(out) if rest else None
     lse = q.new_empty((B, H, N), dtype=torch.float32)
     hq, hk, hv, ho = _frame_heads(q), _frame_heads(k), _frame_heads(v), _frame_heads(out)
     _mark("frame_attn_fwd", "start")
     _lib.check(_lib.load().saf3r_frame_attn_fwd(hq, hk, hv, B, frames, N // frames, H, pat, _ptr(mask), fscale, ho,
-                                                _frame_heads(low) if rest else None, lse.data_ptr(),
-                                                _lib.stream_ptr()))
+                                                _frame_heads(low) if rest else None, lse.data_ptr(), _stream(dev)))
     _mark("frame_attn_fwd", "end")
     return (out, lse, low) if rest else (out, lse)
 
@@ -1016,14 +1017,16 @@ def frame_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
     _frame_like("out", out, q)
     if rest is not None:
         _frame_like("rest", rest, q)
-    if tuple(lse.shape) != (B, H, N) or lse.dtype != torch.float32 or lse.device != q.device:
+    if lse.shape != (B, H, N) or lse.dtype != torch.float32 or lse.get_device() != q.get_device():
         raise ValueError(f"lse must be float32 {(B, H, N)} on {q.device}, got {lse.dtype} {tuple(lse.shape)}")
-    if _elsewhere(q):
+    dev = q.get_device()
+    if dev != _here():
         with torch.cuda.device(q.device):
             return frame_attn_bwd(dout, q, k, v, out, lse, patterns, frames, token_mask, scale, rest, grads)
     lse = lse.contiguous()
     if grads is None:
-        grads = (q.new_empty(q.shape), q.new_empty(q.shape), q.new_empty(q.shape))
+        dq = q.new_empty(q.shape)
+        grads = (dq, torch.empty_like(dq), torch.empty_like(dq))
     else:
         grads = tuple(grads)
         if len(grads) != 3:
@@ -1033,12 +1036,12 @@ def frame_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
     into = [_frame_heads(t, copy=False) for t in grads]
     if None in into:
         raise ValueError("grads need 16-byte aligned rows with strides a multiple of 8")
-    ws = q.new_empty((B, H, N), dtype=torch.float32)  # (saf3r_frame_attn_bwd_workspace_bytes)
+    ws = torch.empty_like(lse)  # (saf3r_frame_attn_bwd_workspace_bytes)
     held = (_frame_heads(dout), _frame_heads(q), _frame_heads(k), _frame_heads(v), _frame_heads(out),
             None if rest is None else _frame_heads(rest))
     _mark("frame_attn_bwd", "start")
     _lib.check(_lib.load().saf3r_frame_attn_bwd(*held, lse.data_ptr(), B, frames, N // frames, H, pat, _ptr(mask), fscale,
-                                                *into, ws.data_ptr(), ws.numel() * 4, _lib.stream_ptr()))
+                                                *into, ws.data_ptr(), ws.numel() * 4, _stream(dev)))
     _mark("frame_attn_bwd", "end")
     return grads
 
@@ -1057,30 +1060,27 @@ def _dtype(name: str, t: torch.Tensor) -> int:
 def _norm_params(shape: tuple, rows: torch.Tensor, rows_dtype, weight, bias=None):
     """(dtype of the parameters, type the kernels read them in, weight, bias): weight and bias of one type and of
     ``shape``, contiguous. Parameters that are neither fp32 nor of the rows' 16-bit type are read as fp32 copies."""
-    kind = None
+    if weight is None and bias is None:
+        return torch.float32, torch.float32, None, None
+    kind, dev = (bias if weight is None else weight).dtype, rows.get_device()
     for n, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
         if t.shape != shape:
             raise ValueError(f"{n} must be {tuple(shape)}, got {tuple(t.shape)}")
-        if t.device != rows.device:
+        if t.get_device() != dev:
             raise ValueError(f"{n} is on {t.device}, the rows on {rows.device}")
-        _dtype(n, t)
-        if kind is not None and t.dtype != kind:
+        if t.dtype != kind:
             raise ValueError("weight and bias must have one dtype")
-        kind = t.dtype
-    kind = torch.float32 if kind is None else kind
-    read = torch.float32
     if kind != torch.float32:
-        if kind == rows_dtype:
-            read = kind
-        else:
+        _dtype("weight and bias", bias if weight is None else weight)
+        if kind != rows_dtype:
             weight, bias = (None if t is None else t.float() for t in (weight, bias))
     if weight is not None and not weight.is_contiguous():
         weight = weight.contiguous()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    return kind, read, weight, bias
+    return kind, kind if kind == rows_dtype else torch.float32, weight, bias
 
 
 def _flat_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -1099,8 +1099,8 @@ def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     """LayerNorm over the last dimension (1 .. 8192 wide, ``saf3r_layer_norm_fwd``): (y, mean, rstd), the statistics
     fp32 of x's leading shape, for ``layer_norm_bwd``. x fp32, bf16 or fp16; y in x's type, or for fp32 x in
     ``out_dtype`` (fp32 arithmetic, rounded once). Not differentiable by itself: see ``autograd.layer_norm``."""
-    _need_cuda(x, weight, bias)
-    shape, dt = x.shape, x.dtype
+    _need_cuda(x)
+    shape, dt, dev = x.shape, x.dtype, x.get_device()
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"x must have a last dimension, got {tuple(shape)}")
     xt = _dtype("x", x)
@@ -1108,19 +1108,30 @@ def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     if out_dtype != dt and (dt != torch.float32 or out_dtype not in _DTYPES):
         raise ValueError(f"{dt} rows give {dt} rows, not {out_dtype}")
     _, read, w, b = _norm_params(shape[-1:], x, out_dtype, weight, bias)
-    if _elsewhere(x):
+    if dev != _here():
         with torch.cuda.device(x.device):
             return layer_norm_fwd(x, weight, bias, eps, out_dtype)
     dim = shape[-1]
     rows, stride = _flat_rows(x)
     y = x.new_empty(shape, dtype=out_dtype)
-    mean, rstd = x.new_empty(shape[:-1], dtype=torch.float32), x.new_empty(shape[:-1], dtype=torch.float32)
+    mean = x.new_empty(shape[:-1], dtype=torch.float32)
+    rstd = torch.empty_like(mean)
     _mark("layer_norm_fwd", "start")
     _lib.check(_lib.load().saf3r_layer_norm_fwd(rows.data_ptr(), stride, xt, mean.numel(), dim, _ptr(w), _ptr(b),
                                                 _DTYPES[read], eps, y.data_ptr(), dim, _DTYPES[out_dtype],
-                                                mean.data_ptr(), rstd.data_ptr(), _lib.stream_ptr()))
+                                                mean.data_ptr(), rstd.data_ptr(), _stream(dev)))
     _mark("layer_norm_fwd", "end")
     return y, mean, rstd
+
+
+def _param_grads(x: torch.Tensor, shape: tuple, dtype, need, workspace_bytes):
+    """(dweight, dbias, workspace, its bytes): None and 0 where they are not needed."""
+    if not (need[0] or need[1]):
+        return None, None, None, 0
+    dw = x.new_empty(shape, dtype=dtype) if need[0] else None
+    db = None if not need[1] else x.new_empty(shape, dtype=dtype) if dw is None else torch.empty_like(dw)
+    nbytes = workspace_bytes()
+    return dw, db, x.new_empty(max(nbytes, 0), dtype=torch.uint8), nbytes
 
 
 def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
@@ -1128,16 +1139,18 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: 
     """Gradients (dx, dweight, dbias) of ``layer_norm_fwd`` (``saf3r_layer_norm_bwd``) from ``dy`` (y's shape and
     type); ``mean`` and ``rstd`` are its results. dweight / dbias are None where ``need_params`` says so, else of
     weight's type (fp32 without a weight). Equal inputs give equal bits."""
-    _need_cuda(dy, x, mean, rstd, weight)
+    _need_cuda(x, dy)
     xt, yt = _dtype("x", x), _dtype("dy", dy)
-    shape = x.shape
-    if dy.shape != shape or dy.device != x.device or len(shape) < 1 or shape[-1] < 1:
+    shape, dev = x.shape, x.get_device()
+    if dy.shape != shape or dy.get_device() != dev or len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"dy must be like x {tuple(shape)} on {x.device}, got {tuple(dy.shape)} on {dy.device}")
+    stats = shape[:-1]
     for n, t in (("mean", mean), ("rstd", rstd)):
-        if t.shape != shape[:-1] or t.dtype != torch.float32 or t.device != x.device:
-            raise ValueError(f"{n} must be float32 {tuple(shape[:-1])}, got {t.dtype} {tuple(t.shape)}")
+        if t.shape != stats or t.dtype != torch.float32 or t.get_device() != dev:
+            raise ValueError(f"{n} must be float32 {tuple(stats)} on {x.device}, got {t.dtype} {tuple(t.shape)} on "
+                             f"{t.device}")
     kind, read, w, _ = _norm_params(shape[-1:], x, dy.dtype, weight)
-    if _elsewhere(x):
+    if dev != _here():
         with torch.cuda.device(x.device):
             return layer_norm_bwd(dy, x, mean, rstd, weight, need_params)
     dim = shape[-1]
@@ -1146,15 +1159,12 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: 
     drows, dstride = _flat_rows(dy)
     mean, rstd = mean.contiguous(), rstd.contiguous()
     dx = x.new_empty(shape)
-    dw, db = (x.new_empty(shape[-1:], dtype=read) if need else None for need in need_params)
-    nbytes, ws = 0, None
-    if dw is not None or db is not None:
-        nbytes = lib.saf3r_layer_norm_bwd_workspace_bytes(mean.numel(), dim)
-        ws = x.new_empty(max(nbytes, 0), dtype=torch.uint8)
+    dw, db, ws, nbytes = _param_grads(x, shape[-1:], read, need_params,
+                                      lambda: lib.saf3r_layer_norm_bwd_workspace_bytes(mean.numel(), dim))
     _mark("layer_norm_bwd", "start")
     _lib.check(lib.saf3r_layer_norm_bwd(drows.data_ptr(), dstride, yt, rows.data_ptr(), stride, xt, mean.numel(), dim,
                                         mean.data_ptr(), rstd.data_ptr(), _ptr(w), _DTYPES[read], dx.data_ptr(), dim,
-                                        _ptr(dw), _ptr(db), _ptr(ws), nbytes, _lib.stream_ptr()))
+                                        _ptr(dw), _ptr(db), _ptr(ws), nbytes, _stream(dev)))
     _mark("layer_norm_bwd", "end")
     if kind != read:
         dw, db = (None if t is None else t.to(kind) for t in (dw, db))
@@ -1202,7 +1212,6 @@ def _rotary_args(x, pos, tables, layout: str, rotary_dim: int | None, norm: bool
         return None, 0, 1, None, None, 0, 0
     B, N, _, _, D = x.shape
     cos, sin = tables
-    _need_cuda(pos, cos, sin)
     if pos.dim() != 3 or pos.shape[:2] != x.shape[:2] or not 1 <= pos.shape[2] <= 8:
         raise ValueError(f"pos must be [{B}, {N}, axes] with 1 to 8 axes, got {tuple(pos.shape)}")
     if pos.dtype != torch.int64 and pos.dtype != torch.int32:
@@ -1217,9 +1226,9 @@ def _rotary_args(x, pos, tables, layout: str, rotary_dim: int | None, norm: bool
     positions = cos.shape[0]
     if positions < 1:
         raise ValueError("the tables hold no position")
-    dev = x.device
-    if pos.device != dev or cos.device != dev or sin.device != dev:
-        raise ValueError(f"pos and the tables must be on {dev}, got {pos.device}, {cos.device} and {sin.device}")
+    dev = x.get_device()
+    if pos.get_device() != dev or cos.get_device() != dev or sin.get_device() != dev:
+        raise ValueError(f"pos and the tables must be on {x.device}, got {pos.device}, {cos.device} and {sin.device}")
     return pos.contiguous(), int(pos.dtype == torch.int64), axes, cos.contiguous(), sin.contiguous(), positions, R
 
 
@@ -1246,12 +1255,12 @@ def head_rotary_fwd(x: torch.Tensor, pos: torch.Tensor | None = None, tables=Non
     section) (``layout`` "half") or (2 j, 2 j + 1) ("interleaved"); positions outside the tables are taken to their
     ends. Returns a contiguous tensor of x's shape and type. Not differentiable by itself: see
     ``autograd.head_rotary``."""
-    _need_cuda(x, weight, bias)
-    xt = _dtype("x", x)
+    _need_cuda(x)
+    xt, dev = _dtype("x", x), x.get_device()
     p, pos64, axes, cos, sin, positions, R = _rotary_args(x, pos, tables, layout, rotary_dim, norm, weight, bias)
     B, N, G, H, D = x.shape
     _, read, w, b = _norm_params((G, D), x, x.dtype, weight, bias)
-    if _elsewhere(x):
+    if dev != _here():
         with torch.cuda.device(x.device):
             return head_rotary_fwd(x, pos, tables, layout, rotary_dim, norm, weight, bias, eps)
     y = x.new_empty(x.shape)
@@ -1259,7 +1268,7 @@ def head_rotary_fwd(x: torch.Tensor, pos: torch.Tensor | None = None, tables=Non
     _mark("head_rotary_fwd", "start")
     _lib.check(_lib.load().saf3r_head_rotary_fwd(
         hx, xt, B, N, G, H, D, _ptr(p), pos64, axes, _ptr(cos), _ptr(sin), positions, R, layout == "interleaved",
-        bool(norm), _ptr(w), _ptr(b), _DTYPES[read], eps, hy, _lib.stream_ptr()))
+        bool(norm), _ptr(w), _ptr(b), _DTYPES[read], eps, hy, _stream(dev)))
     _mark("head_rotary_fwd", "end")
     return y
 
@@ -1272,31 +1281,29 @@ def head_rotary_bwd(dy: torch.Tensor, x: torch.Tensor, pos: torch.Tensor | None 
     type), the other arguments those of that call. dweight / dbias [groups, dim] are None without a norm or where
     ``need_params`` says so, else of weight's type (fp32 without a weight). ``out`` (optional) receives dx: a tensor or
     view like x with consecutive elements in a row, not overlapping the inputs. Equal inputs give equal bits."""
-    _need_cuda(dy, x, weight, out)
-    xt = _dtype("x", x)
+    _need_cuda(x, dy)
+    xt, dev = _dtype("x", x), x.get_device()
     p, pos64, axes, cos, sin, positions, R = _rotary_args(x, pos, tables, layout, rotary_dim, norm, weight, None)
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
-        raise ValueError(f"dy must be like x: {x.dtype} {tuple(x.shape)}, got {dy.dtype} {tuple(dy.shape)}")
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.get_device() != dev:
+        raise ValueError(f"dy must be like x: {x.dtype} {tuple(x.shape)} on {x.device}, got {dy.dtype} {tuple(dy.shape)} on "
+                         f"{dy.device}")
     B, N, G, H, D = x.shape
     kind, read, w, _ = _norm_params((G, D), x, x.dtype, weight)
-    if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != x.device
+    if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.get_device() != dev
                             or (D > 1 and out.stride(4) != 1)):
         raise ValueError(f"out must be like x: {x.dtype} {tuple(x.shape)} with consecutive elements in a row")
-    if _elsewhere(x):
+    if dev != _here():
         with torch.cuda.device(x.device):
             return head_rotary_bwd(dy, x, pos, tables, layout, rotary_dim, norm, weight, eps, need_params, out)
     lib = _lib.load()
     dx = x.new_empty(x.shape) if out is None else out
-    dw, db = (x.new_empty((G, D), dtype=read) if need and norm else None for need in need_params)
-    nbytes, ws = 0, None
-    if dw is not None or db is not None:
-        nbytes = lib.saf3r_head_rotary_bwd_workspace_bytes(B, N, G, H, D)
-        ws = x.new_empty(max(nbytes, 0), dtype=torch.uint8)
+    dw, db, ws, nbytes = _param_grads(x, (G, D), read, need_params if norm else (False, False),
+                                      lambda: lib.saf3r_head_rotary_bwd_workspace_bytes(B, N, G, H, D))
     hdy, hx, hdx = _group_heads(dy), _group_heads(x), _group_heads(dx)
     _mark("head_rotary_bwd", "start")
     _lib.check(lib.saf3r_head_rotary_bwd(
         hdy, hx, xt, B, N, G, H, D, _ptr(p), pos64, axes, _ptr(cos), _ptr(sin), positions, R, layout == "interleaved",
-        bool(norm), _ptr(w), _DTYPES[read], eps, hdx, _ptr(dw), _ptr(db), _ptr(ws), nbytes, _lib.stream_ptr()))
+        bool(norm), _ptr(w), _DTYPES[read], eps, hdx, _ptr(dw), _ptr(db), _ptr(ws), nbytes, _stream(dev)))
     _mark("head_rotary_bwd", "end")
     if kind != read:
         dw, db = (None if t is None else t.to(kind) for t in (dw, db))
