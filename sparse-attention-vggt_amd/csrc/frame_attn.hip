@@ -308,32 +308,88 @@ __device__ __forceinline__ void clear_rows(const Stager& s, __bf16* xt, __bf16* 
   }
 }
 
+// The tiles of a walk that hold a token which is there, in order. Whether 64 tiles hold one is found at once, a tile a lane
+// (a tile that its range cuts off counts without a look).
+template <bool MASK, int MODE>
+struct Tiles {
+  const FaItem& it;
+  const uint8_t* mask;
+  int na, nw, base;
+  uint64_t some;  // of the tiles base .. base + 63
+
+  __device__ Tiles(const FaItem& item, const uint8_t* m) : it(item), mask(m), base(0), some(0) {
+    na = tiles_of<kTokens<MODE>>(it.a1 - it.a0);
+    nw = na + tiles_of<kTokens<MODE>>(it.b1 - it.b0);
+    if constexpr (MASK) look(0);
+  }
+
+  __device__ void look(int first) {
+    base = first;
+    const int i = first + (int)(tid_x() & 63);
+    bool any = false;
+    if (i < nw) {
+      int start, end;
+      walk_tile<kTokens<MODE>>(it, na, i, &start, &end);
+      any = start + kTokens<MODE> > end;
+      if (!any) {
+        typedef u32x4 bytes __attribute__((aligned(1)));
+        u32x4 x{};
+#pragma unroll
+        for (int c = 0; c < kTokens<MODE>; c += 16) x |= *reinterpret_cast<const bytes*>(mask + start + c);
+        any = (x[0] | x[1] | x[2] | x[3]) != 0;
+      }
+    }
+    some = __ballot(any);
+  }
+
+  // The n-th tile behind tile i that holds one, nw behind the last.
+  __device__ int after(int i, int n) {
+    if constexpr (!MASK) return min(i + n, nw);
+    while (true) {
+      const int at = i + 1 - base;
+      const uint64_t left = at < 64 ? some >> at : 0;
+      if (left) {
+        i += 1 + __builtin_ctzll(left);
+        if (--n == 0) return i;
+      } else {
+        i = base + 63;
+        if (i + 1 >= nw) return nw;
+        look(i + 1);
+      }
+    }
+  }
+};
+
 // The walk of a work-group over its ranges. Together: the four waves of a group use each of its tiles, staged in two buffers with
-// one barrier a tile. Alone: wave w of n takes tiles w, w + n, ... of 32 tokens in two buffers of its own, without barriers; the
-// callers add up what the waves found. load(start, end) -> the lane's share of what belongs to a tile,
+// one barrier a tile. Alone: wave w of n takes the tiles w, w + n, ... (of those that hold a token) in two buffers of its own,
+// without barriers; the callers add up what the waves found. load(start, end) -> the lane's share of what belongs to a tile,
 // bits(share) -> the rows that are there, publish(share, buffer) before and tile(buffer, bits) with the rows in LDS.
 template <bool MASK, int MODE, typename Load, typename Bits, typename Publish, typename Tile>
-__device__ __forceinline__ void walk(const FaItem& it, const Stager& st, __bf16 (*lds)[2][kTokens<MODE> * kHeadDim],
-                                     int wave, bool active, Load load, Bits bits, Publish publish, Tile tile) {
+__device__ __forceinline__ void walk(const FaItem& it, const Stager& st, const uint8_t* mask,
+                                     __bf16 (*lds)[2][kTokens<MODE> * kHeadDim], int wave, bool active, Load load,
+                                     Bits bits, Publish publish, Tile tile) {
   constexpr int kN = kTokens<MODE>;
-  const int na = tiles_of<kN>(it.a1 - it.a0), nw = na + tiles_of<kN>(it.b1 - it.b0);
+  if constexpr (MASK)
+    if (!__syncthreads_or(active)) return;  // no row of its own: nothing to walk for
+  Tiles<MASK, MODE> tiles(it, mask);
+  const int nw = tiles.nw;
   auto fetch = [&](int i, int buf) {
     int start, end;
-    walk_tile<kN>(it, na, i, &start, &end);
+    walk_tile<kN>(it, tiles.na, i, &start, &end);
     end = min(end, start + kN);
     const auto share = load(start, end);
     stage<MODE>(st, start, end, lds[buf][0], lds[buf][1]);
     return share;
   };
-  if constexpr (MASK)
-    if (!__syncthreads_or(active)) return;  // no row of its own: nothing to walk for
   if constexpr (kAlone<MODE>) {
-    if (!active || wave >= nw) return;
-    auto now = fetch(wave, 2 * wave), next = now;
-    if (wave + MODE < nw) next = fetch(wave + MODE, 2 * wave + 1);
-    int buf = 2 * wave;
-    for (int i = wave; i < nw; i += MODE) {
-      if (i + MODE < nw)
+    if (!active) return;
+    int i = tiles.after(-1, wave + 1);
+    if (i >= nw) return;
+    int buf = 2 * wave, behind = tiles.after(i, MODE);
+    auto now = fetch(i, buf), next = now;
+    if (behind < nw) next = fetch(behind, buf + 1);
+    while (true) {
+      if (behind < nw)
         wait_vm<8>();  // all but the next tile's copies
       else
         wait_vm<0>();
@@ -341,25 +397,49 @@ __device__ __forceinline__ void walk(const FaItem& it, const Stager& st, __bf16 
       if constexpr (MASK) clear_rows<MODE>(st, lds[buf][0], lds[buf][1], there);
       publish(now, buf);
       if (there) tile(buf, there);
+      i = behind;
+      if (i >= nw) return;
+      behind = tiles.after(i, MODE);
       now = next;
       wait_lds();  // this tile's reads, before its buffer is filled again
-      if (i + 2 * MODE < nw) next = fetch(i + 2 * MODE, buf);
+      if (behind < nw) next = fetch(behind, buf);
       buf ^= 1;
     }
-  } else {
+  } else if constexpr (!MASK) {  // (every tile: the same loop with less to decide, 150 us in place of 175 in dK and dV)
     if (nw == 0) return;
     constexpr int kGroups = MODE == kPairs ? 2 : 1;
     const int group = wave >> 2, buf0 = 2 * group;
     auto now = fetch(min(group, nw - 1), buf0);
-    for (int i = group, step = 0; step * kGroups < nw; i += kGroups, ++step) {  // (groups step alike, to the last barrier)
+    for (int i = group, step = 0; step * kGroups < nw; i += kGroups, ++step) {
       const int buf = buf0 + (step & 1);
       const uint64_t there = bits(now);
       wait_vm<0>();
-      if constexpr (MASK) clear_rows<MODE>(st, lds[buf][0], lds[buf][1], there);
       if ((wave & 3) == 0) publish(now, buf);
       __syncthreads();
       if (i + kGroups < nw) now = fetch(i + kGroups, buf ^ 1);
-      if (active && there && i < nw) tile(buf, there);  // (a tile without a row changes nothing)
+      if (active && there && i < nw) tile(buf, there);
+    }
+  } else {
+    // first: the tile of the first group, own: of the wave's group (all groups step alike, to the last barrier)
+    int first = tiles.after(-1, 1), last = MODE == kPairs ? tiles.after(first, 1) : first;
+    if (first >= nw) return;
+    const int group = MODE == kPairs ? wave >> 2 : 0;
+    int own = group ? last : first;
+    const int buf0 = 2 * group;
+    auto now = fetch(min(own, nw - 1), buf0);
+    for (int step = 0; first < nw; ++step) {
+      const int buf = buf0 + (step & 1);
+      const bool has = MODE != kPairs || own < nw;
+      const uint64_t there = bits(now);
+      wait_vm<0>();
+      clear_rows<MODE>(st, lds[buf][0], lds[buf][1], there);
+      if ((wave & 3) == 0) publish(now, buf);
+      __syncthreads();
+      first = tiles.after(last, 1);
+      last = MODE == kPairs ? tiles.after(first, 1) : first;
+      own = group ? last : first;
+      if (own < nw) now = fetch(own, buf ^ 1);
+      if (active && there && has) tile(buf, there);  // (a tile without a row changes nothing)
     }
   }
 }
@@ -457,7 +537,7 @@ __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether ? 3 : 2) fra
   const Stager st = stager<MODE>(p.k.ptr + it.clip * p.k.clip + it.head * p.k.head, p.k.token,
                                   p.v.ptr + it.clip * p.v.clip + it.head * p.v.head, p.v.token, p.wide, wave, lane);
   walk<MASK, MODE>(
-      it, st, lds, wave, active, [&](int start, int end) { return mask_byte<MASK>(mask, start, end); },
+      it, st, mask, lds, wave, active, [&](int start, int end) { return mask_byte<MASK>(mask, start, end); },
       [](uint8_t b) { return __ballot(b != 0); }, [](uint8_t, int) {},
       [&](int buf, uint64_t bits) {
         const __bf16 *kt = lds[buf][0], *vt = lds[buf][1];
@@ -651,7 +731,7 @@ __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether ? 3 : 2) fra
   const Stager st = stager<MODE>(p.k.ptr + it.clip * p.k.clip + it.head * p.k.head, p.k.token,
                                   p.v.ptr + it.clip * p.v.clip + it.head * p.v.head, p.v.token, p.wide, wave, lane);
   walk<MASK, MODE>(
-      it, st, lds, wave, active, [&](int start, int end) { return mask_byte<MASK>(mask, start, end); },
+      it, st, mask, lds, wave, active, [&](int start, int end) { return mask_byte<MASK>(mask, start, end); },
       [](uint8_t b) { return __ballot(b != 0); }, [](uint8_t, int) {},
       [&](int buf, uint64_t bits) {
         const __bf16 *kt = lds[buf][0], *vt = lds[buf][1];
@@ -754,7 +834,7 @@ __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether && !MASK ? 3
                                   p.doo.ptr + it.clip * p.doo.clip + it.head * p.doo.head, p.doo.token, p.wide, wave,
                                   lane);
   walk<MASK, MODE>(
-      it, st, lds, wave, active,
+      it, st, mask, lds, wave, active,
       [&](int start, int end) {
         const int tok = start + lane;  // (end: at most the tile's)
         RowStats x;
