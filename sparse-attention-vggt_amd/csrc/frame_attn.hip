@@ -1330,34 +1330,49 @@ constexpr int64_t kEightUpTo = 256;
 constexpr int kEightFrom = 768;
 // Up to one work-group a compute unit, pairs of groups, on long walks (3 heads of 8192 tokens, 192 work-groups: 82 / 99 /
 // 127, together 109 / 133 / 200; 16 of 2048, 256: 29 / 36 / 42 and 34 / 42 / 58; 4 clips of 16 of 512: 13.9 / 18.3 / 19.1
-// and 14.7 / 18.1 / 21.0; 10 of 8 of 256: 10.0 / 13.2 / 11.7 and 9.8 / 12.4 / 12.7).
+// and 14.7 / 18.1 / 21.0; 10 of 8 of 256: 10.0 / 13.2 / 11.7 and 9.8 / 12.4 / 12.7). Shorter walks count by their share of the
+// longest: few long ones bound a launch, whatever runs beside them (2 clips of 32 x 77 tokens, 2 heads dense, 5 local, 9
+// on the first frame: 32 / 39 / 44 and 41 / 50 / 68; 2 of 22 x 269, 1, 6 and 9: 91 / 116 / 133 and 93 / 114 / 165).
 constexpr int64_t kPairsUpTo = 256;
 constexpr int kPairsFrom = 512;
 
-// Tokens of the longest walk of a launch.
+// Tokens that a work-group of a class walks, and the most of a launch.
+static int fa_walked(const FaParams& p, const FaClass& c) {
+  return c.walk == kAll ? p.N : c.walk == kFirstOwn ? 2 * p.T : c.walk == kNone ? 0 : p.T;
+}
 static int fa_longest(const FaParams& p) {
   int longest = 0;
-  for (const FaClass& c : p.cls)
-    longest = std::max(longest, c.walk == kAll ? p.N : c.walk == kFirstOwn ? 2 * p.T : c.walk == kNone ? 0 : p.T);
+  for (const FaClass& c : p.cls) longest = std::max(longest, fa_walked(p, c));
   return longest;
 }
 
-// Whether the backward pass over keys takes 64 rows a wave (without a mask, for launches of more than kPairsUpTo
-// work-groups n of 128 rows; n256: work-groups of 256). Those run one a compute unit, in rounds of 256 that take 7 units of
-// time a walked tile where 256 work-groups of 128 rows take 4, and start and end without another to fill the time, about
-// five tiles. (16 dense heads, long and short in us: 2050 tokens, 1 round against 2, 64 and 75; 4096, 1 and 2, 133 and 155;
-// 6144, 2 and 3, 330 and 307; 7168, 2 and 4, 386 and 473; 10240, 3 and 5, 810 and 816; 12288, 3 and 6, 1021 and 1145;
-// 20 frames of 1374, 8 and 14, 411 and 365; 8 of them, 3 and 6, 151 and 147; 60 of 250, 4 and 8, 72 and 61.)
-static bool fa_takes_long(int64_t n, int64_t n256, int longest) {
+// The n work-groups of a launch as so many of its longest walk (in tiles, one more for the rest of a work-group).
+static int64_t fa_load(const FaParams& p, int64_t n) {
+  const int64_t longest = tiles_of<kTile>(fa_longest(p)) + 1;
+  int64_t tiles = 0;
+  for (int i = 0; i < kFaClasses; ++i) {
+    const int64_t end = i + 1 < kFaClasses ? std::min<int64_t>(p.cls[i + 1].start, n) : n;
+    const int64_t walk = tiles_of<kTile>(fa_walked(p, p.cls[i])) + 1;
+    tiles += std::max<int64_t>(0, end - p.cls[i].start) * walk;
+  }
+  return ceil_div(tiles, longest);
+}
+
+// Whether the backward pass over keys takes 64 rows a wave (without a mask, where groups walk together): `load` and
+// `load256` of its launches of 128 and 256 rows a work-group. The wide ones run one a compute unit, in rounds of 256 that
+// take 7 units of time a walked tile where 256 work-groups of 128 rows take 4, and start and end without another to fill the
+// time, about five tiles. (16 dense heads, long and short in us: 2050 tokens, 1 round against 2, 64 and 75; 4096, 1 and 2,
+// 133 and 155; 6144, 2 and 3, 330 and 307; 7168, 2 and 4, 386 and 473; 10240, 3 and 5, 810 and 816; 12288, 3 and 6, 1021
+// and 1145; 20 frames of 1374, 8 and 14, 411 and 365; 8 of them, 3 and 6, 151 and 147; 60 of 250, 4 and 8, 72 and 61.)
+static bool fa_takes_long(int64_t load, int64_t load256, int longest) {
   const int64_t tiles = tiles_of<kTile>(longest);
-  return 7 * ceil_div(n256, 256) * (tiles + 5) <= 4 * ceil_div(n, 256) * (tiles + 1);
+  return 7 * ceil_div(load256, 256) * (tiles + 5) <= 4 * ceil_div(load, 256) * (tiles + 1);
 }
 
 // The mode of a launch and its classes; n: its work-groups.
 static int fa_mode(FaParams* p, const int32_t* patterns, int frames, bool keys, int64_t* n) {
   *n = make_classes(p, patterns, frames, kRows<kTogether>, keys);
-  if (*n > kPairsUpTo) return kTogether;
-  if (*n >= kAloneBelow) return fa_longest(*p) >= kPairsFrom ? kPairs : kTogether;
+  if (*n >= kAloneBelow) return fa_load(*p, *n) <= kPairsUpTo && fa_longest(*p) >= kPairsFrom ? kPairs : kTogether;
   *n = make_classes(p, patterns, frames, kRows<4>, keys);
   return *n <= kEightUpTo && fa_longest(*p) >= kEightFrom ? 8 : 4;
 }
@@ -1460,10 +1475,10 @@ extern "C" int saf3r_frame_attn_bwd(const saf3r_heads* dout, const saf3r_heads* 
   int64_t n, nk;
   const int mode = fa_mode(&p, patterns, frames, false, &n), mode_k = fa_mode(&pk, patterns, frames, true, &nk);
   bool long_k = false;
-  if (!masked && nk > kPairsUpTo) {
+  if (!masked && mode_k == kTogether) {
     FaParams wide = pk;
     const int64_t n256 = make_classes(&wide, patterns, frames, 256, true);
-    long_k = fa_takes_long(nk, n256, fa_longest(wide));
+    long_k = fa_takes_long(fa_load(pk, nk), fa_load(wide, n256), fa_longest(wide));
     if (long_k) {
       pk = wide;
       nk = n256;
