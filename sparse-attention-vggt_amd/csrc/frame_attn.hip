@@ -7,12 +7,12 @@
 //   D = sum_d dO O,  dP = dO V^T,  dS = P (dP - D),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO
 //
 // Every pattern gives a query tile (or, in the backward pass over keys, a key tile) at most two ranges of
-// consecutive tokens on the other side: all, the first frame, the own frame. A work-group of four waves owns a
-// tile of rows and walks the other side in tiles of 64 tokens that all its waves read from LDS (two buffers, the
-// next tile copied by LDS-DMA while the current one is used). Matrix products are v_mfma_f32_32x32x16_bf16 and none of their results crosses lanes: a
-// product whose rows are summed over next (P, dS) leaves its 32x32 result with one column per lane and the rows
-// 8 (i / 4) + 4 (lane / 32) + i % 4, and the other operand of the next product is read from LDS with the
-// transposing read in that same row order (two groups of four rows per 16).
+// consecutive tokens on the other side: all, the first frame, the own frame. A work-group owns a tile of rows and walks
+// the other side in tiles of tokens read from LDS (two buffers, the next tile copied by LDS-DMA while the current one is
+// used); launches of few rows share the walk among more waves (see the modes below). Matrix products are
+// v_mfma_f32_32x32x16_bf16 and none of their results crosses lanes: a product whose rows are summed over next (P, dS)
+// leaves its 32x32 result with one column per lane and the rows 8 (i / 4) + 4 (lane / 32) + i % 4, and the other operand
+// of the next product is read from LDS with the transposing read in that same row order (two groups of four rows per 16).
 //
 // The probabilities and dS are rounded to bf16 as operands of the second product, which is what the matrix
 // cores take; everything else (S, dP, the statistics, all sums) is fp32.
@@ -514,7 +514,11 @@ __device__ __forceinline__ void mask_scores(f32x16& s, uint64_t bits, int half, 
 // bf16 the probabilities, at the same relative precision for any m at or below the row's maximum).
 //
 // A wave owns 32 rows and three waves share a SIMD. (64 rows a wave, two waves: the same rate over long walks, 1.4
-// times the time over 522 tokens.) The other modes join their sums at the end.
+// times the time over 522 tokens.) The modes that share a walk join their sums at the end.
+//
+// Bound by the issue of vector instructions: fma, exponential, add and half a conversion an element against 16 matrix
+// products a tile. 12 frames of 1374 tokens, 10 of 16 heads dense: 870 us, 849 TFLOP/s of the pairs (1357 is what a
+// large matrix product reaches here); 8 x 1374 frames 101 us; 522 tokens 11 us.
 // ---------------------------------------------------------------------------------------
 template <bool MASK, int MODE>
 __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether ? 3 : 2) frame_attn_fwd_kernel(const FaParams p) {
@@ -681,7 +685,10 @@ __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether ? 3 : 2) fra
 // ---------------------------------------------------------------------------------------
 // Backward over queries: D and dQ. A wave owns 32 query rows as columns of S^T and dP^T = V dO^T;
 // dQ^T += K^T dS^T.
-// The sums of dP start at -D. Three waves a SIMD (64 rows a wave and two waves: the same rate). 
+// The sums of dP start at -D. Three waves a SIMD (64 rows a wave and two waves: the same rate).
+//
+// Matrix and vector pipes are about equally busy (24 products a tile against fma, exponential, product and half a
+// conversion an element): 12 frames of 1374, 10 of 16 heads dense 1120 us, 990 TFLOP/s; 8 x 1374 frames 120 us.
 // ---------------------------------------------------------------------------------------
 template <bool MASK, int MODE>
 __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether ? 3 : 2) frame_attn_dq_kernel(const FaParams p) {
@@ -801,7 +808,7 @@ __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether ? 3 : 2) fra
 // dV^T += dO^T P, dK^T += Q^T dS. The sums of S start at -lse / scale and those of dP at -D of their rows (from LDS); a
 // query that is not there starts at -inf, so that its probabilities are zero. Three waves a SIMD without a mask (four
 // registers spilled to hold them: 8 x 1374 frames 161 us against 174); with one, three spill too much (254 us against
-// 200 on the masked mix).
+// 200 on the masked mix). 32 products a tile: 8 x 1374 frames 150 us, 825 TFLOP/s of the pairs.
 // ---------------------------------------------------------------------------------------
 struct RowStats {
   float ls, dl;
@@ -958,7 +965,10 @@ __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether && !MASK ? 3
 // its own matrix products and vector work: a half tile (32 queries) is 32 products in a fixed order, with the
 // exponentials and roundings of one group placed behind the products of the other (32 cycles each, room for seven
 // vector instructions) and the LDS reads a phase ahead. (Compiler's order, two-phase loop: 686 TFLOP/s over 12 frames
-// of 1374 tokens, 16 heads.)
+// of 1374 tokens, 16 heads.) 12 frames of 1374, 10 of 16 heads dense: 1310 us, 1130 TFLOP/s of the pairs.
+//
+// The products are inline assembly, for which the compiler keeps no distance to the instructions that read their results:
+// nothing but this order may touch them, so the kernel must not spill (tests/test_frame_attn_build.py).
 // ---------------------------------------------------------------------------------------
 struct DkvRows {
   bf16x8 q[4], d[4];  // row operands of Q and dO
