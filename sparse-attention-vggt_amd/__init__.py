@@ -8,8 +8,10 @@ Layers
 ``patch``   plugin surface of the reference (``patch_model``, ``update_args_per_forward``,
             ``HeadwiseSparseAttentionWrapper``), driving the kernels below.
 ``ops``     torch-facing wrappers of the C ABI in ``include/saf3r_hip.h``.
+``autograd`` differentiable forms of the training kernels (attention over frames, head norm and rotary
+            positions, LayerNorm).
 ``csrc``    gfx950 HIP kernels (prologue, block pooling / selection, block-sparse MFMA attention,
-            gather attention, per-frame token top-k) built into ``libsaf3r_hip.so``.
+            gather attention, per-frame token top-k, the training operators) built into ``libsaf3r_hip.so``.
 ``synth``   seeded synthetic workloads of the benchmark configurations.
 ``vggt``    the VGGT global-attention module shape (``Attention`` with qkv / q_norm / k_norm /
             rope / proj) used when no host model is supplied.
