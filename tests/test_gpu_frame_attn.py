@@ -358,3 +358,93 @@ def test_shared_walks(ops, pattern, B, F, T, H, masked):
     if masked:
         for n in ("out", "dq", "dk", "dv"):
             assert (got[n].cpu()[~mask] == 0).all(), n
+
+
+@pytest.mark.parametrize("N,H", [(5000, 1), (11000, 1), (9001, 3), (8400, 16)])
+def test_long_masked_walks(ops, N, H):
+    """Walks of more tiles than are looked at at once, with stretches of padding longer than that: sampled heads against
+    64 bits on the GPU, in every way that a launch shares its walks."""
+    q, k, v, do = (t.to(DEV) for t in inputs(1, N, H, N))
+    mask = torch.rand(1, N, generator=torch.Generator().manual_seed(N)) < 0.8
+    mask[0, 40: N // 2 + 77] = False
+    mask[0, N - 333:] = False
+    mask = mask.to(DEV)
+    for t, bad in zip((q, k, v, do), (math.nan, math.inf, -math.inf, math.nan)):
+        t[~mask] = bad
+    pat = [ops.DENSE] * H
+    out, lse, rest = ops.frame_attn_fwd(q, k, v, pat, token_mask=mask, rest=True)
+    grads = ops.frame_attn_bwd(do, q, k, v, out, lse, pat, token_mask=mask, rest=rest)
+    for t in (out, *grads):
+        assert (t[~mask] == 0).all()
+    assert (lse.transpose(1, 2)[~mask] == -math.inf).all()
+    for h in sorted({0, H - 1}):
+        Q, K, V, G = (t[0, mask[0], h].double() for t in (q, k, v, do))
+        s = Q @ K.t().contiguous() * 0.125
+        L = torch.logsumexp(s, -1)
+        p = torch.exp(s - L[:, None])
+        o = p @ V
+        ds = p * (G @ V.t().contiguous() - (G * o).sum(-1, keepdim=True)) * 0.125
+        assert (lse[0, h, mask[0]].double() - L).abs().max() < 1e-5 * L.abs().max()
+        for name, t, w in (("out", out, o), ("dq", grads[0], ds @ K), ("dk", grads[1], ds.t().contiguous() @ Q),
+                           ("dv", grads[2], p.t().contiguous() @ G)):
+            rel = float((t[0, mask[0], h].double() - w).norm() / w.norm())
+            # a result's rounding and its operands' (P, dS, D), each at most U of magnitudes that add in quadrature
+            assert rel < 2 * R.U, (name, h, rel)
+
+
+@pytest.mark.parametrize("pattern,B,F,T,H", [("mix", 1, 2, 40, 64), ("mix", 1, 300, 1, 5), ("anchor_local", 2, 50, 7, 3),
+                                             ("mix", 5, 1, 1, 64)])
+def test_many_heads_and_small_frames(ops, pattern, B, F, T, H):
+    q, k, v, do = inputs(B, F * T, H, H + T)
+    check(ops, q, k, v, do, patterns_of(ops, pattern, H), F)
+
+
+def test_one_tensor_for_all_and_broadcast_gradient(ops):
+    """q, k and v are one tensor; dout is one row for all tokens, read in place."""
+    B, N, H = 2, 200, 3
+    x = inputs(B, N, H, 21)[0]
+    do = inputs(B, N, H, 22)[3][:, :1, :, :]
+    pat = patterns_of(ops, "mix", H)
+    want = check(ops, x, x, x, do.expand(B, N, H, 64), pat, 2)
+    gx, gdo = x.to(DEV), do.to(DEV).expand(B, N, H, 64)
+    out, lse, rest = ops.frame_attn_fwd(gx, gx, gx, pat, frames=2, rest=True)
+    for n, t in zip(("dq", "dk", "dv"), ops.frame_attn_bwd(gdo, gx, gx, gx, out, lse, pat, frames=2, rest=rest)):
+        assert torch.equal(t, want[n]), n
+    bad = torch.empty(B, 1, H, 64, dtype=torch.bfloat16, device=DEV).expand(B, N, H, 64)
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.frame_attn_bwd(gdo, gx, gx, gx, out, lse, pat, frames=2, rest=rest, grads=(bad, *want_like(gx, 2)))
+
+
+def want_like(t, n):
+    return [torch.empty_like(t) for _ in range(n)]
+
+
+@pytest.mark.parametrize("B,F,T,H", [(1, 1, 900, 2), (2, 2, 300, 14), (1, 1, 2060, 16)])
+def test_shared_walks_captured(ops, B, F, T, H):
+    """Launches that share their walks in a graph whose inputs and mask change between the replays."""
+    N = F * T
+    pat = [ops.DENSE] * H
+    gen = torch.Generator().manual_seed(T)
+    bufs = [t.to(DEV) for t in inputs(B, N, H, 1)]
+    mask = torch.ones(B, N, dtype=torch.bool, device=DEV)
+
+    def run():
+        res = []
+        for m in (None, mask):
+            out, lse, rest = ops.frame_attn_fwd(*bufs[:3], pat, frames=F, token_mask=m, rest=True)
+            res += [out, lse, *ops.frame_attn_bwd(bufs[3], *bufs[:3], out, lse, pat, frames=F, token_mask=m, rest=rest)]
+        return res
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for seed in (3, 4, 5):
+        for dst, src in zip(bufs, inputs(B, N, H, seed)):
+            dst.copy_(src)
+        mask.copy_(torch.rand(B, N, generator=gen) < 0.3 * (seed - 2))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got)), seed
