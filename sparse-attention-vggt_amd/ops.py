@@ -1025,7 +1025,7 @@ def frame_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
             return frame_attn_bwd(dout, q, k, v, out, lse, patterns, frames, token_mask, scale, rest, grads)
     lse = lse.contiguous()
     if grads is None:
-        dq = q.new_empty(q.shape)
+        dq = torch.empty_like(out) if out.is_contiguous() else q.new_empty(q.shape)
         grads = (dq, torch.empty_like(dq), torch.empty_like(dq))
     else:
         grads = tuple(grads)
@@ -1084,7 +1084,7 @@ def _norm_params(shape: tuple, rows: torch.Tensor, rows_dtype, weight, bias=None
 
 
 def _flat_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """``t`` as rows with consecutive elements (a copy where its strides do not allow that view), and the row stride."""
+    """``t`` as rows with consecutive elements (itself where it is contiguous, a copy where its strides do not allow that view), and the row stride."""
     dim = t.shape[-1]
     if t.is_contiguous():
         return t, dim
@@ -1113,7 +1113,7 @@ def layer_norm_fwd(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
             return layer_norm_fwd(x, weight, bias, eps, out_dtype)
     dim = shape[-1]
     rows, stride = _flat_rows(x)
-    y = x.new_empty(shape, dtype=out_dtype)
+    y = torch.empty_like(x) if rows is x and out_dtype == dt else x.new_empty(shape, dtype=out_dtype)
     mean = x.new_empty(shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
     _mark("layer_norm_fwd", "start")
@@ -1158,7 +1158,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: 
     rows, stride = _flat_rows(x)
     drows, dstride = _flat_rows(dy)
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    dx = x.new_empty(shape)
+    dx = torch.empty_like(x) if rows is x else x.new_empty(shape)
     dw, db, ws, nbytes = _param_grads(x, shape[-1:], read, need_params,
                                       lambda: lib.saf3r_layer_norm_bwd_workspace_bytes(mean.numel(), dim))
     _mark("layer_norm_bwd", "start")
