@@ -364,10 +364,11 @@ struct Tiles {
 // one barrier a tile. Alone: wave w of n takes the tiles w, w + n, ... (of those that hold a token) in two buffers of its own,
 // without barriers; the callers add up what the waves found. load(start, end) -> the lane's share of what belongs to a tile,
 // bits(share) -> the rows that are there, publish(share, buffer) before and tile(buffer, bits) with the rows in LDS.
-template <bool MASK, int MODE, typename Load, typename Bits, typename Publish, typename Tile>
+// rows() reads the own rows, once the first tiles are on their way.
+template <bool MASK, int MODE, typename Rows, typename Load, typename Bits, typename Publish, typename Tile>
 __device__ __forceinline__ void walk(const FaItem& it, const Stager& st, const uint8_t* mask,
-                                     __bf16 (*lds)[2][kTokens<MODE> * kHeadDim], int wave, bool active, Load load,
-                                     Bits bits, Publish publish, Tile tile) {
+                                     __bf16 (*lds)[2][kTokens<MODE> * kHeadDim], int wave, bool active, Rows rows,
+                                     Load load, Bits bits, Publish publish, Tile tile) {
   constexpr int kN = kTokens<MODE>;
   if constexpr (MASK)
     if (!__syncthreads_or(active)) return;  // no row of its own: nothing to walk for
@@ -388,6 +389,7 @@ __device__ __forceinline__ void walk(const FaItem& it, const Stager& st, const u
     int buf = 2 * wave, behind = tiles.after(i, MODE);
     auto now = fetch(i, buf), next = now;
     if (behind < nw) next = fetch(behind, buf + 1);
+    rows();
     while (true) {
       if (behind < nw)
         wait_vm<8>();  // all but the next tile's copies
@@ -410,6 +412,7 @@ __device__ __forceinline__ void walk(const FaItem& it, const Stager& st, const u
     constexpr int kGroups = MODE == kPairs ? 2 : 1;
     const int group = wave >> 2, buf0 = 2 * group;
     auto now = fetch(min(group, nw - 1), buf0);
+    rows();
     for (int i = group, step = 0; step * kGroups < nw; i += kGroups, ++step) {
       const int buf = buf0 + (step & 1);
       const uint64_t there = bits(now);
@@ -427,6 +430,7 @@ __device__ __forceinline__ void walk(const FaItem& it, const Stager& st, const u
     int own = group ? last : first;
     const int buf0 = 2 * group;
     auto now = fetch(min(own, nw - 1), buf0);
+    rows();
     for (int step = 0; first < nw; ++step) {
       const int buf = buf0 + (step & 1);
       const bool has = MODE != kPairs || own < nw;
@@ -541,7 +545,8 @@ __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether ? 3 : 2) fra
   const Stager st = stager<MODE>(p.k.ptr + it.clip * p.k.clip + it.head * p.k.head, p.k.token,
                                   p.v.ptr + it.clip * p.v.clip + it.head * p.v.head, p.v.token, p.wide, wave, lane);
   walk<MASK, MODE>(
-      it, st, mask, lds, wave, active, [&](int start, int end) { return mask_byte<MASK>(mask, start, end); },
+      it, st, mask, lds, wave, active, [] {},
+      [&](int start, int end) { return mask_byte<MASK>(mask, start, end); },
       [](uint8_t b) { return __ballot(b != 0); }, [](uint8_t, int) {},
       [&](int buf, uint64_t bits) {
         const __bf16 *kt = lds[buf][0], *vt = lds[buf][1];
@@ -706,47 +711,57 @@ __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether ? 3 : 2) fra
   const uint8_t* mask = MASK ? p.mask + (int64_t)it.clip * p.N : nullptr;
   const int64_t stat = ((int64_t)it.clip * p.H + it.head) * p.N;
   const int first = it.row0 + (kAlone<MODE> ? 0 : (wave & 3) * 32), r = first + (lane & 31);
-  const float ls = r < it.row_end ? p.lse[stat + r] : -__builtin_inff();
-  const bool valid = ls != -__builtin_inff(), active = __any(valid);  // not: rows without a key, or not there
+  const bool active = __any(r < it.row_end && (!MASK || mask[r]));
 
-  bf16x8 qf[4] = {}, dof[4] = {};
-  float d = 0.f;
-  if (valid) {
-    const __bf16* qp = p.q.ptr + it.clip * p.q.clip + it.head * p.q.head + r * p.q.token + 8 * h;
-    const __bf16* dp = p.doo.ptr + it.clip * p.doo.clip + it.head * p.doo.head + r * p.doo.token + 8 * h;
-    const __bf16* op = p.o.ptr + it.clip * p.o.clip + it.head * p.o.head + r * p.o.token + 8 * h;
-    bf16x8 of[4], rf[4] = {};
+  bf16x8 qf[4], dof[4];
+  float lse2 = __builtin_inff();  // rows without a key, or not there: probabilities of zero
+  f32x16 dq[2] = {}, from;        // from: where the sums of dP start
+  auto rows = [&] {
+    float ls = -__builtin_inff(), d = 0.f;
+    bf16x8 of[4] = {}, rf[4] = {};
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) qf[ks] = dof[ks] = bf16x8{};
+    if (r < it.row_end) {
+      const __bf16* qp = p.q.ptr + it.clip * p.q.clip + it.head * p.q.head + r * p.q.token + 8 * h;
+      const __bf16* dp = p.doo.ptr + it.clip * p.doo.clip + it.head * p.doo.head + r * p.doo.token + 8 * h;
+      const __bf16* op = p.o.ptr + it.clip * p.o.clip + it.head * p.o.head + r * p.o.token + 8 * h;
+      ls = p.lse[stat + r];
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
+        dof[ks] = *reinterpret_cast<const bf16x8*>(dp + 16 * ks);
+        of[ks] = *reinterpret_cast<const bf16x8*>(op + 16 * ks);
+      }
+      if (p.rest.ptr) {
+        const __bf16* rp = p.rest.ptr + it.clip * p.rest.clip + it.head * p.rest.head + r * p.rest.token + 8 * h;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) rf[ks] = *reinterpret_cast<const bf16x8*>(rp + 16 * ks);
+      }
+    }
+    const bool valid = ls != -__builtin_inff();
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
-      dof[ks] = *reinterpret_cast<const bf16x8*>(dp + 16 * ks);
-      of[ks] = *reinterpret_cast<const bf16x8*>(op + 16 * ks);
-    }
-    if (p.rest.ptr) {
-      const __bf16* rp = p.rest.ptr + it.clip * p.rest.clip + it.head * p.rest.head + r * p.rest.token + 8 * h;
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) rf[ks] = *reinterpret_cast<const bf16x8*>(rp + 16 * ks);
-    }
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
+      qf[ks] = valid ? qf[ks] : bf16x8{};
+      dof[ks] = valid ? dof[ks] : bf16x8{};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         d += (float)dof[ks][j] * (float)of[ks][j];
         d += (float)dof[ks][j] * (float)rf[ks][j];
       }
-  }
-  d = pair_sum(d);
-  if (h == 0 && r < it.row_end && wave < kRows<MODE> / 32) p.delta[stat + r] = d;
-  const float lse2 = valid ? ls * kLog2e : __builtin_inff();
-  f32x16 dq[2] = {}, from;  // from: where the sums of dP start
+    }
+    d = valid ? pair_sum(d) : 0.f;
+    if (h == 0 && r < it.row_end && wave < kRows<MODE> / 32) p.delta[stat + r] = d;
+    if (valid) lse2 = ls * kLog2e;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) from[j] = -d;
+    for (int j = 0; j < 16; ++j) from[j] = -d;
+  };
 
   const bool fine = it.a1 - it.a0 + it.b1 - it.b0 <= kFineUpTo<MODE>;
   const Stager st = stager<MODE>(p.k.ptr + it.clip * p.k.clip + it.head * p.k.head, p.k.token,
                                   p.v.ptr + it.clip * p.v.clip + it.head * p.v.head, p.v.token, p.wide, wave, lane);
   walk<MASK, MODE>(
-      it, st, mask, lds, wave, active, [&](int start, int end) { return mask_byte<MASK>(mask, start, end); },
+      it, st, mask, lds, wave, active, rows,
+      [&](int start, int end) { return mask_byte<MASK>(mask, start, end); },
       [](uint8_t b) { return __ballot(b != 0); }, [](uint8_t, int) {},
       [&](int buf, uint64_t bits) {
         const __bf16 *kt = lds[buf][0], *vt = lds[buf][1];
@@ -859,7 +874,7 @@ __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether && !MASK ? 3
                                   p.doo.ptr + it.clip * p.doo.clip + it.head * p.doo.head, p.doo.token, p.wide, wave,
                                   lane);
   walk<MASK, MODE>(
-      it, st, mask, lds, wave, active,
+      it, st, mask, lds, wave, active, [] {},
       [&](int start, int end) {
         const int tok = start + lane;  // (end: at most the tile's)
         RowStats x;
