@@ -112,7 +112,13 @@ __device__ inline FaItem fa_item(const FaParams& p, int rows) {
     s.walk = in ? x.walk : s.walk;
     s.heads = in ? x.heads : s.heads;
   }
-  const int j = bid - s.start, run = j / s.per_clip, t = j - run * s.per_clip;
+  // Work-groups go to the eight XCDs in turn: eight runs (a head of a clip) side by side, so that a run's rows are read
+  // through one L2. What eight do not divide comes behind. (60 clips of 120 tokens, 16 heads, forward / dQ / dK and dV: 22 /
+  // 29 / 32 us, run by run 26 / 31 / 34; 8192 tokens: the same.)
+  const int j = bid - s.start, even = (__builtin_popcountll(s.heads) * p.clips & ~7) * s.per_clip;
+  const bool in_turn = j < even;
+  const int k = in_turn ? j >> 3 : j - even, nth_run = k / s.per_clip, t = k - nth_run * s.per_clip;
+  const int run = in_turn ? 8 * nth_run + (j & 7) : even / s.per_clip + nth_run;
   FaItem it;
   const int nth = run / p.clips;
   it.clip = run - nth * p.clips;
