@@ -98,7 +98,9 @@ def trained_attention(attn: Attention, x: torch.Tensor, pos) -> torch.Tensor:
     S, T, C = x.shape
     if attn.head_dim != HEAD_DIM:
         raise NotImplementedError("the kernels are built for head_dim 64")
-    y = autograd.module_attention(attn, attn.qkv(x).to(torch.bfloat16), pos, [ops.DENSE] * attn.num_heads)
+    # (patch coordinates are at most the number of patches: tables of T + 1 need no read from the device)
+    y = autograd.module_attention(attn, attn.qkv(x).to(torch.bfloat16), pos, [ops.DENSE] * attn.num_heads,
+                                  positions=T + 1)
     if y.dtype != attn.proj.weight.dtype and not torch.is_autocast_enabled("cuda"):
         y = y.to(attn.proj.weight.dtype)
     return attn.proj_drop(attn.proj(y))

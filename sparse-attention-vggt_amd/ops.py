@@ -201,9 +201,10 @@ def rope_tables(positions: int, base: float = 100.0, device="cuda"):
     ``rope.py:100-115`` does (angles = position * inv_freq in fp32, then cos / sin), cached."""
     key = (int(positions), float(base), str(device))
     if key not in _rope_cache:
-        inv = rope_inv_freq(base)
-        ang = torch.arange(int(positions), dtype=torch.float32)[:, None] * inv[None, :]
-        _rope_cache[key] = (ang.cos().contiguous().to(device), ang.sin().contiguous().to(device))
+        with torch.inference_mode(False):  # (kept: a training step may save them for its backward pass)
+            inv = rope_inv_freq(base)
+            ang = torch.arange(int(positions), dtype=torch.float32)[:, None] * inv[None, :]
+            _rope_cache[key] = (ang.cos().contiguous().to(device), ang.sin().contiguous().to(device))
     return _rope_cache[key]
 
 

@@ -251,3 +251,13 @@ def test_rotary_tables(pkg):
                 dict(positions=4, section=2, scaling="ntk", factor=2.0)):
         with pytest.raises(ValueError):
             ops.rotary_tables(device="cpu", **bad)
+
+
+def test_kept_tables_of_an_inference_run(pkg):
+    """Tables that a run without gradients made first can be saved by a training step."""
+    ops = import_module(pkg.__name__ + ".ops")
+    with torch.inference_mode():
+        kept = ops.rope_tables(7, 77.0, "cpu")
+    assert not any(t.is_inference() for t in kept)
+    x = torch.ones(7, 16, requires_grad=True)
+    (x * ops.rope_tables(7, 77.0, "cpu")[0]).sum().backward()
