@@ -1444,7 +1444,8 @@ static void fa_launch(bool mask, int mode, F f) {
 }
 
 static int fa_grid(const char* who, int64_t total) {
-  if (total > 0x7fffffff) return fail(SAF3R_ERR_UNSUPPORTED, "%s: too many row tiles for one launch", who);
+  // (a launch counts its threads in 32 bits)
+  if (total > 0xffffffffll / 512) return fail(SAF3R_ERR_UNSUPPORTED, "%s: too many row tiles for one launch", who);
   return SAF3R_OK;
 }
 

@@ -301,7 +301,8 @@ extern "C" int saf3r_layer_norm_fwd(const void* x, int64_t x_stride, int x_type,
     return ln_types(x_type, y_type, param_type, [&](auto tx, auto ty, auto tp) {
       constexpr int kTpr = decltype(tpr)::value;
       const int64_t grid = (rows + 256 / kTpr - 1) / (256 / kTpr);
-      if (grid > 0x7fffffff) return fail(SAF3R_ERR_UNSUPPORTED, "%s: too many rows for one launch", who);
+      // (a launch counts its threads in 32 bits)
+      if (grid > 0xffffffffll / 256) return fail(SAF3R_ERR_UNSUPPORTED, "%s: too many rows for one launch", who);
       hipLaunchKernelGGL(
           (layer_norm_fwd_kernel<decltype(tx), decltype(ty), decltype(tp), decltype(some)::value, decltype(nv)::value,
                                  kTpr>),

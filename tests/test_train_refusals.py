@@ -111,6 +111,13 @@ def test_rotary_results_on_each_other(L, bwd):
             refused(L, rotary(L, bwd, y=heads(L, **{stride: 0}), clips=2, norm=norm), INVALID, "overlap")
 
 
+def test_launches_beyond_32_bits_of_threads(L):
+    for call in (attn_fwd, attn_bwd):
+        kw = {} if call is attn_fwd else {"nbytes": 1 << 40}
+        refused(L, call(L, clips=1 << 23, frames=1, tokens=1, **kw), UNSUPPORTED, "too many row tiles")
+    refused(L, norm(L, rows=(1 << 24) * 32), UNSUPPORTED, "too many rows for one launch")
+
+
 def rotary(L, bwd=False, x=None, y=None, dy=None, type=BF16, clips=1, tokens=3, groups=2, n=2, dim=64, pos=256, pos64=1,
            axes=2, cos=256, sin=256, positions=9, rot=64, inter=0, norm=1, w=256, b=256, pt=FP32, eps=1e-5, ws=256,
            nbytes=1 << 20):
