@@ -93,14 +93,13 @@ def frame_local_attention(attn: Attention, x: torch.Tensor, pos, num_special: in
     return attn.proj_drop(attn.proj(y))
 
 
-def trained_attention(attn: Attention, x: torch.Tensor, pos) -> torch.Tensor:
-    """``attn`` over each sequence of x [S, T, C], differentiable, through the package kernels."""
-    S, T, C = x.shape
+def trained_attention(attn: Attention, x: torch.Tensor, pos, positions: int | None = None) -> torch.Tensor:
+    """``attn`` over each sequence of x [S, T, C], differentiable, through the package kernels. ``positions``: more
+    than any position (default: the largest one is read from the device, which a graph cannot capture)."""
     if attn.head_dim != HEAD_DIM:
         raise NotImplementedError("the kernels are built for head_dim 64")
-    # (patch coordinates are at most the number of patches: tables of T + 1 need no read from the device)
     y = autograd.module_attention(attn, attn.qkv(x).to(torch.bfloat16), pos, [ops.DENSE] * attn.num_heads,
-                                  positions=T + 1)
+                                  positions=positions)
     if y.dtype != attn.proj.weight.dtype and not torch.is_autocast_enabled("cuda"):
         y = y.to(attn.proj.weight.dtype)
     return attn.proj_drop(attn.proj(y))
@@ -129,14 +128,15 @@ class Block(nn.Module):
         return autograd.layer_norm(x, norm.weight, norm.bias, norm.eps,
                                    torch.get_autocast_dtype("cuda") if cast else None)
 
-    def forward(self, x, pos=None):
+    def forward(self, x, pos=None, positions: int | None = None):
+        """``positions`` (``"saf3r_train"`` only): more than any of ``pos``, see ``trained_attention``."""
         h = self._norm(self.norm1, x)
         if self.frame_attention == "saf3r" and not isinstance(self.attn, Attention):
             raise RuntimeError("frame_attention='saf3r' is for unpatched frame blocks")
         if self.frame_attention == "saf3r":
             a = frame_local_attention(self.attn, h, pos, self.num_special)
         elif self.frame_attention == "saf3r_train" and isinstance(self.attn, Attention):
-            a = trained_attention(self.attn, h, pos)
+            a = trained_attention(self.attn, h, pos, positions)
         else:
             a = self.attn(h, pos=pos)
         x = x + self.ls1(a)
@@ -258,6 +258,12 @@ class Aggregator(nn.Module):
         frame = torch.cat([torch.zeros(self.patch_start_idx, 2, dtype=patch.dtype, device=device), patch], dim=0)
         return frame[None].expand(S, -1, -1).contiguous()
 
+    @staticmethod
+    def _block(block, x, pos, positions: int):
+        if type(block).forward is Block.forward and block.frame_attention == "saf3r_train":
+            return block(x, pos=pos, positions=positions)
+        return block(x, pos=pos)
+
     def forward(self, images: torch.Tensor):
         """images [1, S, 3, H, W] in [0, 1] -> (list of [1, S, T, 2C] per layer, patch_start_idx)."""
         B, S, c, H, W = images.shape
@@ -273,15 +279,17 @@ class Aggregator(nn.Module):
         tokens = torch.cat([_expand_special(self.camera_token, S).to(dt),
                             _expand_special(self.register_token, S).to(dt), patch_tokens], dim=1)  # [S, T, C]
         T = tokens.shape[1]
-        pos = None
+        pos = gpos = None
+        gh, gw = H // self.patch_size, W // self.patch_size
+        positions = max(gh, gw) + 1  # (the patch grid bounds every position, whatever the number of views)
         if self.rope is not None:
-            pos = self.positions(S, H // self.patch_size, W // self.patch_size, images.device)
+            pos = self.positions(S, gh, gw, images.device)
+            gpos = pos.reshape(1, S * T, 2)
         outputs = []
         for i in range(self.depth):
-            tokens = self.frame_blocks[i](tokens.reshape(S, T, C), pos=pos)
+            tokens = self._block(self.frame_blocks[i], tokens.reshape(S, T, C), pos, positions)
             frame_out = tokens.reshape(1, S, T, C)
-            tokens = self.global_blocks[i](tokens.reshape(1, S * T, C),
-                                           pos=None if pos is None else pos.reshape(1, S * T, 2))
+            tokens = self._block(self.global_blocks[i], tokens.reshape(1, S * T, C), gpos, positions)
             global_out = tokens.reshape(1, S, T, C)
             outputs.append(torch.cat([frame_out, global_out], dim=-1))
         return outputs, self.patch_start_idx

@@ -1,0 +1,57 @@
+"""What the training path makes of a model's modules: the rotary tables it asks for, the modules that it computes itself
+and those that it leaves alone or refuses (CPU: the kernels' functions are replaced by torch's)."""
+from importlib import import_module
+
+import pytest
+import torch
+import torch.nn.functional as F
+from torch import nn
+
+BF = torch.bfloat16
+
+
+@pytest.fixture
+def mods(pkg, monkeypatch):
+    """(autograd, ops, aggregator, vggt, calls): the two functions that launch kernels return plain values and note their
+    arguments."""
+    ad, ops, agg, vggt = (import_module(pkg.__name__ + m) for m in (".autograd", ".ops", ".aggregator", ".vggt"))
+    calls = {"attention": [], "norm": []}
+
+    def qkv_attention(qkv, patterns, frames=1, pos=None, tables=None, norm=False, weight=None, bias=None, eps=1e-5,
+                      token_mask=None, scale=None):
+        calls["attention"].append({"pos": pos, "tables": tables, "norm": norm, "weight": weight, "bias": bias})
+        return qkv[..., 2 * len(patterns) * 64:]
+
+    def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
+        calls["norm"].append(x.shape)
+        return F.layer_norm(x, x.shape[-1:], weight, bias, eps)
+    monkeypatch.setattr(ad, "qkv_attention", qkv_attention)
+    monkeypatch.setattr(ad, "layer_norm", layer_norm)
+    return ad, ops, agg, vggt, calls
+
+
+def test_tables_hold_every_position(mods):
+    """A block that is called with few tokens of far positions (a pruned sequence) is rotated by their own angles."""
+    _, ops, agg, _, calls = mods
+    block = agg.Block(64, 1, qk_norm=True, rope=agg.RotaryPositionEmbedding2D(100.0))
+    block.frame_attention = "saf3r_train"
+    pos = torch.tensor([[[0, 0], [7, 20], [3, 2]]])
+    block(torch.randn(1, 3, 64), pos=pos)
+    (call,) = calls["attention"]
+    cos, sin = call["tables"]
+    assert cos.shape[0] > 20 and sin.shape == cos.shape
+    assert torch.equal(cos[:21], ops.rope_tables(21, 100.0, "cpu")[0])
+
+
+def test_tables_go_by_the_patch_grid(mods, monkeypatch):
+    """Steps over different numbers of views share the tables of their grid, and read no position back."""
+    _, ops, agg, _, calls = mods
+    model = agg.VGGTAggregatorModel(img_size=28, embed_dim=64, depth=1, num_heads=1, dino_depth=1, dino_dim=64,
+                                    dino_heads=1, frame_attention="saf3r_train")
+    monkeypatch.setattr(ops, "_rope_cache", {})
+    monkeypatch.setattr(torch.Tensor, "item", lambda t: pytest.fail("a read from the device"))
+    for views in (1, 2, 5):
+        model(torch.rand(1, views, 3, 28, 42))
+    rotated = [c for c in calls["attention"] if c["tables"] is not None]
+    assert len(rotated) == 6 and len(ops._rope_cache) == 1
+    assert all(c["tables"][0].shape[0] == 4 and int(c["pos"].max()) == 3 for c in rotated)
