@@ -23,7 +23,8 @@ fused SDPA kernels (flash / memory-efficient only, never the math path), or, wit
 ``frame_attention="saf3r"``, through this package's kernels as the frame-local pattern over the
 frames' tokens (identical arithmetic: every token attends to the tokens of its own frame). With
 ``frame_attention="saf3r_train"`` every block's norms and the attention of unpatched blocks run through the
-differentiable kernels (``autograd``), for training steps.
+differentiable kernels (``autograd``), for training steps; norms and attentions of a class with a forward of its own, or
+with hooks, are called as they are.
 """
 from __future__ import annotations
 
@@ -120,8 +121,9 @@ class Block(nn.Module):
         self.frame_attention = "sdpa"  # "saf3r", "saf3r_train": the package kernels (see module doc)
         self.num_special = 0
 
-    def _norm(self, norm: nn.LayerNorm, x):
-        if self.frame_attention != "saf3r_train":
+    def _norm(self, norm: nn.Module, x):
+        if self.frame_attention != "saf3r_train" or not autograd.computed_as(norm, nn.LayerNorm) \
+                or len(norm.normalized_shape) != 1:
             return norm(x)
         # (under autocast the products that follow take their input in the autocast type)
         cast = torch.is_autocast_enabled("cuda") and x.dtype == torch.float32
@@ -135,7 +137,7 @@ class Block(nn.Module):
             raise RuntimeError("frame_attention='saf3r' is for unpatched frame blocks")
         if self.frame_attention == "saf3r":
             a = frame_local_attention(self.attn, h, pos, self.num_special)
-        elif self.frame_attention == "saf3r_train" and isinstance(self.attn, Attention):
+        elif self.frame_attention == "saf3r_train" and autograd.computed_as(self.attn, Attention):
             a = trained_attention(self.attn, h, pos, positions)
         else:
             a = self.attn(h, pos=pos)

@@ -147,6 +147,15 @@ def qkv_attention(qkv: torch.Tensor, patterns: Sequence[int], frames: int = 1, p
                                norm, eps, token_mask, scale)
 
 
+def computed_as(module: torch.nn.Module, kind: type) -> bool:
+    """Whether calling ``module`` is ``kind``'s forward and nothing else, so that a kernel can stand for the call: no
+    forward of a subclass or of the instance, no hooks."""
+    own = module.__dict__
+    return (isinstance(module, kind) and type(module).forward is kind.forward and "forward" not in own
+            and not (own["_forward_hooks"] or own["_forward_pre_hooks"] or own["_backward_hooks"]
+                     or own["_backward_pre_hooks"]))
+
+
 def module_attention(attn, qkv: torch.Tensor, pos: torch.Tensor | None, patterns: Sequence[int], frames: int = 1,
                      positions: int | None = None, token_mask: torch.Tensor | None = None) -> torch.Tensor:
     """``qkv_attention`` with the norms, rotary positions and scale of an ``Attention``-shaped module (``q_norm``,

@@ -55,3 +55,72 @@ def test_tables_go_by_the_patch_grid(mods, monkeypatch):
     rotated = [c for c in calls["attention"] if c["tables"] is not None]
     assert len(rotated) == 6 and len(ops._rope_cache) == 1
     assert all(c["tables"][0].shape[0] == 4 and int(c["pos"].max()) == 3 for c in rotated)
+
+
+class ScaledNorm(nn.LayerNorm):
+    """A norm that is a LayerNorm by its class and not by what it computes."""
+
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+class Doubled:
+    """A forward that belongs to an instance."""
+
+    def __init__(self, module):
+        self.module = module
+
+    def __call__(self, x):
+        return 2 * type(self.module).forward(self.module, x)
+
+
+def double_weight(module, args):
+    nn.init.constant_(module.weight, 2.0)
+
+
+def customised(kind, dim):
+    """A LayerNorm whose call gives twice LayerNorm's result."""
+    norm = ScaledNorm(dim) if kind == "subclass" else nn.LayerNorm(dim)
+    if kind == "hook":
+        norm.register_forward_hook(lambda m, args, y: 2 * y)
+    elif kind == "pre-hook":  # (as a weight that is made from others for every call)
+        norm.register_forward_pre_hook(double_weight)
+    elif kind == "instance":
+        norm.forward = Doubled(norm)
+    return norm
+
+
+KINDS = ("subclass", "hook", "pre-hook", "instance")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_norms_with_a_forward_of_their_own(mods, kind):
+    _, _, agg, _, calls = mods
+    block = agg.Block(64, 1)
+    block.norm2 = customised(kind, 64)
+    x = torch.randn(1, 4, 64)
+    with torch.no_grad():
+        block.frame_attention = "saf3r_train"
+        h = block._norm(block.norm1, x)
+        assert len(calls["norm"]) == 1 and torch.equal(h, F.layer_norm(x, (64,)))
+        assert torch.equal(block._norm(block.norm2, x), 2 * h) and len(calls["norm"]) == 1
+        block.norm1 = nn.LayerNorm((4, 64))  # over two dimensions
+        assert torch.equal(block._norm(block.norm1, x), F.layer_norm(x, (4, 64))) and len(calls["norm"]) == 1
+
+
+@pytest.mark.parametrize("kind", ["subclass", "hook"])
+def test_attentions_with_a_forward_of_their_own(mods, kind):
+    _, _, agg, vggt, calls = mods
+    block = agg.Block(64, 1)
+    block.frame_attention = "saf3r_train"
+    seen = []
+    if kind == "subclass":
+        class Marked(vggt.Attention):
+            def forward(self, x, pos=None):
+                seen.append(1)
+                return super().forward(x, pos)
+        block.attn.__class__ = Marked
+    else:
+        block.attn.register_forward_hook(lambda m, args, y: seen.append(1))
+    block(torch.randn(1, 4, 64))
+    assert seen and not calls["attention"]
