@@ -156,23 +156,40 @@ def computed_as(module: torch.nn.Module, kind: type) -> bool:
                      or own["_backward_pre_hooks"]))
 
 
+def _head_norms(attn):
+    """(norm, eps, weight, bias) of ``q_norm`` and ``k_norm``, which are one kind: LayerNorm over a head's elements with the
+    same eps and the same parameters, or Identity. Others are refused: they would be trained as something else."""
+    q, k = attn.q_norm, attn.k_norm
+    norm = isinstance(q, torch.nn.LayerNorm)
+    kind = torch.nn.LayerNorm if norm else torch.nn.Identity
+    for name, m in (("q_norm", q), ("k_norm", k)):
+        if not isinstance(m, (torch.nn.LayerNorm, torch.nn.Identity)):
+            raise NotImplementedError(f"{name} {type(m).__name__} is not LayerNorm / Identity")
+        if not isinstance(m, kind):
+            raise NotImplementedError(f"q_norm {type(q).__name__} and k_norm {type(k).__name__} differ")
+        if not computed_as(m, kind):
+            raise NotImplementedError(f"{name} {type(m).__name__} has a forward of its own or hooks")
+    if not norm:
+        return False, 1e-5, None, None
+    if k.eps != q.eps:
+        raise NotImplementedError("q_norm and k_norm of different eps")
+    pairs = ((q.weight, k.weight), (q.bias, k.bias))
+    if any((a is None) != (b is None) for a, b in pairs):
+        raise NotImplementedError("q_norm and k_norm differ in their parameters")
+    for m in (q, k):
+        if tuple(m.normalized_shape) != (HEAD_DIM,):
+            raise NotImplementedError(f"q_norm / k_norm over {tuple(m.normalized_shape)} and not over a head's {HEAD_DIM}")
+    return True, q.eps, *(None if a is None else torch.stack([a, b]) for a, b in pairs)
+
+
 def module_attention(attn, qkv: torch.Tensor, pos: torch.Tensor | None, patterns: Sequence[int], frames: int = 1,
                      positions: int | None = None, token_mask: torch.Tensor | None = None) -> torch.Tensor:
     """``qkv_attention`` with the norms, rotary positions and scale of an ``Attention``-shaped module (``q_norm``,
-    ``k_norm``, ``rope``, ``scale``): qkv [clips, tokens, 3 * heads * 64], pos int [clips, tokens, 2]. ``positions``:
-    length of the rotary tables (default: the largest position + 1, which costs one device-to-host read)."""
-    weight = bias = None
-    eps, norm = 1e-5, isinstance(attn.q_norm, torch.nn.LayerNorm)
-    if norm:
-        eps = attn.q_norm.eps
-        if attn.k_norm.eps != eps:
-            raise NotImplementedError("q_norm and k_norm of different eps")
-        if attn.q_norm.weight is not None:
-            weight = torch.stack([attn.q_norm.weight, attn.k_norm.weight])
-        if attn.q_norm.bias is not None:
-            bias = torch.stack([attn.q_norm.bias, attn.k_norm.bias])
-    elif not isinstance(attn.q_norm, torch.nn.Identity):
-        raise NotImplementedError(f"q_norm {type(attn.q_norm).__name__} is not LayerNorm / Identity")
+    ``k_norm``, ``rope`` by its ``base_frequency``, ``scale``): qkv [clips, tokens, 3 * heads * 64], pos int [clips,
+    tokens, 2]. ``positions``: length of the rotary tables (default: the largest position + 1, which costs one
+    device-to-host read); positions behind it are taken to its end. Raises NotImplementedError for norms that the
+    kernels do not compute: other kinds, or two different ones."""
+    norm, eps, weight, bias = _head_norms(attn)
     tables = None
     if attn.rope is not None and pos is not None:
         n = int(pos.max().item()) + 1 if positions is None else positions

@@ -124,3 +124,42 @@ def test_attentions_with_a_forward_of_their_own(mods, kind):
         block.attn.register_forward_hook(lambda m, args, y: seen.append(1))
     block(torch.randn(1, 4, 64))
     assert seen and not calls["attention"]
+
+
+@pytest.mark.parametrize("name", ["q_norm", "k_norm"])
+@pytest.mark.parametrize("kind", [*KINDS, "identity", "other", "eps", "weight", "bias", "shape"])
+def test_head_norms_that_are_refused(mods, name, kind):
+    """Norms of q and k that the kernels do not compute, or that are not alike."""
+    ad, ops, _, vggt, calls = mods
+    attn = vggt.Attention(128, 2, qk_norm=True)
+    qkv = torch.randn(1, 4, 384).to(BF)
+    ad.module_attention(attn, qkv, None, [ops.DENSE] * 2)
+    (call,) = calls["attention"]
+    assert call["norm"] and call["weight"].shape == (2, 64)
+    setattr(attn, name, {"identity": nn.Identity, "other": lambda: nn.RMSNorm(64),
+                         "eps": lambda: nn.LayerNorm(64, eps=1e-3),
+                         "weight": lambda: nn.LayerNorm(64, elementwise_affine=False),
+                         "bias": lambda: nn.LayerNorm(64, bias=False),
+                         "shape": lambda: nn.LayerNorm((2, 64))}.get(kind, lambda: customised(kind, 64))())
+    if kind == "pre-hook":
+        nn.init.ones_(getattr(attn, name).weight)
+    with pytest.raises(NotImplementedError, match="norm"):
+        ad.module_attention(attn, qkv, None, [ops.DENSE] * 2)
+    assert len(calls["attention"]) == 1
+
+
+def test_head_norms_that_are_computed(mods):
+    ad, ops, _, vggt, calls = mods
+    qkv = torch.randn(1, 4, 384).to(BF)
+    for norm, weight, bias in ((nn.Identity, False, False), (lambda: nn.LayerNorm(64), True, True),
+                               (lambda: nn.LayerNorm(64, bias=False), True, False),
+                               (lambda: nn.LayerNorm(64, elementwise_affine=False), False, False)):
+        attn = vggt.Attention(128, 2)
+        attn.q_norm, attn.k_norm = norm(), norm()
+        ad.module_attention(attn, qkv, None, [ops.DENSE] * 2)
+        call = calls["attention"][-1]
+        assert call["norm"] == isinstance(attn.q_norm, nn.LayerNorm)
+        assert (call["weight"] is not None) == weight and (call["bias"] is not None) == bias
+    with pytest.raises(NotImplementedError, match="Identity and k_norm LayerNorm"):
+        attn.q_norm = nn.Identity()
+        ad.module_attention(attn, qkv, None, [ops.DENSE] * 2)
