@@ -187,8 +187,11 @@ def module_attention(attn, qkv: torch.Tensor, pos: torch.Tensor | None, patterns
     """``qkv_attention`` with the norms, rotary positions and scale of an ``Attention``-shaped module (``q_norm``,
     ``k_norm``, ``rope`` by its ``base_frequency``, ``scale``): qkv [clips, tokens, 3 * heads * 64], pos int [clips,
     tokens, 2]. ``positions``: length of the rotary tables (default: the largest position + 1, which costs one
-    device-to-host read); positions behind it are taken to its end. Raises NotImplementedError for norms that the
-    kernels do not compute: other kinds, or two different ones."""
+    device-to-host read); positions behind it are taken to its end. Raises NotImplementedError for what the kernels do not
+    compute: norms of other kinds (or two different ones), and dropout of the probabilities (``attn_drop``) in training."""
+    drop = getattr(attn, "attn_drop", 0.0)
+    if getattr(attn, "training", False) and getattr(drop, "p", drop):
+        raise NotImplementedError(f"attn_drop {getattr(drop, 'p', drop)}: no dropout of the probabilities in training")
     norm, eps, weight, bias = _head_norms(attn)
     tables = None
     if attn.rope is not None and pos is not None:

@@ -163,3 +163,22 @@ def test_head_norms_that_are_computed(mods):
     with pytest.raises(NotImplementedError, match="Identity and k_norm LayerNorm"):
         attn.q_norm = nn.Identity()
         ad.module_attention(attn, qkv, None, [ops.DENSE] * 2)
+
+
+def test_dropout_is_refused_in_training(mods):
+    """Dropout of the probabilities is no part of the kernels: refused where it would be applied, and only there."""
+    ad, ops, agg, vggt, calls = mods
+    qkv = torch.randn(1, 4, 384).to(BF)
+    attn = vggt.Attention(128, 2, attn_drop=0.1)
+    with pytest.raises(NotImplementedError, match="attn_drop 0.1"):
+        ad.module_attention(attn, qkv, None, [ops.DENSE] * 2)
+    attn.eval()
+    ad.module_attention(attn, qkv, None, [ops.DENSE] * 2)
+    attn.train()
+    attn.attn_drop.p = 0.0
+    ad.module_attention(attn, qkv, None, [ops.DENSE] * 2)
+    del attn.attn_drop
+    attn.attn_drop = 0.2  # (a plain number, as some modules keep it)
+    with pytest.raises(NotImplementedError, match="attn_drop 0.2"):
+        ad.module_attention(attn, qkv, None, [ops.DENSE] * 2)
+    assert len(calls["attention"]) == 2
