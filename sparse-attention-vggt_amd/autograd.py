@@ -44,7 +44,8 @@ class _HeadRotary(torch.autograd.Function):
     def forward(ctx, x, weight, bias, pos, cos, sin, layout, rotary_dim, norm, eps):
         tables = None if cos is None else (cos, sin)
         y = ops.head_rotary_fwd(x, pos, tables, layout, rotary_dim, norm, weight, bias, eps)
-        ctx.save_for_backward(x, weight, pos, cos, sin)
+        # (without the norm x is not read again: its memory is the caller's)
+        ctx.save_for_backward(x if norm else None, weight, pos, cos, sin)
         ctx.args = (layout, rotary_dim, norm, eps, None if bias is None else bias.dtype)
         return y
 
@@ -53,8 +54,8 @@ class _HeadRotary(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, pos, cos, sin = ctx.saved_tensors
         layout, rotary_dim, norm, eps, bias_dtype = ctx.args
-        dx, dw, db = ops.head_rotary_bwd(dy, x, pos, None if cos is None else (cos, sin), layout, rotary_dim, norm,
-                                         weight, eps, need_params=ctx.needs_input_grad[1:3])
+        dx, dw, db = ops.head_rotary_bwd(dy, x if norm else dy, pos, None if cos is None else (cos, sin), layout,
+                                         rotary_dim, norm, weight, eps, need_params=ctx.needs_input_grad[1:3])
         return (dx, dw, db if db is None else db.to(bias_dtype), *(None,) * 7)
 
 

@@ -1279,9 +1279,10 @@ def head_rotary_bwd(dy: torch.Tensor, x: torch.Tensor, pos: torch.Tensor | None 
                     weight: torch.Tensor | None = None, eps: float = 1e-5,
                     need_params: tuple[bool, bool] = (True, True), out: torch.Tensor | None = None):
     """Gradients (dx, dweight, dbias) of ``head_rotary_fwd`` (``saf3r_head_rotary_bwd``) from ``dy`` (x's shape and
-    type), the other arguments those of that call. dweight / dbias [groups, dim] are None without a norm or where
-    ``need_params`` says so, else of weight's type (fp32 without a weight). ``out`` (optional) receives dx: a tensor or
-    view like x with consecutive elements in a row, not overlapping the inputs. Equal inputs give equal bits."""
+    type), the other arguments those of that call. Without a norm x is not read. dweight / dbias [groups, dim] are None
+    without a norm or where ``need_params`` says so, else of weight's type (fp32 without a weight). ``out`` (optional)
+    receives dx: a tensor or view like x with consecutive elements in a row, not overlapping the inputs. Equal inputs
+    give equal bits."""
     _need_cuda(x, dy)
     xt, dev = _dtype("x", x), x.get_device()
     p, pos64, axes, cos, sin, positions, R = _rotary_args(x, pos, tables, layout, rotary_dim, norm, weight, None)
@@ -1300,7 +1301,7 @@ def head_rotary_bwd(dy: torch.Tensor, x: torch.Tensor, pos: torch.Tensor | None 
     dx = x.new_empty(x.shape) if out is None else out
     dw, db, ws, nbytes = _param_grads(x, (G, D), read, need_params if norm else (False, False),
                                       lambda: lib.saf3r_head_rotary_bwd_workspace_bytes(B, N, G, H, D))
-    hdy, hx, hdx = _group_heads(dy), _group_heads(x), _group_heads(dx)
+    hdy, hx, hdx = _group_heads(dy), _group_heads(x) if norm else None, _group_heads(dx)
     _mark("head_rotary_bwd", "start")
     _lib.check(lib.saf3r_head_rotary_bwd(
         hdy, hx, xt, B, N, G, H, D, _ptr(p), pos64, axes, _ptr(cos), _ptr(sin), positions, R, layout == "interleaved",

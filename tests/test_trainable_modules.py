@@ -182,3 +182,26 @@ def test_dropout_is_refused_in_training(mods):
     with pytest.raises(NotImplementedError, match="attn_drop 0.2"):
         ad.module_attention(attn, qkv, None, [ops.DENSE] * 2)
     assert len(calls["attention"]) == 2
+
+
+@pytest.mark.parametrize("norm", [False, True])
+def test_rotary_keeps_what_its_backward_pass_reads(mods, monkeypatch, norm):
+    """Without the norm the rows are not kept for the backward pass, and may change before it."""
+    ad, ops, _, _, _ = mods
+    read = []
+
+    def bwd(dy, x, *args, **kw):
+        read.append(x)
+        return 3 * dy, None, None
+    monkeypatch.setattr(ops, "head_rotary_fwd", lambda x, *args: 3 * x)
+    monkeypatch.setattr(ops, "head_rotary_bwd", bwd)
+    leaf = torch.randn(1, 4, 2, 3, 64, requires_grad=True)
+    x = leaf * 1.0
+    pos, tables = torch.zeros(1, 4, 1, dtype=torch.long), (torch.ones(1, 32), torch.zeros(1, 32))
+    y = ad.head_rotary(x, pos, tables, norm=norm)
+    assert (y.grad_fn.saved_tensors[0] is None) == (not norm)
+    if not norm:
+        with torch.no_grad():
+            x.zero_()
+    y.backward(torch.ones_like(y))
+    assert torch.equal(leaf.grad, torch.full_like(leaf, 3.0)) and read[0].shape == leaf.shape
