@@ -1385,9 +1385,10 @@ constexpr int kEightFrom = 768;
 constexpr int64_t kPairsUpTo = 256;
 constexpr int kPairsFrom = 512;
 
-// Tokens that a work-group of a class walks, and the most of a launch.
+// Tokens that a work-group of a class walks (of a lone frame once), and the most of a launch.
 static int fa_walked(const FaParams& p, const FaClass& c) {
-  return c.walk == kAll ? p.N : c.walk == kFirstOwn ? 2 * p.T : c.walk == kNone ? 0 : p.T;
+  if (c.walk == kFirstOwn) return p.N > p.T ? 2 * p.T : p.T;  // (two frames are at most N)
+  return c.walk == kAll ? p.N : c.walk == kNone ? 0 : p.T;
 }
 static int fa_longest(const FaParams& p) {
   int longest = 0;
