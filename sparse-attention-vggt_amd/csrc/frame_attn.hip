@@ -1007,7 +1007,7 @@ __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether && !MASK ? 3
 // of 1374 tokens, 16 heads.) 12 frames of 1374, 10 of 16 heads dense: 1310 us, 1130 TFLOP/s of the pairs.
 //
 // The products are inline assembly, for which the compiler keeps no distance to the instructions that read their results:
-// nothing but this order may touch them, so the kernel must not spill (tests/test_frame_attn_build.py).
+// nothing but this order may touch them, so the kernel must not spill (tests/test_frame_attn_build.py, _order.py).
 // ---------------------------------------------------------------------------------------
 struct DkvRows {
   bf16x8 q[4], d[4];  // row operands of Q and dO
@@ -1241,8 +1241,11 @@ __global__ void __launch_bounds__(256, 1) frame_attn_dkv_long_kernel(const FaPar
              },
              first_half(i + 1));
   }
-  // the last products are done before the sums are read
-  asm volatile("s_nop 15\n\ts_nop 15"
+  // The last products are done before the sums are read: the wait stands right behind the loop, where no copy of a sum can
+  // come ahead of it, and the statement that takes the sums keeps their first use behind it.
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile(""
                : "+a"(A.dk[0][0]), "+a"(A.dk[0][1]), "+a"(A.dk[1][0]), "+a"(A.dk[1][1]), "+a"(A.dv[0][0]),
                  "+a"(A.dv[0][1]), "+a"(A.dv[1][0]), "+a"(A.dv[1][1]));
 #pragma unroll
