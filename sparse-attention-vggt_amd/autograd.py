@@ -125,7 +125,10 @@ class _QkvAttention(torch.autograd.Function):
                            token_mask, scale, rest, grads=(dqk[:, :, 0], dqk[:, :, 1], dx[:, :, 2]))
         dw = db = None
         if prologue:
-            _, dw, db = ops.head_rotary_bwd(dqk, x[:, :, :2], pos, None if cos is None else (cos, sin), norm=norm,
+            rows = x[:, :, :2]
+            if norm and token_mask is not None:  # (the norm's sums take every row: zeros where a token is not there)
+                rows = torch.where((token_mask != 0)[:, :, None, None, None], rows, 0.0)
+            _, dw, db = ops.head_rotary_bwd(dqk, rows, pos, None if cos is None else (cos, sin), norm=norm,
                                             weight=weight, eps=eps, need_params=ctx.needs_input_grad[1:3],
                                             out=dx[:, :, :2])
         return (dqkv, dw, db if db is None else db.to(bias_dtype), *(None,) * 9)
@@ -138,7 +141,8 @@ def qkv_attention(qkv: torch.Tensor, patterns: Sequence[int], frames: int = 1, p
     """A layer's attention between its two projections: qkv bf16 [clips, tokens, 3 * heads * 64] (the qkv Linear's
     output) -> bf16 [clips, tokens, heads * 64]. Norm of q and k over the head dimension (``norm``, ``weight`` / ``bias``
     [2, 64]: q's, k's), rotary positions (``tables``, ``pos`` [clips, tokens, axes], half layout), then
-    ``frame_attention``. The gradients of qkv are written in place into one buffer."""
+    ``frame_attention``. The gradients of qkv are written in place into one buffer. What the rows of tokens that
+    ``token_mask`` removes hold reaches no result and no gradient; their own gradients are zeros."""
     _, _, width = qkv.shape
     if width != 3 * len(patterns) * HEAD_DIM or qkv.dtype != torch.bfloat16:
         raise ValueError(f"qkv must be bfloat16 [clips, tokens, {3 * len(patterns) * HEAD_DIM}], got {qkv.dtype} "
