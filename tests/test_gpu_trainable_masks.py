@@ -41,3 +41,24 @@ def test_padded_rows_of_a_qkv_buffer(mods, norm, rotate, value):
     for a, b in zip(got, want):
         assert torch.isfinite(a).all() and torch.equal(a, b)
     assert not got[1][~mask].any()
+
+
+@pytest.mark.parametrize("shape,layout", [((2, 37, 2, 3, 64), "half"), ((1, 5, 1, 2, 48), "interleaved")])
+def test_inverse_rotation_of_a_broadcast_gradient(mods, shape, layout):
+    """Without a norm only the gradient is read, whatever its strides and whatever the rows hold by then."""
+    ad, ops = mods
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(shape, generator=g).to(BF).to(DEV)
+    pos = torch.randint(0, 30, (*shape[:2], 1), generator=g).to(DEV)
+    tables = ops.rotary_tables(30, shape[-1], device=DEV)
+    dy = torch.randn(shape[:4], generator=g).to(BF).to(DEV)[..., None].expand(shape)
+    want, _, _ = ops.head_rotary_bwd(dy.contiguous(), x, pos, tables, layout)
+    got, dw, db = ops.head_rotary_bwd(dy, torch.full_like(x, float("nan")), pos, tables, layout)
+    assert torch.equal(got, want) and dw is None and db is None
+    leaf = x.clone().requires_grad_()
+    row = leaf * 1.0
+    y = ad.head_rotary(row, pos, tables, layout)
+    with torch.no_grad():
+        row.zero_()
+    y.backward(dy)
+    assert torch.equal(leaf.grad, want)
