@@ -599,7 +599,7 @@ int saf3r_layer_norm_bwd(const void* dy, int64_t dy_stride, int y_type, const vo
                          int param_type, void* dx, int64_t dx_stride, void* dweight, void* dbias, void* workspace,
                          int64_t workspace_bytes, void* stream);
 
-/* Workspace bytes of saf3r_layer_norm_bwd (at most 8192 * dim), -1 for sizes that it rejects. */
+/* Workspace bytes of saf3r_layer_norm_bwd (at most 4096 * dim), -1 for sizes that it rejects. */
 int64_t saf3r_layer_norm_bwd_workspace_bytes(int64_t rows, int dim);
 
 #ifdef __cplusplus

@@ -527,7 +527,7 @@ __device__ __forceinline__ void mask_scores(f32x16& s, uint64_t bits, int half, 
 // times the time over 522 tokens.) The modes that share a walk join their sums at the end.
 //
 // Bound by the issue of vector instructions: fma, exponential, add and half a conversion an element against 16 matrix
-// products a tile. 12 frames of 1374 tokens, 10 of 16 heads dense: 870 us, 849 TFLOP/s of the pairs (1357 is what a
+// products a tile (vector pipe busy 58% of the time, matrix pipe 41%, seldom both). 12 frames of 1374 tokens, 10 of 16 heads dense: 870 us, 849 TFLOP/s of the pairs (1357 is what a
 // large matrix product reaches here); 8 x 1374 frames 101 us; 522 tokens 11 us.
 // ---------------------------------------------------------------------------------------
 template <bool MASK, int MODE>
@@ -698,12 +698,14 @@ __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether ? 3 : 2) fra
 // dQ^T += K^T dS^T.
 // The sums of dP start at -D. Three waves a SIMD (64 rows a wave and two waves: the same rate).
 //
-// Matrix and vector pipes are about equally busy (24 products a tile against fma, exponential, product and half a
-// conversion an element): 12 frames of 1374, 10 of 16 heads dense 1120 us, 990 TFLOP/s; 8 x 1374 frames 120 us.
+// Matrix and vector pipes are about equally busy, 51% each and seldom both (24 products a tile against fma, exponential,
+// product and half a conversion an element): 12 frames of 1374, 10 of 16 heads dense 1120 us, 990 TFLOP/s; 8 x 1374 frames 120 us.
 //
 // The dS of a row add up to zero, so that what its keys have in common cancels in dQ, and the roundings of dS do not: over
 // a few keys that are alike dQ loses another bit. Short walks add what the rounding took away (a third more products: 5% of
-// the time over 60 x 120 tokens, 30% over 8 x 1374; waves that walk alone wait for memory anyway, 3% over 256 tokens).
+// the time over 60 x 120 tokens, 30% over 8 x 1374; waves that walk alone wait for memory anyway, 3% over 256 tokens). What
+// is short goes by the mode, and the mode by the whole launch: dQ of a clip of 129 to 512 tokens is finer in a launch of few
+// rows than in one of many.
 // ---------------------------------------------------------------------------------------
 template <int MODE>
 constexpr int kFineUpTo = kAlone<MODE> ? 512 : 128;
@@ -1004,7 +1006,8 @@ __global__ void __launch_bounds__(kThreads<MODE>, MODE == kTogether && !MASK ? 3
 // its own matrix products and vector work: a half tile (32 queries) is 32 products in a fixed order, with the
 // exponentials and roundings of one group placed behind the products of the other (32 cycles each, room for seven
 // vector instructions) and the LDS reads a phase ahead. (Compiler's order, two-phase loop: 686 TFLOP/s over 12 frames
-// of 1374 tokens, 16 heads.) 12 frames of 1374, 10 of 16 heads dense: 1310 us, 1130 TFLOP/s of the pairs.
+// of 1374 tokens, 16 heads.) 12 frames of 1374, 10 of 16 heads dense: 1310 us, 1130 TFLOP/s of the pairs; matrix pipe busy
+// 53%, vector pipe 44%.
 //
 // The products are inline assembly, for which the compiler keeps no distance to the instructions that read their results:
 // nothing but this order may touch them, so the kernel must not spill (tests/test_frame_attn_build.py, _order.py).

@@ -8,9 +8,9 @@
 // sums of its columns in registers while its work-group walks its rows, one work-group writes one partial row, and a
 // second kernel adds the partial rows in a fixed order (no atomics: equal inputs give equal bits). A lane reads eight
 // elements at a time, also where a row is not aligned to that or ends inside them.
-// Measured: 87936 rows of 1024, fp32 to bf16: forward 95 us for 540 MB (5.7 TB/s), backward 156 us for 900 MB (5.8
-// TB/s) and 5 us for the sums, which a copy does not surpass; 4097 rows of 1027, fp32: 10 and 14 us (16 and 28 with
-// single elements).
+// Measured: 87936 rows of 1024, fp32 to bf16: forward 94 us for 540 MB (5.7 TB/s), backward 156 us for 900 MB (5.8
+// TB/s) and 5 us for the sums (a 4 GiB copy, read and written: 4.8 TB/s); 4097 rows of 1027, fp32: 10 and 15 us (16 and 28
+// with single elements).
 #include "row_ops.h"
 
 namespace saf3r {

@@ -50,8 +50,7 @@ struct RotParams {
 struct RotLane {
   int a, b;      // element offsets
   int axis;      // -1: passed through
-  int table;     // first table column (the second vector's: + table2)
-  int table2;
+  int table;     // first table column
   bool on;
 };
 
@@ -61,7 +60,7 @@ __device__ inline RotLane rot_lane(const RotParams& p, int t) {
   const int turned = p.rot / (2 * VE);
   r.on = t * 2 * VE < p.dim;
   r.axis = -1;
-  r.table = r.table2 = 0;
+  r.table = 0;
   if (t >= turned || !p.cosine) {
     r.a = t * 2 * VE;
     r.b = r.a + VE;
@@ -73,7 +72,6 @@ __device__ inline RotLane rot_lane(const RotParams& p, int t) {
     r.b = r.a + VE;
     r.axis = r.a / S;
     r.table = (r.a - r.axis * S) / 2;
-    r.table2 = VE / 2;
   } else {
     const int per = S / (2 * VE);
     r.axis = t / per;

@@ -1011,7 +1011,9 @@ def frame_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
     output; ``out``, ``lse`` and ``rest`` are its results, the other arguments those of that call (without ``rest``
     dq and dk carry the rounding of out: 1.5 to 2 times their error). ``grads`` (optional): three
     bf16 tensors or views of q's shape that receive them (rows 16-byte aligned, strides a multiple of 8, not
-    overlapping the inputs). The results do not depend on the order in which the GPU runs the work."""
+    overlapping the inputs). The results do not depend on the order in which the GPU runs the work: equal calls give equal
+    bits. How a launch shares its walks goes by all of its rows, so the last bits of a clip's results (and, up to 512
+    tokens, the accuracy of its dq) are its own only in launches of one size."""
     pat, mask, fscale = _frame_args(q, k, v, patterns, frames, token_mask, scale)
     B, N, H, _ = q.shape
     _frame_like("dout", dout, q)
