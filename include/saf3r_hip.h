@@ -123,6 +123,13 @@ enum saf3r_dtype {
   SAF3R_FP16 = 2
 };
 
+/* Activations of saf3r_linear_fwd: none, z Phi(z) (Phi: the normal distribution function), and its tanh form. */
+enum saf3r_activation {
+  SAF3R_NO_ACTIVATION = 0,
+  SAF3R_GELU = 1,
+  SAF3R_GELU_TANH = 2
+};
+
 /* Rows of several heads where another kernel left them: the row of (clip b, token t, group g, head h) starts at
  * ptr + b*clip_stride + t*token_stride + g*group_stride + h*head_stride elements, its elements are consecutive.
  * (saf3r_frame_attn_*: one group, group_stride is not read.) */
@@ -601,6 +608,47 @@ int saf3r_layer_norm_bwd(const void* dy, int64_t dy_stride, int y_type, const vo
 
 /* Workspace bytes of saf3r_layer_norm_bwd (at most 4096 * dim), -1 for sizes that it rejects. */
 int64_t saf3r_layer_norm_bwd_workspace_bytes(int64_t rows, int dim);
+
+/*
+ * Linear layer with its epilogue: y = residual + gate drop(act(x w^T + bias)), rows of `out` from rows of `in`.
+ *   x [rows][in], w [out][in]: bf16 or fp16 (`type`), rows at 16-byte alignment (strides multiples of 8 elements), `in` a
+ *   multiple of 8 (pad both with zeros otherwise).
+ *   bias, gate: [out] of param_type (fp32 or `type`), NULL: none. activation: enum saf3r_activation.
+ *   drop: 65536 times the probability of dropping an element, 0 .. 65536 (0: no dropout); state: device int64 [2], the seed
+ *   and the stream (its low 32 bits) of the keep mask, a function of them and of the element's row and column: sixteen bits
+ *   of a counter-based generator, compared with `drop`. Kept elements are multiplied by 65536 / (65536 - drop).
+ *   residual: rows of y's type, or NULL. y: rows of y_type (fp32 or `type`).
+ *   kept: rows of `type` that receive x w^T + bias, for the backward pass, or NULL.
+ *   Sums are fp32, y and kept are each rounded once. Equal calls give equal bits.
+ *   workspace: saf3r_linear_fwd_workspace_bytes, 16-byte aligned, for this call alone until it is done on its stream.
+ * ref: the Linear layers, layer scale and residual of layers/block.py:26-105, layers/mlp.py.
+ */
+int saf3r_linear_fwd(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int type, int64_t rows, int in,
+                     int out, const void* bias, const void* gate, int param_type, int activation, int drop,
+                     const int64_t* state, const void* residual, int64_t res_stride, void* y, int64_t y_stride,
+                     int y_type, void* kept, int64_t kept_stride, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of saf3r_linear_fwd (0 for most sizes), -1 for sizes that it rejects. */
+int64_t saf3r_linear_fwd_workspace_bytes(int64_t rows, int in, int out);
+
+/*
+ * Gradients of saf3r_linear_fwd from dy (rows of y_type; it is the residual's gradient itself), each may be NULL:
+ *   dx (rows of `type`), dw [out][in] (rows of dw_type: fp32 or `type`), dbias and dgate [out] of param_type.
+ *   kept: as written by the forward pass, for an activation or dgate. gate, activation, drop and state: of that call.
+ *   x and w: rows at 16-byte alignment; where `in` is no multiple of 8 the elements up to the next one are read (and
+ *   reach no result). The sums have a fixed order.
+ *   workspace: saf3r_linear_bwd_workspace_bytes, 16-byte aligned, for this call alone until it is done on its stream.
+ */
+int saf3r_linear_bwd(const void* dy, int64_t dy_stride, int y_type, const void* x, int64_t x_stride, const void* w,
+                     int64_t w_stride, int type, int64_t rows, int in, int out, const void* kept, int64_t kept_stride,
+                     const void* gate, int param_type, int activation, int drop, const int64_t* state, void* dx,
+                     int64_t dx_stride, void* dw, int64_t dw_stride, int dw_type, void* dbias, void* dgate,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of saf3r_linear_bwd, -1 for sizes that it rejects. own_dz: whether anything lies between dy and the
+ * products: a gate, an activation, dropout, dy of another type than `type` or in rows that are not 16-byte aligned, `out` no
+ * multiple of 8. */
+int64_t saf3r_linear_bwd_workspace_bytes(int64_t rows, int in, int out, int own_dz);
 
 #ifdef __cplusplus
 }

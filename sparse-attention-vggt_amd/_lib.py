@@ -25,11 +25,13 @@ EXPORTS = (
     "saf3r_frame_attn_fwd", "saf3r_frame_attn_bwd", "saf3r_frame_attn_bwd_workspace_bytes",
     "saf3r_head_rotary_fwd", "saf3r_head_rotary_bwd", "saf3r_head_rotary_bwd_workspace_bytes",
     "saf3r_layer_norm_fwd", "saf3r_layer_norm_bwd", "saf3r_layer_norm_bwd_workspace_bytes",
+    "saf3r_linear_fwd", "saf3r_linear_fwd_workspace_bytes", "saf3r_linear_bwd", "saf3r_linear_bwd_workspace_bytes",
 )
 ABI_VERSION = 13
 PACK_LN_BF16, PACK_POS_INT64 = 1, 2  # enum saf3r_pack_param_flags
 GATHER_QK_FP32, GATHER_V_FP32, GATHER_OUT_FP32 = 1, 2, 4  # enum saf3r_gather_dtype
 FP32, BF16, FP16 = 0, 1, 2  # enum saf3r_dtype
+NO_ACTIVATION, GELU, GELU_TANH = 0, 1, 2  # enum saf3r_activation
 SAF3R_OK, SAF3R_ERR_INVALID, SAF3R_ERR_UNSUPPORTED, SAF3R_ERR_LAUNCH, SAF3R_ERR_INJECTED = range(5)
 
 _lib = None
@@ -116,6 +118,12 @@ def load():
         "saf3r_layer_norm_fwd": ([p, i64, i32, i64, i32, p, p, i32, f32, p, i64, i32, p, p, p], i32),
         "saf3r_layer_norm_bwd": ([p, i64, i32, p, i64, i32, i64, i32, p, p, p, i32, p, i64, p, p, p, i64, p], i32),
         "saf3r_layer_norm_bwd_workspace_bytes": ([i64, i32], i64),
+        "saf3r_linear_fwd": ([p, i64, p, i64, i32, i64, i32, i32, p, p, i32, i32, i32, p, p, i64, p, i64, i32, p, i64, p,
+                              i64, p], i32),
+        "saf3r_linear_fwd_workspace_bytes": ([i64, i32, i32], i64),
+        "saf3r_linear_bwd": ([p, i64, i32, p, i64, p, i64, i32, i64, i32, i32, p, i64, p, i32, i32, i32, p, p, i64, p, i64,
+                              i32, p, p, p, i64, p], i32),
+        "saf3r_linear_bwd_workspace_bytes": ([i64, i32, i32, i32], i64),
         "saf3r_frame_topk_scores": ([p, i64, i32, i32, i32, i32, i32, i32, i32, i32, p, i64, p, p, p], i32),
     }
     if lib.saf3r_abi_version() != ABI_VERSION:  # (no arguments, int result: ctypes' defaults)

@@ -1,0 +1,102 @@
+// Before the products of a linear layer's backward pass: the gradient behind the epilogue, and its sums over rows.
+//   dz = dy gate keep/(1-p) act'(kept),  dbias = sum dz,  dgate = sum dy keep/(1-p) act(kept)
+// dz is rounded to the operands' type, which the matrix products read; the sums take it unrounded.
+//
+// Bound by HBM: dy and kept are read and dz is written once. A work-group of 256 owns 256 columns of a range of rows, eight
+// rows at a time; a lane keeps the sums of its eight columns, and every work-group writes one partial row (summed in a fixed
+// order by sum_parts: equal inputs give equal bits).
+#include "linear.h"
+
+namespace saf3r {
+
+template <typename T, typename TY, bool VEC>
+__global__ void __launch_bounds__(256) linear_grad_kernel(const LinearGradParams p) {
+  __shared__ float lds[256 * 8];
+  const int lane = tid_x() & 31, slot = tid_x() >> 5;
+  const int col = (bid_x() * 32 + lane) * 8, cnt = p.n - col;
+  const int64_t begin = bid_y() * p.part_rows, end = begin + p.part_rows < p.rows ? begin + p.part_rows : p.rows;
+  float db[8], dg[8], gate[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    db[e] = dg[e] = 0.f;
+    gate[e] = 1.f;
+  }
+  DropKey key{};
+  if (p.drop.limit) key = drop_key(p.drop);
+  if (col < p.n) {
+    if (p.gate) epi_load<T>(p.gate, p.param32, VEC, col, cnt, gate);
+#pragma unroll 2
+    for (int64_t row = begin + slot; row < end; row += 8) {
+      float g[8], z[8];
+      if constexpr (VEC)
+        load_vec<8>((const TY*)p.dy + row * p.ld_dy + col, g);
+      else
+        load_some<8>((const TY*)p.dy + row * p.ld_dy + col, cnt, g);
+      if (p.kept) epi_load<T>(p.kept, false, VEC, row * p.ld_kept + col, cnt, z);
+      if (p.drop.limit) drop8(key, p.drop.limit, p.drop.scale, (uint32_t)col >> 3, (uint64_t)row, g);
+      if (p.kept) {
+        if (p.act == SAF3R_GELU) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float a;
+            const float d = act_slope(SAF3R_GELU, z[e], &a);
+            dg[e] += g[e] * a;
+            g[e] *= d;
+          }
+        } else if (p.act == SAF3R_GELU_TANH) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float a;
+            const float d = act_slope(SAF3R_GELU_TANH, z[e], &a);
+            dg[e] += g[e] * a;
+            g[e] *= d;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dg[e] += g[e] * z[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        g[e] *= gate[e];
+        db[e] += g[e];
+      }
+      if (p.dz) store_vec<8>((T*)p.dz + row * p.ld_dz + col, g);
+    }
+  }
+  if (!p.part) return;
+  add_slots<8, 32>(dg, lds);
+  add_slots<8, 32>(db, lds);
+  if (tid_x() < 32 && col < p.n) {
+    float* to = p.part + (int64_t)bid_y() * 2 * p.n + col;
+    if constexpr (VEC) {
+      store_vec<8>(to, dg);
+      store_vec<8>(to + p.n, db);
+    } else {
+      store_some<8>(to, cnt, dg);
+      store_some<8>(to + p.n, cnt, db);
+    }
+  }
+}
+
+// Partial rows: work-groups for four on a compute unit, with at least 16 rows each.
+int64_t linear_grad_parts(int64_t rows, int n) {
+  const int64_t strips = (n + 255) / 256;
+  return std::max<int64_t>(1, std::min<int64_t>((1024 + strips - 1) / strips, rows / 16));
+}
+
+int linear_grad(const char* who, const LinearGradParams& p, int type, bool dy32, bool vec, int64_t parts,
+                hipStream_t stream) {
+  const dim3 grid((uint32_t)((p.n + 255) / 256), (uint32_t)parts);
+  auto go = [&](auto t, auto ty) {
+    if (vec)
+      hipLaunchKernelGGL((linear_grad_kernel<decltype(t), decltype(ty), true>), grid, dim3(256), 0, stream, p);
+    else
+      hipLaunchKernelGGL((linear_grad_kernel<decltype(t), decltype(ty), false>), grid, dim3(256), 0, stream, p);
+    return check_launch(who);
+  };
+  if (type == SAF3R_BF16) return dy32 ? go(__bf16(), float()) : go(__bf16(), __bf16());
+  return dy32 ? go(_Float16(), float()) : go(_Float16(), _Float16());
+}
+
+}  // namespace saf3r

@@ -1312,3 +1312,183 @@ def head_rotary_bwd(dy: torch.Tensor, x: torch.Tensor, pos: torch.Tensor | None 
     if kind != read:
         dw, db = (None if t is None else t.to(kind) for t in (dw, db))
     return dx, dw, db
+
+
+# ---- linear layers with their epilogue, and their gradients --------------------------------------------------
+
+ACTIVATIONS = {None: _lib.NO_ACTIVATION, "gelu": _lib.GELU, "gelu_tanh": _lib.GELU_TANH}
+
+
+def dropout_state(device="cuda") -> torch.Tensor:
+    """A state of the keep masks, (seed, stream) as int64 [2] on the device, drawn from torch's generator there: every call
+    another one, ``torch.manual_seed`` repeats them, and a graph that captured the call draws a new one in every replay."""
+    return torch.randint(-(1 << 63), (1 << 63) - 1, (2,), dtype=torch.int64, device=device)
+
+
+def _drop(p: float, state: torch.Tensor | None, dev: int) -> tuple[int, torch.Tensor | None]:
+    """(65536 times the probability, the state or None) as the C entries take them."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout {p}: a probability")
+    limit = round(p * 65536)
+    if limit == 0:
+        return 0, None
+    if state is None or state.dtype != torch.int64 or state.shape != (2,) or state.get_device() != dev:
+        raise ValueError("dropout needs its state: int64 [2] on the rows' device (ops.dropout_state)")
+    return limit, state.contiguous()
+
+
+def _column_params(n: int, rows: torch.Tensor, **params):
+    """(type they are read in, the tensors): parameters of n columns, of one type, contiguous. Those that are neither fp32
+    nor of the rows' type are read as fp32 copies. Without any, the rows' type."""
+    kind, dev = None, rows.get_device()
+    for name, t in params.items():
+        if t is None:
+            continue
+        if t.shape != (n,) or t.get_device() != dev:
+            raise ValueError(f"{name} must be [{n}] on {rows.device}, got {tuple(t.shape)} on {t.device}")
+        if kind is not None and t.dtype != kind:
+            raise ValueError(f"{' and '.join(params)} must have one dtype")
+        kind = t.dtype
+        _dtype(name, t)
+    if kind is None:
+        return rows.dtype, *params.values()
+    read = kind if kind in (torch.float32, rows.dtype) else torch.float32
+    return read, *(None if t is None else t.to(read).contiguous() for t in params.values())
+
+
+def _operand(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t`` as rows that the products can read (16-byte aligned, a multiple of eight elements) and the row stride: itself,
+    or a copy with zeros behind each row."""
+    dim = t.shape[-1]
+    rows, stride = _flat_rows(t)
+    if not (dim % 8 or stride % 8 or stride < dim or rows.data_ptr() % 16):
+        return rows, stride
+    wide = -(-dim // 8) * 8
+    padded = t.new_zeros((*t.shape[:-1], wide))
+    padded[..., :dim] = t
+    return padded, wide
+
+
+def _linear_args(x, weight, activation):
+    if not (x.is_cuda and weight.is_cuda):
+        raise ValueError("saf3r kernels take GPU tensors")
+    if x.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != x.dtype:
+        raise ValueError(f"x and weight must be bfloat16 or float16 of one dtype, got {x.dtype} and {weight.dtype}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"weight must be [out, in] for rows of in, got {tuple(weight.shape)} for {tuple(x.shape)}")
+    if weight.get_device() != x.get_device():
+        raise ValueError(f"weight is on {weight.device}, x on {x.device}")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation {activation!r}: one of {tuple(ACTIVATIONS)}")
+    return ACTIVATIONS[activation]
+
+
+def linear_fwd(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+               gate: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+               out_dtype: torch.dtype | None = None, dropout: float = 0.0, state: torch.Tensor | None = None,
+               keep: bool = False):
+    """``residual + gate * drop(act(x weight^T + bias))`` in one product with its epilogue (``saf3r_linear_fwd``). x bf16 or
+    fp16 [..., in], weight [out, in] of x's type; bias and gate [out], fp32 or of x's type; ``activation`` None, "gelu" or
+    "gelu_tanh"; residual [..., out] fp32 or of x's type. ``dropout``: probability (rounded to 1/65536), with ``state`` of
+    ``dropout_state``. The result is of residual's type, or without one of ``out_dtype`` (x's type or fp32); sums are fp32,
+    rounded once. With ``keep`` a second tensor of x's type holds x weight^T + bias, for ``linear_bwd``. Rows that are not
+    16-byte aligned, or widths that 8 does not divide, cost a copy of x or the weight. Not differentiable by itself: see
+    ``autograd.linear``."""
+    act = _linear_args(x, weight, activation)
+    dev = x.get_device()
+    n, k = weight.shape
+    shape = (*x.shape[:-1], n)
+    if residual is not None:
+        if residual.shape != shape or residual.get_device() != dev or residual.dtype not in (torch.float32, x.dtype):
+            raise ValueError(f"residual must be float32 or {x.dtype} {shape} on {x.device}, got {residual.dtype} "
+                             f"{tuple(residual.shape)} on {residual.device}")
+        if out_dtype not in (None, residual.dtype):
+            raise ValueError(f"a {residual.dtype} residual gives {residual.dtype}, not {out_dtype}")
+        out_dtype = residual.dtype
+    elif out_dtype is None:
+        out_dtype = x.dtype
+    elif out_dtype not in (torch.float32, x.dtype):
+        raise ValueError(f"{x.dtype} rows give {x.dtype} or float32, not {out_dtype}")
+    read, bias, gate = _column_params(n, x, bias=bias, gate=gate)
+    limit, drop_state = _drop(dropout, state, dev)
+    if dev != _here():
+        with torch.cuda.device(x.device):
+            return linear_fwd(x, weight, bias, activation, gate, residual, out_dtype, dropout, state, keep)
+    lib = _lib.load()
+    rows, stride = _operand(x)
+    w, wstride = _operand(weight)
+    res, res_stride = (None, 0) if residual is None else _flat_rows(residual)
+    y = x.new_empty(shape, dtype=out_dtype)
+    kept = x.new_empty(shape) if keep else None
+    count, wide = y.numel() // n, -(-k // 8) * 8
+    nbytes = lib.saf3r_linear_fwd_workspace_bytes(count, wide, n)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
+    _mark("linear_fwd", "start")
+    _lib.check(lib.saf3r_linear_fwd(rows.data_ptr(), stride, w.data_ptr(), wstride, _DTYPES[x.dtype], count, wide, n,
+                                    _ptr(bias), _ptr(gate), _DTYPES[read], act, limit, _ptr(drop_state), _ptr(res),
+                                    res_stride, y.data_ptr(), n, _DTYPES[out_dtype], _ptr(kept), n, _ptr(ws),
+                                    max(nbytes, 0), _stream(dev)))
+    _mark("linear_fwd", "end")
+    return (y, kept) if keep else y
+
+
+def linear_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, kept: torch.Tensor | None = None,
+               activation: str | None = None, gate: torch.Tensor | None = None, dropout: float = 0.0,
+               state: torch.Tensor | None = None, need: tuple[bool, bool, bool, bool] = (True, True, True, True),
+               weight_dtype: torch.dtype | None = None, param_dtype: torch.dtype | None = None):
+    """Gradients (dx, dweight, dbias, dgate) of ``linear_fwd`` (``saf3r_linear_bwd``) from ``dy``, fp32 or of x's type, of
+    y's shape (it is the residual's gradient itself). ``kept`` is the forward pass's, read for an activation or the
+    gate's gradient; the other arguments are those of that call. ``need``: which of the four are computed, the others are
+    None (dgate also without a gate). dweight is of ``weight_dtype`` (the weight's type or fp32), dbias and dgate of gate's
+    type, without one of ``param_dtype`` (default x's). Equal inputs give equal bits."""
+    act = _linear_args(x, weight, activation)
+    dev = x.get_device()
+    n, k = weight.shape
+    shape = (*x.shape[:-1], n)
+    if dy.shape != shape or dy.get_device() != dev or dy.dtype not in (torch.float32, x.dtype):
+        raise ValueError(f"dy must be float32 or {x.dtype} {shape} on {x.device}, got {dy.dtype} {tuple(dy.shape)} on "
+                         f"{dy.device}")
+    need_dx, need_dw, need_db, need_dg = (bool(v) for v in need)
+    need_dg = need_dg and gate is not None
+    if kept is not None:
+        if kept.shape != shape or kept.dtype != x.dtype or kept.get_device() != dev:
+            raise ValueError(f"kept must be {x.dtype} {shape} on {x.device}, got {kept.dtype} {tuple(kept.shape)} on "
+                             f"{kept.device}")
+    elif activation is not None or need_dg:
+        raise ValueError("the gradients of an activation and of a gate need what the forward pass kept (keep=True)")
+    weight_dtype = x.dtype if weight_dtype is None else weight_dtype
+    if weight_dtype not in (torch.float32, x.dtype):
+        raise ValueError(f"dweight is {x.dtype} or float32, not {weight_dtype}")
+    kind = gate.dtype if gate is not None else x.dtype if param_dtype is None else param_dtype
+    if kind not in _DTYPES:
+        raise ValueError(f"gradients of parameters in float32, bfloat16 or float16, not {kind}")
+    read, gate = _column_params(n, x, gate=gate)
+    if gate is None:
+        read = kind if kind == x.dtype else torch.float32
+    limit, drop_state = _drop(dropout, state, dev)
+    if dev != _here():
+        with torch.cuda.device(x.device):
+            return linear_bwd(dy, x, weight, kept, activation, gate, dropout, state, need, weight_dtype, kind)
+    lib = _lib.load()
+    drows, dstride = _flat_rows(dy)
+    zrows, zstride = (None, 0) if kept is None else _flat_rows(kept)
+    rows, stride = _operand(x) if need_dw else (x, k)
+    w, wstride = _operand(weight) if need_dx else (weight, k)
+    dx = x.new_empty(x.shape) if need_dx else None
+    dw = x.new_empty((n, k), dtype=weight_dtype) if need_dw else None
+    db = x.new_empty(n, dtype=read) if need_db else None
+    dg = x.new_empty(n, dtype=read) if need_dg else None
+    own_dz = (need_dx or need_dw) and bool(activation is not None or gate is not None or limit or dy.dtype != x.dtype or n % 8
+                                           or dstride % 8 or dstride < n or drows.data_ptr() % 16)
+    count = dy.numel() // n
+    nbytes = lib.saf3r_linear_bwd_workspace_bytes(count, k, n, own_dz)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
+    _mark("linear_bwd", "start")
+    _lib.check(lib.saf3r_linear_bwd(drows.data_ptr(), dstride, _DTYPES[dy.dtype], rows.data_ptr(), stride, w.data_ptr(), wstride,
+                                    _DTYPES[x.dtype], count, k, n, _ptr(zrows), zstride, _ptr(gate), _DTYPES[read], act,
+                                    limit, _ptr(drop_state), _ptr(dx), k, _ptr(dw), k, _DTYPES[weight_dtype], _ptr(db),
+                                    _ptr(dg), _ptr(ws), max(nbytes, 0), _stream(dev)))
+    _mark("linear_bwd", "end")
+    if kind != read:
+        db, dg = (None if t is None else t.to(kind) for t in (db, dg))
+    return dx, dw, db, dg
