@@ -650,6 +650,45 @@ int saf3r_linear_bwd(const void* dy, int64_t dy_stride, int y_type, const void* 
  * multiple of 8. */
 int64_t saf3r_linear_bwd_workspace_bytes(int64_t rows, int in, int out, int own_dz);
 
+/*
+ * End of a branch and the norm before the next one: h = x + gate branch keep / (1 - p), y = LayerNorm(h), rows of `dim`
+ * elements (1 .. 8192).
+ *   x, h: rows of x_type; h is rounded to it before the norm. branch, y: rows of y_type (x_type, or a 16-bit type for an
+ *   fp32 stream). gate, weight, bias: [dim] of param_type (fp32 or y_type), NULL: ones, ones, zeros.
+ *   drop, state: as of saf3r_linear_fwd. mean, rstd: fp32 [rows], for the backward pass.
+ *   All arithmetic is fp32, h and y are each rounded once.
+ * ref: the residual, layer scale and norms of layers/block.py:26-105.
+ */
+int saf3r_residual_norm_fwd(const void* x, int64_t x_stride, int x_type, const void* branch, int64_t branch_stride,
+                            int y_type, int64_t rows, int dim, const void* gate, const void* weight, const void* bias,
+                            int param_type, int drop, const int64_t* state, float eps, void* h, int64_t h_stride, void* y,
+                            int64_t y_stride, float* mean, float* rstd, void* stream);
+
+/*
+ * Gradients of saf3r_residual_norm_fwd from dh (rows of x_type, or NULL: zeros) and dy (rows of y_type): dx (rows of
+ * x_type), dbranch (rows of y_type), dgate / dweight / dbias [dim] of param_type; dbranch and the last three may be NULL.
+ *   h, mean, rstd: results of that call; branch is read for dgate only. The sums over rows have a fixed order.
+ *   workspace: saf3r_residual_norm_bwd_workspace_bytes when one of dgate, dweight, dbias is given, 16-byte aligned, for
+ *   this call alone until it is done on its stream.
+ */
+int saf3r_residual_norm_bwd(const void* dh, int64_t dh_stride, const void* dy, int64_t dy_stride, int y_type,
+                            const void* h, int64_t h_stride, int x_type, const void* branch, int64_t branch_stride,
+                            int64_t rows, int dim, const float* mean, const float* rstd, const void* gate,
+                            const void* weight, int param_type, int drop, const int64_t* state, void* dx,
+                            int64_t dx_stride, void* dbranch, int64_t dbranch_stride, void* dgate, void* dweight,
+                            void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of saf3r_residual_norm_bwd (at most 6144 * dim), -1 for sizes that it rejects. */
+int64_t saf3r_residual_norm_bwd_workspace_bytes(int64_t rows, int dim);
+
+/*
+ * Dropout by itself, and its gradient (the same function of dy): y = x keep / (1 - p), rows of `dim` elements of `type`.
+ *   drop, state: as of saf3r_linear_fwd; a dropped element is zero whatever x holds. y may be x.
+ * No counterpart in the reference (torch's dropout, whose masks are stored for the backward pass).
+ */
+int saf3r_dropout(const void* x, int64_t x_stride, int type, int64_t rows, int dim, int drop, const int64_t* state,
+                  void* y, int64_t y_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,6 +26,7 @@ EXPORTS = (
     "saf3r_head_rotary_fwd", "saf3r_head_rotary_bwd", "saf3r_head_rotary_bwd_workspace_bytes",
     "saf3r_layer_norm_fwd", "saf3r_layer_norm_bwd", "saf3r_layer_norm_bwd_workspace_bytes",
     "saf3r_linear_fwd", "saf3r_linear_fwd_workspace_bytes", "saf3r_linear_bwd", "saf3r_linear_bwd_workspace_bytes",
+    "saf3r_residual_norm_fwd", "saf3r_residual_norm_bwd", "saf3r_residual_norm_bwd_workspace_bytes", "saf3r_dropout",
 )
 ABI_VERSION = 13
 PACK_LN_BF16, PACK_POS_INT64 = 1, 2  # enum saf3r_pack_param_flags
@@ -124,6 +125,12 @@ def load():
         "saf3r_linear_bwd": ([p, i64, i32, p, i64, p, i64, i32, i64, i32, i32, p, i64, p, i32, i32, i32, p, p, i64, p, i64,
                               i32, p, p, p, i64, p], i32),
         "saf3r_linear_bwd_workspace_bytes": ([i64, i32, i32, i32], i64),
+        "saf3r_residual_norm_fwd": ([p, i64, i32, p, i64, i32, i64, i32, p, p, p, i32, i32, p, f32, p, i64, p, i64, p, p, p],
+                                    i32),
+        "saf3r_residual_norm_bwd": ([p, i64, p, i64, i32, p, i64, i32, p, i64, i64, i32, p, p, p, p, i32, i32, p, p, i64, p,
+                                     i64, p, p, p, p, i64, p], i32),
+        "saf3r_residual_norm_bwd_workspace_bytes": ([i64, i32], i64),
+        "saf3r_dropout": ([p, i64, i32, i64, i32, i32, p, p, i64, p], i32),
         "saf3r_frame_topk_scores": ([p, i64, i32, i32, i32, i32, i32, i32, i32, i32, p, i64, p, p, p], i32),
     }
     if lib.saf3r_abi_version() != ABI_VERSION:  # (no arguments, int result: ctypes' defaults)

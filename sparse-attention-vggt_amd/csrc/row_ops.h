@@ -166,6 +166,9 @@ inline int param_check(const char* who, int param_type, int half) {
 // dweight / dbias (each may be null) of n columns from `parts` partial rows [part][2][n], in part order per slice.
 int sum_parts(const char* who, const float* part, int64_t parts, int n, void* dweight, void* dbias, int type,
               hipStream_t stream);
+// the same of three gradients from [part][3][n]
+int sum_parts3(const char* who, const float* part, int64_t parts, int n, void* a, void* b, void* c, int type,
+               hipStream_t stream);
 
 // A row tensor's pointer and stride (elements) as the row kernels need them; written rows do not overlap.
 inline int row_check(const char* who, const void* ptr, int64_t stride, int dim, int type, bool written) {

@@ -4,10 +4,10 @@
 namespace saf3r {
 
 struct PartParams {
-  const float* part;  // [parts][2][n]
+  const float* part;  // [parts][outs][n]
   int64_t parts;
-  int n;
-  void* out[2];
+  int n, outs;
+  void* out[3];
   int type;
 };
 
@@ -18,7 +18,7 @@ constexpr int kSumCols = 16, kSumSlices = 64;
 __global__ void __launch_bounds__(kSumCols* kSumSlices) sum_parts_kernel(const PartParams p) {
   __shared__ float lds[kSumSlices][kSumCols + 1];
   const int col = tid_x() % kSumCols, slice = tid_x() / kSumCols;
-  const int64_t n2 = 2 * (int64_t)p.n, c = (int64_t)bid_x() * kSumCols + col;  // column of [2][n]
+  const int64_t n2 = p.outs * (int64_t)p.n, c = (int64_t)bid_x() * kSumCols + col;  // column of [outs][n]
   float s[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < n2) {
     const float* at = p.part + c;
@@ -42,10 +42,10 @@ __global__ void __launch_bounds__(kSumCols* kSumSlices) sum_parts_kernel(const P
   __syncthreads();
   if (slice || c >= n2) return;
   s[0] = (lds[0][col] + lds[1][col]) + (lds[2][col] + lds[3][col]);
-  const int which = c >= p.n;
+  const int which = (c >= p.n) + (c >= 2 * (int64_t)p.n);
   void* out = p.out[which];
   if (!out) return;
-  const int64_t at = c - (which ? p.n : 0);
+  const int64_t at = c - which * (int64_t)p.n;
   if (p.type == SAF3R_FP32)
     ((float*)out)[at] = s[0];
   else if (p.type == SAF3R_BF16)
@@ -54,12 +54,20 @@ __global__ void __launch_bounds__(kSumCols* kSumSlices) sum_parts_kernel(const P
     ((_Float16*)out)[at] = (_Float16)s[0];
 }
 
-int sum_parts(const char* who, const float* part, int64_t parts, int n, void* dweight, void* dbias, int type,
-              hipStream_t stream) {
-  const PartParams p = {part, parts, n, {dweight, dbias}, type};
-  hipLaunchKernelGGL(sum_parts_kernel, dim3((uint32_t)((2 * (int64_t)n + kSumCols - 1) / kSumCols)),
+static int launch(const char* who, const PartParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL(sum_parts_kernel, dim3((uint32_t)((p.outs * (int64_t)p.n + kSumCols - 1) / kSumCols)),
                      dim3(kSumCols * kSumSlices), 0, stream, p);
   return check_launch(who);
+}
+
+int sum_parts(const char* who, const float* part, int64_t parts, int n, void* dweight, void* dbias, int type,
+              hipStream_t stream) {
+  return launch(who, {part, parts, n, 2, {dweight, dbias, nullptr}, type}, stream);
+}
+
+int sum_parts3(const char* who, const float* part, int64_t parts, int n, void* a, void* b, void* c, int type,
+               hipStream_t stream) {
+  return launch(who, {part, parts, n, 3, {a, b, c}, type}, stream);
 }
 
 }  // namespace saf3r

@@ -1492,3 +1492,123 @@ def linear_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, kept: to
     if kind != read:
         db, dg = (None if t is None else t.to(kind) for t in (db, dg))
     return dx, dw, db, dg
+
+
+# ---- the gated residual with the norm behind it, and dropout --------------------------------------------------
+
+def _residual_args(x, branch, out_dtype, **rows):
+    """(type of branch and y, the stream's and its type as the C entries take them)."""
+    shape, dt, dev = x.shape, x.dtype, x.get_device()
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"the stream must have a last dimension, got {tuple(shape)}")
+    xt = _dtype("the stream", x)
+    if out_dtype not in _DTYPES or (out_dtype != dt and dt != torch.float32):
+        raise ValueError(f"a {dt} stream takes branches and gives rows of its own type (fp32: any), not {out_dtype}")
+    for name, t, kind in [("branch", branch, out_dtype), *((n, *v) for n, v in rows.items())]:
+        if t is not None and (t.shape != shape or t.dtype != kind or t.get_device() != dev):
+            raise ValueError(f"{name} must be {kind} {tuple(shape)} on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return xt, _DTYPES[out_dtype]
+
+
+def residual_norm_fwd(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tensor | None = None,
+                      weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
+                      out_dtype: torch.dtype | None = None, dropout: float = 0.0, state: torch.Tensor | None = None):
+    """``h = x + gate * drop(branch)`` and ``y = LayerNorm(h)`` over the last dimension (1 .. 8192 wide) in one pass
+    (``saf3r_residual_norm_fwd``): (h, y, mean, rstd), the statistics fp32 of x's leading shape, for ``residual_norm_bwd``.
+    The stream x and h fp32, bf16 or fp16; branch and y in x's type, or for an fp32 stream in ``out_dtype`` (default: the
+    branch's type). gate, weight and bias [dim] of one type. ``dropout``, ``state``: as of ``linear_fwd``. y is the norm
+    of h as it is stored. Not differentiable by itself: see ``autograd.residual_norm``."""
+    _need_cuda(x, branch)
+    out_dtype = branch.dtype if out_dtype is None else out_dtype
+    xt, yt = _residual_args(x, branch, out_dtype)
+    dim, dev = x.shape[-1], x.get_device()
+    read, gate, w, b = _column_params(dim, branch, gate=gate, weight=weight, bias=bias)
+    limit, drop_state = _drop(dropout, state, dev)
+    if dev != _here():
+        with torch.cuda.device(x.device):
+            return residual_norm_fwd(x, branch, gate, weight, bias, eps, out_dtype, dropout, state)
+    rows, stride = _flat_rows(x)
+    brows, bstride = _flat_rows(branch)
+    h = x.new_empty(x.shape)
+    y = x.new_empty(x.shape, dtype=out_dtype)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    _mark("residual_norm_fwd", "start")
+    _lib.check(_lib.load().saf3r_residual_norm_fwd(
+        rows.data_ptr(), stride, xt, brows.data_ptr(), bstride, yt, mean.numel(), dim, _ptr(gate), _ptr(w), _ptr(b),
+        _DTYPES[read], limit, _ptr(drop_state), eps, h.data_ptr(), dim, y.data_ptr(), dim, mean.data_ptr(), rstd.data_ptr(),
+        _stream(dev)))
+    _mark("residual_norm_fwd", "end")
+    return h, y, mean, rstd
+
+
+def residual_norm_bwd(dh: torch.Tensor | None, dy: torch.Tensor, h: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                      branch: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                      weight: torch.Tensor | None = None, dropout: float = 0.0, state: torch.Tensor | None = None,
+                      need: tuple[bool, bool, bool, bool] = (True, True, True, True)):
+    """Gradients (dx, dbranch, dgate, dweight, dbias) of ``residual_norm_fwd`` (``saf3r_residual_norm_bwd``) from ``dh`` (of
+    h's type; None: zeros) and ``dy`` (of y's type); ``h``, ``mean`` and ``rstd`` are its results, the other arguments
+    those of that call (``branch`` is read for the gate's gradient only). ``need``: whether dbranch, dgate, dweight and
+    dbias are computed; the others are None, dgate also without a gate. The parameters' gradients are of their type
+    (without one of y's). Equal inputs give equal bits."""
+    _need_cuda(h, dy)
+    dev, dim = h.get_device(), h.shape[-1] if h.dim() else 0
+    xt, yt = _residual_args(h, branch, dy.dtype, dy=(dy, dy.dtype), dh=(dh, h.dtype))
+    stats = h.shape[:-1]
+    for n, t in (("mean", mean), ("rstd", rstd)):
+        if t.shape != stats or t.dtype != torch.float32 or t.get_device() != dev:
+            raise ValueError(f"{n} must be float32 {tuple(stats)} on {h.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    need_db, need_dg, need_dw, need_dbias = (bool(v) for v in need)
+    need_dg = need_dg and gate is not None
+    if need_dg and branch is None:
+        raise ValueError("the gate's gradient needs the branch")
+    kind = next((t.dtype for t in (gate, weight) if t is not None), dy.dtype)
+    read, g, w = _column_params(dim, dy, gate=gate, weight=weight)
+    limit, drop_state = _drop(dropout, state, dev)
+    if dev != _here():
+        with torch.cuda.device(h.device):
+            return residual_norm_bwd(dh, dy, h, mean, rstd, branch, gate, weight, dropout, state, need)
+    lib = _lib.load()
+    up, up_stride = (None, 0) if dh is None else _flat_rows(dh)
+    drows, dstride = _flat_rows(dy)
+    hrows, hstride = _flat_rows(h)
+    brows, bstride = _flat_rows(branch) if need_dg else (None, 0)
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    dx = h.new_empty(h.shape)
+    dbranch = dy.new_empty(h.shape) if need_db else None
+    dg, dw, db = (h.new_empty(dim, dtype=read) if n else None for n in (need_dg, need_dw, need_dbias))
+    nbytes = lib.saf3r_residual_norm_bwd_workspace_bytes(mean.numel(), dim) if need_dg or need_dw or need_dbias else 0
+    ws = h.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
+    _mark("residual_norm_bwd", "start")
+    _lib.check(lib.saf3r_residual_norm_bwd(
+        _ptr(up), up_stride, drows.data_ptr(), dstride, yt, hrows.data_ptr(), hstride, xt, _ptr(brows), bstride, mean.numel(),
+        dim, mean.data_ptr(), rstd.data_ptr(), _ptr(g), _ptr(w), _DTYPES[read], limit, _ptr(drop_state), dx.data_ptr(), dim,
+        _ptr(dbranch), dim, _ptr(dg), _ptr(dw), _ptr(db), _ptr(ws), max(nbytes, 0), _stream(dev)))
+    _mark("residual_norm_bwd", "end")
+    if kind != read:
+        dg, dw, db = (None if t is None else t.to(kind) for t in (dg, dw, db))
+    return dx, dbranch, dg, dw, db
+
+
+def dropout(x: torch.Tensor, p: float, state: torch.Tensor) -> torch.Tensor:
+    """``x * keep / (1 - p)`` (``saf3r_dropout``), fp32, bf16 or fp16 [..., dim], p rounded to 1/65536. The keep mask is a
+    function of ``state`` (``dropout_state``) and of an element's place in x [rows, dim]; nothing is stored, and the
+    gradient is the same function of dy. A dropped element is zero whatever x holds."""
+    _need_cuda(x)
+    xt, dev = _dtype("x", x), x.get_device()
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must have a last dimension, got {tuple(x.shape)}")
+    limit, drop_state = _drop(p, state, dev)
+    if dev != _here():
+        with torch.cuda.device(x.device):
+            return dropout(x, p, state)
+    if limit == 0:
+        return x.clone(memory_format=torch.contiguous_format)
+    rows, stride = _flat_rows(x)
+    dim = x.shape[-1]
+    y = x.new_empty(x.shape)
+    _mark("dropout", "start")
+    _lib.check(_lib.load().saf3r_dropout(rows.data_ptr(), stride, xt, x.numel() // dim, dim, limit, drop_state.data_ptr(),
+                                         y.data_ptr(), dim, _stream(dev)))
+    _mark("dropout", "end")
+    return y
