@@ -119,19 +119,43 @@ __device__ __forceinline__ void epi_store(void* p, bool f32, bool vec, int64_t a
   }
 }
 
-// The epilogue of columns col .. col + 7 (col % 8 == 0, col < n) of a row that is there.
+// The parameters of columns col .. col + 7 (col % 8 == 0, col < n).
 template <typename T>
-__device__ __forceinline__ void epilogue8(const EpiParams& e, const DropKey& key, int64_t row, int col, float (&x)[8]) {
+struct EpiCols {
+  float bias[8], gate[8];
+  __device__ __forceinline__ void load(const EpiParams& e, int col) {
+    if (e.bias) epi_load<T>(e.bias, e.param32, e.vec, col, e.n - col, bias);
+    if (e.gate) epi_load<T>(e.gate, e.param32, e.vec, col, e.n - col, gate);
+  }
+};
+
+// The elements at which eight columns of a row start.
+struct EpiPlace {
+  int64_t res, y, kept;
+  __device__ __forceinline__ void init(const EpiParams& e, int64_t row, int col) {
+    res = row * e.ld_res + col;
+    y = row * e.ld_y + col;
+    kept = row * e.ld_kept + col;
+  }
+  __device__ __forceinline__ void down(const EpiParams& e, int rows) {
+    res += rows * e.ld_res;
+    y += rows * e.ld_y;
+    kept += rows * e.ld_kept;
+  }
+};
+
+// The epilogue of columns col .. col + 7 of a row that is there.
+template <typename T>
+__device__ __forceinline__ void epilogue8(const EpiParams& e, const DropKey& key, const EpiCols<T>& c, const EpiPlace& at,
+                                          int64_t row, int col, float (&x)[8]) {
   const int cnt = e.n - col;
   float r[8];
-  if (e.res) epi_load<T>(e.res, e.y32, e.vec, row * e.ld_res + col, cnt, r);
+  if (e.res) epi_load<T>(e.res, e.y32, e.vec, at.res, cnt, r);
   if (e.bias) {
-    float b[8];
-    epi_load<T>(e.bias, e.param32, e.vec, col, cnt, b);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] += b[j];
+    for (int j = 0; j < 8; ++j) x[j] += c.bias[j];
   }
-  if (e.kept) epi_store<T>(e.kept, false, e.vec, row * e.ld_kept + col, cnt, x);
+  if (e.kept) epi_store<T>(e.kept, false, e.vec, at.kept, cnt, x);
   if (e.act != SAF3R_NO_ACTIVATION) {
     if (e.act == SAF3R_GELU) {
 #pragma unroll
@@ -143,16 +167,23 @@ __device__ __forceinline__ void epilogue8(const EpiParams& e, const DropKey& key
   }
   if (e.drop.limit) drop8(key, e.drop.limit, e.drop.scale, (uint32_t)col >> 3, (uint64_t)row, x);
   if (e.gate) {
-    float g[8];
-    epi_load<T>(e.gate, e.param32, e.vec, col, cnt, g);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] *= g[j];
+    for (int j = 0; j < 8; ++j) x[j] *= c.gate[j];
   }
   if (e.res) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] += r[j];
   }
-  epi_store<T>(e.y, e.y32, e.vec, row * e.ld_y + col, cnt, x);
+  epi_store<T>(e.y, e.y32, e.vec, at.y, cnt, x);
+}
+
+template <typename T>
+__device__ __forceinline__ void epilogue8(const EpiParams& e, const DropKey& key, int64_t row, int col, float (&x)[8]) {
+  EpiCols<T> c;
+  EpiPlace at;
+  c.load(e, col);
+  at.init(e, row, col);
+  epilogue8<T>(e, key, c, at, row, col, x);
 }
 
 // First step of a backward pass (linear_grad.hip): dz = dy gate keep/(1-p) act'(kept), rounded to the operands' type, and the

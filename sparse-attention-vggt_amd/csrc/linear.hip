@@ -26,7 +26,6 @@ struct GemmParams {
 };
 
 constexpr int kUnit = 16384;        // bytes of a unit: 128 rows (or columns) x 64 of the reduction
-constexpr int kSlots = 5;           // units in LDS: 80 KB, two work-groups a compute unit
 constexpr int kUnitRows = 128;
 
 // How a wave copies its quarter of a unit: four instructions of 1 KB. ROWS: instruction j of wave w takes rows 8 (4 j + w)
@@ -34,23 +33,25 @@ constexpr int kUnitRows = 128;
 // row (the lanes' sources are, the LDS side of such a copy is linear).
 template <bool COLS>
 struct Copy {
-  uint32_t off[4];  // byte offset of the lane's chunk from the unit's base
-  int at;           // its place along the reduction: element (ROWS) or row (COLS, instruction 0)
+  const char* base;  // the unit's first row or column, step 0
+  uint32_t off[4];   // byte offset of the lane's chunk
+  int at;            // its place along the reduction: element (ROWS) or row (COLS, instruction 0)
 
-  __device__ __forceinline__ void init(int wave, int lane, int first, int count, int64_t ld) {
+  // unit u of an operand of `count` rows (columns) from `first` (a unit behind the last one reads the first one's)
+  __device__ __forceinline__ void init(int wave, int lane, const char* operand, int first, int count, int64_t ld) {
+    first = first < count ? first : 0;
+    base = operand + (COLS ? (int64_t)first * 2 : first * ld);
     if constexpr (COLS) {
       const int kr = 4 * wave + (lane >> 4), chunk = (lane & 15) ^ ((kr & 3) << 2);
       // columns behind the last are the last chunk's: their results are not stored
       const int last = (count - 1) / 8 * 8 - first;
-      const int c = chunk * 8 < last ? chunk * 8 : (last > 0 ? last : 0);
+      const int c = chunk * 8 < last ? chunk * 8 : last;
       at = kr;
 #pragma unroll
       for (int j = 0; j < 4; ++j) off[j] = (uint32_t)((16 * j + kr) * ld + c * 2);
     } else {
-      const int r = 8 * wave + (lane >> 3);
-      const int chunk = (lane & 7) ^ swz8(r);
+      const int r = 8 * wave + (lane >> 3), chunk = (lane & 7) ^ swz8(r), last = count - 1 - first;
       at = chunk * 8;
-      const int last = count - 1 - first > 0 ? count - 1 - first : 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int row = r + 32 * j < last ? r + 32 * j : last;
@@ -59,18 +60,61 @@ struct Copy {
     }
   }
 
-  __device__ __forceinline__ void issue(const char* base, uint32_t lds) const {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) dma16s(base, off[j], lds + j * 4096);
-  }
-
-  // the last step of a reduction that 64 does not divide: `left` elements or rows are there
-  __device__ __forceinline__ void issue_tail(const char* base, uint32_t lds, int left) const {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool there = at + (COLS ? 16 * j : 0) < left;
-      dma16(there ? base + off[j] : (const char*)&kZeros, lds + j * 4096);
+  // instruction J of step * its bytes to `lds`; with ANY only the first `left` elements (rows) of the step are there, zeros
+  // in place of the others
+  template <int J, bool ANY>
+  __device__ __forceinline__ void issue(int64_t step_bytes, uint32_t lds, int left) const {
+    if constexpr (ANY) {
+      const bool there = at + (COLS ? 16 * J : 0) < left;
+      dma16(there ? base + step_bytes + off[J] : (const char*)&kZeros, lds + J * 4096);
+    } else {
+      dma16s(base + step_bytes, off[J], lds + J * 4096);
     }
+  }
+};
+
+// The copies of a work-group of four waves: units 0 .. UB - 1 of a step are B's, the next UA are A's. With ANY a step may be
+// the last one, of which `left` of 64 is there, or behind it: zeros are copied, so that every step copies and waits alike.
+template <bool ACOLS, bool BCOLS, int UA, int UB, int SLOTS>
+struct Feed {
+  Copy<ACOLS> a[UA];
+  Copy<BCOLS> b[UB];
+  int64_t astep, bstep;
+  uint32_t lds0;
+  int s0, s1, left, tail;
+
+  __device__ __forceinline__ void init(const GemmParams& p, int split, int m0, int n0, int wave, int lane, const char* lds) {
+#pragma unroll
+    for (int u = 0; u < UA; ++u) a[u].init(wave, lane, p.a, m0 + u * kUnitRows, p.m, p.lda);
+#pragma unroll
+    for (int u = 0; u < UB; ++u) b[u].init(wave, lane, p.b, n0 + u * kUnitRows, p.n, p.ldb);
+    astep = ACOLS ? 64 * p.lda : 128;
+    bstep = BCOLS ? 64 * p.ldb : 128;
+    lds0 = lds_addr(lds) + wave * 1024;
+    s0 = split * p.split_steps;
+    s1 = s0 + p.split_steps < p.steps ? s0 + p.split_steps : p.steps;
+    left = p.k - (p.steps - 1) * 64;                       // elements of the last step
+    tail = left < 64 && s1 == p.steps ? p.steps - 1 : -1;  // the step with fewer than 64
+  }
+  // steps of this split whose 64 elements are there
+  __device__ __forceinline__ int whole() const { return tail < 0 ? s1 : s1 - 1; }
+  static __device__ __forceinline__ int after(int slot, int n) { return slot + n >= SLOTS ? slot + n - SLOTS : slot + n; }
+
+  template <int U, int J, bool ANY>
+  __device__ __forceinline__ void one(int step, int slot) const {
+    const uint32_t to = lds0 + slot * kUnit;
+    const int there = ANY ? (step >= s1 ? 0 : step == tail ? left : 64) : 64;
+    if constexpr (U < UB)
+      b[U].template issue<J, ANY>(step * bstep, to, there);
+    else
+      a[U - UB].template issue<J, ANY>(step * astep, to, there);
+  }
+  template <int U>
+  __device__ __forceinline__ void unit(int step, int slot) const {
+    one<U, 0, true>(step, slot);
+    one<U, 1, true>(step, slot);
+    one<U, 2, true>(step, slot);
+    one<U, 3, true>(step, slot);
   }
 };
 
@@ -109,79 +153,107 @@ struct Frags {
   }
 };
 
-// Tile of a work-group: 128 UA rows by 128 columns, four waves in two rows of two; each wave owns 64 x 64 of every 128 x 128.
-// Units (128 x 64 of an operand) go through a ring of five LDS slots, in the order B, A0, (A1) of every step of 64: the
-// fragments of B stay in registers for the step, so its slot and A0's are free again after the first half of it. A phase is
-// the 16 products of one A unit: wait for its unit, one barrier, copies into the slots that the last phase freed, LDS reads,
-// products. Copies are under way for two phases. Two work-groups share a compute unit, so that one's epilogue, waits and
-// barriers lie under the other's products.
-template <typename T, bool ACOLS, bool BCOLS, int UA>
-__global__ void __launch_bounds__(256, 2) gemm_kernel(const GemmParams p) {
+// Work-groups go to the eight XCDs in turn: each XCD takes a contiguous range of the tiles, which go by groups of eight rows
+// of tiles, so that the work-groups of an XCD share operand rows in its L2.
+struct Place {
+  int tm, tn, split;
+};
+__device__ __forceinline__ Place place_of(const GemmParams& p) {
+  const int tiles = p.tiles_m * p.tiles_n, all = tiles * p.splits;
+  int id = bid_x();
+  const int q = all / 8, r = all % 8, x = id % 8;
+  id = x * q + (x < r ? x : r) + id / 8;
+  Place at;
+  at.split = p.splits > 1 ? id / tiles : 0;
+  id -= at.split * tiles;
+  const int per = 8 * p.tiles_n, g = id / per, in = id - g * per;
+  const int rows = p.tiles_m - 8 * g < 8 ? p.tiles_m - 8 * g : 8;
+  at.tn = in / rows;
+  at.tm = 8 * g + in - at.tn * rows;
+  return at;
+}
+
+// Results of 32 rows by 64 columns of a wave, two blocks x0, x1 (a lane holds row l % 32, columns 8 q + 4 (l / 32) + e in
+// element 4 q + e), through the wave's own part of LDS: read back, eight lanes hold a row, each eight columns, so that every
+// load and store of the epilogue takes whole lines. (Eight columns a lane of 32 rows, straight from the registers: four
+// requests a line, and 87936 x 1024 to 4096 took 840 us.)
+constexpr int kTurnRow = 68;                  // floats: 16-byte places of 16 rows are distinct banks
+constexpr int kTurnBytes = 32 * kTurnRow * 4;  // of a wave
+
+template <typename T>
+__device__ __forceinline__ void finish_rows(const GemmParams& p, const DropKey& key, const EpiCols<T>& cols, int split,
+                                            int row0, int col0, float* turn, const f32x16& x0, const f32x16& x1) {
+  const int lane = tid_x() & 63;
+  float* to = turn + (lane & 31) * kTurnRow + 4 * (lane >> 5);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    *reinterpret_cast<f32x4*>(to + 8 * q) = f32x4{x0[4 * q], x0[4 * q + 1], x0[4 * q + 2], x0[4 * q + 3]};
+    *reinterpret_cast<f32x4*>(to + 32 + 8 * q) = f32x4{x1[4 * q], x1[4 * q + 1], x1[4 * q + 2], x1[4 * q + 3]};
+  }
+  asm volatile("" ::: "memory");  // (a wave's LDS accesses stay in their order)
+  const int col = col0 + 8 * (lane & 7);
+  int row = row0 + (lane >> 3);
+  const float* from = turn + (lane >> 3) * kTurnRow + 8 * (lane & 7);
+  EpiPlace at;
+  at.init(p.epi, row, col);
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    float v[8];
+    load_vec<8>(from + pass * 8 * kTurnRow, v);
+    if (row < p.m && col < p.n) {
+      if (p.splits > 1)
+        store_vec<8>(p.part + ((int64_t)split * p.m + row) * p.ldp + col, v);
+      else
+        epilogue8<T>(p.epi, key, cols, at, row, col, v);
+    }
+    row += 8;
+    at.down(p.epi, 8);
+  }
+  asm volatile("" ::: "memory");
+}
+
+// Nothing moves across: the order of products, LDS reads and copies is the one written down.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// This wave's copies but the last N are there and all that it read from LDS has come back; then every wave's.
+template <int N>
+__device__ __forceinline__ void arrive() {
+  wait_vm<N>();
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  barrier_only();
+}
+
+// f(Int<0>()), f(Int<1>()), .., f(Int<N - 1>())
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void each(F f) {
+  if constexpr (I < N) {
+    f(Int<I>());
+    each<N, I + 1>(f);
+  }
+}
+
+// Tiles of 256 x 128 (UA 2; 80 KB of LDS, two work-groups a compute unit, so that one's epilogue lies under the other's
+// products) and 128 x 128 (UA 1). Four waves in two rows of two; each owns 64 x 64 of every unit of A. Units (128 x 64 of an
+// operand) go through a ring of LDS slots. A step of 64 is four groups of products (16 of the reduction each) of every A unit;
+// fragments are read into the registers that the groups before have done with:
+//   UA 2   group    0        1     |    2        3      4      5     |   6           7
+//          reads    B A0 k3        |  A1 k0 k1  A1 k2  A1 k3         | B A0 k0' k1'  B A0 k2'     (': of the next step)
+//          copies   A0"     A0" A0"|  A1'     A1' A1'  A1' B" B" B"  | B"           A0"
+// The first barrier waits for A1 of this step and frees B A0, the second waits for B A0 of the next step and frees A1.
+//   UA 1   group    0      1     |    2            3
+//          reads    B A k3       |  B A k0' k1'   B A k2'
+//          copies                |  B, A of the step whose place is free
+template <typename T, bool ACOLS, bool BCOLS, int UA, int SLOTS>
+__global__ void __launch_bounds__(256, SLOTS > 5 ? 1 : 2) gemm_kernel(const GemmParams p) {
   typedef typename Half<T>::vec8 vec8;
-  __shared__ __attribute__((aligned(16))) char lds[kSlots * kUnit];
+  typedef Feed<ACOLS, BCOLS, UA, 1, SLOTS> F;
+  __shared__ __attribute__((aligned(16))) char lds[SLOTS * kUnit];
   const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6);
   const int wm = wave >> 1, wn = wave & 1;
-
-  // Work-groups go to the eight XCDs in turn: each XCD takes a contiguous range of the tiles, which go by groups of eight
-  // rows of tiles, so that the work-groups of an XCD share operand rows in its L2.
-  const int tiles = p.tiles_m * p.tiles_n;
-  int id = bid_x(), split = 0;
-  const int all = tiles * p.splits;
-  {
-    const int q = all / 8, r = all % 8, x = id % 8;
-    id = x * q + (x < r ? x : r) + id / 8;
-  }
-  if (p.splits > 1) {
-    split = id / tiles;
-    id -= split * tiles;
-  }
-  int tm, tn;
-  {
-    const int per = 8 * p.tiles_n, g = id / per, in = id - g * per;
-    const int rows = p.tiles_m - 8 * g < 8 ? p.tiles_m - 8 * g : 8;
-    tn = in / rows;
-    tm = 8 * g + in - tn * rows;
-  }
-  const int m0 = tm * (kUnitRows * UA), n0 = tn * kUnitRows;
-  const int s0 = split * p.split_steps;
-  const int s1 = s0 + p.split_steps < p.steps ? s0 + p.split_steps : p.steps;
-  const int left = p.k - (p.steps - 1) * 64;           // elements of the last step
-  const int tail = left < 64 && s1 == p.steps ? p.steps - 1 : -1;  // the step with fewer than 64
-
-  Copy<ACOLS> ca[UA];
-  Copy<BCOLS> cb;
-  const char* abase[UA];
-#pragma unroll
-  for (int u = 0; u < UA; ++u) {
-    const int first = m0 + u * kUnitRows < p.m ? m0 + u * kUnitRows : 0;  // (a unit without a row reads the first one's)
-    ca[u].init(wave, lane, first, p.m, p.lda);
-    abase[u] = p.a + (ACOLS ? (int64_t)first * 2 : first * p.lda);
-  }
-  cb.init(wave, lane, n0, p.n, p.ldb);
-  const char* bbase = p.b + (BCOLS ? (int64_t)n0 * 2 : n0 * p.ldb);
-  const int64_t astep = ACOLS ? 64 * p.lda : 128, bstep = BCOLS ? 64 * p.ldb : 128;
-  const uint32_t lds0 = lds_addr(lds) + wave * 1024;
-
-  int put = 0;  // slot of the next unit that is copied
-  auto copy = [&](auto which, int step) {
-    constexpr int u = decltype(which)::value;  // 0: B, 1 + a: unit a of A
-    const uint32_t to = lds0 + put * kUnit;
-    put = put == kSlots - 1 ? 0 : put + 1;
-    if constexpr (u == 0) {
-      const char* base = bbase + step * bstep;
-      if (step == tail)
-        cb.issue_tail(base, to, left);
-      else
-        cb.issue(base, to);
-    } else {
-      const char* base = abase[u - 1] + step * astep;
-      if (step == tail)
-        ca[u - 1].issue_tail(base, to, left);
-      else
-        ca[u - 1].issue(base, to);
-    }
-  };
-
+  const Place at = place_of(p);
+  const int m0 = at.tm * (kUnitRows * UA), n0 = at.tn * kUnitRows;
+  F feed;
+  feed.init(p, at.split, m0, n0, wave, lane, lds);
   Frags<ACOLS, T> fa;
   Frags<BCOLS, T> fb;
   fa.init(lane, wm);
@@ -195,123 +267,285 @@ __global__ void __launch_bounds__(256, 2) gemm_kernel(const GemmParams p) {
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[u][i][j][e] = 0.f;
-
-  int got = 0;  // slot of the next unit that is read
-  auto next = [&]() {
-    const char* r = lds + got * kUnit;
-    got = got == kSlots - 1 ? 0 : got + 1;
-    return r;
+  vec8 af[2][4], bf[2][4];
+  auto read_a = [&](int slot, int i, int ks) { af[i][ks] = fa.get(lds + slot * kUnit, i, ks); };
+  auto read_b = [&](int slot, int j, int ks) { bf[j][ks] = fb.get(lds + slot * kUnit, j, ks); };
+  // read n of B and A of ks
+  auto read_ba = [&](int n, int b_slot, int a_slot, int ks) {
+    if (n < 2)
+      read_b(b_slot, n, ks);
+    else if (n < 4)
+      read_a(a_slot, n - 2, ks);
   };
-  // LDS reads of the last phase are done before the barrier that frees their slots
-  auto arrive = [&]() {
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-    barrier_only();
-  };
-  vec8 bf[2][4];
-  auto phase = [&](auto which, const char* ua) {
-    constexpr int u = decltype(which)::value;
-    vec8 af[2][4];
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) af[i][ks] = fa.get(ua, i, ks);
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[u][i][j] = Half<T>::mma32(bf[j][ks], af[i][ks], acc[u][i][j]);
-  };
-  auto read_b = [&](const char* ub) {
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) bf[j][ks] = fb.get(ub, j, ks);
+  // the products of ks of a unit, hook(n) behind the n-th of four
+  auto products = [&](auto which, auto at_k, auto hook) {
+    constexpr int u = decltype(which)::value, ks = decltype(at_k)::value;
+    each<4>([&](auto n) {
+      constexpr int i = decltype(n)::value / 2, j = decltype(n)::value % 2;
+      acc[u][i][j] = Half<T>::mma32(bf[j][ks], af[i][ks], acc[u][i][j]);
+      hook(n);
+      fence();
+    });
   };
 
-  copy(Int<0>(), s0);
-  copy(Int<1>(), s0);
-  if constexpr (UA == 2) copy(Int<2>(), s0);
-  if (s0 + 1 < s1) copy(Int<0>(), s0 + 1);
-#pragma unroll 1
-  for (int s = s0; s < s1 - 1; ++s) {
-    // (copies behind the ones that are waited for: A1 of this step and B of the next, or B of the next)
-    if constexpr (UA == 2)
-      wait_vm<8>();
-    else
-      wait_vm<4>();
-    arrive();
-    copy(Int<1>(), s + 1);
-    if constexpr (UA == 1) {
-      if (s + 2 < s1) copy(Int<0>(), s + 2);
-    }
-    const char* ub = next();
-    const char* ua = next();
-    read_b(ub);
-    phase(Int<0>(), ua);
-    if constexpr (UA == 2) {
-      wait_vm<8>();
-      arrive();
-      copy(Int<2>(), s + 1);
-      if (s + 2 < s1) copy(Int<0>(), s + 2);
-      phase(Int<1>(), next());
-    }
-  }
-  if constexpr (UA == 2)
-    wait_vm<4>();
-  else
-    wait_vm<0>();
-  arrive();
-  {
-    const char* ub = next();
-    const char* ua = next();
-    read_b(ub);
-    phase(Int<0>(), ua);
-  }
+  int s = feed.s0, slot = 0;  // slot: of B of this step
+  const int s1 = feed.s1, whole = feed.whole();
   if constexpr (UA == 2) {
-    wait_vm<0>();
-    arrive();
-    phase(Int<1>(), next());
+    feed.template unit<0>(s, 0);
+    feed.template unit<1>(s, 1);
+    feed.template unit<2>(s, 2);
+    feed.template unit<0>(s + 1, 3);
+    wait_vm<8>();
+    barrier_only();
+#pragma unroll
+    for (int ks = 0; ks < 3; ++ks)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) read_ba(n, 0, 1, ks);
+    fence();
+    auto step = [&](auto any, int s) {
+      constexpr bool kAny = decltype(any)::value;
+      const int a0 = F::after(slot, 1), a1 = F::after(slot, 2), b_next = F::after(slot, 3), a0_next = F::after(slot, 4);
+      products(Int<0>(), Int<0>(), [&](auto n) {
+        constexpr int m = decltype(n)::value;
+        read_ba(m, slot, a0, 3);
+        if constexpr (m == 1) feed.template one<1, 1, kAny>(s + 1, a0_next);
+      });
+      products(Int<0>(), Int<1>(), [&](auto n) {
+        constexpr int m = decltype(n)::value;
+        if constexpr (m == 0) feed.template one<1, 2, kAny>(s + 1, a0_next);
+        if constexpr (m == 2) feed.template one<1, 3, kAny>(s + 1, a0_next);
+      });
+      arrive<8>();  // (behind A1: B and A0 of the next step)
+      products(Int<0>(), Int<2>(), [&](auto n) {
+        constexpr int m = decltype(n)::value;
+        read_a(a1, m % 2, m / 2);
+        if constexpr (m == 2) feed.template one<2, 0, kAny>(s + 1, slot);
+      });
+      products(Int<0>(), Int<3>(), [&](auto n) {
+        constexpr int m = decltype(n)::value;
+        if constexpr (m % 2 == 1) read_a(a1, m / 2, 2);
+        if constexpr (m == 0) feed.template one<2, 1, kAny>(s + 1, slot);
+        if constexpr (m == 2) feed.template one<2, 2, kAny>(s + 1, slot);
+      });
+      products(Int<1>(), Int<0>(), [&](auto n) {
+        constexpr int m = decltype(n)::value;
+        if constexpr (m % 2 == 1) read_a(a1, m / 2, 3);
+        if constexpr (m == 0) feed.template one<2, 3, kAny>(s + 1, slot);
+        if constexpr (m == 2) feed.template one<0, 0, kAny>(s + 2, a0);
+      });
+      products(Int<1>(), Int<1>(), [&](auto n) {
+        constexpr int m = decltype(n)::value;
+        if constexpr (m == 0) feed.template one<0, 1, kAny>(s + 2, a0);
+        if constexpr (m == 2) feed.template one<0, 2, kAny>(s + 2, a0);
+      });
+      arrive<7>();  // (behind A0 of the next step: its A1 and three instructions of B behind it)
+      products(Int<1>(), Int<2>(), [&](auto n) {
+        constexpr int m = decltype(n)::value;
+        read_ba(m, b_next, a0_next, 0);
+        read_ba(m, b_next, a0_next, 1);
+        if constexpr (m == 2) feed.template one<0, 3, kAny>(s + 2, a0);
+      });
+      products(Int<1>(), Int<3>(), [&](auto n) {
+        constexpr int m = decltype(n)::value;
+        read_ba(m, b_next, a0_next, 2);
+        if constexpr (m == 1) feed.template one<1, 0, kAny>(s + 2, a1);
+      });
+      slot = b_next;
+    };
+    // (A0 of the second step, whose first instruction belongs to the step before)
+    feed.template one<1, 0, true>(s + 1, 4);
+#pragma unroll 1
+    for (; s + 2 < whole; ++s) step(Int<0>(), s);
+#pragma unroll 1
+    for (; s < s1; ++s) step(Int<1>(), s);
+  } else {
+    constexpr int kAhead = SLOTS / 2;  // steps whose units have a place
+    each<kAhead>([&](auto n) {
+      constexpr int i = decltype(n)::value;
+      feed.template unit<0>(s + i, 2 * i);
+      feed.template unit<1>(s + i, 2 * i + 1);
+    });
+    wait_vm<8 * (kAhead - 1)>();
+    barrier_only();
+#pragma unroll
+    for (int ks = 0; ks < 3; ++ks)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) read_ba(n, 0, 1, ks);
+    fence();
+    auto step = [&](auto any, int s) {
+      constexpr bool kAny = decltype(any)::value;
+      const int a0 = F::after(slot, 1), b_next = F::after(slot, 2), a_next = F::after(slot, 3);
+      products(Int<0>(), Int<0>(), [&](auto n) { read_ba(decltype(n)::value, slot, a0, 3); });
+      products(Int<0>(), Int<1>(), [&](auto) {});
+      arrive<8 * (kAhead - 2)>();
+      products(Int<0>(), Int<2>(), [&](auto n) {
+        constexpr int m = decltype(n)::value;
+        read_ba(m, b_next, a_next, 0);
+        read_ba(m, b_next, a_next, 1);
+        feed.template one<0, m, kAny>(s + kAhead, slot);
+      });
+      products(Int<0>(), Int<3>(), [&](auto n) {
+        constexpr int m = decltype(n)::value;
+        read_ba(m, b_next, a_next, 2);
+        feed.template one<1, m, kAny>(s + kAhead, a0);
+      });
+      slot = b_next;
+    };
+#pragma unroll 1
+    for (; s + kAhead < whole; ++s) step(Int<0>(), s);
+#pragma unroll 1
+    for (; s < s1; ++s) step(Int<1>(), s);
   }
+  wait_vm<0>();  // (no copy is under way when the work-group ends)
 
-  // A lane holds row l % 32 of a block, columns 8 q + 4 (l / 32) + e in element 4 q + e. Exchanged between the halves of the
-  // wave for pairs of q, it holds eight columns in a row: 16 (q / 2) + 8 (l / 32) .. + 7.
-  const int h = lane >> 5;
+  __syncthreads();  // (the slots are read to their end)
+  float* turn = reinterpret_cast<float*>(lds + wave * kTurnBytes);
+  DropKey key{};
+  if (p.epi.drop.limit) key = drop_key(p.epi.drop);
+  EpiCols<T> cols;
+  const int col0 = n0 + 64 * wn;
+  if (p.splits == 1 && col0 + 8 * (lane & 7) < p.n) cols.load(p.epi, col0 + 8 * (lane & 7));
+#pragma unroll 1
+  for (int blk = 0; blk < UA * 2; ++blk) {
+    f32x16 x0, x1;
+    switch (blk) {
+      case 0: x0 = acc[0][0][0], x1 = acc[0][0][1]; break;
+      case 1: x0 = acc[0][1][0], x1 = acc[0][1][1]; break;
+      case 2: x0 = acc[UA - 1][0][0], x1 = acc[UA - 1][0][1]; break;
+      default: x0 = acc[UA - 1][1][0], x1 = acc[UA - 1][1][1]; break;
+    }
+    finish_rows<T>(p, key, cols, at.split, m0 + (blk >> 1) * kUnitRows + 64 * wm + 32 * (blk & 1), col0, turn, x0, x1);
+  }
+}
+
+// 256 x 256 tile of four waves, one a SIMD: each owns 64 rows of both A units by a whole unit of B (128 x 128 in all, 256 sums a
+// lane), which reads 32 KB of LDS for 128 products, a third less than two waves of 128 x 64, and copies a third less than
+// tiles of 256 x 128. Every product is followed by at most a read and a copy, which issue under it (a 32x32x16 product
+// holds the pipe for 32 cycles). A step is four groups of 16 products:
+//   group    A0 k0 k1    |  A0 k2 k3    A1 k0 k1    A1 k2 k3
+//   reads    B A0 k2 k3  |  A1 k0 k1    A1 k2 k3    B A0 k0' k1'     (': of the next step)
+//   copies   B0"         |  B1"         A0"         A1"
+// into the registers, and slots, that the groups before have done with. The barrier waits for A1 of this step and B0 B1 A0 of
+// the next one; it frees B0 B1 A0 of this one and A1 of the last. The data path takes 28 cycles for an instruction of 1 KB,
+// 64 of them a step of 2048 cycles of products: they are spread evenly (in a burst behind the barrier, 8192^3 takes 902 us
+// in place of 820).
+template <typename T, bool ACOLS, bool BCOLS>
+__global__ void __launch_bounds__(256, 1) gemm_wide_kernel(const GemmParams p) {
+  typedef typename Half<T>::vec8 vec8;
+  typedef Feed<ACOLS, BCOLS, 2, 2, 10> F;
+  __shared__ __attribute__((aligned(16))) char lds[10 * kUnit];
+  const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const Place at = place_of(p);
+  const int m0 = at.tm * 256, n0 = at.tn * 256;
+  F feed;
+  feed.init(p, at.split, m0, n0, wave, lane, lds);
+  Frags<ACOLS, T> fa;
+  Frags<BCOLS, T> fb[2];
+  fa.init(lane, wm);
+  fb[0].init(lane, 0);
+  fb[1].init(lane, 1);
+  f32x16 acc[2][2][4];  // [unit][row block][column block]
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[u][i][j][e] = 0.f;
+  vec8 af[2][4], bf[4][4];
+  auto read_a = [&](int slot, int i, int ks) { af[i][ks] = fa.get(lds + slot * kUnit, i, ks); };
+  auto read_b = [&](int slot, int j, int ks) { bf[j][ks] = fb[j >> 1].get(lds + slot * kUnit, j & 1, ks); };
+  // read n of B and A of ks and ks + 1
+  auto read_ba = [&](int n, int b_slot, int a_slot, int ks) {
+    if (n < 8)
+      read_b(b_slot, n % 4, ks + n / 4);
+    else if (n < 12)
+      read_a(a_slot, n % 2, ks + (n - 8) / 2);
+  };
+  // the products of ks and ks + 1 of a unit, hook(n) behind the n-th of 16
+  auto products = [&](auto which, auto first, auto hook) {
+    constexpr int u = decltype(which)::value, k0 = decltype(first)::value;
+    each<16>([&](auto n) {
+      constexpr int m = decltype(n)::value, ks = k0 + m / 8, i = m / 4 % 2, j = m % 4;
+      acc[u][i][j] = Half<T>::mma32(bf[j][ks], af[i][ks], acc[u][i][j]);
+      hook(n);
+      fence();
+    });
+  };
+
+  int s = feed.s0, slot = 0;  // slot: of B0 of this step
+  each<2>([&](auto n) {
+    constexpr int i = decltype(n)::value;
+    feed.template unit<0>(s + i, 4 * i);
+    feed.template unit<1>(s + i, 4 * i + 1);
+    feed.template unit<2>(s + i, 4 * i + 2);
+    feed.template unit<3>(s + i, 4 * i + 3);
+  });
+  wait_vm<20>();
+  barrier_only();
+#pragma unroll
+  for (int n = 0; n < 12; ++n) read_ba(n, wn, 2, 0);
+  fence();
+  auto step = [&](auto any, int s) {
+    constexpr bool kAny = decltype(any)::value;
+    const int b_at = F::after(slot, wn), a0 = F::after(slot, 2), a1 = F::after(slot, 3);
+    const int b_next = F::after(slot, 4 + wn), a0_next = F::after(slot, 6);
+    const int to0 = F::after(slot, 8), to1 = F::after(slot, 9), to3 = F::after(slot, 1);
+    products(Int<0>(), Int<0>(), [&](auto n) {
+      constexpr int m = decltype(n)::value;
+      read_ba(m, b_at, a0, 2);
+      if constexpr (m % 4 == 1) feed.template one<0, m / 4, kAny>(s + 2, to0);
+    });
+    arrive<8>();  // (behind A0 of the next step: its A1 and B0 of the step after it)
+    products(Int<0>(), Int<2>(), [&](auto n) {
+      constexpr int m = decltype(n)::value;
+      if constexpr (m % 4 == 0) read_a(a1, m / 4 % 2, m / 8);
+      if constexpr (m % 4 == 1) feed.template one<1, m / 4, kAny>(s + 2, to1);
+    });
+    products(Int<1>(), Int<0>(), [&](auto n) {
+      constexpr int m = decltype(n)::value;
+      if constexpr (m % 2 == 0 && m < 8) read_a(a1, m / 2 % 2, 2 + m / 4);
+      if constexpr (m % 4 == 1) feed.template one<2, m / 4, kAny>(s + 2, slot);
+    });
+    products(Int<1>(), Int<2>(), [&](auto n) {
+      constexpr int m = decltype(n)::value;
+      read_ba(m, b_next, a0_next, 0);
+      if constexpr (m % 4 == 1) feed.template one<3, m / 4, kAny>(s + 2, to3);
+    });
+    slot = F::after(slot, 4);
+  };
+  const int s1 = feed.s1, whole = feed.whole();
+#pragma unroll 1
+  for (; s + 2 < whole; ++s) step(Int<0>(), s);
+#pragma unroll 1
+  for (; s < s1; ++s) step(Int<1>(), s);
+  wait_vm<0>();  // (no copy is under way when the work-group ends)
+
+  __syncthreads();  // (the slots are read to their end)
+  float* turn = reinterpret_cast<float*>(lds + wave * kTurnBytes);
   DropKey key{};
   if (p.epi.drop.limit) key = drop_key(p.epi.drop);
 #pragma unroll 1
-  for (int blk = 0; blk < UA * 4; ++blk) {
-    f32x16 x;
-    switch (blk) {
-      case 0: x = acc[0][0][0]; break;
-      case 1: x = acc[0][0][1]; break;
-      case 2: x = acc[0][1][0]; break;
-      case 3: x = acc[0][1][1]; break;
-      case 4: x = acc[UA - 1][0][0]; break;
-      case 5: x = acc[UA - 1][0][1]; break;
-      case 6: x = acc[UA - 1][1][0]; break;
-      default: x = acc[UA - 1][1][1]; break;
-    }
-    const int row = m0 + (blk >> 2) * kUnitRows + 64 * wm + 32 * ((blk >> 1) & 1) + (lane & 31);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int col = n0 + 64 * wn + 32 * (blk & 1) + 16 * half + 8 * h;
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // (as scalars first: the bits of a vector's element were taken from its first one)
-        const float lo = x[8 * half + e], hi = x[8 * half + 4 + e];
-        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi),
-                                                        false, false);
-        v[e] = __builtin_bit_cast(float, (uint32_t)r[0]);
-        v[4 + e] = __builtin_bit_cast(float, (uint32_t)r[1]);
+  for (int part = 0; part < 2; ++part) {
+    EpiCols<T> cols;
+    const int col0 = n0 + 128 * wn + 64 * part;
+    if (p.splits == 1 && col0 + 8 * (lane & 7) < p.n) cols.load(p.epi, col0 + 8 * (lane & 7));
+#pragma unroll 1
+    for (int blk = 0; blk < 4; ++blk) {
+      f32x16 x0, x1;
+      switch (4 * part + blk) {
+        case 0: x0 = acc[0][0][0], x1 = acc[0][0][1]; break;
+        case 1: x0 = acc[0][1][0], x1 = acc[0][1][1]; break;
+        case 2: x0 = acc[1][0][0], x1 = acc[1][0][1]; break;
+        case 3: x0 = acc[1][1][0], x1 = acc[1][1][1]; break;
+        case 4: x0 = acc[0][0][2], x1 = acc[0][0][3]; break;
+        case 5: x0 = acc[0][1][2], x1 = acc[0][1][3]; break;
+        case 6: x0 = acc[1][0][2], x1 = acc[1][0][3]; break;
+        default: x0 = acc[1][1][2], x1 = acc[1][1][3]; break;
       }
-      if (row < p.m && col < p.n) {
-        if (p.splits > 1)
-          store_vec<8>(p.part + ((int64_t)split * p.m + row) * p.ldp + col, v);
-        else
-          epilogue8<T>(p.epi, key, row, col, v);
-      }
+      finish_rows<T>(p, key, cols, at.split, m0 + (blk >> 1) * kUnitRows + 64 * wm + 32 * (blk & 1), col0, turn, x0, x1);
     }
   }
 }
@@ -403,26 +637,57 @@ __global__ void __launch_bounds__(256) join_kernel(const GemmParams p) {
 constexpr int kMaxSize = 1 << 21;         // widths of a layer (a unit's byte offsets stay in 32 bits)
 constexpr int64_t kMaxRows = 0x7fffff00;  // rows of a layer
 
-// How a product is split: tiles of 256 or 128 rows, splits of the reduction.
+// How a product runs: the kernel for few rows, or tiles of 128 UA by 128 UB and splits of the reduction.
 struct Plan {
   bool few;
-  int ua, splits, split_steps, steps, tiles_m, tiles_n;
+  int ua, ub, splits, split_steps, steps, tiles_m, tiles_n;
 };
 
+// Microseconds of a product with `wgs` work-groups of one kind and `steps` steps each, from what single kinds took over 70 to
+// 87936 rows, widths of 128 to 6144 and 1 to 16 splits: start and end; a step while every work-group has a compute unit of
+// its own (few of them, and more with their number: the card's clock goes down under load); of two on a unit, a step of the
+// slower and, with 512, of the whole card. A round behind the first costs half of one at least.
+static double tile_time(int kind, int64_t wgs, int64_t steps) {
+  constexpr struct {
+    double ends, alone, shared, two, full;
+    int places;
+  } kKinds[3] = {{8.5, 0.31, 0.16, 0.72, 1.00, 512}, {11.0, 0.49, 0.44, 1.20, 1.75, 512}, {19.0, 0.97, 0.60, 1.57, 1.57, 256}};
+  const auto& k = kKinds[kind];
+  const double x = (double)wgs / 256;
+  if (wgs <= 256) return k.ends + (double)steps * (k.alone + k.shared * x * x);
+  if (wgs <= k.places) return k.ends + (double)steps * (k.two + (k.full - k.two) * (x - 1));
+  const int64_t halves = (2 * wgs + k.places - 1) / k.places;
+  const double end = kind == 2 ? k.ends : 0.5 * k.ends;  // (of two on a unit, one ends under the other)
+  return k.ends + 0.5 * (double)halves * (double)steps * k.full + 0.5 * (double)(halves - 2) * end;
+}
+
+// Tiles and splits of the least such time. Splits have two steps at least; their join is a launch more, and writes and reads
+// the partial sums once (5.5 TB/s). Against one kind and split for all sizes: 4096 x 1024 from 1041 rows 27.6 -> 16.3 us,
+// 1024 x 1024 from 2748 rows 24 -> 15, 128 x 512 from 20000 rows 24.6 -> 18.9, 10992 x 1024 from 4096 105 -> 93.
 static Plan plan_of(int64_t m, int n, int64_t k, bool rows_kind) {
   Plan r{};
   r.steps = (int)((k + 63) / 64);
   r.few = rows_kind && m <= 64;
-  r.tiles_n = (n + 127) / 128;
-  const int64_t big = (m + 255) / 256 * r.tiles_n;
-  r.ua = big >= 384 ? 2 : 1;
-  r.tiles_m = (int)((m + 128 * r.ua - 1) / (128 * r.ua));
-  const int64_t tiles = (int64_t)r.tiles_m * r.tiles_n;
-  // splits of at least four steps that fill the 512 places
-  int64_t splits = tiles >= 384 ? 1 : std::min<int64_t>(512 / tiles, r.steps / 4);
-  if (splits < 1) splits = 1;
-  r.split_steps = (int)((r.steps + splits - 1) / splits);
-  r.splits = (r.steps + r.split_steps - 1) / r.split_steps;
+  double best = 1e300;
+  for (int kind = 0; kind < 3; ++kind) {
+    const int ua = kind ? 2 : 1, ub = kind == 2 ? 2 : 1;
+    const int64_t tm = (m + 128 * ua - 1) / (128 * ua), tn = ((int64_t)n + 128 * ub - 1) / (128 * ub);
+    for (int splits = 1; splits <= 64; splits += splits < 4 ? 1 : splits < 8 ? 2 : splits < 16 ? 4 : 8) {
+      if (splits > 1 && (r.steps < 2 * splits || tm * tn * splits > 1024)) break;
+      const int per = (r.steps + splits - 1) / splits, used = (r.steps + per - 1) / per;
+      double t = tile_time(kind, tm * tn * used, per);
+      if (used > 1) t += 2.5 + (double)used * (double)m * n * 8 / 5.5e6;
+      if (t < best) {
+        best = t;
+        r.ua = ua;
+        r.ub = ub;
+        r.splits = used;
+        r.split_steps = per;
+        r.tiles_m = (int)tm;
+        r.tiles_n = (int)tn;
+      }
+    }
+  }
   return r;
 }
 
@@ -465,10 +730,15 @@ static int product(const char* who, const void* a, int64_t lda, const void* b, i
   p.ldp = (n + 7) / 8 * 8;
   const int64_t grid = (int64_t)r.tiles_m * r.tiles_n * r.splits;
   if (grid > 0xffffffffll / 256) return fail(SAF3R_ERR_UNSUPPORTED, "%s: too many tiles for one launch", who);
-  if (r.ua == 2)
-    hipLaunchKernelGGL((gemm_kernel<T, ACOLS, BCOLS, 2>), dim3((uint32_t)grid), dim3(256), 0, stream, p);
+  const dim3 wgs((uint32_t)grid);
+  if (r.ub == 2)
+    hipLaunchKernelGGL((gemm_wide_kernel<T, ACOLS, BCOLS>), wgs, dim3(256), 0, stream, p);
+  else if (r.ua == 2)
+    hipLaunchKernelGGL((gemm_kernel<T, ACOLS, BCOLS, 2, 5>), wgs, dim3(256), 0, stream, p);
+  else if (grid <= 256)  // (one a compute unit: twice the units on their way)
+    hipLaunchKernelGGL((gemm_kernel<T, ACOLS, BCOLS, 1, 10>), wgs, dim3(256), 0, stream, p);
   else
-    hipLaunchKernelGGL((gemm_kernel<T, ACOLS, BCOLS, 1>), dim3((uint32_t)grid), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((gemm_kernel<T, ACOLS, BCOLS, 1, 4>), wgs, dim3(256), 0, stream, p);
   if (int e = check_launch(who)) return e;
   if (r.splits == 1) return SAF3R_OK;
   const int64_t threads = m * (p.ldp / 8);
