@@ -611,8 +611,8 @@ int64_t saf3r_layer_norm_bwd_workspace_bytes(int64_t rows, int dim);
 
 /*
  * Linear layer with its epilogue: y = residual + gate drop(act(x w^T + bias)), rows of `out` from rows of `in`.
- *   x [rows][in], w [out][in]: bf16 or fp16 (`type`), rows at 16-byte alignment (strides multiples of 8 elements), `in` a
- *   multiple of 8 (pad both with zeros otherwise).
+ *   x [rows][in], w [out][in]: bf16 or fp16 (`type`), any strides and alignment. Of an operand whose rows are not at 16-byte
+ *   alignment, or of no multiple of 8 elements, the workspace takes a copy first.
  *   bias, gate: [out] of param_type (fp32 or `type`), NULL: none. activation: enum saf3r_activation.
  *   drop: 65536 times the probability of dropping an element, 0 .. 65536 (0: no dropout); state: device int64 [2], the seed
  *   and the stream (its low 32 bits) of the keep mask, a function of them and of the element's row and column: sixteen bits
@@ -628,15 +628,15 @@ int saf3r_linear_fwd(const void* x, int64_t x_stride, const void* w, int64_t w_s
                      const int64_t* state, const void* residual, int64_t res_stride, void* y, int64_t y_stride,
                      int y_type, void* kept, int64_t kept_stride, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Workspace bytes of saf3r_linear_fwd (0 for most sizes), -1 for sizes that it rejects. */
-int64_t saf3r_linear_fwd_workspace_bytes(int64_t rows, int in, int out);
+/* Workspace bytes of saf3r_linear_fwd (0 for most sizes), -1 for sizes that it rejects. copies: 1: of x, 2: of w (their
+ * pointer is no multiple of 16 bytes, their stride or `in` none of 8 elements, or the stride is less than `in`). */
+int64_t saf3r_linear_fwd_workspace_bytes(int64_t rows, int in, int out, int copies);
 
 /*
  * Gradients of saf3r_linear_fwd from dy (rows of y_type; it is the residual's gradient itself), each may be NULL:
  *   dx (rows of `type`), dw [out][in] (rows of dw_type: fp32 or `type`), dbias and dgate [out] of param_type.
  *   kept: as written by the forward pass, for an activation or dgate. gate, activation, drop and state: of that call.
- *   x and w: rows at 16-byte alignment; where `in` is no multiple of 8 the elements up to the next one are read (and
- *   reach no result). The sums have a fixed order.
+ *   The sums have a fixed order: equal calls give equal bits.
  *   workspace: saf3r_linear_bwd_workspace_bytes, 16-byte aligned, for this call alone until it is done on its stream.
  */
 int saf3r_linear_bwd(const void* dy, int64_t dy_stride, int y_type, const void* x, int64_t x_stride, const void* w,
@@ -645,10 +645,10 @@ int saf3r_linear_bwd(const void* dy, int64_t dy_stride, int y_type, const void* 
                      int64_t dx_stride, void* dw, int64_t dw_stride, int dw_type, void* dbias, void* dgate,
                      void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Workspace bytes of saf3r_linear_bwd, -1 for sizes that it rejects. own_dz: whether anything lies between dy and the
- * products: a gate, an activation, dropout, dy of another type than `type` or in rows that are not 16-byte aligned, `out` no
- * multiple of 8. */
-int64_t saf3r_linear_bwd_workspace_bytes(int64_t rows, int in, int out, int own_dz);
+/* Workspace bytes of saf3r_linear_bwd, -1 for sizes that it rejects. copies: 1: of x (for dw), 2: of w (for dx), both as of
+ * saf3r_linear_fwd_workspace_bytes; 4: dz (dx or dw is asked for, and anything lies between dy and the products: a gate, an
+ * activation, dropout, another type than `type`, or rows that would be copied as x's are). */
+int64_t saf3r_linear_bwd_workspace_bytes(int64_t rows, int in, int out, int copies);
 
 /*
  * End of a branch and the norm before the next one: h = x + gate branch keep / (1 - p), y = LayerNorm(h), rows of `dim`

@@ -752,6 +752,36 @@ __global__ void __launch_bounds__(256) zero_rows_kernel(T* y, int64_t ld, int64_
   for (int64_t at = (int64_t)bid_x() * 256 + tid_x(); at < count; at += step) y[at / n * ld + at % n] = (T)0.f;
 }
 
+// Up to two matrices as rows of width8 (the next multiple of eight) elements with zeros behind `width`: operands whose rows
+// are not 16-byte aligned. A thread moves eight elements.
+struct PadParams {
+  const uint16_t* from[2];
+  uint16_t* to[2];
+  int64_t stride[2], rows[2];
+  int64_t vectors;  // of both
+  int width;
+};
+__global__ void __launch_bounds__(256) pad_rows_kernel(const PadParams p) {
+  int64_t at = (int64_t)bid_x() * 256 + tid_x();
+  if (at >= p.vectors) return;
+  const int groups = (p.width + 7) / 8;
+  const int which = at >= p.rows[0] * groups;
+  if (which) at -= p.rows[0] * groups;
+  const int64_t row = at / groups;
+  const int c = (int)(at - row * groups) * 8, n = p.width - c;
+  const uint16_t* from = p.from[which] + row * p.stride[which] + c;
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+  typedef u16x8 any __attribute__((aligned(2)));
+  u16x8 v;
+  if (n >= 8) {
+    v = *reinterpret_cast<const any*>(from);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? from[e] : (uint16_t)0;
+  }
+  *reinterpret_cast<u16x8*>(p.to[which] + (row * groups) * 8 + c) = v;
+}
+
 static bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 static int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 static int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -778,14 +808,43 @@ static int types_check(const char* who, int type, int param_type, int y_type, in
   return param_check(who, param_type, type);
 }
 
-// An operand of the products: `width` elements a row, read to the next multiple of eight.
-static int operand_check(const char* who, const char* name, const void* p, int64_t stride, int64_t width) {
+// An operand of the products, and whether they read it where it lies: rows at 16-byte alignment, of a multiple of eight.
+static int operand_check(const char* who, const char* name, const void* p, int64_t stride) {
   if (!p) return fail(SAF3R_ERR_INVALID, "%s: null %s", who, name);
-  if (!aligned16(p) || stride % 8) return fail(SAF3R_ERR_INVALID, "%s: rows of %s must be 16-byte aligned", who, name);
-  if (stride < round8(width) || stride > 2 * kMaxSize)
-    return fail(SAF3R_ERR_INVALID, "%s: row stride %lld of %s for rows of %lld", who, (long long)stride, name,
-                (long long)width);
+  if ((uintptr_t)p % 2) return fail(SAF3R_ERR_INVALID, "%s: rows of %s must be aligned to their elements", who, name);
+  if (stride < 0) return fail(SAF3R_ERR_INVALID, "%s: row stride %lld of %s", who, (long long)stride, name);
   return SAF3R_OK;
+}
+static bool in_place(const void* p, int64_t stride, int width) {
+  return aligned16(p) && stride % 8 == 0 && width % 8 == 0 && stride >= width && stride <= 2 * kMaxSize;
+}
+// bytes of an operand's copy
+static int64_t pad_bytes(int64_t rows, int width) { return round256(rows * round8(width) * 2); }
+
+// Copies the operands that are asked for to ws, one behind the other; their pointers and strides become the copies'.
+static int pad_operands(const char* who, char* ws, int width, const void** x, int64_t* x_stride, int64_t x_rows, bool pad_x,
+                        const void** w, int64_t* w_stride, int64_t w_rows, bool pad_w, hipStream_t stream) {
+  if (!pad_x && !pad_w) return SAF3R_OK;
+  PadParams p{};
+  p.width = width;
+  int n = 0;
+  auto add = [&](const void** t, int64_t* stride, int64_t rows) {
+    p.from[n] = (const uint16_t*)*t;
+    p.to[n] = (uint16_t*)ws;
+    p.stride[n] = *stride;
+    p.rows[n] = rows;
+    p.vectors += rows * (round8(width) / 8);
+    *t = ws;
+    *stride = round8(width);
+    ws += pad_bytes(rows, width);
+    ++n;
+  };
+  if (pad_x) add(x, x_stride, x_rows);
+  if (pad_w) add(w, w_stride, w_rows);
+  const int64_t grid = (p.vectors + 255) / 256;
+  if (grid > 0xffffffffll / 256) return fail(SAF3R_ERR_UNSUPPORTED, "%s: too many rows for one launch", who);
+  hipLaunchKernelGGL(pad_rows_kernel, dim3((uint32_t)grid), dim3(256), 0, stream, p);
+  return check_launch(who);
 }
 
 // rows of n that eight-element vectors can read or write
@@ -795,10 +854,12 @@ static bool vec_rows(const void* p, int64_t stride) { return aligned16(p) && str
 
 using namespace saf3r;
 
-extern "C" int64_t saf3r_linear_fwd_workspace_bytes(int64_t rows, int in, int out) {
+extern "C" int64_t saf3r_linear_fwd_workspace_bytes(int64_t rows, int in, int out, int copies) {
   const char* who = "saf3r_linear_fwd_workspace_bytes";
   if (sizes_check(who, rows, in, out)) return -1;
-  return rows ? part_bytes(plan_of(rows, out, in, true), rows, out) : 0;
+  if (rows == 0) return 0;
+  return part_bytes(plan_of(rows, out, in, true), rows, out) + (copies & 1 ? pad_bytes(rows, in) : 0) +
+         (copies & 2 ? pad_bytes(out, in) : 0);
 }
 
 extern "C" int saf3r_linear_fwd(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int type, int64_t rows,
@@ -813,9 +874,8 @@ extern "C" int saf3r_linear_fwd(const void* x, int64_t x_stride, const void* w, 
   EpiParams epi{};
   if (int e = drop_check(who, drop, state, &epi.drop)) return e;
   if (rows == 0) return SAF3R_OK;
-  if (in % 8) return fail(SAF3R_ERR_INVALID, "%s: rows of %d: the reduction must be a multiple of 8 (pad with zeros)", who, in);
-  if (int e = operand_check(who, "x", x, x_stride, in)) return e;
-  if (int e = operand_check(who, "w", w, w_stride, in)) return e;
+  if (int e = operand_check(who, "x", x, x_stride)) return e;
+  if (int e = operand_check(who, "w", w, w_stride)) return e;
   if (!y) return fail(SAF3R_ERR_INVALID, "%s: null y", who);
   if (int e = row_check(who, y, y_stride, out, y_type, true)) return e;
   if (kept)
@@ -825,7 +885,8 @@ extern "C" int saf3r_linear_fwd(const void* x, int64_t x_stride, const void* w, 
   for (const void* p : {bias, gate})
     if (p)
       if (int e = row_check(who, p, 0, out, param_type, false)) return e;
-  const int64_t need = saf3r_linear_fwd_workspace_bytes(rows, in, out);
+  const bool pad_x = !in_place(x, x_stride, in), pad_w = !in_place(w, w_stride, in);
+  const int64_t need = saf3r_linear_fwd_workspace_bytes(rows, in, out, pad_x + 2 * pad_w);
   if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace))))
     return fail(SAF3R_ERR_INVALID, "%s: workspace of %lld bytes: %lld, 16-byte aligned, are needed", who,
                 (long long)workspace_bytes, (long long)need);
@@ -844,29 +905,33 @@ extern "C" int saf3r_linear_fwd(const void* x, int64_t x_stride, const void* w, 
   epi.vec = out % 8 == 0 && vec_rows(y, y_stride) && aligned16(bias) && aligned16(gate) &&
             (!kept || vec_rows(kept, kept_stride)) && (!residual || vec_rows(residual, res_stride));
   const hipStream_t s = (hipStream_t)stream;
+  char* copies = (char*)workspace + part_bytes(plan_of(rows, out, in, true), rows, out);
+  if (int e = pad_operands(who, copies, in, &x, &x_stride, rows, pad_x, &w, &w_stride, out, pad_w, s)) return e;
+  const int k = (int)round8(in);  // (zeros behind `in` in both)
   if (type == SAF3R_BF16)
-    return product<__bf16, false, false>(who, x, x_stride, w, w_stride, rows, out, in, epi, workspace, s);
-  return product<_Float16, false, false>(who, x, x_stride, w, w_stride, rows, out, in, epi, workspace, s);
+    return product<__bf16, false, false>(who, x, x_stride, w, w_stride, rows, out, k, epi, workspace, s);
+  return product<_Float16, false, false>(who, x, x_stride, w, w_stride, rows, out, k, epi, workspace, s);
 }
 
-// Workspace of a backward pass: dz, the partial sums over rows, the split products (one after the other).
+// Workspace of a backward pass: dz, the partial sums over rows, copies of x and w, the split products (one after the other).
 struct BwdSizes {
-  int64_t dz, sums, products;
+  int64_t dz, sums, copies, products;
+  int64_t all() const { return dz + sums + copies + products; }
 };
-static BwdSizes bwd_sizes(int64_t rows, int in, int out, bool own_dz) {
+static BwdSizes bwd_sizes(int64_t rows, int in, int out, bool own_dz, bool pad_x, bool pad_w) {
   BwdSizes r{};
   if (rows == 0) return r;
+  r.copies = (pad_x ? pad_bytes(rows, in) : 0) + (pad_w ? pad_bytes(out, in) : 0);
   r.dz = own_dz ? round256(rows * round8(out) * 2) : 0;
   r.sums = round256(linear_grad_parts(rows, out) * 2 * out * 4);
   r.products = std::max(part_bytes(plan_of(rows, in, out, false), rows, in), part_bytes(plan_of(out, in, rows, false), out, in));
   return r;
 }
 
-extern "C" int64_t saf3r_linear_bwd_workspace_bytes(int64_t rows, int in, int out, int own_dz) {
+extern "C" int64_t saf3r_linear_bwd_workspace_bytes(int64_t rows, int in, int out, int copies) {
   const char* who = "saf3r_linear_bwd_workspace_bytes";
   if (sizes_check(who, rows, in, out)) return -1;
-  const BwdSizes r = bwd_sizes(rows, in, out, own_dz);
-  return r.dz + r.sums + r.products;
+  return bwd_sizes(rows, in, out, copies & 4, copies & 1, copies & 2).all();
 }
 
 extern "C" int saf3r_linear_bwd(const void* dy, int64_t dy_stride, int y_type, const void* x, int64_t x_stride,
@@ -891,9 +956,9 @@ extern "C" int saf3r_linear_bwd(const void* dy, int64_t dy_stride, int y_type, c
     if (!dy) return fail(SAF3R_ERR_INVALID, "%s: null dy", who);
     if (int e = row_check(who, dy, dy_stride, out, y_type, false)) return e;
     if (dw)
-      if (int e = operand_check(who, "x", x, x_stride, in)) return e;
+      if (int e = operand_check(who, "x", x, x_stride)) return e;
     if (dx) {
-      if (int e = operand_check(who, "w", w, w_stride, in)) return e;
+      if (int e = operand_check(who, "w", w, w_stride)) return e;
       if (int e = row_check(who, dx, dx_stride, in, type, true)) return e;
     }
     if ((activation != SAF3R_NO_ACTIVATION || dgate) && !kept)
@@ -904,10 +969,11 @@ extern "C" int saf3r_linear_bwd(const void* dy, int64_t dy_stride, int y_type, c
       if (int e = row_check(who, gate, 0, out, param_type, false)) return e;
   }
   // dy itself is the products' operand where nothing lies between
-  const bool own_dz = (dx || dw) && (activation != SAF3R_NO_ACTIVATION || gate || drop || y_type != type || out % 8 ||
-                                     !vec_rows(dy, dy_stride) || dy_stride < out || dy_stride > 2 * kMaxSize);
-  const BwdSizes size = bwd_sizes(rows, in, out, own_dz);
-  const int64_t need = size.dz + size.sums + size.products;
+  const bool own_dz = (dx || dw) && (activation != SAF3R_NO_ACTIVATION || gate || drop || y_type != type ||
+                                     !in_place(dy, dy_stride, out));
+  const bool pad_x = dw && !in_place(x, x_stride, in), pad_w = dx && !in_place(w, w_stride, in);
+  const BwdSizes size = bwd_sizes(rows, in, out, own_dz, pad_x, pad_w);
+  const int64_t need = size.all();
   if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace))))
     return fail(SAF3R_ERR_INVALID, "%s: workspace of %lld bytes: %lld, 16-byte aligned, are needed", who,
                 (long long)workspace_bytes, (long long)need);
@@ -951,7 +1017,9 @@ extern "C" int saf3r_linear_bwd(const void* dy, int64_t dy_stride, int y_type, c
       ld_dz = g.ld_dz;
     }
   }
-  void* part = ws + size.dz + size.sums;
+  if (int e = pad_operands(who, ws + size.dz + size.sums, in, &x, &x_stride, rows, pad_x, &w, &w_stride, out, pad_w, s))
+    return e;
+  void* part = ws + size.dz + size.sums + size.copies;
   auto plain = [&](void* y, int64_t ld, bool y32, int n) {
     EpiParams epi{};
     epi.y = y;

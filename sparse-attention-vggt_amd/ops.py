@@ -1334,53 +1334,58 @@ def _drop(p: float, state: torch.Tensor | None, dev: int) -> tuple[int, torch.Te
         return 0, None
     if state is None or state.dtype != torch.int64 or state.shape != (2,) or state.get_device() != dev:
         raise ValueError("dropout needs its state: int64 [2] on the rows' device (ops.dropout_state)")
-    return limit, state.contiguous()
+    return limit, state if state.is_contiguous() else state.contiguous()
 
 
-def _column_params(n: int, rows: torch.Tensor, **params):
-    """(type they are read in, the tensors): parameters of n columns, of one type, contiguous. Those that are neither fp32
+def _column_params(n: int, dt: torch.dtype, dev: int, names: tuple, params: tuple):
+    """(type they are read in, *the tensors): parameters of n columns, of one type, contiguous. Those that are neither fp32
     nor of the rows' type are read as fp32 copies. Without any, the rows' type."""
-    kind, dev = None, rows.get_device()
-    for name, t in params.items():
+    kind = None
+    for name, t in zip(names, params):
         if t is None:
             continue
-        if t.shape != (n,) or t.get_device() != dev:
-            raise ValueError(f"{name} must be [{n}] on {rows.device}, got {tuple(t.shape)} on {t.device}")
-        if kind is not None and t.dtype != kind:
-            raise ValueError(f"{' and '.join(params)} must have one dtype")
-        kind = t.dtype
-        _dtype(name, t)
+        if kind is None:
+            kind = t.dtype
+            if kind not in _DTYPES:
+                raise ValueError(f"{name} must be float32, bfloat16 or float16, got {kind}")
+        elif t.dtype != kind:
+            raise ValueError(f"{' and '.join(names)} must have one dtype")
+        if t.dim() != 1 or t.shape[0] != n or t.get_device() != dev:
+            raise ValueError(f"{name} must be [{n}] on the rows' device, got {tuple(t.shape)} on {t.device}")
     if kind is None:
-        return rows.dtype, *params.values()
-    read = kind if kind in (torch.float32, rows.dtype) else torch.float32
-    return read, *(None if t is None else t.to(read).contiguous() for t in params.values())
-
-
-def _operand(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """``t`` as rows that the products can read (16-byte aligned, a multiple of eight elements) and the row stride: itself,
-    or a copy with zeros behind each row."""
-    dim = t.shape[-1]
-    rows, stride = _flat_rows(t)
-    if not (dim % 8 or stride % 8 or stride < dim or rows.data_ptr() % 16):
-        return rows, stride
-    wide = -(-dim // 8) * 8
-    padded = t.new_zeros((*t.shape[:-1], wide))
-    padded[..., :dim] = t
-    return padded, wide
+        return dt, *params
+    if kind == dt or kind == torch.float32:
+        return kind, *(t if t is None or t.is_contiguous() else t.contiguous() for t in params)
+    return torch.float32, *(None if t is None else t.float() for t in params)
 
 
 def _linear_args(x, weight, activation):
+    """(the activation as the C entries take it, out, in)."""
+    dt = x.dtype
     if not (x.is_cuda and weight.is_cuda):
         raise ValueError("saf3r kernels take GPU tensors")
-    if x.dtype not in (torch.bfloat16, torch.float16) or weight.dtype != x.dtype:
-        raise ValueError(f"x and weight must be bfloat16 or float16 of one dtype, got {x.dtype} and {weight.dtype}")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
-        raise ValueError(f"weight must be [out, in] for rows of in, got {tuple(weight.shape)} for {tuple(x.shape)}")
+    if (dt != torch.bfloat16 and dt != torch.float16) or weight.dtype != dt:
+        raise ValueError(f"x and weight must be bfloat16 or float16 of one dtype, got {dt} and {weight.dtype}")
+    shape = weight.shape
+    if len(shape) != 2 or x.dim() < 1 or x.shape[-1] != shape[1] or not (shape[0] and shape[1]):
+        raise ValueError(f"weight must be [out, in] for rows of in, got {tuple(shape)} for {tuple(x.shape)}")
     if weight.get_device() != x.get_device():
         raise ValueError(f"weight is on {weight.device}, x on {x.device}")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation {activation!r}: one of {tuple(ACTIVATIONS)}")
-    return ACTIVATIONS[activation]
+    return ACTIVATIONS[activation], shape[0], shape[1]
+
+
+def _copied(ptr: int, stride: int, dim: int) -> bool:
+    """Whether the products take a copy of rows (``saf3r_linear_fwd_workspace_bytes``)."""
+    return bool((ptr & 15) | ((stride | dim) & 7)) or stride < dim or stride > 1 << 22
+
+
+@lru_cache(maxsize=4096)
+def _linear_bytes(backward: bool, rows: int, n_in: int, n_out: int, copies: int) -> int:
+    lib = _lib.load()
+    size = lib.saf3r_linear_bwd_workspace_bytes if backward else lib.saf3r_linear_fwd_workspace_bytes
+    return max(size(rows, n_in, n_out, copies), 0)
 
 
 def linear_fwd(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
@@ -1394,40 +1399,39 @@ def linear_fwd(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     rounded once. With ``keep`` a second tensor of x's type holds x weight^T + bias, for ``linear_bwd``. Rows that are not
     16-byte aligned, or widths that 8 does not divide, cost a copy of x or the weight. Not differentiable by itself: see
     ``autograd.linear``."""
-    act = _linear_args(x, weight, activation)
-    dev = x.get_device()
-    n, k = weight.shape
+    act, n, k = _linear_args(x, weight, activation)
+    dev, dt = x.get_device(), x.dtype
     shape = (*x.shape[:-1], n)
+    res, res_stride = None, 0
     if residual is not None:
-        if residual.shape != shape or residual.get_device() != dev or residual.dtype not in (torch.float32, x.dtype):
-            raise ValueError(f"residual must be float32 or {x.dtype} {shape} on {x.device}, got {residual.dtype} "
-                             f"{tuple(residual.shape)} on {residual.device}")
-        if out_dtype not in (None, residual.dtype):
-            raise ValueError(f"a {residual.dtype} residual gives {residual.dtype}, not {out_dtype}")
-        out_dtype = residual.dtype
+        kind = residual.dtype
+        if residual.shape != shape or residual.get_device() != dev or (kind != torch.float32 and kind != dt):
+            raise ValueError(f"residual must be float32 or {dt} {shape} on {x.device}, got {kind} {tuple(residual.shape)} on "
+                             f"{residual.device}")
+        if out_dtype is not None and out_dtype != kind:
+            raise ValueError(f"a {kind} residual gives {kind}, not {out_dtype}")
+        out_dtype = kind
+        res, res_stride = _flat_rows(residual)
     elif out_dtype is None:
-        out_dtype = x.dtype
-    elif out_dtype not in (torch.float32, x.dtype):
-        raise ValueError(f"{x.dtype} rows give {x.dtype} or float32, not {out_dtype}")
-    read, bias, gate = _column_params(n, x, bias=bias, gate=gate)
-    limit, drop_state = _drop(dropout, state, dev)
+        out_dtype = dt
+    elif out_dtype != torch.float32 and out_dtype != dt:
+        raise ValueError(f"{dt} rows give {dt} or float32, not {out_dtype}")
+    read, b, g = _column_params(n, dt, dev, ("bias", "gate"), (bias, gate))
+    limit, drop_state = _drop(dropout, state, dev) if dropout else (0, None)
     if dev != _here():
         with torch.cuda.device(x.device):
             return linear_fwd(x, weight, bias, activation, gate, residual, out_dtype, dropout, state, keep)
-    lib = _lib.load()
-    rows, stride = _operand(x)
-    w, wstride = _operand(weight)
-    res, res_stride = (None, 0) if residual is None else _flat_rows(residual)
-    y = x.new_empty(shape, dtype=out_dtype)
+    rows, stride = _flat_rows(x)
+    w, wstride = _flat_rows(weight)
+    y = x.new_empty(shape) if out_dtype == dt else x.new_empty(shape, dtype=out_dtype)
     kept = x.new_empty(shape) if keep else None
-    count, wide = y.numel() // n, -(-k // 8) * 8
-    nbytes = lib.saf3r_linear_fwd_workspace_bytes(count, wide, n)
-    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
+    xp, wp, count = rows.data_ptr(), w.data_ptr(), y.numel() // n
+    nbytes = _linear_bytes(False, count, k, n, _copied(xp, stride, k) | _copied(wp, wstride, k) << 1)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _mark("linear_fwd", "start")
-    _lib.check(lib.saf3r_linear_fwd(rows.data_ptr(), stride, w.data_ptr(), wstride, _DTYPES[x.dtype], count, wide, n,
-                                    _ptr(bias), _ptr(gate), _DTYPES[read], act, limit, _ptr(drop_state), _ptr(res),
-                                    res_stride, y.data_ptr(), n, _DTYPES[out_dtype], _ptr(kept), n, _ptr(ws),
-                                    max(nbytes, 0), _stream(dev)))
+    _lib.check(_lib.load().saf3r_linear_fwd(xp, stride, wp, wstride, _DTYPES[dt], count, k, n, _ptr(b), _ptr(g),
+                                            _DTYPES[read], act, limit, _ptr(drop_state), _ptr(res), res_stride, y.data_ptr(),
+                                            n, _DTYPES[out_dtype], _ptr(kept), n, _ptr(ws), nbytes, _stream(dev)))
     _mark("linear_fwd", "end")
     return (y, kept) if keep else y
 
@@ -1441,53 +1445,52 @@ def linear_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, kept: to
     gate's gradient; the other arguments are those of that call. ``need``: which of the four are computed, the others are
     None (dgate also without a gate). dweight is of ``weight_dtype`` (the weight's type or fp32), dbias and dgate of gate's
     type, without one of ``param_dtype`` (default x's). Equal inputs give equal bits."""
-    act = _linear_args(x, weight, activation)
-    dev = x.get_device()
-    n, k = weight.shape
+    act, n, k = _linear_args(x, weight, activation)
+    dev, dt = x.get_device(), x.dtype
     shape = (*x.shape[:-1], n)
-    if dy.shape != shape or dy.get_device() != dev or dy.dtype not in (torch.float32, x.dtype):
-        raise ValueError(f"dy must be float32 or {x.dtype} {shape} on {x.device}, got {dy.dtype} {tuple(dy.shape)} on "
-                         f"{dy.device}")
-    need_dx, need_dw, need_db, need_dg = (bool(v) for v in need)
+    if dy.shape != shape or dy.get_device() != dev or (dy.dtype != torch.float32 and dy.dtype != dt):
+        raise ValueError(f"dy must be float32 or {dt} {shape} on {x.device}, got {dy.dtype} {tuple(dy.shape)} on {dy.device}")
+    need_dx, need_dw, need_db, need_dg = need
     need_dg = need_dg and gate is not None
+    zrows, zstride = None, 0
     if kept is not None:
-        if kept.shape != shape or kept.dtype != x.dtype or kept.get_device() != dev:
-            raise ValueError(f"kept must be {x.dtype} {shape} on {x.device}, got {kept.dtype} {tuple(kept.shape)} on "
-                             f"{kept.device}")
-    elif activation is not None or need_dg:
+        if kept.shape != shape or kept.dtype != dt or kept.get_device() != dev:
+            raise ValueError(f"kept must be {dt} {shape} on {x.device}, got {kept.dtype} {tuple(kept.shape)} on {kept.device}")
+        zrows, zstride = _flat_rows(kept)
+    elif act or need_dg:
         raise ValueError("the gradients of an activation and of a gate need what the forward pass kept (keep=True)")
-    weight_dtype = x.dtype if weight_dtype is None else weight_dtype
-    if weight_dtype not in (torch.float32, x.dtype):
-        raise ValueError(f"dweight is {x.dtype} or float32, not {weight_dtype}")
-    kind = gate.dtype if gate is not None else x.dtype if param_dtype is None else param_dtype
+    if weight_dtype is None:
+        weight_dtype = dt
+    elif weight_dtype != torch.float32 and weight_dtype != dt:
+        raise ValueError(f"dweight is {dt} or float32, not {weight_dtype}")
+    kind = gate.dtype if gate is not None else dt if param_dtype is None else param_dtype
     if kind not in _DTYPES:
         raise ValueError(f"gradients of parameters in float32, bfloat16 or float16, not {kind}")
-    read, gate = _column_params(n, x, gate=gate)
-    if gate is None:
-        read = kind if kind == x.dtype else torch.float32
-    limit, drop_state = _drop(dropout, state, dev)
+    read, g = _column_params(n, dt, dev, ("gate",), (gate,))
+    if g is None and kind != dt:
+        read = torch.float32
+    limit, drop_state = _drop(dropout, state, dev) if dropout else (0, None)
     if dev != _here():
         with torch.cuda.device(x.device):
             return linear_bwd(dy, x, weight, kept, activation, gate, dropout, state, need, weight_dtype, kind)
-    lib = _lib.load()
     drows, dstride = _flat_rows(dy)
-    zrows, zstride = (None, 0) if kept is None else _flat_rows(kept)
-    rows, stride = _operand(x) if need_dw else (x, k)
-    w, wstride = _operand(weight) if need_dx else (weight, k)
+    rows, stride = _flat_rows(x)
+    w, wstride = _flat_rows(weight)
     dx = x.new_empty(x.shape) if need_dx else None
-    dw = x.new_empty((n, k), dtype=weight_dtype) if need_dw else None
+    dw = None if not need_dw else x.new_empty((n, k)) if weight_dtype == dt else x.new_empty((n, k), dtype=weight_dtype)
     db = x.new_empty(n, dtype=read) if need_db else None
     dg = x.new_empty(n, dtype=read) if need_dg else None
-    own_dz = (need_dx or need_dw) and bool(activation is not None or gate is not None or limit or dy.dtype != x.dtype or n % 8
-                                           or dstride % 8 or dstride < n or drows.data_ptr() % 16)
-    count = dy.numel() // n
-    nbytes = lib.saf3r_linear_bwd_workspace_bytes(count, k, n, own_dz)
-    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
+    dp, xp, wp, count = drows.data_ptr(), rows.data_ptr(), w.data_ptr(), dy.numel() // n
+    own_dz = act or g is not None or limit or dy.dtype != dt or _copied(dp, dstride, n)
+    copies = (need_dw and _copied(xp, stride, k)) | (need_dx and _copied(wp, wstride, k)) << 1 | (
+        4 if own_dz and (need_dx or need_dw) else 0)
+    nbytes = _linear_bytes(True, count, k, n, copies)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _mark("linear_bwd", "start")
-    _lib.check(lib.saf3r_linear_bwd(drows.data_ptr(), dstride, _DTYPES[dy.dtype], rows.data_ptr(), stride, w.data_ptr(), wstride,
-                                    _DTYPES[x.dtype], count, k, n, _ptr(zrows), zstride, _ptr(gate), _DTYPES[read], act,
-                                    limit, _ptr(drop_state), _ptr(dx), k, _ptr(dw), k, _DTYPES[weight_dtype], _ptr(db),
-                                    _ptr(dg), _ptr(ws), max(nbytes, 0), _stream(dev)))
+    _lib.check(_lib.load().saf3r_linear_bwd(dp, dstride, _DTYPES[dy.dtype], xp, stride, wp, wstride, _DTYPES[dt], count, k, n,
+                                            _ptr(zrows), zstride, _ptr(g), _DTYPES[read], act, limit, _ptr(drop_state),
+                                            _ptr(dx), k, _ptr(dw), k, _DTYPES[weight_dtype], _ptr(db), _ptr(dg), _ptr(ws),
+                                            nbytes, _stream(dev)))
     _mark("linear_bwd", "end")
     if kind != read:
         db, dg = (None if t is None else t.to(kind) for t in (db, dg))
@@ -1496,18 +1499,19 @@ def linear_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, kept: to
 
 # ---- the gated residual with the norm behind it, and dropout --------------------------------------------------
 
-def _residual_args(x, branch, out_dtype, **rows):
-    """(type of branch and y, the stream's and its type as the C entries take them)."""
-    shape, dt, dev = x.shape, x.dtype, x.get_device()
+def _residual_types(x, y_dtype) -> None:
+    dt, shape = x.dtype, x.shape
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"the stream must have a last dimension, got {tuple(shape)}")
-    xt = _dtype("the stream", x)
-    if out_dtype not in _DTYPES or (out_dtype != dt and dt != torch.float32):
-        raise ValueError(f"a {dt} stream takes branches and gives rows of its own type (fp32: any), not {out_dtype}")
-    for name, t, kind in [("branch", branch, out_dtype), *((n, *v) for n, v in rows.items())]:
-        if t is not None and (t.shape != shape or t.dtype != kind or t.get_device() != dev):
-            raise ValueError(f"{name} must be {kind} {tuple(shape)} on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return xt, _DTYPES[out_dtype]
+    if dt not in _DTYPES:
+        raise ValueError(f"the stream must be float32, bfloat16 or float16, got {dt}")
+    if y_dtype not in _DTYPES or (y_dtype != dt and dt != torch.float32):
+        raise ValueError(f"a {dt} stream takes branches and gives rows of its own type (fp32: any), not {y_dtype}")
+
+
+def _like_stream(name: str, t, x, kind) -> None:
+    if t.shape != x.shape or t.dtype != kind or t.get_device() != x.get_device():
+        raise ValueError(f"{name} must be {kind} {tuple(x.shape)} on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def residual_norm_fwd(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tensor | None = None,
@@ -1519,25 +1523,29 @@ def residual_norm_fwd(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tensor 
     branch's type). gate, weight and bias [dim] of one type. ``dropout``, ``state``: as of ``linear_fwd``. y is the norm
     of h as it is stored. Not differentiable by itself: see ``autograd.residual_norm``."""
     _need_cuda(x, branch)
-    out_dtype = branch.dtype if out_dtype is None else out_dtype
-    xt, yt = _residual_args(x, branch, out_dtype)
-    dim, dev = x.shape[-1], x.get_device()
-    read, gate, w, b = _column_params(dim, branch, gate=gate, weight=weight, bias=bias)
-    limit, drop_state = _drop(dropout, state, dev)
+    dt = x.dtype
+    if out_dtype is None:
+        out_dtype = branch.dtype
+    _residual_types(x, out_dtype)
+    _like_stream("branch", branch, x, out_dtype)
+    shape, dev = x.shape, x.get_device()
+    dim = shape[-1]
+    read, g, w, b = _column_params(dim, out_dtype, dev, ("gate", "weight", "bias"), (gate, weight, bias))
+    limit, drop_state = _drop(dropout, state, dev) if dropout else (0, None)
     if dev != _here():
         with torch.cuda.device(x.device):
             return residual_norm_fwd(x, branch, gate, weight, bias, eps, out_dtype, dropout, state)
     rows, stride = _flat_rows(x)
     brows, bstride = _flat_rows(branch)
-    h = x.new_empty(x.shape)
-    y = x.new_empty(x.shape, dtype=out_dtype)
-    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    h = torch.empty_like(x) if rows is x else x.new_empty(shape)
+    y = torch.empty_like(branch) if brows is branch else branch.new_empty(shape)
+    mean = x.new_empty(shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
     _mark("residual_norm_fwd", "start")
     _lib.check(_lib.load().saf3r_residual_norm_fwd(
-        rows.data_ptr(), stride, xt, brows.data_ptr(), bstride, yt, mean.numel(), dim, _ptr(gate), _ptr(w), _ptr(b),
-        _DTYPES[read], limit, _ptr(drop_state), eps, h.data_ptr(), dim, y.data_ptr(), dim, mean.data_ptr(), rstd.data_ptr(),
-        _stream(dev)))
+        rows.data_ptr(), stride, _DTYPES[dt], brows.data_ptr(), bstride, _DTYPES[out_dtype], mean.numel(), dim, _ptr(g), _ptr(w),
+        _ptr(b), _DTYPES[read], limit, _ptr(drop_state), eps, h.data_ptr(), dim, y.data_ptr(), dim, mean.data_ptr(),
+        rstd.data_ptr(), _stream(dev)))
     _mark("residual_norm_fwd", "end")
     return h, y, mean, rstd
 
@@ -1552,42 +1560,54 @@ def residual_norm_bwd(dh: torch.Tensor | None, dy: torch.Tensor, h: torch.Tensor
     dbias are computed; the others are None, dgate also without a gate. The parameters' gradients are of their type
     (without one of y's). Equal inputs give equal bits."""
     _need_cuda(h, dy)
-    dev, dim = h.get_device(), h.shape[-1] if h.dim() else 0
-    xt, yt = _residual_args(h, branch, dy.dtype, dy=(dy, dy.dtype), dh=(dh, h.dtype))
-    stats = h.shape[:-1]
+    yt = dy.dtype
+    _residual_types(h, yt)
+    _like_stream("dy", dy, h, yt)
+    need_db, need_dg, need_dw, need_dbias = need
+    need_dg = need_dg and gate is not None
+    up, up_stride, brows, bstride = None, 0, None, 0
+    if dh is not None:
+        _like_stream("dh", dh, h, h.dtype)
+        up, up_stride = _flat_rows(dh)
+    if need_dg:
+        if branch is None:
+            raise ValueError("the gate's gradient needs the branch")
+        _like_stream("branch", branch, h, yt)
+        brows, bstride = _flat_rows(branch)
+    shape, dev = h.shape, h.get_device()
+    dim, stats = shape[-1], shape[:-1]
     for n, t in (("mean", mean), ("rstd", rstd)):
         if t.shape != stats or t.dtype != torch.float32 or t.get_device() != dev:
             raise ValueError(f"{n} must be float32 {tuple(stats)} on {h.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    need_db, need_dg, need_dw, need_dbias = (bool(v) for v in need)
-    need_dg = need_dg and gate is not None
-    if need_dg and branch is None:
-        raise ValueError("the gate's gradient needs the branch")
-    kind = next((t.dtype for t in (gate, weight) if t is not None), dy.dtype)
-    read, g, w = _column_params(dim, dy, gate=gate, weight=weight)
-    limit, drop_state = _drop(dropout, state, dev)
+    kind = gate.dtype if gate is not None else yt if weight is None else weight.dtype
+    read, g, w = _column_params(dim, yt, dev, ("gate", "weight"), (gate, weight))
+    limit, drop_state = _drop(dropout, state, dev) if dropout else (0, None)
     if dev != _here():
         with torch.cuda.device(h.device):
             return residual_norm_bwd(dh, dy, h, mean, rstd, branch, gate, weight, dropout, state, need)
     lib = _lib.load()
-    up, up_stride = (None, 0) if dh is None else _flat_rows(dh)
     drows, dstride = _flat_rows(dy)
     hrows, hstride = _flat_rows(h)
-    brows, bstride = _flat_rows(branch) if need_dg else (None, 0)
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    dx = h.new_empty(h.shape)
-    dbranch = dy.new_empty(h.shape) if need_db else None
+    dx = torch.empty_like(h) if hrows is h else h.new_empty(shape)
+    dbranch = None if not need_db else torch.empty_like(dy) if drows is dy else dy.new_empty(shape)
     dg, dw, db = (h.new_empty(dim, dtype=read) if n else None for n in (need_dg, need_dw, need_dbias))
-    nbytes = lib.saf3r_residual_norm_bwd_workspace_bytes(mean.numel(), dim) if need_dg or need_dw or need_dbias else 0
-    ws = h.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
+    nbytes = _residual_bytes(mean.numel(), dim) if need_dg or need_dw or need_dbias else 0
+    ws = h.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _mark("residual_norm_bwd", "start")
     _lib.check(lib.saf3r_residual_norm_bwd(
-        _ptr(up), up_stride, drows.data_ptr(), dstride, yt, hrows.data_ptr(), hstride, xt, _ptr(brows), bstride, mean.numel(),
-        dim, mean.data_ptr(), rstd.data_ptr(), _ptr(g), _ptr(w), _DTYPES[read], limit, _ptr(drop_state), dx.data_ptr(), dim,
-        _ptr(dbranch), dim, _ptr(dg), _ptr(dw), _ptr(db), _ptr(ws), max(nbytes, 0), _stream(dev)))
+        _ptr(up), up_stride, drows.data_ptr(), dstride, _DTYPES[yt], hrows.data_ptr(), hstride, _DTYPES[h.dtype], _ptr(brows),
+        bstride, mean.numel(), dim, mean.data_ptr(), rstd.data_ptr(), _ptr(g), _ptr(w), _DTYPES[read], limit, _ptr(drop_state),
+        dx.data_ptr(), dim, _ptr(dbranch), dim, _ptr(dg), _ptr(dw), _ptr(db), _ptr(ws), nbytes, _stream(dev)))
     _mark("residual_norm_bwd", "end")
     if kind != read:
         dg, dw, db = (None if t is None else t.to(kind) for t in (dg, dw, db))
     return dx, dbranch, dg, dw, db
+
+
+@lru_cache(maxsize=1024)
+def _residual_bytes(rows: int, dim: int) -> int:
+    return max(_lib.load().saf3r_residual_norm_bwd_workspace_bytes(rows, dim), 0)
 
 
 def dropout(x: torch.Tensor, p: float, state: torch.Tensor) -> torch.Tensor:
