@@ -144,13 +144,11 @@ struct EpiPlace {
   }
 };
 
-// The epilogue of columns col .. col + 7 of a row that is there.
+// The epilogue of columns col .. col + 7 of a row that is there; r: the residual's.
 template <typename T>
 __device__ __forceinline__ void epilogue8(const EpiParams& e, const DropKey& key, const EpiCols<T>& c, const EpiPlace& at,
-                                          int64_t row, int col, float (&x)[8]) {
+                                          int64_t row, int col, const float (&r)[8], float (&x)[8]) {
   const int cnt = e.n - col;
-  float r[8];
-  if (e.res) epi_load<T>(e.res, e.y32, e.vec, at.res, cnt, r);
   if (e.bias) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] += c.bias[j];
@@ -181,9 +179,11 @@ template <typename T>
 __device__ __forceinline__ void epilogue8(const EpiParams& e, const DropKey& key, int64_t row, int col, float (&x)[8]) {
   EpiCols<T> c;
   EpiPlace at;
+  float r[8];
   c.load(e, col);
   at.init(e, row, col);
-  epilogue8<T>(e, key, c, at, row, col, x);
+  if (e.res) epi_load<T>(e.res, e.y32, e.vec, at.res, e.n - col, r);
+  epilogue8<T>(e, key, c, at, row, col, r, x);
 }
 
 // First step of a backward pass (linear_grad.hip): dz = dy gate keep/(1-p) act'(kept), rounded to the operands' type, and the

@@ -74,7 +74,7 @@ struct Copy {
 };
 
 // The copies of a work-group of four waves: units 0 .. UB - 1 of a step are B's, the next UA are A's. With ANY a step may be
-// the last one, of which `left` of 64 is there, or behind it: zeros are copied, so that every step copies and waits alike.
+// the last one, of which `left` of 64 is there.
 template <bool ACOLS, bool BCOLS, int UA, int UB, int SLOTS>
 struct Feed {
   Copy<ACOLS> a[UA];
@@ -103,7 +103,7 @@ struct Feed {
   template <int U, int J, bool ANY>
   __device__ __forceinline__ void one(int step, int slot) const {
     const uint32_t to = lds0 + slot * kUnit;
-    const int there = ANY ? (step >= s1 ? 0 : step == tail ? left : 64) : 64;
+    const int there = ANY && step == tail ? left : 64;
     if constexpr (U < UB)
       b[U].template issue<J, ANY>(step * bstep, to, there);
     else
@@ -111,6 +111,7 @@ struct Feed {
   }
   template <int U>
   __device__ __forceinline__ void unit(int step, int slot) const {
+    if (step >= s1) return;
     one<U, 0, true>(step, slot);
     one<U, 1, true>(step, slot);
     one<U, 2, true>(step, slot);
@@ -183,7 +184,18 @@ constexpr int kTurnBytes = 32 * kTurnRow * 4;  // of a wave
 template <typename T>
 __device__ __forceinline__ void finish_rows(const GemmParams& p, const DropKey& key, const EpiCols<T>& cols, int split,
                                             int row0, int col0, float* turn, const f32x16& x0, const f32x16& x1) {
-  const int lane = tid_x() & 63;
+  const int lane = tid_x() & 63, col = col0 + 8 * (lane & 7);
+  int row = row0 + (lane >> 3);
+  EpiPlace at;
+  at.init(p.epi, row, col);
+  // (the residual is on its way while the rows turn)
+  float res[4][8];
+  if (p.epi.res && p.splits == 1) {
+#pragma unroll
+    for (int pass = 0; pass < 4; ++pass)
+      if (row + 8 * pass < p.m && col < p.n)
+        epi_load<T>(p.epi.res, p.epi.y32, p.epi.vec, at.res + 8 * pass * p.epi.ld_res, p.epi.n - col, res[pass]);
+  }
   float* to = turn + (lane & 31) * kTurnRow + 4 * (lane >> 5);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -191,11 +203,7 @@ __device__ __forceinline__ void finish_rows(const GemmParams& p, const DropKey& 
     *reinterpret_cast<f32x4*>(to + 32 + 8 * q) = f32x4{x1[4 * q], x1[4 * q + 1], x1[4 * q + 2], x1[4 * q + 3]};
   }
   asm volatile("" ::: "memory");  // (a wave's LDS accesses stay in their order)
-  const int col = col0 + 8 * (lane & 7);
-  int row = row0 + (lane >> 3);
   const float* from = turn + (lane >> 3) * kTurnRow + 8 * (lane & 7);
-  EpiPlace at;
-  at.init(p.epi, row, col);
 #pragma unroll
   for (int pass = 0; pass < 4; ++pass) {
     float v[8];
@@ -204,7 +212,7 @@ __device__ __forceinline__ void finish_rows(const GemmParams& p, const DropKey& 
       if (p.splits > 1)
         store_vec<8>(p.part + ((int64_t)split * p.m + row) * p.ldp + col, v);
       else
-        epilogue8<T>(p.epi, key, cols, at, row, col, v);
+        epilogue8<T>(p.epi, key, cols, at, row, col, res[pass], v);
     }
     row += 8;
     at.down(p.epi, 8);
@@ -295,69 +303,83 @@ __global__ void __launch_bounds__(256, SLOTS > 5 ? 1 : 2) gemm_kernel(const Gemm
     feed.template unit<1>(s, 1);
     feed.template unit<2>(s, 2);
     feed.template unit<0>(s + 1, 3);
-    wait_vm<8>();
+    if (s + 1 < s1)
+      wait_vm<8>();
+    else
+      wait_vm<4>();
     barrier_only();
 #pragma unroll
     for (int ks = 0; ks < 3; ++ks)
 #pragma unroll
       for (int n = 0; n < 4; ++n) read_ba(n, 0, 1, ks);
     fence();
-    auto step = [&](auto any, int s) {
-      constexpr bool kAny = decltype(any)::value;
+    // Copies of a step: NEXT: of the next one, LATER: of the one behind it (2: with the check for the last step).
+    auto step = [&](auto next, auto later, int s) {
+      constexpr int kNext = decltype(next)::value, kLater = decltype(later)::value;
       const int a0 = F::after(slot, 1), a1 = F::after(slot, 2), b_next = F::after(slot, 3), a0_next = F::after(slot, 4);
+      auto copy_next = [&](auto unit, auto j, int to) {
+        if constexpr (kNext != 0) feed.template one<decltype(unit)::value, decltype(j)::value, kNext == 2>(s + 1, to);
+      };
+      auto copy_later = [&](auto unit, auto j, int to) {
+        if constexpr (kLater != 0) feed.template one<decltype(unit)::value, decltype(j)::value, kLater == 2>(s + 2, to);
+      };
       products(Int<0>(), Int<0>(), [&](auto n) {
         constexpr int m = decltype(n)::value;
         read_ba(m, slot, a0, 3);
-        if constexpr (m == 1) feed.template one<1, 1, kAny>(s + 1, a0_next);
+        if constexpr (m == 1) copy_next(Int<1>(), Int<1>(), a0_next);
       });
       products(Int<0>(), Int<1>(), [&](auto n) {
         constexpr int m = decltype(n)::value;
-        if constexpr (m == 0) feed.template one<1, 2, kAny>(s + 1, a0_next);
-        if constexpr (m == 2) feed.template one<1, 3, kAny>(s + 1, a0_next);
+        if constexpr (m == 0) copy_next(Int<1>(), Int<2>(), a0_next);
+        if constexpr (m == 2) copy_next(Int<1>(), Int<3>(), a0_next);
       });
-      arrive<8>();  // (behind A1: B and A0 of the next step)
+      arrive<kNext ? 8 : 0>();  // (behind A1: B and A0 of the next step)
       products(Int<0>(), Int<2>(), [&](auto n) {
         constexpr int m = decltype(n)::value;
         read_a(a1, m % 2, m / 2);
-        if constexpr (m == 2) feed.template one<2, 0, kAny>(s + 1, slot);
+        if constexpr (m == 2) copy_next(Int<2>(), Int<0>(), slot);
       });
       products(Int<0>(), Int<3>(), [&](auto n) {
         constexpr int m = decltype(n)::value;
         if constexpr (m % 2 == 1) read_a(a1, m / 2, 2);
-        if constexpr (m == 0) feed.template one<2, 1, kAny>(s + 1, slot);
-        if constexpr (m == 2) feed.template one<2, 2, kAny>(s + 1, slot);
+        if constexpr (m == 0) copy_next(Int<2>(), Int<1>(), slot);
+        if constexpr (m == 2) copy_next(Int<2>(), Int<2>(), slot);
       });
       products(Int<1>(), Int<0>(), [&](auto n) {
         constexpr int m = decltype(n)::value;
         if constexpr (m % 2 == 1) read_a(a1, m / 2, 3);
-        if constexpr (m == 0) feed.template one<2, 3, kAny>(s + 1, slot);
-        if constexpr (m == 2) feed.template one<0, 0, kAny>(s + 2, a0);
+        if constexpr (m == 0) copy_next(Int<2>(), Int<3>(), slot);
+        if constexpr (m == 2) copy_later(Int<0>(), Int<0>(), a0);
       });
       products(Int<1>(), Int<1>(), [&](auto n) {
         constexpr int m = decltype(n)::value;
-        if constexpr (m == 0) feed.template one<0, 1, kAny>(s + 2, a0);
-        if constexpr (m == 2) feed.template one<0, 2, kAny>(s + 2, a0);
+        if constexpr (m == 0) copy_later(Int<0>(), Int<1>(), a0);
+        if constexpr (m == 2) copy_later(Int<0>(), Int<2>(), a0);
       });
-      arrive<7>();  // (behind A0 of the next step: its A1 and three instructions of B behind it)
+      // (behind A0 of the next step: its A1 and three instructions of B behind it)
+      if constexpr (kNext != 0) arrive<kLater ? 7 : 4>();
       products(Int<1>(), Int<2>(), [&](auto n) {
         constexpr int m = decltype(n)::value;
-        read_ba(m, b_next, a0_next, 0);
-        read_ba(m, b_next, a0_next, 1);
-        if constexpr (m == 2) feed.template one<0, 3, kAny>(s + 2, a0);
+        if constexpr (kNext != 0) {
+          read_ba(m, b_next, a0_next, 0);
+          read_ba(m, b_next, a0_next, 1);
+        }
+        if constexpr (m == 2) copy_later(Int<0>(), Int<3>(), a0);
       });
       products(Int<1>(), Int<3>(), [&](auto n) {
         constexpr int m = decltype(n)::value;
-        read_ba(m, b_next, a0_next, 2);
-        if constexpr (m == 1) feed.template one<1, 0, kAny>(s + 2, a1);
+        if constexpr (kNext != 0) read_ba(m, b_next, a0_next, 2);
+        if constexpr (m == 1) copy_later(Int<1>(), Int<0>(), a1);
       });
       slot = b_next;
     };
     // (A0 of the second step, whose first instruction belongs to the step before)
-    feed.template one<1, 0, true>(s + 1, 4);
+    if (s + 1 < s1) feed.template one<1, 0, true>(s + 1, 4);
 #pragma unroll 1
-    for (; s + 2 < whole; ++s) step(Int<0>(), s);
-#pragma unroll 1
-    for (; s < s1; ++s) step(Int<1>(), s);
+    for (; s + 2 < whole; ++s) step(Int<1>(), Int<1>(), s);
+    if (s + 2 < s1) step(Int<1>(), Int<2>(), s++);
+    if (s + 1 < s1) step(Int<2>(), Int<0>(), s++);
+    step(Int<0>(), Int<0>(), s);
   } else {
     constexpr int kAhead = SLOTS / 2;  // steps whose units have a place
     each<kAhead>([&](auto n) {
@@ -365,39 +387,47 @@ __global__ void __launch_bounds__(256, SLOTS > 5 ? 1 : 2) gemm_kernel(const Gemm
       feed.template unit<0>(s + i, 2 * i);
       feed.template unit<1>(s + i, 2 * i + 1);
     });
-    wait_vm<8 * (kAhead - 1)>();
+    if (s1 - s >= kAhead)
+      wait_vm<8 * (kAhead - 1)>();
+    else
+      wait_vm<0>();
     barrier_only();
 #pragma unroll
     for (int ks = 0; ks < 3; ++ks)
 #pragma unroll
       for (int n = 0; n < 4; ++n) read_ba(n, 0, 1, ks);
     fence();
-    auto step = [&](auto any, int s) {
-      constexpr bool kAny = decltype(any)::value;
+    // behind: steps behind the next one whose copies are under way; ahead: copies of step s + kAhead (2: with the check for
+    // the last step)
+    auto step = [&](auto behind, auto ahead, int s) {
+      constexpr int kBehind = decltype(behind)::value, kCopy = decltype(ahead)::value;
       const int a0 = F::after(slot, 1), b_next = F::after(slot, 2), a_next = F::after(slot, 3);
       products(Int<0>(), Int<0>(), [&](auto n) { read_ba(decltype(n)::value, slot, a0, 3); });
       products(Int<0>(), Int<1>(), [&](auto) {});
-      arrive<8 * (kAhead - 2)>();
+      if constexpr (kBehind >= 0) arrive<8 * (kBehind > 0 ? kBehind : 0)>();
       products(Int<0>(), Int<2>(), [&](auto n) {
         constexpr int m = decltype(n)::value;
-        read_ba(m, b_next, a_next, 0);
-        read_ba(m, b_next, a_next, 1);
-        feed.template one<0, m, kAny>(s + kAhead, slot);
+        if constexpr (kBehind >= 0) {
+          read_ba(m, b_next, a_next, 0);
+          read_ba(m, b_next, a_next, 1);
+        }
+        if constexpr (kCopy != 0) feed.template one<0, m, kCopy == 2>(s + kAhead, slot);
       });
       products(Int<0>(), Int<3>(), [&](auto n) {
         constexpr int m = decltype(n)::value;
-        read_ba(m, b_next, a_next, 2);
-        feed.template one<1, m, kAny>(s + kAhead, a0);
+        if constexpr (kBehind >= 0) read_ba(m, b_next, a_next, 2);
+        if constexpr (kCopy != 0) feed.template one<1, m, kCopy == 2>(s + kAhead, a0);
       });
       slot = b_next;
     };
 #pragma unroll 1
-    for (; s + kAhead < whole; ++s) step(Int<0>(), s);
-#pragma unroll 1
-    for (; s < s1; ++s) step(Int<1>(), s);
+    for (; s + kAhead < whole; ++s) step(Int<kAhead - 2>(), Int<1>(), s);
+    if (s + kAhead < s1) step(Int<kAhead - 2>(), Int<2>(), s++);
+    each<kAhead>([&](auto n) {  // the last kAhead steps
+      constexpr int r = kAhead - decltype(n)::value;
+      if (s1 - s == r) step(Int<r - 2>(), Int<0>(), s++);
+    });
   }
-  wait_vm<0>();  // (no copy is under way when the work-group ends)
-
   __syncthreads();  // (the slots are read to their end)
   float* turn = reinterpret_cast<float*>(lds + wave * kTurnBytes);
   DropKey key{};
@@ -483,46 +513,53 @@ __global__ void __launch_bounds__(256, 1) gemm_wide_kernel(const GemmParams p) {
     feed.template unit<2>(s + i, 4 * i + 2);
     feed.template unit<3>(s + i, 4 * i + 3);
   });
-  wait_vm<20>();
+  if (s + 1 < feed.s1)
+    wait_vm<20>();
+  else
+    wait_vm<4>();
   barrier_only();
 #pragma unroll
   for (int n = 0; n < 12; ++n) read_ba(n, wn, 2, 0);
   fence();
-  auto step = [&](auto any, int s) {
-    constexpr bool kAny = decltype(any)::value;
+  // ahead: copies of step s + 2 (2: with the check for the last step; 0: none, and all that is under way is waited for)
+  auto step = [&](auto ahead, int s) {
+    constexpr int kCopy = decltype(ahead)::value;
+    auto copy = [&](auto unit, auto j, int to) {
+      if constexpr (kCopy != 0) feed.template one<decltype(unit)::value, decltype(j)::value, kCopy == 2>(s + 2, to);
+    };
     const int b_at = F::after(slot, wn), a0 = F::after(slot, 2), a1 = F::after(slot, 3);
     const int b_next = F::after(slot, 4 + wn), a0_next = F::after(slot, 6);
     const int to0 = F::after(slot, 8), to1 = F::after(slot, 9), to3 = F::after(slot, 1);
     products(Int<0>(), Int<0>(), [&](auto n) {
       constexpr int m = decltype(n)::value;
       read_ba(m, b_at, a0, 2);
-      if constexpr (m % 4 == 1) feed.template one<0, m / 4, kAny>(s + 2, to0);
+      if constexpr (m % 4 == 1) copy(Int<0>(), Int<m / 4>(), to0);
     });
-    arrive<8>();  // (behind A0 of the next step: its A1 and B0 of the step after it)
+    arrive<kCopy ? 8 : 0>();  // (behind A0 of the next step: its A1 and B0 of the step after it)
     products(Int<0>(), Int<2>(), [&](auto n) {
       constexpr int m = decltype(n)::value;
       if constexpr (m % 4 == 0) read_a(a1, m / 4 % 2, m / 8);
-      if constexpr (m % 4 == 1) feed.template one<1, m / 4, kAny>(s + 2, to1);
+      if constexpr (m % 4 == 1) copy(Int<1>(), Int<m / 4>(), to1);
     });
     products(Int<1>(), Int<0>(), [&](auto n) {
       constexpr int m = decltype(n)::value;
       if constexpr (m % 2 == 0 && m < 8) read_a(a1, m / 2 % 2, 2 + m / 4);
-      if constexpr (m % 4 == 1) feed.template one<2, m / 4, kAny>(s + 2, slot);
+      if constexpr (m % 4 == 1) copy(Int<2>(), Int<m / 4>(), slot);
     });
     products(Int<1>(), Int<2>(), [&](auto n) {
       constexpr int m = decltype(n)::value;
       read_ba(m, b_next, a0_next, 0);
-      if constexpr (m % 4 == 1) feed.template one<3, m / 4, kAny>(s + 2, to3);
+      if constexpr (m % 4 == 1) copy(Int<3>(), Int<m / 4>(), to3);
     });
     slot = F::after(slot, 4);
   };
   const int s1 = feed.s1, whole = feed.whole();
 #pragma unroll 1
-  for (; s + 2 < whole; ++s) step(Int<0>(), s);
+  for (; s + 2 < whole; ++s) step(Int<1>(), s);
 #pragma unroll 1
-  for (; s < s1; ++s) step(Int<1>(), s);
-  wait_vm<0>();  // (no copy is under way when the work-group ends)
-
+  for (; s + 2 < s1; ++s) step(Int<2>(), s);  // (once at most)
+#pragma unroll 1
+  for (; s < s1; ++s) step(Int<0>(), s);
   __syncthreads();  // (the slots are read to their end)
   float* turn = reinterpret_cast<float*>(lds + wave * kTurnBytes);
   DropKey key{};
