@@ -25,16 +25,24 @@ struct GemmParams {
   EpiParams epi;
 };
 
-constexpr int kUnit = 16384;        // bytes of a unit: 128 rows (or columns) x 64 of the reduction
-constexpr int kUnitRows = 128;
+// Unit of an operand: R rows (or columns), 128 or 64, by 64 of the reduction.
+constexpr int unit_bytes(int r) { return r * 128; }
 
-// How a wave copies its quarter of a unit: four instructions of 1 KB. ROWS: instruction j of wave w takes rows 8 (4 j + w)
-// .. + 7 of 128 bytes; COLS: reduction rows 4 (4 j + w) .. + 3 of 256 bytes. The 16-byte chunks of a row are swizzled by the
-// row (the lanes' sources are, the LDS side of such a copy is linear).
-template <bool COLS>
+// How a wave copies its quarter of a unit: R / 32 instructions of 1 KB. ROWS: instruction j of wave w takes rows 8 (4 j + w)
+// .. + 7 of 128 bytes; COLS: of the reduction's 64 rows of 2 R bytes the 1 KB from 4 j + w on. The 16-byte chunks of a row
+// are swizzled by the row (the lanes' sources are, the LDS side of such a copy is linear).
+// Swizzles: ROWS: swz8. COLS: a transposed read takes 64 bytes of four reduction rows for either half of the wave: those fall on
+// 64 different banks when rows of 256 bytes differ in bits 2 and 3 of the chunk, rows of 128 bytes two apart in bit 2.
+template <int R>
+__device__ __forceinline__ int swz_cols(int kr) {
+  return R == 128 ? (kr & 3) << 2 : ((kr >> 1) & 1) << 2;
+}
+
+template <bool COLS, int R>
 struct Copy {
-  const char* base;  // the unit's first row or column, step 0
-  uint32_t off[4];   // byte offset of the lane's chunk
+  static constexpr int kCount = R / 32, kRowChunks = R / 8, kKRows = 512 / R;  // COLS: chunks of a row, rows of 1 KB
+  const char* base;      // the unit's first row or column, step 0
+  uint32_t off[kCount];  // byte offset of the lane's chunk
   int at;            // its place along the reduction: element (ROWS) or row (COLS, instruction 0)
 
   // unit u of an operand of `count` rows (columns) from `first` (a unit behind the last one reads the first one's)
@@ -42,18 +50,18 @@ struct Copy {
     first = first < count ? first : 0;
     base = operand + (COLS ? (int64_t)first * 2 : first * ld);
     if constexpr (COLS) {
-      const int kr = 4 * wave + (lane >> 4), chunk = (lane & 15) ^ ((kr & 3) << 2);
+      const int kr = kKRows * wave + lane / kRowChunks, chunk = (lane % kRowChunks) ^ swz_cols<R>(kr);
       // columns behind the last are the last chunk's: their results are not stored
       const int last = (count - 1) / 8 * 8 - first;
       const int c = chunk * 8 < last ? chunk * 8 : last;
       at = kr;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) off[j] = (uint32_t)((16 * j + kr) * ld + c * 2);
+      for (int j = 0; j < kCount; ++j) off[j] = (uint32_t)((4 * kKRows * j + kr) * ld + c * 2);
     } else {
       const int r = 8 * wave + (lane >> 3), chunk = (lane & 7) ^ swz8(r), last = count - 1 - first;
       at = chunk * 8;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < kCount; ++j) {
         const int row = r + 32 * j < last ? r + 32 * j : last;
         off[j] = (uint32_t)(row * ld + chunk * 16);
       }
@@ -65,7 +73,7 @@ struct Copy {
   template <int J, bool ANY>
   __device__ __forceinline__ void issue(int64_t step_bytes, uint32_t lds, int left) const {
     if constexpr (ANY) {
-      const bool there = at + (COLS ? 16 * J : 0) < left;
+      const bool there = at + (COLS ? 4 * kKRows * J : 0) < left;
       dma16(there ? base + step_bytes + off[J] : (const char*)&kZeros, lds + J * 4096);
     } else {
       dma16s(base + step_bytes, off[J], lds + J * 4096);
@@ -75,19 +83,20 @@ struct Copy {
 
 // The copies of a work-group of four waves: units 0 .. UB - 1 of a step are B's, the next UA are A's. With ANY a step may be
 // the last one, of which `left` of 64 is there.
-template <bool ACOLS, bool BCOLS, int UA, int UB, int SLOTS>
+template <bool ACOLS, bool BCOLS, int UA, int UB, int SLOTS, int R = 128>
 struct Feed {
-  Copy<ACOLS> a[UA];
-  Copy<BCOLS> b[UB];
+  static constexpr int kUnit = unit_bytes(R);
+  Copy<ACOLS, R> a[UA];
+  Copy<BCOLS, R> b[UB];
   int64_t astep, bstep;
   uint32_t lds0;
   int s0, s1, left, tail;
 
   __device__ __forceinline__ void init(const GemmParams& p, int split, int m0, int n0, int wave, int lane, const char* lds) {
 #pragma unroll
-    for (int u = 0; u < UA; ++u) a[u].init(wave, lane, p.a, m0 + u * kUnitRows, p.m, p.lda);
+    for (int u = 0; u < UA; ++u) a[u].init(wave, lane, p.a, m0 + u * R, p.m, p.lda);
 #pragma unroll
-    for (int u = 0; u < UB; ++u) b[u].init(wave, lane, p.b, n0 + u * kUnitRows, p.n, p.ldb);
+    for (int u = 0; u < UB; ++u) b[u].init(wave, lane, p.b, n0 + u * R, p.n, p.ldb);
     astep = ACOLS ? 64 * p.lda : 128;
     bstep = BCOLS ? 64 * p.ldb : 128;
     lds0 = lds_addr(lds) + wave * 1024;
@@ -114,38 +123,41 @@ struct Feed {
     if (step >= s1) return;
     one<U, 0, true>(step, slot);
     one<U, 1, true>(step, slot);
-    one<U, 2, true>(step, slot);
-    one<U, 3, true>(step, slot);
+    if constexpr (R == 128) {
+      one<U, 2, true>(step, slot);
+      one<U, 3, true>(step, slot);
+    }
   }
 };
 
-// Fragments of a wave's 64 rows (columns) of a unit for the 32x32x16 products: lane l holds row l % 32 of a block of 32,
-// elements 16 ks + 8 (l / 32) .. + 7 of the reduction.
-template <bool COLS, typename T>
+// Fragments of a wave's half of a unit (R / 64 blocks of 32 rows or columns) for the 32x32x16 products: lane l holds row l % 32
+// of a block, elements 16 ks + 8 (l / 32) .. + 7 of the reduction.
+template <bool COLS, typename T, int R = 128>
 struct Frags {
   typedef typename Half<T>::vec8 vec8;
-  int addr[COLS ? 2 : 4];
+  static constexpr int kBlocks = R / 64;
+  int addr[COLS ? kBlocks : 4];
 
   __device__ __forceinline__ void init(int lane, int part) {
     const int h = lane >> 5;
     if constexpr (COLS) {
       const int i = lane & 15, kr = 8 * h + (i >> 2), s = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-        addr[b] = kr * 256 + ((((2 * part + b) ^ (i >> 2)) << 2) + s) * 16 + 8 * (i & 1);
+      for (int b = 0; b < kBlocks; ++b)
+        addr[b] = kr * 2 * R + ((4 * (kBlocks * part + b) + s) ^ swz_cols<R>(kr)) * 16 + 8 * (i & 1);
     } else {
       const int r = lane & 31;
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) addr[ks] = (64 * part + r) * 128 + (((2 * ks + h) ^ swz8(r)) << 4);
+      for (int ks = 0; ks < 4; ++ks) addr[ks] = (R / 2 * part + r) * 128 + (((2 * ks + h) ^ swz8(r)) << 4);
     }
   }
 
   __device__ __forceinline__ vec8 get(const char* unit, int block, int ks) const {
     if constexpr (COLS) {
       typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-      const char* p = unit + addr[block] + ks * 4096;
+      const char* p = unit + addr[block] + ks * 32 * R;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 1024));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * R));
       const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
       return __builtin_bit_cast(vec8, u32x4{x[0], x[1], y[0], y[1]});
     } else {
@@ -174,48 +186,49 @@ __device__ __forceinline__ Place place_of(const GemmParams& p) {
   return at;
 }
 
-// Results of 32 rows by 64 columns of a wave, two blocks x0, x1 (a lane holds row l % 32, columns 8 q + 4 (l / 32) + e in
-// element 4 q + e), through the wave's own part of LDS: read back, eight lanes hold a row, each eight columns, so that every
+// Results of 32 rows by 32 NB columns of a wave, blocks x[0], x[1] (a lane holds row l % 32, columns 8 q + 4 (l / 32) + e in
+// element 4 q + e), through the wave's own part of LDS: read back, 4 NB lanes hold a row, each eight columns, so that every
 // load and store of the epilogue takes whole lines. (Eight columns a lane of 32 rows, straight from the registers: four
-// requests a line, and 87936 x 1024 to 4096 took 840 us.)
-constexpr int kTurnRow = 68;                  // floats: 16-byte places of 16 rows are distinct banks
-constexpr int kTurnBytes = 32 * kTurnRow * 4;  // of a wave
+// requests a line, and 87936 x 1024 to 4096 took 840 us in place of 740.)
+constexpr int turn_row(int nb) { return 32 * nb + 4; }           // floats: 16-byte places of 16 rows are distinct banks
+constexpr int turn_bytes(int nb) { return 32 * turn_row(nb) * 4; }  // of a wave
 
-template <typename T>
+template <typename T, int NB>
 __device__ __forceinline__ void finish_rows(const GemmParams& p, const DropKey& key, const EpiCols<T>& cols, int split,
-                                            int row0, int col0, float* turn, const f32x16& x0, const f32x16& x1) {
-  const int lane = tid_x() & 63, col = col0 + 8 * (lane & 7);
-  int row = row0 + (lane >> 3);
+                                            int row0, int col0, float* turn, const f32x16 (&x)[NB]) {
+  constexpr int kLanes = 4 * NB, kRows = 64 / kLanes, kPasses = 32 / kRows;  // lanes of a row, rows of a pass
+  const int lane = tid_x() & 63, col = col0 + 8 * (lane % kLanes);
+  int row = row0 + lane / kLanes;
   EpiPlace at;
   at.init(p.epi, row, col);
   // (the residual is on its way while the rows turn)
-  float res[4][8];
+  float res[kPasses][8];
   if (p.epi.res && p.splits == 1) {
 #pragma unroll
-    for (int pass = 0; pass < 4; ++pass)
-      if (row + 8 * pass < p.m && col < p.n)
-        epi_load<T>(p.epi.res, p.epi.y32, p.epi.vec, at.res + 8 * pass * p.epi.ld_res, p.epi.n - col, res[pass]);
+    for (int pass = 0; pass < kPasses; ++pass)
+      if (row + kRows * pass < p.m && col < p.n)
+        epi_load<T>(p.epi.res, p.epi.y32, p.epi.vec, at.res + kRows * pass * p.epi.ld_res, p.epi.n - col, res[pass]);
   }
-  float* to = turn + (lane & 31) * kTurnRow + 4 * (lane >> 5);
+  float* to = turn + (lane & 31) * turn_row(NB) + 4 * (lane >> 5);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    *reinterpret_cast<f32x4*>(to + 8 * q) = f32x4{x0[4 * q], x0[4 * q + 1], x0[4 * q + 2], x0[4 * q + 3]};
-    *reinterpret_cast<f32x4*>(to + 32 + 8 * q) = f32x4{x1[4 * q], x1[4 * q + 1], x1[4 * q + 2], x1[4 * q + 3]};
-  }
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<f32x4*>(to + 32 * b + 8 * q) = f32x4{x[b][4 * q], x[b][4 * q + 1], x[b][4 * q + 2], x[b][4 * q + 3]};
   asm volatile("" ::: "memory");  // (a wave's LDS accesses stay in their order)
-  const float* from = turn + (lane >> 3) * kTurnRow + 8 * (lane & 7);
+  const float* from = turn + lane / kLanes * turn_row(NB) + 8 * (lane % kLanes);
 #pragma unroll
-  for (int pass = 0; pass < 4; ++pass) {
+  for (int pass = 0; pass < kPasses; ++pass) {
     float v[8];
-    load_vec<8>(from + pass * 8 * kTurnRow, v);
+    load_vec<8>(from + pass * kRows * turn_row(NB), v);
     if (row < p.m && col < p.n) {
       if (p.splits > 1)
         store_vec<8>(p.part + ((int64_t)split * p.m + row) * p.ldp + col, v);
       else
         epilogue8<T>(p.epi, key, cols, at, row, col, res[pass], v);
     }
-    row += 8;
-    at.down(p.epi, 8);
+    row += kRows;
+    at.down(p.epi, kRows);
   }
   asm volatile("" ::: "memory");
 }
@@ -240,35 +253,34 @@ __device__ __forceinline__ void each(F f) {
   }
 }
 
-// Tiles of 256 x 128 (UA 2; 80 KB of LDS, two work-groups a compute unit, so that one's epilogue lies under the other's
-// products) and 128 x 128 (UA 1). Four waves in two rows of two; each owns 64 x 64 of every unit of A. Units (128 x 64 of an
-// operand) go through a ring of LDS slots. A step of 64 is four groups of products (16 of the reduction each) of every A unit;
-// fragments are read into the registers that the groups before have done with:
-//   UA 2   group    0        1     |    2        3      4      5     |   6           7
-//          reads    B A0 k3        |  A1 k0 k1  A1 k2  A1 k3         | B A0 k0' k1'  B A0 k2'     (': of the next step)
-//          copies   A0"     A0" A0"|  A1'     A1' A1'  A1' B" B" B"  | B"           A0"
-// The first barrier waits for A1 of this step and frees B A0, the second waits for B A0 of the next step and frees A1.
-//   UA 1   group    0      1     |    2            3
-//          reads    B A k3       |  B A k0' k1'   B A k2'
-//          copies                |  B, A of the step whose place is free
-template <typename T, bool ACOLS, bool BCOLS, int UA, int SLOTS>
-__global__ void __launch_bounds__(256, SLOTS > 5 ? 1 : 2) gemm_kernel(const GemmParams p) {
+// 256 x 128 tile of four waves in two rows of two, each 64 x 64 of either unit of A; 80 KB of LDS and two work-groups a compute
+// unit, so that one's epilogue lies under the other's products. Units go through a ring of five LDS slots. A step of 64 is four
+// groups of products (16 of the reduction each) of A0, then A1; fragments are read into the registers that the groups before
+// have done with:
+//   group    0          1     |    2        3      4      5     |   6           7
+//   reads    B A0 k3          |  A1 k0 k1  A1 k2  A1 k3         | B A0 k0' k1'  B A0 k2'     (': of the next step)
+//   copies   A0'        A0'   |  A1'       A1'    A1' B" B"     | B"            A0"
+// The first barrier waits for A1 of this step and frees B A0, the second waits for B A0 of the next step and frees A1. The copies
+// are spread (all behind the barriers, 87936 x 4096 to 1024 takes 729 us in place of 690).
+template <typename T, bool ACOLS, bool BCOLS>
+__global__ void __launch_bounds__(256, 2) gemm_pair_kernel(const GemmParams p) {
   typedef typename Half<T>::vec8 vec8;
-  typedef Feed<ACOLS, BCOLS, UA, 1, SLOTS> F;
-  __shared__ __attribute__((aligned(16))) char lds[SLOTS * kUnit];
+  typedef Feed<ACOLS, BCOLS, 2, 1, 5> F;
+  constexpr int kUnit = F::kUnit;
+  __shared__ __attribute__((aligned(16))) char lds[5 * kUnit];
   const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6);
   const int wm = wave >> 1, wn = wave & 1;
   const Place at = place_of(p);
-  const int m0 = at.tm * (kUnitRows * UA), n0 = at.tn * kUnitRows;
+  const int m0 = at.tm * 256, n0 = at.tn * 128;
   F feed;
   feed.init(p, at.split, m0, n0, wave, lane, lds);
   Frags<ACOLS, T> fa;
   Frags<BCOLS, T> fb;
   fa.init(lane, wm);
   fb.init(lane, wn);
-  f32x16 acc[UA][2][2];  // [unit][row block][column block]
+  f32x16 acc[2][2][2];  // [unit][row block][column block]
 #pragma unroll
-  for (int u = 0; u < UA; ++u)
+  for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -298,154 +310,219 @@ __global__ void __launch_bounds__(256, SLOTS > 5 ? 1 : 2) gemm_kernel(const Gemm
 
   int s = feed.s0, slot = 0;  // slot: of B of this step
   const int s1 = feed.s1, whole = feed.whole();
-  if constexpr (UA == 2) {
-    feed.template unit<0>(s, 0);
-    feed.template unit<1>(s, 1);
-    feed.template unit<2>(s, 2);
-    feed.template unit<0>(s + 1, 3);
-    if (s + 1 < s1)
-      wait_vm<8>();
-    else
-      wait_vm<4>();
-    barrier_only();
+      feed.template unit<0>(s, 0);
+      feed.template unit<1>(s, 1);
+      feed.template unit<2>(s, 2);
+      feed.template unit<0>(s + 1, 3);
+      if (s + 1 < s1)
+        wait_vm<8>();
+      else
+        wait_vm<4>();
+      barrier_only();
 #pragma unroll
-    for (int ks = 0; ks < 3; ++ks)
+      for (int ks = 0; ks < 3; ++ks)
 #pragma unroll
-      for (int n = 0; n < 4; ++n) read_ba(n, 0, 1, ks);
-    fence();
-    // Copies of a step: NEXT: of the next one, LATER: of the one behind it (2: with the check for the last step).
-    auto step = [&](auto next, auto later, int s) {
-      constexpr int kNext = decltype(next)::value, kLater = decltype(later)::value;
-      const int a0 = F::after(slot, 1), a1 = F::after(slot, 2), b_next = F::after(slot, 3), a0_next = F::after(slot, 4);
-      auto copy_next = [&](auto unit, auto j, int to) {
-        if constexpr (kNext != 0) feed.template one<decltype(unit)::value, decltype(j)::value, kNext == 2>(s + 1, to);
+        for (int n = 0; n < 4; ++n) read_ba(n, 0, 1, ks);
+      fence();
+      // Copies of a step: NEXT: of the next one, LATER: of the one behind it (2: with the check for the last step).
+      auto step = [&](auto next, auto later, int s) {
+        constexpr int kNext = decltype(next)::value, kLater = decltype(later)::value;
+        const int a0 = F::after(slot, 1), a1 = F::after(slot, 2), b_next = F::after(slot, 3), a0_next = F::after(slot, 4);
+        auto copy_next = [&](auto unit, auto j, int to) {
+          if constexpr (kNext != 0) feed.template one<decltype(unit)::value, decltype(j)::value, kNext == 2>(s + 1, to);
+        };
+        auto copy_later = [&](auto unit, auto j, int to) {
+          if constexpr (kLater != 0) feed.template one<decltype(unit)::value, decltype(j)::value, kLater == 2>(s + 2, to);
+        };
+        products(Int<0>(), Int<0>(), [&](auto n) {
+          constexpr int m = decltype(n)::value;
+          read_ba(m, slot, a0, 3);
+          if constexpr (m == 1) copy_next(Int<1>(), Int<1>(), a0_next);
+        });
+        products(Int<0>(), Int<1>(), [&](auto n) {
+          constexpr int m = decltype(n)::value;
+          if constexpr (m == 0) copy_next(Int<1>(), Int<2>(), a0_next);
+          if constexpr (m == 2) copy_next(Int<1>(), Int<3>(), a0_next);
+        });
+        arrive<kNext ? 8 : 0>();  // (behind A1: B and A0 of the next step)
+        products(Int<0>(), Int<2>(), [&](auto n) {
+          constexpr int m = decltype(n)::value;
+          read_a(a1, m % 2, m / 2);
+          if constexpr (m == 2) copy_next(Int<2>(), Int<0>(), slot);
+        });
+        products(Int<0>(), Int<3>(), [&](auto n) {
+          constexpr int m = decltype(n)::value;
+          if constexpr (m % 2 == 1) read_a(a1, m / 2, 2);
+          if constexpr (m == 0) copy_next(Int<2>(), Int<1>(), slot);
+          if constexpr (m == 2) copy_next(Int<2>(), Int<2>(), slot);
+        });
+        products(Int<1>(), Int<0>(), [&](auto n) {
+          constexpr int m = decltype(n)::value;
+          if constexpr (m % 2 == 1) read_a(a1, m / 2, 3);
+          if constexpr (m == 0) copy_next(Int<2>(), Int<3>(), slot);
+          if constexpr (m == 2) copy_later(Int<0>(), Int<0>(), a0);
+        });
+        products(Int<1>(), Int<1>(), [&](auto n) {
+          constexpr int m = decltype(n)::value;
+          if constexpr (m == 0) copy_later(Int<0>(), Int<1>(), a0);
+          if constexpr (m == 2) copy_later(Int<0>(), Int<2>(), a0);
+        });
+        // (behind A0 of the next step: its A1 and three instructions of B behind it)
+        if constexpr (kNext != 0) arrive<kLater ? 7 : 4>();
+        products(Int<1>(), Int<2>(), [&](auto n) {
+          constexpr int m = decltype(n)::value;
+          if constexpr (kNext != 0) {
+            read_ba(m, b_next, a0_next, 0);
+            read_ba(m, b_next, a0_next, 1);
+          }
+          if constexpr (m == 2) copy_later(Int<0>(), Int<3>(), a0);
+        });
+        products(Int<1>(), Int<3>(), [&](auto n) {
+          constexpr int m = decltype(n)::value;
+          if constexpr (kNext != 0) read_ba(m, b_next, a0_next, 2);
+          if constexpr (m == 1) copy_later(Int<1>(), Int<0>(), a1);
+        });
+        slot = b_next;
       };
-      auto copy_later = [&](auto unit, auto j, int to) {
-        if constexpr (kLater != 0) feed.template one<decltype(unit)::value, decltype(j)::value, kLater == 2>(s + 2, to);
-      };
-      products(Int<0>(), Int<0>(), [&](auto n) {
-        constexpr int m = decltype(n)::value;
-        read_ba(m, slot, a0, 3);
-        if constexpr (m == 1) copy_next(Int<1>(), Int<1>(), a0_next);
-      });
-      products(Int<0>(), Int<1>(), [&](auto n) {
-        constexpr int m = decltype(n)::value;
-        if constexpr (m == 0) copy_next(Int<1>(), Int<2>(), a0_next);
-        if constexpr (m == 2) copy_next(Int<1>(), Int<3>(), a0_next);
-      });
-      arrive<kNext ? 8 : 0>();  // (behind A1: B and A0 of the next step)
-      products(Int<0>(), Int<2>(), [&](auto n) {
-        constexpr int m = decltype(n)::value;
-        read_a(a1, m % 2, m / 2);
-        if constexpr (m == 2) copy_next(Int<2>(), Int<0>(), slot);
-      });
-      products(Int<0>(), Int<3>(), [&](auto n) {
-        constexpr int m = decltype(n)::value;
-        if constexpr (m % 2 == 1) read_a(a1, m / 2, 2);
-        if constexpr (m == 0) copy_next(Int<2>(), Int<1>(), slot);
-        if constexpr (m == 2) copy_next(Int<2>(), Int<2>(), slot);
-      });
-      products(Int<1>(), Int<0>(), [&](auto n) {
-        constexpr int m = decltype(n)::value;
-        if constexpr (m % 2 == 1) read_a(a1, m / 2, 3);
-        if constexpr (m == 0) copy_next(Int<2>(), Int<3>(), slot);
-        if constexpr (m == 2) copy_later(Int<0>(), Int<0>(), a0);
-      });
-      products(Int<1>(), Int<1>(), [&](auto n) {
-        constexpr int m = decltype(n)::value;
-        if constexpr (m == 0) copy_later(Int<0>(), Int<1>(), a0);
-        if constexpr (m == 2) copy_later(Int<0>(), Int<2>(), a0);
-      });
-      // (behind A0 of the next step: its A1 and three instructions of B behind it)
-      if constexpr (kNext != 0) arrive<kLater ? 7 : 4>();
-      products(Int<1>(), Int<2>(), [&](auto n) {
-        constexpr int m = decltype(n)::value;
-        if constexpr (kNext != 0) {
-          read_ba(m, b_next, a0_next, 0);
-          read_ba(m, b_next, a0_next, 1);
-        }
-        if constexpr (m == 2) copy_later(Int<0>(), Int<3>(), a0);
-      });
-      products(Int<1>(), Int<3>(), [&](auto n) {
-        constexpr int m = decltype(n)::value;
-        if constexpr (kNext != 0) read_ba(m, b_next, a0_next, 2);
-        if constexpr (m == 1) copy_later(Int<1>(), Int<0>(), a1);
-      });
-      slot = b_next;
-    };
-    // (A0 of the second step, whose first instruction belongs to the step before)
-    if (s + 1 < s1) feed.template one<1, 0, true>(s + 1, 4);
+      // (A0 of the second step, whose first instruction belongs to the step before)
+      if (s + 1 < s1) feed.template one<1, 0, true>(s + 1, 4);
 #pragma unroll 1
-    for (; s + 2 < whole; ++s) step(Int<1>(), Int<1>(), s);
-    if (s + 2 < s1) step(Int<1>(), Int<2>(), s++);
-    if (s + 1 < s1) step(Int<2>(), Int<0>(), s++);
-    step(Int<0>(), Int<0>(), s);
-  } else {
-    constexpr int kAhead = SLOTS / 2;  // steps whose units have a place
-    each<kAhead>([&](auto n) {
-      constexpr int i = decltype(n)::value;
-      feed.template unit<0>(s + i, 2 * i);
-      feed.template unit<1>(s + i, 2 * i + 1);
-    });
-    if (s1 - s >= kAhead)
-      wait_vm<8 * (kAhead - 1)>();
-    else
-      wait_vm<0>();
-    barrier_only();
-#pragma unroll
-    for (int ks = 0; ks < 3; ++ks)
-#pragma unroll
-      for (int n = 0; n < 4; ++n) read_ba(n, 0, 1, ks);
-    fence();
-    // behind: steps behind the next one whose copies are under way; ahead: copies of step s + kAhead (2: with the check for
-    // the last step)
-    auto step = [&](auto behind, auto ahead, int s) {
-      constexpr int kBehind = decltype(behind)::value, kCopy = decltype(ahead)::value;
-      const int a0 = F::after(slot, 1), b_next = F::after(slot, 2), a_next = F::after(slot, 3);
-      products(Int<0>(), Int<0>(), [&](auto n) { read_ba(decltype(n)::value, slot, a0, 3); });
-      products(Int<0>(), Int<1>(), [&](auto) {});
-      if constexpr (kBehind >= 0) arrive<8 * (kBehind > 0 ? kBehind : 0)>();
-      products(Int<0>(), Int<2>(), [&](auto n) {
-        constexpr int m = decltype(n)::value;
-        if constexpr (kBehind >= 0) {
-          read_ba(m, b_next, a_next, 0);
-          read_ba(m, b_next, a_next, 1);
-        }
-        if constexpr (kCopy != 0) feed.template one<0, m, kCopy == 2>(s + kAhead, slot);
-      });
-      products(Int<0>(), Int<3>(), [&](auto n) {
-        constexpr int m = decltype(n)::value;
-        if constexpr (kBehind >= 0) read_ba(m, b_next, a_next, 2);
-        if constexpr (kCopy != 0) feed.template one<1, m, kCopy == 2>(s + kAhead, a0);
-      });
-      slot = b_next;
-    };
-#pragma unroll 1
-    for (; s + kAhead < whole; ++s) step(Int<kAhead - 2>(), Int<1>(), s);
-    if (s + kAhead < s1) step(Int<kAhead - 2>(), Int<2>(), s++);
-    each<kAhead>([&](auto n) {  // the last kAhead steps
-      constexpr int r = kAhead - decltype(n)::value;
-      if (s1 - s == r) step(Int<r - 2>(), Int<0>(), s++);
-    });
-  }
+      for (; s + 2 < whole; ++s) step(Int<1>(), Int<1>(), s);
+      if (s + 2 < s1) step(Int<1>(), Int<2>(), s++);
+      if (s + 1 < s1) step(Int<2>(), Int<0>(), s++);
+      step(Int<0>(), Int<0>(), s);
+
   __syncthreads();  // (the slots are read to their end)
-  float* turn = reinterpret_cast<float*>(lds + wave * kTurnBytes);
+  float* turn = reinterpret_cast<float*>(lds + wave * turn_bytes(2));
   DropKey key{};
   if (p.epi.drop.limit) key = drop_key(p.epi.drop);
   EpiCols<T> cols;
-  const int col0 = n0 + 64 * wn;
-  if (p.splits == 1 && col0 + 8 * (lane & 7) < p.n) cols.load(p.epi, col0 + 8 * (lane & 7));
+  const int col0 = n0 + 64 * wn, col = col0 + 8 * (lane & 7);
+  if (p.splits == 1 && col < p.n) cols.load(p.epi, col);
 #pragma unroll 1
-  for (int blk = 0; blk < UA * 2; ++blk) {
-    f32x16 x0, x1;
+  for (int blk = 0; blk < 4; ++blk) {
+    f32x16 x[2];
     switch (blk) {
-      case 0: x0 = acc[0][0][0], x1 = acc[0][0][1]; break;
-      case 1: x0 = acc[0][1][0], x1 = acc[0][1][1]; break;
-      case 2: x0 = acc[UA - 1][0][0], x1 = acc[UA - 1][0][1]; break;
-      default: x0 = acc[UA - 1][1][0], x1 = acc[UA - 1][1][1]; break;
+      case 0: x[0] = acc[0][0][0], x[1] = acc[0][0][1]; break;
+      case 1: x[0] = acc[0][1][0], x[1] = acc[0][1][1]; break;
+      case 2: x[0] = acc[1][0][0], x[1] = acc[1][0][1]; break;
+      default: x[0] = acc[1][1][0], x[1] = acc[1][1][1]; break;
     }
-    finish_rows<T>(p, key, cols, at.split, m0 + (blk >> 1) * kUnitRows + 64 * wm + 32 * (blk & 1), col0, turn, x0, x1);
+    finish_rows<T, 2>(p, key, cols, at.split, m0 + 128 * (blk >> 1) + 64 * wm + 32 * (blk & 1), col0, turn, x);
   }
+}
+
+// Tiles of 128 x 128 (NB 2) and 64 x 64 (NB 1) for products with few of the larger ones: four waves in two rows of two, each NB x
+// NB blocks. A step is bound by its copies (32 or 16 instructions of 28 cycles); a short product by its first copies' way and
+// by the epilogue, which smaller tiles spread over more compute units. Units of both operands go through a ring of SLOTS:
+//   group    0        1   |   2            3
+//   reads    B A k3       |  B A k0' k1'   B A k2'
+//   copies                |  B, A of the step whose place is free
+template <typename T, bool ACOLS, bool BCOLS, int NB, int SLOTS>
+__global__ void __launch_bounds__(256, SLOTS * NB > 10 ? 1 : 2) gemm_small_kernel(const GemmParams p) {
+  typedef typename Half<T>::vec8 vec8;
+  constexpr int R = 64 * NB, kPer = R / 32;  // rows of a unit, a wave's instructions for it
+  typedef Feed<ACOLS, BCOLS, 1, 1, SLOTS, R> F;
+  constexpr int kUnit = F::kUnit;
+  __shared__ __attribute__((aligned(16))) char lds[SLOTS * kUnit];
+  const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const Place at = place_of(p);
+  const int m0 = at.tm * R, n0 = at.tn * R;
+  F feed;
+  feed.init(p, at.split, m0, n0, wave, lane, lds);
+  Frags<ACOLS, T, R> fa;
+  Frags<BCOLS, T, R> fb;
+  fa.init(lane, wm);
+  fb.init(lane, wn);
+  f32x16 acc[NB][NB];  // [row block][column block]
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  vec8 af[NB][4], bf[NB][4];
+  // the fragments of ks
+  auto read = [&](int b_slot, int a_slot, int ks) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) bf[j][ks] = fb.get(lds + b_slot * kUnit, j, ks);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) af[i][ks] = fa.get(lds + a_slot * kUnit, i, ks);
+  };
+  // the products of ks, hook(n) behind the n-th
+  auto products = [&](auto at_k, auto hook) {
+    constexpr int ks = decltype(at_k)::value;
+    each<NB * NB>([&](auto n) {
+      constexpr int i = decltype(n)::value / NB, j = decltype(n)::value % NB;
+      acc[i][j] = Half<T>::mma32(bf[j][ks], af[i][ks], acc[i][j]);
+      hook(n);
+      fence();
+    });
+  };
+
+  int s = feed.s0, slot = 0;  // slot: of B of this step
+  const int s1 = feed.s1, whole = feed.whole();
+  constexpr int kAhead = SLOTS / 2;  // steps whose units have a place
+  each<kAhead>([&](auto n) {
+    constexpr int i = decltype(n)::value;
+    feed.template unit<0>(s + i, 2 * i);
+    feed.template unit<1>(s + i, 2 * i + 1);
+  });
+  if (s1 - s >= kAhead)
+    wait_vm<2 * kPer * (kAhead - 1)>();
+  else
+    wait_vm<0>();
+  barrier_only();
+  read(0, 1, 0);
+  read(0, 1, 1);
+  read(0, 1, 2);
+  fence();
+  // behind: steps behind the next one whose copies are under way (-1: there is no next one); ahead: copies of step s + kAhead
+  // (2: with the check for the last step)
+  auto step = [&](auto behind, auto ahead, int s) {
+    constexpr int kBehind = decltype(behind)::value, kCopy = decltype(ahead)::value;
+    const int a0 = F::after(slot, 1), b_next = F::after(slot, 2), a_next = F::after(slot, 3);
+    auto copy = [&](auto unit, auto n, int to) {
+      constexpr int j = decltype(n)::value;
+      if constexpr (kCopy != 0 && j < kPer) feed.template one<decltype(unit)::value, j, kCopy == 2>(s + kAhead, to);
+    };
+    products(Int<0>(), [&](auto n) {
+      if constexpr (decltype(n)::value == 0) read(slot, a0, 3);
+    });
+    products(Int<1>(), [&](auto) {});
+    if constexpr (kBehind >= 0) arrive<2 * kPer * (kBehind > 0 ? kBehind : 0)>();
+    products(Int<2>(), [&](auto n) {
+      constexpr int m = decltype(n)::value;
+      if constexpr (kBehind >= 0 && m == 0) read(b_next, a_next, 0);
+      if constexpr (kBehind >= 0 && m == (NB == 2 ? 2 : 0)) read(b_next, a_next, 1);
+      copy(Int<0>(), n, slot);
+      if constexpr (NB == 1) copy(Int<0>(), Int<1>(), slot);
+    });
+    products(Int<3>(), [&](auto n) {
+      if constexpr (kBehind >= 0 && decltype(n)::value == 0) read(b_next, a_next, 2);
+      copy(Int<1>(), n, a0);
+      if constexpr (NB == 1) copy(Int<1>(), Int<1>(), a0);
+    });
+    slot = b_next;
+  };
+#pragma unroll 1
+  for (; s + kAhead < whole; ++s) step(Int<kAhead - 2>(), Int<1>(), s);
+  if (s + kAhead < s1) step(Int<kAhead - 2>(), Int<2>(), s++);
+  each<kAhead>([&](auto n) {  // the last kAhead steps
+    constexpr int r = kAhead - decltype(n)::value;
+    if (s1 - s == r) step(Int<r - 2>(), Int<0>(), s++);
+  });
+
+  __syncthreads();  // (the slots are read to their end)
+  float* turn = reinterpret_cast<float*>(lds + wave * turn_bytes(NB));
+  DropKey key{};
+  if (p.epi.drop.limit) key = drop_key(p.epi.drop);
+  EpiCols<T> cols;
+  const int col0 = n0 + 32 * NB * wn, col = col0 + 8 * (lane % (4 * NB));
+  if (p.splits == 1 && col < p.n) cols.load(p.epi, col);
+#pragma unroll
+  for (int i = 0; i < NB; ++i) finish_rows<T, NB>(p, key, cols, at.split, m0 + 32 * (NB * wm + i), col0, turn, acc[i]);
 }
 
 // 256 x 256 tile of four waves, one a SIMD: each owns 64 rows of both A units by a whole unit of B (128 x 128 in all, 256 sums a
@@ -463,6 +540,7 @@ template <typename T, bool ACOLS, bool BCOLS>
 __global__ void __launch_bounds__(256, 1) gemm_wide_kernel(const GemmParams p) {
   typedef typename Half<T>::vec8 vec8;
   typedef Feed<ACOLS, BCOLS, 2, 2, 10> F;
+  constexpr int kUnit = F::kUnit;
   __shared__ __attribute__((aligned(16))) char lds[10 * kUnit];
   const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6);
   const int wm = wave >> 1, wn = wave & 1;
@@ -561,7 +639,7 @@ __global__ void __launch_bounds__(256, 1) gemm_wide_kernel(const GemmParams p) {
 #pragma unroll 1
   for (; s < s1; ++s) step(Int<0>(), s);
   __syncthreads();  // (the slots are read to their end)
-  float* turn = reinterpret_cast<float*>(lds + wave * kTurnBytes);
+  float* turn = reinterpret_cast<float*>(lds + wave * turn_bytes(2));
   DropKey key{};
   if (p.epi.drop.limit) key = drop_key(p.epi.drop);
 #pragma unroll 1
@@ -571,18 +649,18 @@ __global__ void __launch_bounds__(256, 1) gemm_wide_kernel(const GemmParams p) {
     if (p.splits == 1 && col0 + 8 * (lane & 7) < p.n) cols.load(p.epi, col0 + 8 * (lane & 7));
 #pragma unroll 1
     for (int blk = 0; blk < 4; ++blk) {
-      f32x16 x0, x1;
+      f32x16 x[2];
       switch (4 * part + blk) {
-        case 0: x0 = acc[0][0][0], x1 = acc[0][0][1]; break;
-        case 1: x0 = acc[0][1][0], x1 = acc[0][1][1]; break;
-        case 2: x0 = acc[1][0][0], x1 = acc[1][0][1]; break;
-        case 3: x0 = acc[1][1][0], x1 = acc[1][1][1]; break;
-        case 4: x0 = acc[0][0][2], x1 = acc[0][0][3]; break;
-        case 5: x0 = acc[0][1][2], x1 = acc[0][1][3]; break;
-        case 6: x0 = acc[1][0][2], x1 = acc[1][0][3]; break;
-        default: x0 = acc[1][1][2], x1 = acc[1][1][3]; break;
+        case 0: x[0] = acc[0][0][0], x[1] = acc[0][0][1]; break;
+        case 1: x[0] = acc[0][1][0], x[1] = acc[0][1][1]; break;
+        case 2: x[0] = acc[1][0][0], x[1] = acc[1][0][1]; break;
+        case 3: x[0] = acc[1][1][0], x[1] = acc[1][1][1]; break;
+        case 4: x[0] = acc[0][0][2], x[1] = acc[0][0][3]; break;
+        case 5: x[0] = acc[0][1][2], x[1] = acc[0][1][3]; break;
+        case 6: x[0] = acc[1][0][2], x[1] = acc[1][0][3]; break;
+        default: x[0] = acc[1][1][2], x[1] = acc[1][1][3]; break;
       }
-      finish_rows<T>(p, key, cols, at.split, m0 + (blk >> 1) * kUnitRows + 64 * wm + 32 * (blk & 1), col0, turn, x0, x1);
+      finish_rows<T, 2>(p, key, cols, at.split, m0 + 128 * (blk >> 1) + 64 * wm + 32 * (blk & 1), col0, turn, x);
     }
   }
 }
@@ -593,7 +671,7 @@ __global__ void __launch_bounds__(256, 1) gemm_wide_kernel(const GemmParams p) {
 template <typename T, int MB>
 __global__ void __launch_bounds__(512) few_rows_kernel(const GemmParams p) {
   typedef typename Half<T>::vec8 vec8;
-  constexpr int kWaves = 8, kAhead = MB >= 4 ? 2 : 4;  // turns of a wave whose loads are under way together
+  constexpr int kWaves = 8, kAhead = 4;  // turns of a wave whose loads are under way together
   __shared__ __attribute__((aligned(16))) float lds[kWaves][MB][16][20];
   const int lane = tid_x() & 63, wave = tid_x() >> 6;
   const int n0 = bid_x() * 16, i = lane & 15, at = (lane >> 4) * 8;
@@ -674,10 +752,12 @@ __global__ void __launch_bounds__(256) join_kernel(const GemmParams p) {
 constexpr int kMaxSize = 1 << 21;         // widths of a layer (a unit's byte offsets stay in 32 bits)
 constexpr int64_t kMaxRows = 0x7fffff00;  // rows of a layer
 
-// How a product runs: the kernel for few rows, or tiles of 128 UA by 128 UB and splits of the reduction.
+// How a product runs: the kernel for few rows, or tiles of one kind and splits of the reduction.
+enum Kind { kTiny, kSmall, kPair, kWide, kKinds };
+constexpr int kTileM[kKinds] = {64, 128, 256, 256}, kTileN[kKinds] = {64, 128, 128, 256};
 struct Plan {
   bool few;
-  int ua, ub, splits, split_steps, steps, tiles_m, tiles_n;
+  int kind, splits, split_steps, steps, tiles_m, tiles_n;
 };
 
 // Microseconds of a product with `wgs` work-groups of one kind and `steps` steps each, from what single kinds took over 70 to
@@ -688,13 +768,16 @@ static double tile_time(int kind, int64_t wgs, int64_t steps) {
   constexpr struct {
     double ends, alone, shared, two, full;
     int places;
-  } kKinds[3] = {{8.5, 0.31, 0.16, 0.72, 1.00, 512}, {11.0, 0.49, 0.44, 1.20, 1.75, 512}, {19.0, 0.97, 0.60, 1.57, 1.57, 256}};
-  const auto& k = kKinds[kind];
+  } kTimes[kKinds] = {{5.5, 0.19, 0.06, 0.30, 0.36, 512},
+                      {7.5, 0.31, 0.16, 0.72, 1.00, 512},
+                      {10.0, 0.49, 0.44, 1.20, 1.75, 512},
+                      {16.0, 0.97, 0.60, 1.57, 1.57, 256}};
+  const auto& k = kTimes[kind];
   const double x = (double)wgs / 256;
   if (wgs <= 256) return k.ends + (double)steps * (k.alone + k.shared * x * x);
   if (wgs <= k.places) return k.ends + (double)steps * (k.two + (k.full - k.two) * (x - 1));
   const int64_t halves = (2 * wgs + k.places - 1) / k.places;
-  const double end = kind == 2 ? k.ends : 0.5 * k.ends;  // (of two on a unit, one ends under the other)
+  const double end = kind == kWide ? k.ends : 0.5 * k.ends;  // (of two on a unit, one ends under the other)
   return k.ends + 0.5 * (double)halves * (double)steps * k.full + 0.5 * (double)(halves - 2) * end;
 }
 
@@ -704,11 +787,10 @@ static double tile_time(int kind, int64_t wgs, int64_t steps) {
 static Plan plan_of(int64_t m, int n, int64_t k, bool rows_kind) {
   Plan r{};
   r.steps = (int)((k + 63) / 64);
-  r.few = rows_kind && m <= 64;
+  r.few = rows_kind && m <= 32;
   double best = 1e300;
-  for (int kind = 0; kind < 3; ++kind) {
-    const int ua = kind ? 2 : 1, ub = kind == 2 ? 2 : 1;
-    const int64_t tm = (m + 128 * ua - 1) / (128 * ua), tn = ((int64_t)n + 128 * ub - 1) / (128 * ub);
+  for (int kind = 0; kind < kKinds; ++kind) {
+    const int64_t tm = (m + kTileM[kind] - 1) / kTileM[kind], tn = ((int64_t)n + kTileN[kind] - 1) / kTileN[kind];
     for (int splits = 1; splits <= 64; splits += splits < 4 ? 1 : splits < 8 ? 2 : splits < 16 ? 4 : 8) {
       if (splits > 1 && (r.steps < 2 * splits || tm * tn * splits > 1024)) break;
       const int per = (r.steps + splits - 1) / splits, used = (r.steps + per - 1) / per;
@@ -716,8 +798,7 @@ static Plan plan_of(int64_t m, int n, int64_t k, bool rows_kind) {
       if (used > 1) t += 2.5 + (double)used * (double)m * n * 8 / 5.5e6;
       if (t < best) {
         best = t;
-        r.ua = ua;
-        r.ub = ub;
+        r.kind = kind;
         r.splits = used;
         r.split_steps = per;
         r.tiles_m = (int)tm;
@@ -752,10 +833,8 @@ static int product(const char* who, const void* a, int64_t lda, const void* b, i
       const dim3 grid((uint32_t)((n + 15) / 16));
       if (m <= 16)
         hipLaunchKernelGGL((few_rows_kernel<T, 1>), grid, dim3(512), 0, stream, p);
-      else if (m <= 32)
-        hipLaunchKernelGGL((few_rows_kernel<T, 2>), grid, dim3(512), 0, stream, p);
       else
-        hipLaunchKernelGGL((few_rows_kernel<T, 4>), grid, dim3(512), 0, stream, p);
+        hipLaunchKernelGGL((few_rows_kernel<T, 2>), grid, dim3(512), 0, stream, p);
       return check_launch(who);
     }
   }
@@ -768,14 +847,16 @@ static int product(const char* who, const void* a, int64_t lda, const void* b, i
   const int64_t grid = (int64_t)r.tiles_m * r.tiles_n * r.splits;
   if (grid > 0xffffffffll / 256) return fail(SAF3R_ERR_UNSUPPORTED, "%s: too many tiles for one launch", who);
   const dim3 wgs((uint32_t)grid);
-  if (r.ub == 2)
+  if (r.kind == kWide)
     hipLaunchKernelGGL((gemm_wide_kernel<T, ACOLS, BCOLS>), wgs, dim3(256), 0, stream, p);
-  else if (r.ua == 2)
-    hipLaunchKernelGGL((gemm_kernel<T, ACOLS, BCOLS, 2, 5>), wgs, dim3(256), 0, stream, p);
+  else if (r.kind == kPair)
+    hipLaunchKernelGGL((gemm_pair_kernel<T, ACOLS, BCOLS>), wgs, dim3(256), 0, stream, p);
+  else if (r.kind == kTiny)
+    hipLaunchKernelGGL((gemm_small_kernel<T, ACOLS, BCOLS, 1, 10>), wgs, dim3(256), 0, stream, p);
   else if (grid <= 256)  // (one a compute unit: twice the units on their way)
-    hipLaunchKernelGGL((gemm_kernel<T, ACOLS, BCOLS, 1, 10>), wgs, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((gemm_small_kernel<T, ACOLS, BCOLS, 2, 10>), wgs, dim3(256), 0, stream, p);
   else
-    hipLaunchKernelGGL((gemm_kernel<T, ACOLS, BCOLS, 1, 4>), wgs, dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((gemm_small_kernel<T, ACOLS, BCOLS, 2, 4>), wgs, dim3(256), 0, stream, p);
   if (int e = check_launch(who)) return e;
   if (r.splits == 1) return SAF3R_OK;
   const int64_t threads = m * (p.ldp / 8);
