@@ -33,34 +33,34 @@ struct Half<_Float16> {
 };
 
 // Both GELUs are z times a share s(z) in (0, 1); the derivative is s + z s'.
-//   exact: s is the normal distribution function by its complement, 1 - s(|z|) = t (c1 + t (c2 + ...)) exp(-z^2 / 2) / 2,
-//   t = 1 / (1 + 0.3275911 |z| / sqrt 2) (Abramowitz and Stegun, 7.1.26: within 7.5e-8), and s' the density, whose
-//   exponential is the same. A library erf costs about three times as many instructions.
+//   exact: s is the normal distribution function by its complement, q = 1 - s(|z|) = t (c1 + t (c2 + ...)) exp(-z^2 / 2) / 2,
+//   t = 1 / (1 + 0.3275911 |z| / sqrt 2) (Abramowitz and Stegun, 7.1.26: within 7.5e-8), so that z s = max(z, 0) - |z| q; s' is
+//   the density, whose exponential is the same. A library erf costs about three times as many instructions.
 //   tanh form: s = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3); s' = 2 s (1 - s) u'.
-// Behind |z| = 15 both are 0 or 1 in fp32: z is held there in the exponents, and below -15 in the products with s and s' too
-// (an infinity times zero would be a NaN, and so small a share of a large enough z a number). A NaN stays one.
-__device__ __forceinline__ float act_share(int act, float z, float* slope) {
-  const float a = fminf(fabsf(z), 15.f);
-  if (act == SAF3R_GELU) {
-    const float t = __builtin_amdgcn_rcpf(1.f + 0.23164189f * a);
-    const float e = __builtin_amdgcn_exp2f(-0.72134752f * a * a);
-    float q = t * (1.061405429f * 0.5f) + (-1.453152027f * 0.5f);
-    q = q * t + 1.421413741f * 0.5f;
-    q = q * t + -0.284496736f * 0.5f;
-    q = q * t + 0.254829592f * 0.5f;
-    q *= t * e;
-    if (slope) *slope = 0.39894228f * e;
-    return z < 0.f ? q : 1.f - q;
-  }
-  const float b = z < 0.f ? -a : a, b2 = b * b;
-  const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.3022082f * b * (1.f + 0.044715f * b2)));
-  if (slope) *slope = s * (1.f - s) * (1.5957691f * (1.f + 0.134145f * b2));
-  return s;
+// Behind |z| = 15 s is 0 or 1 in fp32: z is held there in its products with q, s and s' (an infinity times zero would be a NaN).
+// A NaN stays one.
+__device__ __forceinline__ float gelu_tail(float z, float* e) {  // q
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.23164189f * fabsf(z));
+  *e = __builtin_amdgcn_exp2f(-0.72134752f * z * z);
+  float q = t * (1.061405429f * 0.5f) + (-1.453152027f * 0.5f);
+  q = q * t + 1.421413741f * 0.5f;
+  q = q * t + -0.284496736f * 0.5f;
+  q = q * t + 0.254829592f * 0.5f;
+  return q * t * *e;
+}
+
+__device__ __forceinline__ float tanh_share(float z) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.3022082f * z * (1.f + 0.044715f * z * z)));
 }
 
 __device__ __forceinline__ float act_value(int act, float z) {
   if (act == SAF3R_NO_ACTIVATION) return z;
-  return (z < -15.f ? -15.f : z) * act_share(act, z, nullptr);
+  if (act == SAF3R_GELU) {
+    float e;
+    const float q = gelu_tail(z, &e);
+    return fmaxf(z, 0.f) - fminf(fabsf(z), 15.f) * q;
+  }
+  return fmaxf(z, -15.f) * tanh_share(z);
 }
 
 // act(z) and act'(z)
@@ -69,10 +69,16 @@ __device__ __forceinline__ float act_slope(int act, float z, float* value) {
     *value = z;
     return 1.f;
   }
-  float d;
-  const float s = act_share(act, z, &d), low = z < -15.f ? -15.f : z;
+  const float low = fmaxf(z, -15.f), b = fminf(low, 15.f);
+  if (act == SAF3R_GELU) {
+    float e;
+    const float q = gelu_tail(z, &e);
+    *value = fmaxf(z, 0.f) - fminf(fabsf(z), 15.f) * q;
+    return (z < 0.f ? q : 1.f - q) + b * (0.39894228f * e);
+  }
+  const float s = tanh_share(z);
   *value = low * s;
-  return s + (z > 15.f ? 15.f : low) * d;
+  return s + b * (s * (1.f - s) * (1.5957691f * (1.f + 0.134145f * b * b)));
 }
 
 // y = res + gate drop(act(z + bias)); kept = z + bias. Rows of n columns; `vec`: every row can be read and written in

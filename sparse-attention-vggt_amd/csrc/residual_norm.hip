@@ -212,9 +212,11 @@ static int rn_dispatch(int dim, bool some, F f) {
   return some ? lanes(std::true_type()) : lanes(std::false_type());
 }
 
-// Work-groups of the backward pass (see layer_norm.hip)
-static int64_t rn_parts(int64_t rows, int rows_per_step) {
-  return std::max<int64_t>(1, std::min<int64_t>(512, rows / (rows_per_step > 8 ? rows_per_step : 8)));
+// Work-groups of the backward pass: two a compute unit, three where one has a row of at most 2048 in its registers at a time,
+// with eight rows each at least, so that the partial rows they write are a small part of the rows they read. (10408 rows of 1536
+// with dropout, with their sums: 51 us with two, 47 with three, 48 with four; 5000 of 4096: 79 with two, 94 with four.)
+static int64_t rn_parts(int64_t rows, int dim) {
+  return std::max<int64_t>(1, std::min<int64_t>(dim > 1024 && dim <= 2048 ? 768 : 512, rows / (dim <= 64 ? 32 : 8)));
 }
 
 }  // namespace saf3r
@@ -273,7 +275,7 @@ extern "C" int saf3r_residual_norm_fwd(const void* x, int64_t x_stride, int x_ty
 extern "C" int64_t saf3r_residual_norm_bwd_workspace_bytes(int64_t rows, int dim) {
   const char* who = "saf3r_residual_norm_bwd_workspace_bytes";
   if (ln_check(who, rows, dim, SAF3R_FP32, SAF3R_FP32, SAF3R_FP32)) return -1;
-  return rn_parts(rows, 1) * 3 * dim * 4;
+  return rn_parts(rows, dim) * 3 * dim * 4;
 }
 
 extern "C" int saf3r_residual_norm_bwd(const void* dh, int64_t dh_stride, const void* dy, int64_t dy_stride, int y_type,
@@ -335,7 +337,7 @@ extern "C" int saf3r_residual_norm_bwd(const void* dh, int64_t dh_stride, const 
     rc = rn_dispatch(dim, !vec, [&](auto some, auto nv, auto tpr) {
       return ln_types(x_type, y_type, param_type, [&](auto tx, auto ty, auto tp) {
         constexpr int kTpr = decltype(tpr)::value;
-        parts = rn_parts(rows, 256 / kTpr);
+        parts = rn_parts(rows, dim);
         p.step = parts * (256 / kTpr);
         hipLaunchKernelGGL((residual_norm_bwd_kernel<decltype(tx), decltype(ty), decltype(tp), decltype(some)::value,
                                                      decltype(nv)::value, kTpr>),
