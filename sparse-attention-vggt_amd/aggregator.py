@@ -24,7 +24,9 @@ fused SDPA kernels (flash / memory-efficient only, never the math path), or, wit
 frames' tokens (identical arithmetic: every token attends to the tokens of its own frame). With
 ``frame_attention="saf3r_train"`` every block's norms and the attention of unpatched blocks run through the
 differentiable kernels (``autograd``), for training steps; norms and attentions of a class with a forward of its own, or
-with hooks, are called as they are.
+with hooks, are called as they are. ``frame_attention="saf3r_block"`` runs the products of the blocks with their bias,
+GELU, dropout, layer scale and residual through the kernels too, and the first residual of a block together with its second
+norm; what a module computes differently (another activation, hooks, products in fp32) is called as it is.
 """
 from __future__ import annotations
 
@@ -42,6 +44,9 @@ RESNET_MEAN = (0.485, 0.456, 0.406)
 RESNET_STD = (0.229, 0.224, 0.225)
 
 
+TRAINED = ("saf3r_train", "saf3r_block")  # kinds of frame attention that run through the differentiable kernels
+
+
 class LayerScale(nn.Module):
     def __init__(self, dim: int, init_values: float):
         super().__init__()
@@ -52,14 +57,15 @@ class LayerScale(nn.Module):
 
 
 class Mlp(nn.Module):
-    def __init__(self, dim: int, hidden: int, bias: bool = True):
+    def __init__(self, dim: int, hidden: int, bias: bool = True, drop: float = 0.0):
         super().__init__()
         self.fc1 = nn.Linear(dim, hidden, bias=bias)
         self.act = nn.GELU()
         self.fc2 = nn.Linear(hidden, dim, bias=bias)
+        self.drop = nn.Dropout(drop) if drop else nn.Identity()
 
     def forward(self, x):
-        return self.fc2(self.act(self.fc1(x)))
+        return self.drop(self.fc2(self.drop(self.act(self.fc1(x)))))
 
 
 def frame_local_attention(attn: Attention, x: torch.Tensor, pos, num_special: int) -> torch.Tensor:
@@ -106,23 +112,41 @@ def trained_attention(attn: Attention, x: torch.Tensor, pos, positions: int | No
     return attn.proj_drop(attn.proj(y))
 
 
+def projected_attention(attn: Attention, x: torch.Tensor, pos, positions: int | None = None):
+    """(``attn`` over each sequence of x [S, T, C] before its last dropout, that dropout's probability), differentiable,
+    through the package kernels with both products (``trained_attention`` leaves them to torch)."""
+    if attn.head_dim != HEAD_DIM:
+        raise NotImplementedError("the kernels are built for head_dim 64")
+    y = autograd.module_attention(attn, autograd.module_linear(attn.qkv, x).to(torch.bfloat16), pos,
+                                  [ops.DENSE] * attn.num_heads, positions=positions)
+    if y.dtype != attn.proj.weight.dtype and not torch.is_autocast_enabled("cuda"):
+        y = y.to(attn.proj.weight.dtype)
+    y = autograd.module_linear(attn.proj, y)
+    p = autograd.module_dropout(attn.proj_drop)
+    return (attn.proj_drop(y), 0.0) if p is None else (y, p)
+
+
+def _one_dtype(*params) -> bool:
+    return len({t.dtype for t in params if t is not None}) <= 1
+
+
 class Block(nn.Module):
     """Pre-norm transformer block: x + ls1(attn(norm1(x))), then x + ls2(mlp(norm2(x)))."""
 
     def __init__(self, dim: int, num_heads: int, mlp_ratio: float = 4.0, init_values: float | None = None,
-                 qk_norm: bool = False, rope=None):
+                 qk_norm: bool = False, rope=None, drop: float = 0.0):
         super().__init__()
         self.norm1 = nn.LayerNorm(dim)
-        self.attn = Attention(dim, num_heads, qkv_bias=True, proj_bias=True, qk_norm=qk_norm, rope=rope)
+        self.attn = Attention(dim, num_heads, qkv_bias=True, proj_bias=True, proj_drop=drop, qk_norm=qk_norm, rope=rope)
         self.ls1 = LayerScale(dim, init_values) if init_values else nn.Identity()
         self.norm2 = nn.LayerNorm(dim)
-        self.mlp = Mlp(dim, int(dim * mlp_ratio))
+        self.mlp = Mlp(dim, int(dim * mlp_ratio), drop=drop)
         self.ls2 = LayerScale(dim, init_values) if init_values else nn.Identity()
-        self.frame_attention = "sdpa"  # "saf3r", "saf3r_train": the package kernels (see module doc)
+        self.frame_attention = "sdpa"  # "saf3r", "saf3r_train", "saf3r_block": the package kernels (see module doc)
         self.num_special = 0
 
     def _norm(self, norm: nn.Module, x):
-        if self.frame_attention != "saf3r_train" or not autograd.computed_as(norm, nn.LayerNorm) \
+        if self.frame_attention not in TRAINED or not autograd.computed_as(norm, nn.LayerNorm) \
                 or len(norm.normalized_shape) != 1:
             return norm(x)
         # (under autocast the products that follow take their input in the autocast type)
@@ -130,9 +154,49 @@ class Block(nn.Module):
         return autograd.layer_norm(x, norm.weight, norm.bias, norm.eps,
                                    torch.get_autocast_dtype("cuda") if cast else None)
 
+    @staticmethod
+    def _scale(ls: nn.Module):
+        """(whether the kernels stand for ``ls``, its gate or None)."""
+        if autograd.computed_as(ls, LayerScale):
+            return True, ls.gamma
+        return autograd.computed_as(ls, nn.Identity), None
+
+    def _residual(self, x, a, p: float):
+        """(x + ls1(a with dropout p), norm2 of it)."""
+        fits, gate = self._scale(self.ls1)
+        norm = self.norm2
+        # (the stream's type is what torch's sum would have)
+        stream = torch.promote_types(x.dtype, torch.promote_types(a.dtype, a.dtype if gate is None else gate.dtype))
+        if (fits and autograd.computed_as(norm, nn.LayerNorm) and len(norm.normalized_shape) == 1
+                and _one_dtype(gate, norm.weight, norm.bias) and stream in (a.dtype, torch.float32)):
+            return autograd.residual_norm(x.to(stream), a, gate, norm.weight, norm.bias, norm.eps, p)
+        x = x + self.ls1(autograd.dropout(a, p))
+        return x, self._norm(norm, x)
+
+    def _mlp(self, x, h):
+        """x + ls2(mlp(h)), the residual and the scale in the second product's epilogue."""
+        fits, gate = self._scale(self.ls2)
+        mlp = self.mlp
+        if fits and autograd.computed_as(mlp, Mlp):
+            act, p = autograd.module_activation(mlp.act), autograd.module_dropout(getattr(mlp, "drop", None))
+            dt = autograd.product_dtype(mlp.fc1, h)
+            if (act is not None and p is not None and dt is not None and dt == autograd.product_dtype(mlp.fc2, h.to(dt))
+                    and _one_dtype(gate, mlp.fc2.bias)):
+                u = autograd.linear(h.to(dt), mlp.fc1.weight, mlp.fc1.bias, act, dropout=p)
+                stream = torch.promote_types(x.dtype, torch.promote_types(dt, dt if gate is None else gate.dtype))
+                return autograd.linear(u, mlp.fc2.weight, mlp.fc2.bias, gate=gate, residual=x.to(stream), dropout=p)
+        return x + self.ls2(mlp(h))
+
     def forward(self, x, pos=None, positions: int | None = None):
-        """``positions`` (``"saf3r_train"`` only): more than any of ``pos``, see ``trained_attention``."""
+        """``positions`` (``"saf3r_train"`` and ``"saf3r_block"``): more than any of ``pos``, see ``trained_attention``."""
         h = self._norm(self.norm1, x)
+        if self.frame_attention == "saf3r_block":
+            if autograd.computed_as(self.attn, Attention):
+                a, p = projected_attention(self.attn, h, pos, positions)
+            else:
+                a, p = self.attn(h, pos=pos), 0.0
+            x, h = self._residual(x, a, p)
+            return self._mlp(x, h)
         if self.frame_attention == "saf3r" and not isinstance(self.attn, Attention):
             raise RuntimeError("frame_attention='saf3r' is for unpatched frame blocks")
         if self.frame_attention == "saf3r":
@@ -219,15 +283,15 @@ class Aggregator(nn.Module):
     def __init__(self, img_size: int = 518, patch_size: int = 14, embed_dim: int = 1024, depth: int = 24,
                  num_heads: int = 16, mlp_ratio: float = 4.0, num_register_tokens: int = 4, rope_freq: float = 100.0,
                  init_values: float = 0.01, dino_depth: int = 24, dino_dim: int = 1024, dino_heads: int = 16,
-                 frame_attention: str = "sdpa"):
+                 frame_attention: str = "sdpa", drop: float = 0.0):
         super().__init__()
         if dino_dim != embed_dim:
             raise ValueError("the patch embedding width must equal the aggregator width")
         self.patch_embed = DinoPatchEmbed(img_size, patch_size, dino_dim, dino_depth, dino_heads, num_register_tokens)
         self.rope = RotaryPositionEmbedding2D(rope_freq) if rope_freq > 0 else None
-        self.frame_blocks = nn.ModuleList([Block(embed_dim, num_heads, mlp_ratio, init_values, True, self.rope)
+        self.frame_blocks = nn.ModuleList([Block(embed_dim, num_heads, mlp_ratio, init_values, True, self.rope, drop)
                                            for _ in range(depth)])
-        self.global_blocks = nn.ModuleList([Block(embed_dim, num_heads, mlp_ratio, init_values, True, self.rope)
+        self.global_blocks = nn.ModuleList([Block(embed_dim, num_heads, mlp_ratio, init_values, True, self.rope, drop)
                                             for _ in range(depth)])
         self.depth = depth
         self.patch_size = patch_size
@@ -243,13 +307,14 @@ class Aggregator(nn.Module):
     def set_frame_attention(self, kind: str):
         """"sdpa" (torch's fused kernels) or "saf3r" (the frame-local pattern of the package kernels) for
         the frame blocks and the patch embedding's blocks; "saf3r_train": the differentiable kernels for these and
-        for the norms of the global blocks (their attention too where it is not patched)."""
-        if kind not in ("sdpa", "saf3r", "saf3r_train"):
+        for the norms of the global blocks (their attention too where it is not patched); "saf3r_block": as
+        "saf3r_train", with the products, residuals, layer scales and dropouts of all of these blocks."""
+        if kind not in ("sdpa", "saf3r", *TRAINED):
             raise ValueError(f"frame attention {kind!r}")
         for b in list(self.frame_blocks) + list(self.patch_embed.blocks):
             b.frame_attention = kind
         for b in self.global_blocks:
-            b.frame_attention = "saf3r_train" if kind == "saf3r_train" else "sdpa"
+            b.frame_attention = kind if kind in TRAINED else "sdpa"
         for b in self.frame_blocks:
             b.num_special = self.patch_start_idx
 
@@ -262,7 +327,7 @@ class Aggregator(nn.Module):
 
     @staticmethod
     def _block(block, x, pos, positions: int):
-        if type(block).forward is Block.forward and block.frame_attention == "saf3r_train":
+        if type(block).forward is Block.forward and block.frame_attention in TRAINED:
             return block(x, pos=pos, positions=positions)
         return block(x, pos=pos)
 

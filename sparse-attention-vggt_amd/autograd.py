@@ -1,5 +1,6 @@
-"""Differentiable forms of the training kernels (``ops.frame_attn_*``, ``ops.head_rotary_*``, ``ops.layer_norm_*``) for
-fine-tuning a patched model: the static head patterns with their gradients, the q / k prologue and the block norms.
+"""Differentiable forms of the training kernels (``ops.frame_attn_*``, ``ops.head_rotary_*``, ``ops.layer_norm_*``,
+``ops.linear_*``, ``ops.residual_norm_*``, ``ops.dropout``) for fine-tuning a patched model: the static head patterns with
+their gradients, the q / k prologue, the block norms, and the products, residuals and dropouts around them.
 
 Each function computes its gradients with the backward kernels; nothing is differentiated twice (a second
 derivative raises). Without an input that needs a gradient they run the forward kernels alone. A call captured into
@@ -152,6 +153,101 @@ def qkv_attention(qkv: torch.Tensor, patterns: Sequence[int], frames: int = 1, p
                                norm, eps, token_mask, scale)
 
 
+def _drop_state(p: float, state: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor | None:
+    """The state of a call's keep mask: the one that is given, or a new one."""
+    return state if state is not None or p == 0.0 else ops.dropout_state(x.device)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, gate, residual, activation, out_dtype, dropout, state):
+        low = weight.to(x.dtype)
+        grad = any(ctx.needs_input_grad[:4])
+        keep = grad and (activation is not None or ctx.needs_input_grad[3])
+        res = ops.linear_fwd(x, low, bias, activation, gate, residual, out_dtype, dropout, state, keep)
+        y, kept = res if keep else (res, None)
+        if grad:
+            ctx.save_for_backward(x, low, kept, gate, state)
+        ctx.args = (activation, dropout, weight.dtype, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        need = ctx.needs_input_grad
+        dx = dw = db = dg = None
+        if any(need[:4]):
+            x, low, kept, gate, state = ctx.saved_tensors
+            activation, dropout, weight_dtype, bias_dtype = ctx.args
+            dx, dw, db, dg = ops.linear_bwd(dy, x, low, kept, activation, gate, dropout, state, need[:4],
+                                            torch.float32 if weight_dtype == torch.float32 else None, bias_dtype)
+            dw = None if dw is None else dw.to(weight_dtype)
+            db = None if db is None else db.to(bias_dtype)
+        return dx, dw, db, dg, dy if need[4] else None, None, None, None, None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+           gate: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+           out_dtype: torch.dtype | None = None, dropout: float = 0.0, state: torch.Tensor | None = None) -> torch.Tensor:
+    """``residual + gate * drop(act(x weight^T + bias))`` (``ops.linear_fwd``) with the gradients of x, weight, bias, gate and
+    residual. x bf16 or fp16; a weight of another type (fp32 master weights) is rounded to x's, and an fp32 one's gradient
+    is fp32. ``dropout`` draws a new mask unless ``state`` gives one; the mask is not stored."""
+    return _Linear.apply(x, weight, bias, gate, residual, activation, out_dtype, float(dropout),
+                         _drop_state(dropout, state, x))
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, branch, gate, weight, bias, eps, dropout, state):
+        h, y, mean, rstd = ops.residual_norm_fwd(x, branch, gate, weight, bias, eps, None, dropout, state)
+        ctx.save_for_backward(h, mean, rstd, branch if ctx.needs_input_grad[2] else None, gate, weight, state)
+        ctx.args = (dropout, branch.dtype, None if bias is None else bias.dtype)
+        ctx.set_materialize_grads(False)
+        return h, y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, dy):
+        if dh is None and dy is None:
+            return (None,) * 8
+        h, mean, rstd, branch, gate, weight, state = ctx.saved_tensors
+        dropout, y_dtype, bias_dtype = ctx.args
+        if dy is None:
+            dy = torch.zeros(h.shape, dtype=y_dtype, device=h.device)
+        dx, dbranch, dg, dw, db = ops.residual_norm_bwd(dh, dy, h, mean, rstd, branch, gate, weight, dropout, state,
+                                                        ctx.needs_input_grad[1:5])
+        return dx, dbranch, dg, dw, db if db is None else db.to(bias_dtype), None, None, None
+
+
+def residual_norm(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tensor | None = None,
+                  weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
+                  dropout: float = 0.0, state: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(h, y): ``h = x + gate * drop(branch)`` and ``y = LayerNorm(h)`` in the branch's type (``ops.residual_norm_fwd``) with
+    the gradients of x, branch, gate, weight and bias. ``dropout`` draws a new mask unless ``state`` gives one."""
+    return _ResidualNorm.apply(x, branch, gate, weight, bias, eps, float(dropout), _drop_state(dropout, state, x))
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, state):
+        ctx.save_for_backward(state)
+        ctx.p = p
+        return ops.dropout(x, p, state)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return ops.dropout(dy, ctx.p, ctx.saved_tensors[0]), None, None
+
+
+def dropout(x: torch.Tensor, p: float, training: bool = True, state: torch.Tensor | None = None) -> torch.Tensor:
+    """``x * keep / (1 - p)`` in training (``ops.dropout``) with the gradient of x; the mask is drawn anew unless ``state``
+    gives it, and is not stored."""
+    if not training or p == 0.0:
+        return x
+    return _Dropout.apply(x, float(p), _drop_state(p, state, x))
+
+
 def computed_as(module: torch.nn.Module, kind: type) -> bool:
     """Whether calling ``module`` is ``kind``'s forward and nothing else, so that a kernel can stand for the call: no
     forward of a subclass or of the instance, no hooks."""
@@ -208,3 +304,35 @@ def module_attention(attn, qkv: torch.Tensor, pos: torch.Tensor | None, patterns
         pos = None
     return qkv_attention(qkv, patterns, frames, pos, tables, norm, weight, bias, eps, token_mask,
                          getattr(attn, "scale", None))
+
+
+def product_dtype(m: torch.nn.Module, x: torch.Tensor) -> torch.dtype | None:
+    """The 16-bit type in which ``m(x)`` is computed where m is a plain Linear (autocast's, or that of x and the weight), or
+    None: the kernels do not stand for that call."""
+    if not computed_as(m, torch.nn.Linear):
+        return None
+    auto = torch.is_autocast_enabled("cuda")
+    dt = torch.get_autocast_dtype("cuda") if auto else m.weight.dtype
+    return dt if dt in (torch.bfloat16, torch.float16) and (auto or x.dtype == dt) else None
+
+
+def module_linear(m: torch.nn.Module, x: torch.Tensor) -> torch.Tensor:
+    """``m(x)``: through ``linear`` where the kernels stand for the call (``product_dtype``)."""
+    dt = product_dtype(m, x)
+    return m(x) if dt is None else linear(x.to(dt), m.weight, m.bias)
+
+
+def module_dropout(m: torch.nn.Module | None) -> float | None:
+    """The probability with which ``m`` drops elements now, or None where it is not a plain Dropout or Identity."""
+    if m is None or computed_as(m, torch.nn.Identity):
+        return 0.0
+    if not computed_as(m, torch.nn.Dropout):
+        return None
+    return float(m.p) if m.training else 0.0
+
+
+def module_activation(m: torch.nn.Module) -> str | None:
+    """The name of ``m`` as an activation of ``linear``, or None."""
+    if not computed_as(m, torch.nn.GELU):
+        return None
+    return {"none": "gelu", "tanh": "gelu_tanh"}[m.approximate]

@@ -20,6 +20,9 @@ Configuration (plain dict or attribute object, as the reference's addict ``model
     patch_module.trainable                 True: forwards that need gradients run through the differentiable
                                            kernels (heads of the modes full / dense, global_to_frame /
                                            frame_local, all_to_first, anchor_local and skip; others raise)
+    patch_module.linear_kernels            True: the qkv and output products of the patched layers and their
+                                           output dropout run through the package kernels (``autograd.linear``,
+                                           ``autograd.dropout``), where they are plain modules in 16 bits
 The lazy indices are shared through one ``SelectionState`` per model instead of rebinding the
 aggregator forward: every dino_topk layer after the one holding the first correspondence head
 reads them, exactly the layers the reference copies them to. The non-lazy indices (and the DINO
@@ -34,6 +37,7 @@ import json
 import torch
 from torch import Tensor
 
+from .. import autograd
 from ..layout import HEAD_DIM
 from .utils import compute_qk_topk_indices_batched
 from .wrapper import BaseHeadwiseSparseAttentionWrapper, SelectionState, _get
@@ -82,7 +86,7 @@ def patch_model(model, model_cfg):
         blocks[i].attn = HeadwiseSparseAttentionWrapper(
             orig, layer_idx=i, dino_topk=_get(pm, "topk", 4), lazy_dino_topk=lazy, config=layer_config,
             block_topk=_get(pm, "block_topk", 4), topk_scope=_get(pm, "topk_scope", "frame"), shared=state,
-            trainable=_get(pm, "trainable", False))
+            trainable=_get(pm, "trainable", False), linear_kernels=_get(pm, "linear_kernels", False))
     model.saf3r_selection_state = state
     if has_dino and not lazy:
         install_feature_topk(model, model_cfg)
@@ -170,7 +174,7 @@ class HeadwiseSparseAttentionWrapper(BaseHeadwiseSparseAttentionWrapper):
             raise RuntimeError("HeadwiseSparseAttentionWrapper runs on the GPU kernels only")
         om = self.orig_module
         geom = self.geometry(N)
-        qkv = om.qkv(x).reshape(N, 3 * C)
+        qkv = (autograd.module_linear(om.qkv, x) if self.linear_kernels else om.qkv(x)).reshape(N, 3 * C)
         if qkv.dtype != torch.bfloat16:
             qkv = qkv.to(torch.bfloat16)
         qkv = qkv.contiguous()
@@ -180,5 +184,7 @@ class HeadwiseSparseAttentionWrapper(BaseHeadwiseSparseAttentionWrapper):
         y = out.reshape(B, N, C)
         if not torch.is_autocast_enabled("cuda") and y.dtype != om.proj.weight.dtype:
             y = y.to(om.proj.weight.dtype)
-        y = om.proj(y)
-        return om.proj_drop(y)
+        if not self.linear_kernels:
+            return om.proj_drop(om.proj(y))
+        y, p = autograd.module_linear(om.proj, y), autograd.module_dropout(om.proj_drop)
+        return om.proj_drop(y) if p is None else autograd.dropout(y, p)

@@ -114,6 +114,8 @@ class BaseHeadwiseSparseAttentionWrapper(nn.Module):
             other = sorted({c["mode"] for c, p in zip(self.head_cfg, self.patterns) if p not in ops.STATIC_PATTERNS})
             if other:
                 raise NotImplementedError(f"trainable: no gradients through heads of mode {', '.join(other)}")
+        # linear_kernels: the qkv and output products and the output dropout run through the package kernels
+        self.linear_kernels = bool(kwargs.get("linear_kernels", False))
         # pack Q with the softmax scale folded in (one bf16 rounding of the fp32 q * scale * log2 e), so
         # that the attention walks skip the running maximum; off for tests that compare the plain layout
         self.prescale_q = True
