@@ -628,9 +628,10 @@ int saf3r_linear_fwd(const void* x, int64_t x_stride, const void* w, int64_t w_s
                      const int64_t* state, const void* residual, int64_t res_stride, void* y, int64_t y_stride,
                      int y_type, void* kept, int64_t kept_stride, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Workspace bytes of saf3r_linear_fwd (0 for most sizes), -1 for sizes that it rejects. copies: 1: of x, 2: of w (their
- * pointer is no multiple of 16 bytes, their stride or `in` none of 8 elements, or the stride is less than `in`). */
-int64_t saf3r_linear_fwd_workspace_bytes(int64_t rows, int in, int out, int copies);
+/* Workspace bytes of saf3r_linear_fwd (0 for most sizes), -1 for sizes that it rejects. activation, drop: of that call.
+ * copies: 1: of x, 2: of w (their pointer is no multiple of 16 bytes, their stride or `in` none of 8 elements, or the stride
+ * is less than `in`). */
+int64_t saf3r_linear_fwd_workspace_bytes(int64_t rows, int in, int out, int activation, int drop, int copies);
 
 /*
  * Gradients of saf3r_linear_fwd from dy (rows of y_type; it is the residual's gradient itself), each may be NULL:

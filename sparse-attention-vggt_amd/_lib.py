@@ -121,7 +121,7 @@ def load():
         "saf3r_layer_norm_bwd_workspace_bytes": ([i64, i32], i64),
         "saf3r_linear_fwd": ([p, i64, p, i64, i32, i64, i32, i32, p, p, i32, i32, i32, p, p, i64, p, i64, i32, p, i64, p,
                               i64, p], i32),
-        "saf3r_linear_fwd_workspace_bytes": ([i64, i32, i32, i32], i64),
+        "saf3r_linear_fwd_workspace_bytes": ([i64, i32, i32, i32, i32, i32], i64),
         "saf3r_linear_bwd": ([p, i64, i32, p, i64, p, i64, i32, i64, i32, i32, p, i64, p, i32, i32, i32, p, p, i64, p, i64,
                               i32, p, p, p, i64, p], i32),
         "saf3r_linear_bwd_workspace_bytes": ([i64, i32, i32, i32], i64),

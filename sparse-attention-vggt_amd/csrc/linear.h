@@ -199,14 +199,14 @@ struct LinearGradParams {
   const void* kept;
   const void* gate;
   void* dz;     // null: sums only; columns n .. n8 - 1 are zeros
-  float* part;  // null: no sums; [parts][2][n]
+  float* part;  // null: no sums; [parts][2][n], the gate's where it is asked for
   int64_t ld_dy, ld_kept, ld_dz, rows, part_rows;
   DropParams drop;
   int act, n;
   bool param32;
 };
 int64_t linear_grad_parts(int64_t rows, int n);
-int linear_grad(const char* who, const LinearGradParams& p, int type, bool dy32, bool vec, int64_t parts,
+int linear_grad(const char* who, const LinearGradParams& p, int type, bool dy32, bool vec, bool dgate, int64_t parts,
                 hipStream_t stream);
 
 }  // namespace saf3r

@@ -764,7 +764,8 @@ struct Plan {
 // 87936 rows, widths of 128 to 6144 and 1 to 16 splits: start and end; a step while every work-group has a compute unit of
 // its own (few of them, and more with their number: the card's clock goes down under load); of two on a unit, a step of the
 // slower and, with 512, of the whole card. A round behind the first costs half of one at least.
-static double tile_time(int kind, int64_t wgs, int64_t steps) {
+// `epilogue`: cycles of a value's activation, dropout and residual; the values of a lane are 16 to 256 a tile.
+static double tile_time(int kind, int64_t wgs, int64_t steps, int epilogue) {
   constexpr struct {
     double ends, alone, shared, two, full;
     int places;
@@ -772,7 +773,8 @@ static double tile_time(int kind, int64_t wgs, int64_t steps) {
                       {7.5, 0.31, 0.16, 0.72, 1.00, 512},
                       {10.0, 0.49, 0.44, 1.20, 1.75, 512},
                       {16.0, 0.97, 0.60, 1.57, 1.57, 256}};
-  const auto& k = kTimes[kind];
+  auto k = kTimes[kind];
+  k.ends += (kTileM[kind] * kTileN[kind] / 256) * epilogue / 2100.0;
   const double x = (double)wgs / 256;
   if (wgs <= 256) return k.ends + (double)steps * (k.alone + k.shared * x * x);
   if (wgs <= k.places) return k.ends + (double)steps * (k.two + (k.full - k.two) * (x - 1));
@@ -781,10 +783,13 @@ static double tile_time(int kind, int64_t wgs, int64_t steps) {
   return k.ends + 0.5 * (double)halves * (double)steps * k.full + 0.5 * (double)(halves - 2) * end;
 }
 
+// Cycles of a value's epilogue behind its conversion.
+static int epilogue_cycles(int act, int drop) { return (act != SAF3R_NO_ACTIVATION ? 80 : 0) + (drop ? 70 : 0); }
+
 // Tiles and splits of the least such time. Splits have two steps at least; their join is a launch more, and writes and reads
 // the partial sums once (5.5 TB/s). Against one kind and split for all sizes: 4096 x 1024 from 1041 rows 27.6 -> 16.3 us,
 // 1024 x 1024 from 2748 rows 24 -> 15, 128 x 512 from 20000 rows 24.6 -> 18.9, 10992 x 1024 from 4096 105 -> 93.
-static Plan plan_of(int64_t m, int n, int64_t k, bool rows_kind) {
+static Plan plan_of(int64_t m, int n, int64_t k, bool rows_kind, int epilogue) {
   Plan r{};
   r.steps = (int)((k + 63) / 64);
   r.few = rows_kind && m <= 32;
@@ -794,7 +799,7 @@ static Plan plan_of(int64_t m, int n, int64_t k, bool rows_kind) {
     for (int splits = 1; splits <= 64; splits += splits < 4 ? 1 : splits < 8 ? 2 : splits < 16 ? 4 : 8) {
       if (splits > 1 && (r.steps < 2 * splits || tm * tn * splits > 1024)) break;
       const int per = (r.steps + splits - 1) / splits, used = (r.steps + per - 1) / per;
-      double t = tile_time(kind, tm * tn * used, per);
+      double t = tile_time(kind, tm * tn * used, per, used > 1 ? 0 : epilogue);
       if (used > 1) t += 2.5 + (double)used * (double)m * n * 8 / 5.5e6;
       if (t < best) {
         best = t;
@@ -817,7 +822,7 @@ static int64_t part_bytes(const Plan& r, int64_t m, int n) {
 template <typename T, bool ACOLS, bool BCOLS>
 static int product(const char* who, const void* a, int64_t lda, const void* b, int64_t ldb, int64_t m, int n, int64_t k,
                    const EpiParams& epi, void* part, hipStream_t stream) {
-  const Plan r = plan_of(m, n, k, !ACOLS && !BCOLS);
+  const Plan r = plan_of(m, n, k, !ACOLS && !BCOLS, epilogue_cycles(epi.act, epi.drop.limit));
   GemmParams p{};
   p.a = (const char*)a;
   p.b = (const char*)b;
@@ -972,12 +977,12 @@ static bool vec_rows(const void* p, int64_t stride) { return aligned16(p) && str
 
 using namespace saf3r;
 
-extern "C" int64_t saf3r_linear_fwd_workspace_bytes(int64_t rows, int in, int out, int copies) {
+extern "C" int64_t saf3r_linear_fwd_workspace_bytes(int64_t rows, int in, int out, int activation, int drop, int copies) {
   const char* who = "saf3r_linear_fwd_workspace_bytes";
   if (sizes_check(who, rows, in, out)) return -1;
   if (rows == 0) return 0;
-  return part_bytes(plan_of(rows, out, in, true), rows, out) + (copies & 1 ? pad_bytes(rows, in) : 0) +
-         (copies & 2 ? pad_bytes(out, in) : 0);
+  return part_bytes(plan_of(rows, out, in, true, epilogue_cycles(activation, drop)), rows, out) +
+         (copies & 1 ? pad_bytes(rows, in) : 0) + (copies & 2 ? pad_bytes(out, in) : 0);
 }
 
 extern "C" int saf3r_linear_fwd(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int type, int64_t rows,
@@ -1004,7 +1009,7 @@ extern "C" int saf3r_linear_fwd(const void* x, int64_t x_stride, const void* w, 
     if (p)
       if (int e = row_check(who, p, 0, out, param_type, false)) return e;
   const bool pad_x = !in_place(x, x_stride, in), pad_w = !in_place(w, w_stride, in);
-  const int64_t need = saf3r_linear_fwd_workspace_bytes(rows, in, out, pad_x + 2 * pad_w);
+  const int64_t need = saf3r_linear_fwd_workspace_bytes(rows, in, out, activation, drop, pad_x + 2 * pad_w);
   if (workspace_bytes < need || (need > 0 && (!workspace || !aligned16(workspace))))
     return fail(SAF3R_ERR_INVALID, "%s: workspace of %lld bytes: %lld, 16-byte aligned, are needed", who,
                 (long long)workspace_bytes, (long long)need);
@@ -1023,7 +1028,7 @@ extern "C" int saf3r_linear_fwd(const void* x, int64_t x_stride, const void* w, 
   epi.vec = out % 8 == 0 && vec_rows(y, y_stride) && aligned16(bias) && aligned16(gate) &&
             (!kept || vec_rows(kept, kept_stride)) && (!residual || vec_rows(residual, res_stride));
   const hipStream_t s = (hipStream_t)stream;
-  char* copies = (char*)workspace + part_bytes(plan_of(rows, out, in, true), rows, out);
+  char* copies = (char*)workspace + part_bytes(plan_of(rows, out, in, true, epilogue_cycles(activation, drop)), rows, out);
   if (int e = pad_operands(who, copies, in, &x, &x_stride, rows, pad_x, &w, &w_stride, out, pad_w, s)) return e;
   const int k = (int)round8(in);  // (zeros behind `in` in both)
   if (type == SAF3R_BF16)
@@ -1042,7 +1047,7 @@ static BwdSizes bwd_sizes(int64_t rows, int in, int out, bool own_dz, bool pad_x
   r.copies = (pad_x ? pad_bytes(rows, in) : 0) + (pad_w ? pad_bytes(out, in) : 0);
   r.dz = own_dz ? round256(rows * round8(out) * 2) : 0;
   r.sums = round256(linear_grad_parts(rows, out) * 2 * out * 4);
-  r.products = std::max(part_bytes(plan_of(rows, in, out, false), rows, in), part_bytes(plan_of(out, in, rows, false), out, in));
+  r.products = std::max(part_bytes(plan_of(rows, in, out, false, 0), rows, in), part_bytes(plan_of(out, in, rows, false, 0), out, in));
   return r;
 }
 
@@ -1127,7 +1132,7 @@ extern "C" int saf3r_linear_bwd(const void* dy, int64_t dy_stride, int y_type, c
     g.n = out;
     g.param32 = param_type == SAF3R_FP32;
     const bool vec = out % 8 == 0 && vec_rows(dy, dy_stride) && aligned16(gate) && (!g.kept || vec_rows(kept, kept_stride));
-    if (int e = linear_grad(who, g, type, y_type == SAF3R_FP32, vec, parts, s)) return e;
+    if (int e = linear_grad(who, g, type, y_type == SAF3R_FP32, vec, dgate != nullptr, parts, s)) return e;
     if (sums)
       if (int e = sum_parts(who, g.part, parts, out, dgate, dbias, param_type, s)) return e;
     if (own_dz) {

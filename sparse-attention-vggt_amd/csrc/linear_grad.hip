@@ -9,7 +9,7 @@
 
 namespace saf3r {
 
-template <typename T, typename TY, bool VEC>
+template <typename T, typename TY, bool VEC, bool DGATE>
 __global__ void __launch_bounds__(256) linear_grad_kernel(const LinearGradParams p) {
   __shared__ float lds[256 * 8];
   const int lane = tid_x() & 31, slot = tid_x() >> 5;
@@ -35,23 +35,20 @@ __global__ void __launch_bounds__(256) linear_grad_kernel(const LinearGradParams
       if (p.kept) epi_load<T>(p.kept, false, VEC, row * p.ld_kept + col, cnt, z);
       if (p.drop.limit) drop8(key, p.drop.limit, p.drop.scale, (uint32_t)col >> 3, (uint64_t)row, g);
       if (p.kept) {
+        auto slopes = [&](int act) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float a;
+            const float d = act_slope(act, z[e], &a);
+            if constexpr (DGATE) dg[e] += g[e] * a;
+            g[e] *= d;
+          }
+        };
         if (p.act == SAF3R_GELU) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float a;
-            const float d = act_slope(SAF3R_GELU, z[e], &a);
-            dg[e] += g[e] * a;
-            g[e] *= d;
-          }
+          slopes(SAF3R_GELU);
         } else if (p.act == SAF3R_GELU_TANH) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float a;
-            const float d = act_slope(SAF3R_GELU_TANH, z[e], &a);
-            dg[e] += g[e] * a;
-            g[e] *= d;
-          }
-        } else {
+          slopes(SAF3R_GELU_TANH);
+        } else if constexpr (DGATE) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) dg[e] += g[e] * z[e];
         }
@@ -65,15 +62,15 @@ __global__ void __launch_bounds__(256) linear_grad_kernel(const LinearGradParams
     }
   }
   if (!p.part) return;
-  add_slots<8, 32>(dg, lds);
+  if constexpr (DGATE) add_slots<8, 32>(dg, lds);
   add_slots<8, 32>(db, lds);
   if (tid_x() < 32 && col < p.n) {
     float* to = p.part + (int64_t)bid_y() * 2 * p.n + col;
     if constexpr (VEC) {
-      store_vec<8>(to, dg);
+      if constexpr (DGATE) store_vec<8>(to, dg);
       store_vec<8>(to + p.n, db);
     } else {
-      store_some<8>(to, cnt, dg);
+      if constexpr (DGATE) store_some<8>(to, cnt, dg);
       store_some<8>(to + p.n, cnt, db);
     }
   }
@@ -85,15 +82,17 @@ int64_t linear_grad_parts(int64_t rows, int n) {
   return std::max<int64_t>(1, std::min<int64_t>((1024 + strips - 1) / strips, rows / 16));
 }
 
-int linear_grad(const char* who, const LinearGradParams& p, int type, bool dy32, bool vec, int64_t parts,
+int linear_grad(const char* who, const LinearGradParams& p, int type, bool dy32, bool vec, bool dgate, int64_t parts,
                 hipStream_t stream) {
   const dim3 grid((uint32_t)((p.n + 255) / 256), (uint32_t)parts);
-  auto go = [&](auto t, auto ty) {
-    if (vec)
-      hipLaunchKernelGGL((linear_grad_kernel<decltype(t), decltype(ty), true>), grid, dim3(256), 0, stream, p);
-    else
-      hipLaunchKernelGGL((linear_grad_kernel<decltype(t), decltype(ty), false>), grid, dim3(256), 0, stream, p);
+  auto one = [&](auto t, auto ty, auto v, auto dg) {
+    hipLaunchKernelGGL((linear_grad_kernel<decltype(t), decltype(ty), decltype(v)::value, decltype(dg)::value>), grid,
+                       dim3(256), 0, stream, p);
     return check_launch(who);
+  };
+  auto go = [&](auto t, auto ty) {
+    if (dgate) return vec ? one(t, ty, Int<1>(), Int<1>()) : one(t, ty, Int<0>(), Int<1>());
+    return vec ? one(t, ty, Int<1>(), Int<0>()) : one(t, ty, Int<0>(), Int<0>());
   };
   if (type == SAF3R_BF16) return dy32 ? go(__bf16(), float()) : go(__bf16(), __bf16());
   return dy32 ? go(_Float16(), float()) : go(_Float16(), _Float16());

@@ -1382,10 +1382,13 @@ def _copied(ptr: int, stride: int, dim: int) -> bool:
 
 
 @lru_cache(maxsize=4096)
-def _linear_bytes(backward: bool, rows: int, n_in: int, n_out: int, copies: int) -> int:
-    lib = _lib.load()
-    size = lib.saf3r_linear_bwd_workspace_bytes if backward else lib.saf3r_linear_fwd_workspace_bytes
-    return max(size(rows, n_in, n_out, copies), 0)
+def _linear_fwd_bytes(*sizes: int) -> int:
+    return max(_lib.load().saf3r_linear_fwd_workspace_bytes(*sizes), 0)
+
+
+@lru_cache(maxsize=4096)
+def _linear_bwd_bytes(*sizes: int) -> int:
+    return max(_lib.load().saf3r_linear_bwd_workspace_bytes(*sizes), 0)
 
 
 def linear_fwd(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
@@ -1426,7 +1429,7 @@ def linear_fwd(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     y = x.new_empty(shape) if out_dtype == dt else x.new_empty(shape, dtype=out_dtype)
     kept = x.new_empty(shape) if keep else None
     xp, wp, count = rows.data_ptr(), w.data_ptr(), y.numel() // n
-    nbytes = _linear_bytes(False, count, k, n, _copied(xp, stride, k) | _copied(wp, wstride, k) << 1)
+    nbytes = _linear_fwd_bytes(count, k, n, act, limit, _copied(xp, stride, k) | _copied(wp, wstride, k) << 1)
     ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _mark("linear_fwd", "start")
     _lib.check(_lib.load().saf3r_linear_fwd(xp, stride, wp, wstride, _DTYPES[dt], count, k, n, _ptr(b), _ptr(g),
@@ -1484,7 +1487,7 @@ def linear_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, kept: to
     own_dz = act or g is not None or limit or dy.dtype != dt or _copied(dp, dstride, n)
     copies = (need_dw and _copied(xp, stride, k)) | (need_dx and _copied(wp, wstride, k)) << 1 | (
         4 if own_dz and (need_dx or need_dw) else 0)
-    nbytes = _linear_bytes(True, count, k, n, copies)
+    nbytes = _linear_bwd_bytes(count, k, n, copies)
     ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _mark("linear_bwd", "start")
     _lib.check(_lib.load().saf3r_linear_bwd(dp, dstride, _DTYPES[dy.dtype], xp, stride, wp, wstride, _DTYPES[dt], count, k, n,

@@ -85,8 +85,9 @@ def test_linear(L, bwd):
         no(INVALID, "aligned", bias=258)
         no(INVALID, "aligned", kept=257)
         size = L.load().saf3r_linear_fwd_workspace_bytes
-        assert size(3, 64, 32, 0) == 0 and size(3, 60, 32, 1) > 0 and size(3, 60, 32, 3) > size(3, 60, 32, 2) > 0
-        assert size(0, 64, 32, 3) == 0 and size(3, 0, 32, 0) == -1 and size(130, 4096, 64, 0) > 0
+        assert size(3, 64, 32, 1, 9, 0) == 0 and size(3, 60, 32, 0, 0, 1) > 0
+        assert size(3, 60, 32, 0, 0, 3) > size(3, 60, 32, 0, 0, 2) > 0
+        assert size(0, 64, 32, 0, 0, 3) == 0 and size(3, 0, 32, 0, 0, 0) == -1 and size(130, 4096, 64, 0, 0, 0) > 0
         no(INVALID, "workspace", k=60, nbytes=0)
         no(INVALID, "workspace", x=258, wsp=None)
         assert linear(L, rows=0, x=None, y=None) == 0
