@@ -752,6 +752,8 @@ __global__ void __launch_bounds__(256) join_kernel(const GemmParams p) {
 constexpr int kMaxSize = 1 << 21;         // widths of a layer (a unit's byte offsets stay in 32 bits)
 constexpr int64_t kMaxRows = 0x7fffff00;  // rows of a layer
 
+constexpr int64_t kMaxTiles = 0xffffffffll / 256;  // (a launch counts its threads in 32 bits)
+
 // How a product runs: the kernel for few rows, or tiles of one kind and splits of the reduction.
 enum Kind { kTiny, kSmall, kPair, kWide, kKinds };
 constexpr int kTileM[kKinds] = {64, 128, 256, 256}, kTileN[kKinds] = {64, 128, 128, 256};
@@ -769,8 +771,8 @@ static double tile_time(int kind, int64_t wgs, int64_t steps, int epilogue) {
   constexpr struct {
     double ends, alone, shared, two, full;
     int places;
-  } kTimes[kKinds] = {{5.5, 0.19, 0.06, 0.30, 0.36, 512},
-                      {7.5, 0.31, 0.16, 0.72, 1.00, 512},
+  } kTimes[kKinds] = {{5.5, 0.19, 0.06, 0.30, 0.45, 512},
+                      {7.5, 0.31, 0.18, 0.72, 1.00, 512},
                       {10.0, 0.49, 0.44, 1.20, 1.75, 512},
                       {16.0, 0.97, 0.60, 1.57, 1.57, 256}};
   auto k = kTimes[kind];
@@ -796,6 +798,7 @@ static Plan plan_of(int64_t m, int n, int64_t k, bool rows_kind, int epilogue) {
   double best = 1e300;
   for (int kind = 0; kind < kKinds; ++kind) {
     const int64_t tm = (m + kTileM[kind] - 1) / kTileM[kind], tn = ((int64_t)n + kTileN[kind] - 1) / kTileN[kind];
+    if (kind != kWide && tm * tn > kMaxTiles) continue;
     for (int splits = 1; splits <= 64; splits += splits < 4 ? 1 : splits < 8 ? 2 : splits < 16 ? 4 : 8) {
       if (splits > 1 && (r.steps < 2 * splits || tm * tn * splits > 1024)) break;
       const int per = (r.steps + splits - 1) / splits, used = (r.steps + per - 1) / per;
@@ -850,7 +853,7 @@ static int product(const char* who, const void* a, int64_t lda, const void* b, i
   p.part = (float*)part;
   p.ldp = (n + 7) / 8 * 8;
   const int64_t grid = (int64_t)r.tiles_m * r.tiles_n * r.splits;
-  if (grid > 0xffffffffll / 256) return fail(SAF3R_ERR_UNSUPPORTED, "%s: too many tiles for one launch", who);
+  if (grid > kMaxTiles) return fail(SAF3R_ERR_UNSUPPORTED, "%s: too many tiles for one launch", who);
   const dim3 wgs((uint32_t)grid);
   if (r.kind == kWide)
     hipLaunchKernelGGL((gemm_wide_kernel<T, ACOLS, BCOLS>), wgs, dim3(256), 0, stream, p);

@@ -75,7 +75,7 @@ def rounded(value, tol, dtype):
 def linear(x, w, bias, kind, gate, residual, factor):
     """{name: (value, bound before its rounding)} of kept and y; every input fp64 (or None), factor of keep_factor."""
     K = x.shape[1]
-    b = torch.zeros(w.shape[0], dtype=torch.float64) if bias is None else bias
+    b = torch.zeros(w.shape[0], dtype=torch.float64, device=x.device) if bias is None else bias
     z = x @ w.T + b
     z_tol = (K + 4) * E32 * (x.abs() @ w.abs().T + b.abs())
     a, _, a_tol, _ = activation(kind, z)
@@ -91,7 +91,7 @@ def linear_bwd(dy, x, w, kept, kind, gate, factor, dtype):
     """The same of dx, dweight, dbias and dgate from kept as it is stored; dz is rounded to dtype for the products."""
     rows, N = dy.shape
     a, slope, a_tol, s_tol = activation(kind, torch.zeros_like(dy) if kept is None else kept)
-    g = torch.ones(N, dtype=torch.float64) if gate is None else gate
+    g = torch.ones(N, dtype=torch.float64, device=dy.device) if gate is None else gate
     dd = dy * g * factor
     dz = dd * slope
     dz_tol = dd.abs() * s_tol + 6 * E32 * dz.abs()

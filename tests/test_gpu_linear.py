@@ -21,7 +21,7 @@ def ops(pkg):
 
 
 def close(got, want, tol, name):
-    got = got.double().cpu()
+    got = got.double().to(want.device)
     assert got.shape == want.shape, (name, got.shape, want.shape)
     err = (got - want).abs()
     bad = ~(err <= tol)
@@ -41,20 +41,20 @@ def inputs(rows, k, n, dt, seed=0, bias=True, gate=True, residual=None, pdt=None
             "dy": (0.1 * rnd(rows, n)).to(ydt), "state": torch.randint(-(1 << 62), 1 << 62, (2,), generator=g)}
 
 
-def double(*ts):
-    return [None if t is None else t.detach().cpu().double() for t in ts]
+def double(where, *ts):
+    return [None if t is None else t.detach().to(where).double() for t in ts]
 
 
-def check(ops, i, act=None, p=0.0, out_dtype=None, put=None):
-    """Forward and backward of inputs i; ``put`` moves them to the GPU in a layout of its own."""
+def check(ops, i, act=None, p=0.0, out_dtype=None, put=None, where="cpu"):
+    """Forward and backward of inputs i; ``put`` moves them to the GPU in a layout of its own; the formulas on ``where``."""
     put = put or (lambda name, t: t.to(DEV))
     d = {n: None if t is None else put(n, t) for n, t in i.items()}
     dt, n = i["x"].dtype, i["weight"].shape[0]
     rows = i["x"].shape[0]
-    factor = R.keep_factor(p, i["state"], rows, n)
+    factor = R.keep_factor(p, i["state"], rows, n).to(where)
     args = dict(activation=act, gate=d["gate"], dropout=p, state=d["state"])
     y, kept = ops.linear_fwd(d["x"], d["weight"], d["bias"], residual=d["residual"], out_dtype=out_dtype, keep=True, **args)
-    x, w, b, g, res, dy = double(*(i[k] for k in ("x", "weight", "bias", "gate", "residual", "dy")))
+    x, w, b, g, res, dy = double(where, *(i[k] for k in ("x", "weight", "bias", "gate", "residual", "dy")))
     ref = R.linear(x, w, b, act, g, res, factor)
     assert kept.dtype == dt and y.dtype == (i["residual"].dtype if res is not None else out_dtype or dt)
     close(kept, ref["kept"][0], R.rounded(*ref["kept"], dt), "kept")
@@ -62,7 +62,7 @@ def check(ops, i, act=None, p=0.0, out_dtype=None, put=None):
     assert torch.equal(y, ops.linear_fwd(d["x"], d["weight"], d["bias"], residual=d["residual"], out_dtype=out_dtype,
                                          **args))
     grads = ops.linear_bwd(d["dy"], d["x"], d["weight"], kept, **args)
-    ref = R.linear_bwd(dy, x, w, kept.double().cpu(), act, g, factor, dt)
+    ref = R.linear_bwd(dy, x, w, kept.double().to(where), act, g, factor, dt)
     pdt = dt if i["gate"] is None else i["gate"].dtype
     for name, got, kind in zip(("dx", "dweight", "dbias", "dgate"), grads, (dt, dt, pdt, pdt)):
         if name == "dgate" and g is None:
@@ -117,6 +117,23 @@ def test_tiles_of_256_rows(ops, rows, k, n):
     check(ops, inputs(rows, k, n, BF, seed=8), "gelu", 0.1)
 
 
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("rows,k,n", [(4001, 1030, 2050), (10411, 1544, 6150), (10901, 4104, 1000), (70003, 72, 130),
+                                      (5000, 520, 1030)])
+def test_ragged_tiles_of_every_size(ops, rows, k, n, dt):
+    """Tiles of 64 to 256 rows and columns that end inside the matrices, in all three products, with reductions that 64 does
+    not divide (the formulas in 64 bits on the GPU)."""
+    check(ops, inputs(rows, k, n, dt, seed=30, gate=False), None, where=DEV)
+    check(ops, inputs(rows, k, n, dt, seed=31, residual=F32), "gelu", 0.1, where=DEV)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3])
+@pytest.mark.parametrize("k,n", [(64, 64), (128, 4096), (192, 72), (256, 1000), (320, 128)])
+def test_few_steps(ops, rows, k, n):
+    """Reductions of one to five steps over few to many rows."""
+    check(ops, inputs(64 * rows + 1, k, n, BF, seed=32), "gelu")
+
+
 @pytest.mark.parametrize("rows,k,n", [(130, 4104, 136), (70, 2048, 64)])
 def test_split_reductions(ops, rows, k, n):
     check(ops, inputs(rows, k, n, BF, seed=9, residual=F32), "gelu_tanh", 0.1)
@@ -126,6 +143,38 @@ def test_long_reduction_over_rows(ops):
     """The weight's gradient sums over many rows, split among work-groups."""
     check(ops, inputs(20011, 40, 24, BF, seed=10, gate=False))
     check(ops, inputs(9001, 130, 70, FP, seed=11), "gelu")
+
+
+def test_offsets_beyond_32_bits(ops):
+    """Operands and results of more than 2^31 elements: rows from both ends against 64 bits, the sums over all rows."""
+    rows, wide, narrow = 530_011, 4104, 72
+    g = torch.Generator(device=DEV).manual_seed(6)
+
+    def rnd(*shape):
+        return torch.randn(*shape, generator=g, device=DEV, dtype=BF)
+    far = torch.cat([torch.arange(3), torch.arange(rows - 130, rows)]).to(DEV)
+    state = torch.tensor([9, 1], device=DEV)
+    keep = torch.cat([R.keep_bits((9, 1), 3, wide), R.keep_bits((9, 1), 130, wide, rows - 130)]).to(DEV)
+    for k, n in ((wide, narrow), (narrow, wide)):
+        x, w = rnd(rows, k), rnd(n, k) / math.sqrt(k)
+        y = ops.linear_fwd(x, w, dropout=0.25 if n == wide else 0.0, state=state)
+        factor = (keep >= 16384).double() * (4 / 3) if n == wide else 1.0
+        z, z_tol = R.linear(x[far].double(), w.double(), None, None, None, None, torch.ones(1, 1, device=DEV))["kept"]
+        close(y[far], z * factor, R.rounded(z * factor, (z_tol + 4 * R.E32 * z.abs()) * factor, BF), "y")
+        dy = rnd(rows, n)
+        dx, dw, db, _ = ops.linear_bwd(dy, x, w)
+        d = dy[far].double()
+        want, tol = d @ w.double(), (n + 2) * R.E32 * (d.abs() @ w.double().abs())
+        close(dx[far], want, R.rounded(want, tol, BF), "dx")
+        want = torch.zeros(n, k, dtype=torch.float64, device=DEV)
+        size = torch.zeros_like(want)
+        for a, b in zip(dy.split(65536), x.split(65536)):
+            want += a.double().t().contiguous() @ b.double()
+            size += a.double().abs().t().contiguous() @ b.double().abs()
+        # (sums of half a million products: the bound of n * 2^-24 is a tenth of them; these are split, of random sign, and
+        # held to 2^-10 of their magnitudes, a sixtieth of that bound)
+        close(dw, want, R.rounded(want, 2.0 ** -10 * size, BF), "dweight")
+        del x, w, y, dy, dx
 
 
 @pytest.mark.parametrize("p", [0.0, 0.5, 1.0])

@@ -207,6 +207,28 @@ def test_dropout_layouts(ops):
     assert ((y == 0) | (y == math.inf)).all() and (y == 0).any()
 
 
+def test_offsets_beyond_32_bits(ops):
+    """Rows of more than 2^31 elements in all: those of the far end."""
+    rows, dim = 262_211, 8192
+    far = torch.arange(rows - 40, rows, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(6)
+    x = torch.randn(rows, dim, generator=g, device=DEV, dtype=BF)
+    state = torch.tensor([9, 1], device=DEV)
+    factor = ((R.keep_bits((9, 1), 40, dim, rows - 40) >= 16384).double() * (4 / 3)).to(DEV)
+    y = ops.dropout(x, 0.25, state)
+    want = x[far].double() * factor
+    assert ((y[far].double() - want).abs() <= R.rounded(want, 2 * R.E32 * want.abs(), BF)).all()
+    h, z, mean, rstd = ops.residual_norm_fwd(x, y, dropout=0.25, state=state)
+    want = x[far].double() + y[far].double() * factor
+    assert ((h[far].double() - want).abs() <= R.rounded(want, 4 * R.E32 * want.abs(), BF)).all()
+    dx, db, *_ = ops.residual_norm_bwd(x, z, h, mean, rstd, dropout=0.25, state=state, need=(True, False, False, False))
+    few = ops.residual_norm_bwd(x[far], z[far], h[far], mean[far], rstd[far], need=(True, False, False, False))
+    assert torch.equal(dx[far], few[0])
+    # (the branch's: of the unrounded gradient of the stream)
+    want = dx[far].double() * factor
+    assert ((db[far].double() - want).abs() <= R.rounded(want, 2 * R.half_step(BF) * want.abs(), BF)).all()
+
+
 def test_masks_are_independent(ops):
     """Shares of kept elements, by column and between states, within five standard deviations."""
     x = torch.ones(4096, 512, device=DEV)
