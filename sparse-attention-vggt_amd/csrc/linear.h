@@ -201,9 +201,11 @@ struct LinearGradParams {
   void* dz;     // null: sums only; columns n .. n8 - 1 are zeros
   float* part;  // null: no sums; [parts][2][n], the gate's where it is asked for
   int64_t ld_dy, ld_kept, ld_dz, rows, part_rows;
+  void* dgate;  // where one work-group has all rows (direct): the sums themselves, each may be null
+  void* dbias;
   DropParams drop;
   int act, n;
-  bool param32;
+  bool param32, direct;
 };
 int64_t linear_grad_parts(int64_t rows, int n);
 int linear_grad(const char* who, const LinearGradParams& p, int type, bool dy32, bool vec, bool dgate, int64_t parts,

@@ -171,9 +171,8 @@ struct Frags {
 struct Place {
   int tm, tn, split;
 };
-__device__ __forceinline__ Place place_of(const GemmParams& p) {
+__device__ __forceinline__ Place place_of(const GemmParams& p, int id) {
   const int tiles = p.tiles_m * p.tiles_n, all = tiles * p.splits;
-  int id = bid_x();
   const int q = all / 8, r = all % 8, x = id % 8;
   id = x * q + (x < r ? x : r) + id / 8;
   Place at;
@@ -270,7 +269,7 @@ __global__ void __launch_bounds__(256, 2) gemm_pair_kernel(const GemmParams p) {
   __shared__ __attribute__((aligned(16))) char lds[5 * kUnit];
   const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6);
   const int wm = wave >> 1, wn = wave & 1;
-  const Place at = place_of(p);
+  const Place at = place_of(p, bid_x());
   const int m0 = at.tm * 256, n0 = at.tn * 128;
   F feed;
   feed.init(p, at.split, m0, n0, wave, lane, lds);
@@ -419,15 +418,14 @@ __global__ void __launch_bounds__(256, 2) gemm_pair_kernel(const GemmParams p) {
 //   reads    B A k3       |  B A k0' k1'   B A k2'
 //   copies                |  B, A of the step whose place is free
 template <typename T, bool ACOLS, bool BCOLS, int NB, int SLOTS>
-__global__ void __launch_bounds__(256, SLOTS * NB > 10 ? 1 : 2) gemm_small_kernel(const GemmParams p) {
+__device__ __forceinline__ void small_tile(const GemmParams& p, int id, char* lds) {
   typedef typename Half<T>::vec8 vec8;
   constexpr int R = 64 * NB, kPer = R / 32;  // rows of a unit, a wave's instructions for it
   typedef Feed<ACOLS, BCOLS, 1, 1, SLOTS, R> F;
   constexpr int kUnit = F::kUnit;
-  __shared__ __attribute__((aligned(16))) char lds[SLOTS * kUnit];
   const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6);
   const int wm = wave >> 1, wn = wave & 1;
-  const Place at = place_of(p);
+  const Place at = place_of(p, id);
   const int m0 = at.tm * R, n0 = at.tn * R;
   F feed;
   feed.init(p, at.split, m0, n0, wave, lane, lds);
@@ -525,6 +523,27 @@ __global__ void __launch_bounds__(256, SLOTS * NB > 10 ? 1 : 2) gemm_small_kerne
   for (int i = 0; i < NB; ++i) finish_rows<T, NB>(p, key, cols, at.split, m0 + 32 * (NB * wm + i), col0, turn, acc[i]);
 }
 
+template <typename T, bool ACOLS, bool BCOLS, int NB, int SLOTS>
+__global__ void __launch_bounds__(256, SLOTS * NB > 10 ? 1 : 2) gemm_small_kernel(const GemmParams p) {
+  __shared__ __attribute__((aligned(16))) char lds[SLOTS * unit_bytes(64 * NB)];
+  small_tile<T, ACOLS, BCOLS, NB, SLOTS>(p, bid_x(), lds);
+}
+
+// Both products of a small backward pass, dx in the first work-groups and dW in the rest: neither fills the card, and a launch
+// is saved (1041 x 1024 to 4096: 37 -> 31 us, 64 x 1024 to 4096: 17 -> 13).
+struct BothParams {
+  GemmParams dx, dw;
+  int first;  // work-groups of dx
+};
+template <typename T, int NB, int SLOTS>
+__global__ void __launch_bounds__(256, SLOTS * NB > 10 ? 1 : 2) gemm_both_kernel(const BothParams p) {
+  __shared__ __attribute__((aligned(16))) char lds[SLOTS * unit_bytes(64 * NB)];
+  if (bid_x() < p.first)
+    small_tile<T, false, true, NB, SLOTS>(p.dx, bid_x(), lds);
+  else
+    small_tile<T, true, true, NB, SLOTS>(p.dw, bid_x() - p.first, lds);
+}
+
 // 256 x 256 tile of four waves, one a SIMD: each owns 64 rows of both A units by a whole unit of B (128 x 128 in all, 256 sums a
 // lane), which reads 32 KB of LDS for 128 products, a third less than two waves of 128 x 64, and copies a third less than
 // tiles of 256 x 128. Every product is followed by at most a read and a copy, which issue under it (a 32x32x16 product
@@ -544,7 +563,7 @@ __global__ void __launch_bounds__(256, 1) gemm_wide_kernel(const GemmParams p) {
   __shared__ __attribute__((aligned(16))) char lds[10 * kUnit];
   const int lane = tid_x() & 63, wave = __builtin_amdgcn_readfirstlane(tid_x() >> 6);
   const int wm = wave >> 1, wn = wave & 1;
-  const Place at = place_of(p);
+  const Place at = place_of(p, bid_x());
   const int m0 = at.tm * 256, n0 = at.tn * 256;
   F feed;
   feed.init(p, at.split, m0, n0, wave, lane, lds);
@@ -759,6 +778,7 @@ enum Kind { kTiny, kSmall, kPair, kWide, kKinds };
 constexpr int kTileM[kKinds] = {64, 128, 256, 256}, kTileN[kKinds] = {64, 128, 128, 256};
 struct Plan {
   bool few;
+  double time;
   int kind, splits, split_steps, steps, tiles_m, tiles_n;
 };
 
@@ -795,7 +815,7 @@ static Plan plan_of(int64_t m, int n, int64_t k, bool rows_kind, int epilogue) {
   Plan r{};
   r.steps = (int)((k + 63) / 64);
   r.few = rows_kind && m <= 32;
-  double best = 1e300;
+  r.time = 1e300;
   for (int kind = 0; kind < kKinds; ++kind) {
     const int64_t tm = (m + kTileM[kind] - 1) / kTileM[kind], tn = ((int64_t)n + kTileN[kind] - 1) / kTileN[kind];
     if (kind != kWide && tm * tn > kMaxTiles) continue;
@@ -804,8 +824,8 @@ static Plan plan_of(int64_t m, int n, int64_t k, bool rows_kind, int epilogue) {
       const int per = (r.steps + splits - 1) / splits, used = (r.steps + per - 1) / per;
       double t = tile_time(kind, tm * tn * used, per, used > 1 ? 0 : epilogue);
       if (used > 1) t += 2.5 + (double)used * (double)m * n * 8 / 5.5e6;
-      if (t < best) {
-        best = t;
+      if (t < r.time) {
+        r.time = t;
         r.kind = kind;
         r.splits = used;
         r.split_steps = per;
@@ -821,11 +841,9 @@ static int64_t part_bytes(const Plan& r, int64_t m, int n) {
   return r.few || r.splits == 1 ? 0 : (int64_t)r.splits * m * ((n + 7) / 8 * 8) * 4;
 }
 
-// C = A B with the plan's kernels; `part` holds part_bytes.
-template <typename T, bool ACOLS, bool BCOLS>
-static int product(const char* who, const void* a, int64_t lda, const void* b, int64_t ldb, int64_t m, int n, int64_t k,
-                   const EpiParams& epi, void* part, hipStream_t stream) {
-  const Plan r = plan_of(m, n, k, !ACOLS && !BCOLS, epilogue_cycles(epi.act, epi.drop.limit));
+// The operands, sizes and splits of a product C = A B; `part` holds part_bytes.
+static GemmParams params_of(const Plan& r, const void* a, int64_t lda, const void* b, int64_t ldb, int64_t m, int n, int64_t k,
+                            const EpiParams& epi, void* part) {
   GemmParams p{};
   p.a = (const char*)a;
   p.b = (const char*)b;
@@ -836,22 +854,36 @@ static int product(const char* who, const void* a, int64_t lda, const void* b, i
   p.k = (int)k;
   p.epi = epi;
   p.steps = r.steps;
-  if constexpr (!ACOLS && !BCOLS) {
-    if (r.few) {
-      const dim3 grid((uint32_t)((n + 15) / 16));
-      if (m <= 16)
-        hipLaunchKernelGGL((few_rows_kernel<T, 1>), grid, dim3(512), 0, stream, p);
-      else
-        hipLaunchKernelGGL((few_rows_kernel<T, 2>), grid, dim3(512), 0, stream, p);
-      return check_launch(who);
-    }
-  }
   p.split_steps = r.split_steps;
   p.splits = r.splits;
   p.tiles_m = r.tiles_m;
   p.tiles_n = r.tiles_n;
   p.part = (float*)part;
   p.ldp = (n + 7) / 8 * 8;
+  return p;
+}
+
+template <typename T>
+static int join(const char* who, const GemmParams& p, hipStream_t stream) {
+  if (p.splits == 1) return SAF3R_OK;
+  const int64_t threads = p.m * (p.ldp / 8);
+  hipLaunchKernelGGL((join_kernel<T>), dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, stream, p);
+  return check_launch(who);
+}
+
+// The product with the plan's kernels.
+template <typename T, bool ACOLS, bool BCOLS>
+static int product(const char* who, const Plan& r, const GemmParams& p, hipStream_t stream) {
+  if constexpr (!ACOLS && !BCOLS) {
+    if (r.few) {
+      const dim3 grid((uint32_t)((p.n + 15) / 16));
+      if (p.m <= 16)
+        hipLaunchKernelGGL((few_rows_kernel<T, 1>), grid, dim3(512), 0, stream, p);
+      else
+        hipLaunchKernelGGL((few_rows_kernel<T, 2>), grid, dim3(512), 0, stream, p);
+      return check_launch(who);
+    }
+  }
   const int64_t grid = (int64_t)r.tiles_m * r.tiles_n * r.splits;
   if (grid > kMaxTiles) return fail(SAF3R_ERR_UNSUPPORTED, "%s: too many tiles for one launch", who);
   const dim3 wgs((uint32_t)grid);
@@ -866,10 +898,48 @@ static int product(const char* who, const void* a, int64_t lda, const void* b, i
   else
     hipLaunchKernelGGL((gemm_small_kernel<T, ACOLS, BCOLS, 2, 4>), wgs, dim3(256), 0, stream, p);
   if (int e = check_launch(who)) return e;
-  if (r.splits == 1) return SAF3R_OK;
-  const int64_t threads = m * (p.ldp / 8);
-  hipLaunchKernelGGL((join_kernel<T>), dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, stream, p);
-  return check_launch(who);
+  return join<T>(who, p, stream);
+}
+
+// Both products of a backward pass. Where both are small they run in one launch, with tiles of one kind and each with its own
+// splits: the order of every sum, and so every bit, is that of the product by itself.
+template <typename T>
+static int both_products(const char* who, Plan rx, GemmParams dx, Plan rw, GemmParams dw, hipStream_t stream) {
+  if (rx.kind <= kSmall && rw.kind <= kSmall) {
+    int kind = -1;
+    double best = rx.time + rw.time;
+    for (int c : {kTiny, kSmall}) {
+      const int64_t wgs = (int64_t)((dx.m + kTileM[c] - 1) / kTileM[c]) * ((dx.n + kTileN[c] - 1) / kTileN[c]) * dx.splits +
+                          (int64_t)((dw.m + kTileM[c] - 1) / kTileM[c]) * ((dw.n + kTileN[c] - 1) / kTileN[c]) * dw.splits;
+      if (wgs > 1024) continue;
+      const double t = tile_time(c, wgs, std::max(dx.split_steps, dw.split_steps), 0) + (dx.splits > 1 ? 2.5 : 0) +
+                       (dw.splits > 1 ? 2.5 : 0);
+      if (t < best) {
+        best = t;
+        kind = c;
+      }
+    }
+    if (kind >= 0) {
+      BothParams p{dx, dw, 0};
+      for (GemmParams* g : {&p.dx, &p.dw}) {
+        g->tiles_m = (g->m + kTileM[kind] - 1) / kTileM[kind];
+        g->tiles_n = (g->n + kTileN[kind] - 1) / kTileN[kind];
+      }
+      p.first = p.dx.tiles_m * p.dx.tiles_n * p.dx.splits;
+      const int wgs = p.first + p.dw.tiles_m * p.dw.tiles_n * p.dw.splits;
+      if (kind == kTiny)
+        hipLaunchKernelGGL((gemm_both_kernel<T, 1, 10>), dim3((uint32_t)wgs), dim3(256), 0, stream, p);
+      else if (wgs <= 256)
+        hipLaunchKernelGGL((gemm_both_kernel<T, 2, 10>), dim3((uint32_t)wgs), dim3(256), 0, stream, p);
+      else
+        hipLaunchKernelGGL((gemm_both_kernel<T, 2, 4>), dim3((uint32_t)wgs), dim3(256), 0, stream, p);
+      if (int e = check_launch(who)) return e;
+      if (int e = join<T>(who, p.dx, stream)) return e;
+      return join<T>(who, p.dw, stream);
+    }
+  }
+  if (int e = product<T, false, true>(who, rx, dx, stream)) return e;
+  return product<T, true, true>(who, rw, dw, stream);
 }
 
 // (`step`: threads of the grid)
@@ -1031,18 +1101,18 @@ extern "C" int saf3r_linear_fwd(const void* x, int64_t x_stride, const void* w, 
   epi.vec = out % 8 == 0 && vec_rows(y, y_stride) && aligned16(bias) && aligned16(gate) &&
             (!kept || vec_rows(kept, kept_stride)) && (!residual || vec_rows(residual, res_stride));
   const hipStream_t s = (hipStream_t)stream;
-  char* copies = (char*)workspace + part_bytes(plan_of(rows, out, in, true, epilogue_cycles(activation, drop)), rows, out);
+  const Plan plan = plan_of(rows, out, in, true, epilogue_cycles(activation, drop));
+  char* copies = (char*)workspace + part_bytes(plan, rows, out);
   if (int e = pad_operands(who, copies, in, &x, &x_stride, rows, pad_x, &w, &w_stride, out, pad_w, s)) return e;
-  const int k = (int)round8(in);  // (zeros behind `in` in both)
-  if (type == SAF3R_BF16)
-    return product<__bf16, false, false>(who, x, x_stride, w, w_stride, rows, out, k, epi, workspace, s);
-  return product<_Float16, false, false>(who, x, x_stride, w, w_stride, rows, out, k, epi, workspace, s);
+  // (zeros behind `in` in both)
+  const GemmParams p = params_of(plan, x, x_stride, w, w_stride, rows, out, round8(in), epi, workspace);
+  return type == SAF3R_BF16 ? product<__bf16, false, false>(who, plan, p, s) : product<_Float16, false, false>(who, plan, p, s);
 }
 
-// Workspace of a backward pass: dz, the partial sums over rows, copies of x and w, the split products (one after the other).
+// Workspace of a backward pass: dz, the partial sums over rows, copies of x and w, the splits of dx and of dW.
 struct BwdSizes {
-  int64_t dz, sums, copies, products;
-  int64_t all() const { return dz + sums + copies + products; }
+  int64_t dz, sums, copies, dx, dw;
+  int64_t all() const { return dz + sums + copies + dx + dw; }
 };
 static BwdSizes bwd_sizes(int64_t rows, int in, int out, bool own_dz, bool pad_x, bool pad_w) {
   BwdSizes r{};
@@ -1050,7 +1120,8 @@ static BwdSizes bwd_sizes(int64_t rows, int in, int out, bool own_dz, bool pad_x
   r.copies = (pad_x ? pad_bytes(rows, in) : 0) + (pad_w ? pad_bytes(out, in) : 0);
   r.dz = own_dz ? round256(rows * round8(out) * 2) : 0;
   r.sums = round256(linear_grad_parts(rows, out) * 2 * out * 4);
-  r.products = std::max(part_bytes(plan_of(rows, in, out, false, 0), rows, in), part_bytes(plan_of(out, in, rows, false, 0), out, in));
+  r.dx = round256(part_bytes(plan_of(rows, in, out, false, 0), rows, in));
+  r.dw = round256(part_bytes(plan_of(out, in, rows, false, 0), out, in));
   return r;
 }
 
@@ -1131,12 +1202,15 @@ extern "C" int saf3r_linear_bwd(const void* dy, int64_t dy_stride, int y_type, c
     g.ld_dz = round8(out);
     g.rows = rows;
     g.part_rows = (rows + parts - 1) / parts;
+    g.dgate = dgate;
+    g.dbias = dbias;
+    g.direct = parts == 1;
     g.act = activation;
     g.n = out;
     g.param32 = param_type == SAF3R_FP32;
     const bool vec = out % 8 == 0 && vec_rows(dy, dy_stride) && aligned16(gate) && (!g.kept || vec_rows(kept, kept_stride));
     if (int e = linear_grad(who, g, type, y_type == SAF3R_FP32, vec, dgate != nullptr, parts, s)) return e;
-    if (sums)
+    if (sums && !g.direct)
       if (int e = sum_parts(who, g.part, parts, out, dgate, dbias, param_type, s)) return e;
     if (own_dz) {
       dz = ws;
@@ -1145,7 +1219,7 @@ extern "C" int saf3r_linear_bwd(const void* dy, int64_t dy_stride, int y_type, c
   }
   if (int e = pad_operands(who, ws + size.dz + size.sums, in, &x, &x_stride, rows, pad_x, &w, &w_stride, out, pad_w, s))
     return e;
-  void* part = ws + size.dz + size.sums + size.copies;
+  char* part = ws + size.dz + size.sums + size.copies;
   auto plain = [&](void* y, int64_t ld, bool y32, int n) {
     EpiParams epi{};
     epi.y = y;
@@ -1155,15 +1229,15 @@ extern "C" int saf3r_linear_bwd(const void* dy, int64_t dy_stride, int y_type, c
     epi.vec = n % 8 == 0 && vec_rows(y, ld);
     return epi;
   };
+  const Plan rx = plan_of(rows, in, out, false, 0), rw = plan_of(out, in, rows, false, 0);
+  const GemmParams px = params_of(rx, dz, ld_dz, w, w_stride, rows, in, out, plain(dx, dx_stride, false, in), part);
+  const GemmParams pw =
+      params_of(rw, dz, ld_dz, x, x_stride, out, in, rows, plain(dw, dw_stride, dw_type == SAF3R_FP32, in), part + size.dx);
   auto go = [&](auto t) {
     typedef decltype(t) T;
-    if (dx)
-      if (int e = product<T, false, true>(who, dz, ld_dz, w, w_stride, rows, in, out, plain(dx, dx_stride, false, in), part, s))
-        return e;
-    if (dw)
-      return product<T, true, true>(who, dz, ld_dz, x, x_stride, out, in, rows, plain(dw, dw_stride, dw_type == SAF3R_FP32, in),
-                                    part, s);
-    return (int)SAF3R_OK;
+    if (dx && dw) return both_products<T>(who, rx, px, rw, pw, s);
+    if (dx) return product<T, false, true>(who, rx, px, s);
+    return dw ? product<T, true, true>(who, rw, pw, s) : (int)SAF3R_OK;
   };
   return type == SAF3R_BF16 ? go(__bf16()) : go(_Float16());
 }

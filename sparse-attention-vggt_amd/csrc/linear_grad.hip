@@ -64,7 +64,10 @@ __global__ void __launch_bounds__(256) linear_grad_kernel(const LinearGradParams
   if (!p.part) return;
   if constexpr (DGATE) add_slots<8, 32>(dg, lds);
   add_slots<8, 32>(db, lds);
-  if (tid_x() < 32 && col < p.n) {
+  if (tid_x() < 32 && col < p.n && p.direct) {
+    if (DGATE && p.dgate) epi_store<T>(p.dgate, p.param32, false, col, cnt, dg);
+    if (p.dbias) epi_store<T>(p.dbias, p.param32, false, col, cnt, db);
+  } else if (tid_x() < 32 && col < p.n) {
     float* to = p.part + (int64_t)bid_y() * 2 * p.n + col;
     if constexpr (VEC) {
       if constexpr (DGATE) store_vec<8>(to, dg);
@@ -76,10 +79,11 @@ __global__ void __launch_bounds__(256) linear_grad_kernel(const LinearGradParams
   }
 }
 
-// Partial rows: work-groups for four on a compute unit, with at least 16 rows each.
+// Partial rows: work-groups for four on a compute unit, with at least eight rows each; up to 32 rows one work-group has them
+// all and writes the sums itself, which saves the launch of their second step.
 int64_t linear_grad_parts(int64_t rows, int n) {
   const int64_t strips = (n + 255) / 256;
-  return std::max<int64_t>(1, std::min<int64_t>((1024 + strips - 1) / strips, rows / 16));
+  return rows <= 32 ? 1 : std::max<int64_t>(1, std::min<int64_t>((1024 + strips - 1) / strips, rows / 8));
 }
 
 int linear_grad(const char* who, const LinearGradParams& p, int type, bool dy32, bool vec, bool dgate, int64_t parts,
