@@ -46,16 +46,25 @@ __device__ __forceinline__ void philox(const DropKey& key, uint32_t group, uint6
   w[3] = c3;
 }
 
-// x *= keep / (1 - p) for the eight columns from 8 * group of a row. A dropped element is zero whatever x holds.
+// x *= keep / (1 - p) for the eight columns from 8 * group of a row. A dropped element is zero whatever x holds; so is z's, which
+// a gradient multiplies by x (an infinity there would be a NaN).
 __device__ __forceinline__ void drop8(const DropKey& key, int limit, float scale, uint32_t group, uint64_t row,
-                                      float (&x)[8]) {
+                                      float (&x)[8], float (&z)[8]) {
   uint32_t w[4];
   philox(key, group, row, w);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const uint32_t bits = j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xFFFFu;
-    x[j] = (int)bits >= limit ? x[j] * scale : 0.f;
+    const bool keep = (int)bits >= limit;
+    x[j] = keep ? x[j] * scale : 0.f;
+    z[j] = keep ? z[j] : 0.f;
   }
+}
+
+__device__ __forceinline__ void drop8(const DropKey& key, int limit, float scale, uint32_t group, uint64_t row,
+                                      float (&x)[8]) {
+  float none[8] = {};
+  drop8(key, limit, scale, group, row, x, none);
 }
 
 inline int drop_check(const char* who, int limit, const int64_t* state, DropParams* p) {

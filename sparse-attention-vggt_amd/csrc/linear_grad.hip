@@ -1,6 +1,8 @@
 // Before the products of a linear layer's backward pass: the gradient behind the epilogue, and its sums over rows.
 //   dz = dy gate keep/(1-p) act'(kept),  dbias = sum dz,  dgate = sum dy keep/(1-p) act(kept)
-// dz is rounded to the operands' type, which the matrix products read; the sums take it unrounded.
+// dz is rounded to the operands' type, which the matrix products read; the sums take it unrounded. kept is of that type too, so
+// that act and act' are those of a z that is off by half a step: in fp32 it would be written and read at twice the bytes
+// (87936 x 4096: 720 MB more in either pass, about 150 us each).
 //
 // Bound by HBM: dy and kept are read and dz is written once. A work-group of 256 owns 256 columns of a range of rows, eight
 // rows at a time; a lane keeps the sums of its eight columns, and every work-group writes one partial row (summed in a fixed
@@ -27,13 +29,13 @@ __global__ void __launch_bounds__(256) linear_grad_kernel(const LinearGradParams
     if (p.gate) epi_load<T>(p.gate, p.param32, VEC, col, cnt, gate);
 #pragma unroll 2
     for (int64_t row = begin + slot; row < end; row += 8) {
-      float g[8], z[8];
+      float g[8], z[8] = {};
       if constexpr (VEC)
         load_vec<8>((const TY*)p.dy + row * p.ld_dy + col, g);
       else
         load_some<8>((const TY*)p.dy + row * p.ld_dy + col, cnt, g);
       if (p.kept) epi_load<T>(p.kept, false, VEC, row * p.ld_kept + col, cnt, z);
-      if (p.drop.limit) drop8(key, p.drop.limit, p.drop.scale, (uint32_t)col >> 3, (uint64_t)row, g);
+      if (p.drop.limit) drop8(key, p.drop.limit, p.drop.scale, (uint32_t)col >> 3, (uint64_t)row, g, z);
       if (p.kept) {
         auto slopes = [&](int act) {
 #pragma unroll

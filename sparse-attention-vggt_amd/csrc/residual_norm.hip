@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(256) residual_norm_bwd_kernel(const RnParams p
             f[e] = g[j][e];
           }
           put<SOME, kVe>((TX*)p.y + row * p.y_stride + c, p.dim - c, g[j]);
-          if (p.drop.limit) drop8(key, p.drop.limit, p.drop.scale, (uint32_t)c >> 3, (uint64_t)row, f);
+          if (p.drop.limit) drop8(key, p.drop.limit, p.drop.scale, (uint32_t)c >> 3, (uint64_t)row, f, d[j]);
 #pragma unroll
           for (int e = 0; e < kVe; ++e) {
             dg[j][e] += f[e] * d[j][e];

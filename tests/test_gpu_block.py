@@ -6,6 +6,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 import torch.nn.functional as F
 
 import block_ref as R
@@ -237,6 +238,23 @@ def test_block_in_a_graph(mods):
         for a, b in zip(got, want):
             assert torch.equal(a, b)
     assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+
+
+def test_checkpointed_block(mods):
+    """A block that is computed again in its backward pass drops the same elements again."""
+    ad, ops, agg, _, _ = mods
+    torch.manual_seed(1)
+    block = agg.Block(128, 2, 2.0, 0.5, drop=0.3).to(BF).to(DEV)
+    block.frame_attention = "saf3r_block"
+    x = torch.randn(2, 70, 128, device=DEV).to(BF).requires_grad_()
+    dout = torch.randn(2, 70, 128, device=DEV).to(BF)
+    res = []
+    for again in (False, True):
+        torch.manual_seed(3)
+        y = torch.utils.checkpoint.checkpoint(block, x, use_reentrant=False) if again else block(x)
+        res.append((y.detach(), *torch.autograd.grad(y, [x, *block.parameters()], dout)))
+    for a, b in zip(*res):
+        assert torch.equal(a, b)
 
 
 def test_patched_layer(mods):

@@ -265,6 +265,26 @@ def test_values_at_the_ends(ops):
         assert slope[3, 0] == 1.0 and slope[5].isnan().any() and slope[rest].isfinite().all()
 
 
+@pytest.mark.parametrize("act", [None, "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("rows,k,n", [(20, 64, 72), (300, 40, 130)])
+def test_infinities_in_dropped_places(ops, act, rows, k, n):
+    """What a dropped element holds reaches neither the result nor a gradient."""
+    i = inputs(rows, k, n, BF, 9)
+    dropped = R.keep_factor(0.5, i["state"], rows, n) == 0
+    x = i["x"].clone()
+    x[3] = math.inf  # (row 3 is infinities or NaN before the mask)
+    y = ops.linear_fwd(x.to(DEV), i["weight"].to(DEV), None, act, None, i["residual"], None, 0.5, i["state"].to(DEV)).cpu()
+    assert (y[3][dropped[3]] == 0).all() and not y[3][~dropped[3]].isfinite().all()
+    kept = torch.randn(rows, n, generator=torch.Generator().manual_seed(1)).to(BF)
+    res = []
+    for value in (1.0, math.inf, -math.inf, math.nan):
+        z = torch.where(dropped, torch.tensor(value, dtype=BF), kept)
+        res.append(ops.linear_bwd(i["dy"].to(DEV), i["x"].to(DEV), i["weight"].to(DEV), z.to(DEV), act, i["gate"].to(DEV), 0.5,
+                                  i["state"].to(DEV)))
+    for other in res[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(res[0], other))
+
+
 def test_gradients_by_differences(ops):
     """The gradient of <y, dy> along random directions against differences of the forward kernel in fp32 results; the inputs
     are multiples of 2^-6, so that moved inputs are exact."""

@@ -115,6 +115,23 @@ def test_many_rows(ops):
     check(ops, inputs(9001, 129, F32, BF, 5), 0.1)
 
 
+@pytest.mark.parametrize("rows,dim", [(20, 64), (9, 1027), (5, 2048)])
+def test_infinities_in_dropped_places(ops, rows, dim):
+    """What a dropped element of the branch holds reaches neither a result nor a gradient."""
+    i = inputs(rows, dim, F32, BF, 11)
+    dropped = R.keep_factor(0.5, i["state"], rows, dim) == 0
+    d = {n: t.to(DEV) for n, t in i.items()}
+    res = []
+    for value in (1.0, math.inf, -math.inf, math.nan):
+        branch = torch.where(dropped, torch.tensor(value, dtype=BF), i["branch"]).to(DEV)
+        h, y, mean, rstd = ops.residual_norm_fwd(d["x"], branch, d["gate"], d["weight"], d["bias"], dropout=0.5,
+                                                 state=d["state"])
+        res.append((h, y, *ops.residual_norm_bwd(d["dh"], d["dy"], h, mean, rstd, branch, d["gate"], d["weight"], 0.5,
+                                                 d["state"])))
+    for other in res[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(res[0], other))
+
+
 def test_without_a_gradient_of_the_stream(ops):
     check(ops, inputs(50, 96, F32, BF, 6), with_dh=False)
 
