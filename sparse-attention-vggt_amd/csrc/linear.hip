@@ -246,6 +246,17 @@ __device__ __forceinline__ void arrive() {
   barrier_only();
 }
 
+// Before the first step, behind the wait for its copies: scalar loads have come back too, and the epilogue's flags are loaded
+// (flags_there) before. Left to the compiler they are loaded ahead of the steps' loop, and with a scalar load under way at its
+// start every step waits for all of its LDS reads before its first product.
+__device__ __forceinline__ void flags_there(const GemmParams& p) {
+  asm volatile("" ::"s"((int)p.epi.y32), "s"((int)p.epi.vec), "s"((int)p.epi.param32));
+}
+__device__ __forceinline__ void start() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  barrier_only();
+}
+
 // f(Int<0>()), f(Int<1>()), .., f(Int<N - 1>())
 template <int N, int I = 0, typename F>
 __device__ __forceinline__ void each(F f) {
@@ -310,6 +321,7 @@ __global__ void __launch_bounds__(256, 2) gemm_pair_kernel(const GemmParams p) {
     });
   };
 
+  flags_there(p);
   int s = feed.s0, slot = 0;  // slot: of B of this step
   const int s1 = feed.s1, whole = feed.whole();
       feed.template unit<0>(s, 0);
@@ -320,7 +332,7 @@ __global__ void __launch_bounds__(256, 2) gemm_pair_kernel(const GemmParams p) {
         wait_vm<8>();
       else
         wait_vm<4>();
-      barrier_only();
+      start();
 #pragma unroll
       for (int ks = 0; ks < 3; ++ks)
 #pragma unroll
@@ -462,6 +474,7 @@ __device__ __forceinline__ void small_tile(const GemmParams& p, int id, char* ld
     });
   };
 
+  flags_there(p);
   int s = feed.s0, slot = 0;  // slot: of B of this step
   const int s1 = feed.s1, whole = feed.whole();
   constexpr int kAhead = SLOTS / 2;  // steps whose units have a place
@@ -474,7 +487,7 @@ __device__ __forceinline__ void small_tile(const GemmParams& p, int id, char* ld
     wait_vm<2 * kPer * (kAhead - 1)>();
   else
     wait_vm<0>();
-  barrier_only();
+  start();
   read(0, 1, 0);
   read(0, 1, 1);
   read(0, 1, 2);
@@ -605,6 +618,7 @@ __global__ void __launch_bounds__(256, 1) gemm_wide_kernel(const GemmParams p) {
     });
   };
 
+  flags_there(p);
   int s = feed.s0, slot = 0;  // slot: of B0 of this step
   each<2>([&](auto n) {
     constexpr int i = decltype(n)::value;
@@ -617,7 +631,7 @@ __global__ void __launch_bounds__(256, 1) gemm_wide_kernel(const GemmParams p) {
     wait_vm<20>();
   else
     wait_vm<4>();
-  barrier_only();
+  start();
 #pragma unroll
   for (int n = 0; n < 12; ++n) read_ba(n, wn, 2, 0);
   fence();
