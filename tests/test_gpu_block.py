@@ -3,6 +3,7 @@
 ``linear_kernels``; against the same in 64 bits with the same masks."""
 import importlib
 import math
+import threading
 
 import pytest
 import torch
@@ -238,6 +239,79 @@ def test_block_in_a_graph(mods):
         for a, b in zip(got, want):
             assert torch.equal(a, b)
     assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+
+
+def test_no_rows_with_gradients(mods):
+    ad, ops, _, _, _ = mods
+    w, b, g = (torch.randn(*s, device=DEV).to(BF).requires_grad_() for s in ((72, 64), (72,), (72,)))
+    x = torch.zeros(0, 64, device=DEV, dtype=BF, requires_grad=True)
+    ad.linear(x, w, b, "gelu", g, dropout=0.3).sum().backward()
+    assert x.grad.shape == x.shape and all(not t.grad.any() for t in (w, b, g))
+    stream = torch.zeros(0, 3, 72, device=DEV, requires_grad=True)
+    g.grad = None
+    h, y = ad.residual_norm(stream, torch.zeros(0, 3, 72, device=DEV, dtype=BF), g, dropout=0.3)
+    (h.sum() + y.sum()).backward()
+    assert h.shape == stream.grad.shape and not g.grad.any()
+    z = torch.zeros(0, 5, device=DEV, requires_grad=True)
+    ad.dropout(z, 0.5).sum().backward()
+    assert z.grad.shape == z.shape
+
+
+def test_one_weight_twice_and_the_rows_as_residual(mods):
+    ad, ops, _, _, _ = mods
+    g = torch.Generator().manual_seed(7)
+    w = (torch.randn(64, 64, generator=g) / 8).to(BF).to(DEV).requires_grad_()
+    x = torch.randn(50, 64, generator=g).to(BF).to(DEV).requires_grad_()
+    dy = torch.randn(50, 64, generator=g).to(BF).to(DEV)
+    y = ad.linear(ad.linear(x, w, residual=x), w, activation="gelu")
+    y.backward(dy)
+    w2, x2 = (t.detach().double().requires_grad_() for t in (w, x))
+    want = torch.nn.functional.gelu((x2 @ w2.t() + x2) @ w2.t())
+    want.backward(dy.double())
+    tol = 2 * R.half_step(BF) * 7 ** 0.5  # seven roundings at most, forward and backward, each of a value's own size or less
+    assert rel(y, want) < tol and rel(x.grad, x2.grad) < tol and rel(w.grad, w2.grad) < tol
+
+
+def test_two_graphs_and_two_threads(mods):
+    """Graphs that are replayed on two streams at a time, and threads that call at a time, have workspaces of their own."""
+    _, ops, _, _, _ = mods
+    g = torch.Generator().manual_seed(8)
+    w, b, gate = ((torch.randn(*s, generator=g) / 8).to(BF).to(DEV) for s in ((72, 1032), (72,), (72,)))
+    xs = [torch.randn(300, 1032, generator=g).to(BF).to(DEV) for _ in range(2)]
+    dys = [torch.randn(300, 72, generator=g).to(BF).to(DEV) for _ in range(2)]
+    state = torch.tensor([3, 4], device=DEV)
+
+    def step(i):
+        y, kept = ops.linear_fwd(xs[i], w, b, "gelu", gate, dropout=0.2, state=state, keep=True)
+        return (y, *ops.linear_bwd(dys[i], xs[i], w, kept, "gelu", gate, 0.2, state))
+    want = [[t.clone() for t in step(i)] for i in range(2)]
+    torch.cuda.synchronize()
+    graphs, held = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph):
+            held.append(step(i))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(held[i], want[i]))
+    same = {}
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(5):
+                res = step(i)
+            streams[i].synchronize()
+            same[i] = all(torch.equal(a, b) for a, b in zip(res, want[i]))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert same == {0: True, 1: True}
 
 
 def test_checkpointed_block(mods):
