@@ -8,8 +8,8 @@
 // under 8192^3) for a few hundred rows or more, by the bytes of W below. Measured, bf16, launches in a graph:
 //   8192^3                  800 to 825 us (1330 to 1380 TFLOP/s)
 //   87936 x 1024 to 4096    690 to 720, with GELU and the kept values 860 to 900; dx 641, dW 555 to 580
-//   10992 x 4096 to 1024    90, with gate, dropout and an fp32 residual 119; dx 94, dW 92
-//   1041 x 1024 to 4096     20.5, with GELU and the kept values 24; dx 21.5, dW 16, both together 27
+//   10992 x 4096 to 1024    90, with gate, dropout and an fp32 residual 119; dx 93, dW 87
+//   1041 x 1024 to 4096     19.5, with GELU and the kept values 23; dx 20.5, dW 15, both together 26
 //   4 x 1024 to 4096        4.6
 #include "linear.h"
 
@@ -434,10 +434,13 @@ __global__ void __launch_bounds__(256, 2) gemm_pair_kernel(const GemmParams p) {
 
 // Tiles of 128 x 128 (NB 2) and 64 x 64 (NB 1) for products with few of the larger ones: four waves in two rows of two, each NB x
 // NB blocks. A step is bound by its copies (32 or 16 instructions of 28 cycles); a short product by its first copies' way and
-// by the epilogue, which smaller tiles spread over more compute units. Units of both operands go through a ring of SLOTS:
-//   group    0        1   |   2            3
-//   reads    B A k3       |  B A k0' k1'   B A k2'
-//   copies                |  B, A of the step whose place is free
+// by the epilogue, which smaller tiles spread over more compute units. Units of both operands go through a ring of SLOTS. A step is
+// four groups of NB x NB products; of 128 x 128, with the barrier behind the second product of group 1 (of 64 x 64 behind group 1):
+//   group    0        1         2         3
+//   reads    B A k3   | B A k0'  B A k1'   B A k2'     (': of the next step)
+//   copies            |          B         A           (of the step whose place is free)
+// Reads and copies are spread, one or two behind a product: the four waves read together behind a barrier, and eight reads at
+// once hold up the products (dW of 10992 x 1024 to 4096 92.6 -> 87 us, 1041 x 4096 to 1024 21.2 -> 20.3).
 template <typename T, bool ACOLS, bool BCOLS, int NB, int SLOTS>
 __device__ __forceinline__ void small_tile(const GemmParams& p, int id, char* lds) {
   typedef typename Half<T>::vec8 vec8;
@@ -475,7 +478,7 @@ __device__ __forceinline__ void small_tile(const GemmParams& p, int id, char* ld
     each<NB * NB>([&](auto n) {
       constexpr int i = decltype(n)::value / NB, j = decltype(n)::value % NB;
       acc[i][j] = Half<T>::mma32(bf[j][ks], af[i][ks], acc[i][j]);
-      hook(n);
+      hook(at_k, n);
       fence();
     });
   };
@@ -507,23 +510,43 @@ __device__ __forceinline__ void small_tile(const GemmParams& p, int id, char* ld
       constexpr int j = decltype(n)::value;
       if constexpr (kCopy != 0 && j < kPer) feed.template one<decltype(unit)::value, j, kCopy == 2>(s + kAhead, to);
     };
-    products(Int<0>(), [&](auto n) {
-      if constexpr (decltype(n)::value == 0) read(slot, a0, 3);
-    });
-    products(Int<1>(), [&](auto) {});
-    if constexpr (kBehind >= 0) arrive<2 * kPer * (kBehind > 0 ? kBehind : 0)>();
-    products(Int<2>(), [&](auto n) {
-      constexpr int m = decltype(n)::value;
-      if constexpr (kBehind >= 0 && m == 0) read(b_next, a_next, 0);
-      if constexpr (kBehind >= 0 && m == (NB == 2 ? 2 : 0)) read(b_next, a_next, 1);
-      copy(Int<0>(), n, slot);
-      if constexpr (NB == 1) copy(Int<0>(), Int<1>(), slot);
-    });
-    products(Int<3>(), [&](auto n) {
-      if constexpr (kBehind >= 0 && decltype(n)::value == 0) read(b_next, a_next, 2);
-      copy(Int<1>(), n, a0);
-      if constexpr (NB == 1) copy(Int<1>(), Int<1>(), a0);
-    });
+    // fragment f of ks: B's blocks, then A's
+    auto read_one = [&](int f, int b_slot, int a_slot, int ks) {
+      if (f < NB)
+        bf[f][ks] = fb.get(lds + b_slot * kUnit, f, ks);
+      else
+        af[f - NB][ks] = fa.get(lds + a_slot * kUnit, f - NB, ks);
+    };
+    auto hook = [&](auto at_k, auto n) {
+      constexpr int i = NB * NB * decltype(at_k)::value + decltype(n)::value;  // products of this step so far
+      constexpr bool kNext = kBehind >= 0;
+      if constexpr (NB == 1) {
+        if constexpr (i == 0) read(slot, a0, 3);
+        if constexpr (kNext && i == 2) read(b_next, a_next, 0);
+        if constexpr (kNext && i == 2) read(b_next, a_next, 1);
+        if constexpr (kNext && i == 3) read(b_next, a_next, 2);
+        if constexpr (i >= 2) {
+          copy(Int<i - 2>(), Int<0>(), i == 2 ? slot : a0);
+          copy(Int<i - 2>(), Int<1>(), i == 2 ? slot : a0);
+        }
+      } else {
+        if constexpr (i < 2) {
+          read_one(2 * i, slot, a0, 3);
+          read_one(2 * i + 1, slot, a0, 3);
+        }
+        if constexpr (kNext && i >= 6 && i < 8) {
+          read_one(2 * i - 12, b_next, a_next, 0);
+          read_one(2 * i - 11, b_next, a_next, 0);
+        }
+        if constexpr (kNext && i >= 8) read_one(i % 4, b_next, a_next, i / 4 - 1);
+        if constexpr (i >= 8) copy(Int<i / 4 - 2>(), Int<i % 4>(), i < 12 ? slot : a0);
+      }
+      if constexpr (kNext && i == (NB == 1 ? 1 : 5)) arrive<2 * kPer * (kBehind > 0 ? kBehind : 0)>();
+    };
+    products(Int<0>(), hook);
+    products(Int<1>(), hook);
+    products(Int<2>(), hook);
+    products(Int<3>(), hook);
     slot = b_next;
   };
 #pragma unroll 1
