@@ -598,8 +598,8 @@ __global__ void __launch_bounds__(256, SLOTS * NB > 10 ? 1 : 2) gemm_both_kernel
 //   copies   B0"         |  B1"         A0"         A1"
 // into the registers, and slots, that the groups before have done with. The barrier waits for A1 of this step and B0 B1 A0 of
 // the next one; it frees B0 B1 A0 of this one and A1 of the last. The data path takes 28 cycles for an instruction of 1 KB
-// at the hit rates of these products (15 from the L2, 40 to 50 from behind it), 64 of them a step of 2048 cycles of products: they are spread evenly (in a burst behind the barrier, 8192^3 takes 902 us
-// in place of 820).
+// at the hit rates of these products (15 from the L2, 40 to 50 from behind it), 64 of them a step of 2048 cycles of
+// products: they are spread evenly (in a burst behind the barrier, 8192^3 takes 902 us in place of 820).
 template <typename T, bool ACOLS, bool BCOLS>
 __global__ void __launch_bounds__(256, 1) gemm_wide_kernel(const GemmParams p) {
   typedef typename Half<T>::vec8 vec8;
