@@ -679,7 +679,7 @@ int saf3r_residual_norm_bwd(const void* dh, int64_t dh_stride, const void* dy, i
                             int64_t dx_stride, void* dbranch, int64_t dbranch_stride, void* dgate, void* dweight,
                             void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Workspace bytes of saf3r_residual_norm_bwd (at most 6144 * dim), -1 for sizes that it rejects. */
+/* Workspace bytes of saf3r_residual_norm_bwd (at most 9216 * dim), -1 for sizes that it rejects. */
 int64_t saf3r_residual_norm_bwd_workspace_bytes(int64_t rows, int dim);
 
 /*
