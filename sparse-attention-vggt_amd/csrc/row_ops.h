@@ -12,14 +12,16 @@ namespace saf3r {
 template <int N>
 using Int = std::integral_constant<int, N>;
 
-// VE elements of T at p (16-byte aligned for VE > 1) as floats.
+// VE elements of T at p (for VE > 1 aligned to 16 bytes, a shorter vector to its size) as floats. (Eight floats lie at 16 bytes as
+// anything else does: their own type promises 32.)
 template <int VE, typename T>
 __device__ __forceinline__ void load_vec(const T* p, float (&x)[VE]) {
   typedef T vec __attribute__((ext_vector_type(VE)));
+  typedef vec at16 __attribute__((aligned(sizeof(vec) < 16 ? sizeof(vec) : 16)));
   if constexpr (VE == 1) {
     x[0] = (float)p[0];
   } else {
-    const vec v = *reinterpret_cast<const vec*>(p);
+    const vec v = *reinterpret_cast<const at16*>(p);
 #pragma unroll
     for (int e = 0; e < VE; ++e) x[e] = (float)v[e];
   }
@@ -28,13 +30,14 @@ __device__ __forceinline__ void load_vec(const T* p, float (&x)[VE]) {
 template <int VE, typename T>
 __device__ __forceinline__ void store_vec(T* p, const float (&x)[VE]) {
   typedef T vec __attribute__((ext_vector_type(VE)));
+  typedef vec at16 __attribute__((aligned(sizeof(vec) < 16 ? sizeof(vec) : 16)));
   if constexpr (VE == 1) {
     p[0] = (T)x[0];
   } else {
     vec v;
 #pragma unroll
     for (int e = 0; e < VE; ++e) v[e] = (T)x[e];
-    *reinterpret_cast<vec*>(p) = v;
+    *reinterpret_cast<at16*>(p) = v;
   }
 }
 
