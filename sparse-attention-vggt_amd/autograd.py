@@ -166,8 +166,9 @@ class _Linear(torch.autograd.Function):
         keep = grad and (activation is not None or ctx.needs_input_grad[3])
         res = ops.linear_fwd(x, low, bias, activation, gate, residual, out_dtype, dropout, state, keep)
         y, kept = res if keep else (res, None)
-        if grad:
-            ctx.save_for_backward(x, low, kept, gate, state)
+        if grad:  # (x is read for the weight's gradient only, the weight for x's)
+            ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, low if ctx.needs_input_grad[0] else None, kept, gate,
+                                  state)
         ctx.args = (activation, dropout, weight.dtype, None if bias is None else bias.dtype)
         return y
 

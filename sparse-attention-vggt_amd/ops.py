@@ -1439,26 +1439,57 @@ def linear_fwd(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     return (y, kept) if keep else y
 
 
-def linear_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, kept: torch.Tensor | None = None,
+def _some_linear_args(dy, x, weight, kept, activation):
+    """``_linear_args`` of a backward pass without x, the weight or both, and the rows' type: the one that is there names it (of the
+    sums alone nothing is rounded to it)."""
+    if not dy.is_cuda:
+        raise ValueError("saf3r kernels take GPU tensors")
+    if dy.dim() < 1 or dy.shape[-1] < 1:
+        raise ValueError(f"dy must have a last dimension, got {tuple(dy.shape)}")
+    there = [t.dtype for t in (x, weight, kept, dy) if t is not None and t.dtype in (torch.bfloat16, torch.float16)]
+    dt, n, k = there[0] if there else torch.bfloat16, dy.shape[-1], 1
+    for name, t in (("x", x), ("weight", weight)):
+        if t is None:
+            continue
+        lead = (*dy.shape[:-1],) if t is x else (n,)
+        if t.dim() < 1 or t.shape[:-1] != lead or not t.shape[-1] or t.dtype != dt or t.get_device() != dy.get_device():
+            raise ValueError(f"{name} must be bfloat16 or float16 {(*lead, 'in')} on {dy.device}, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+        k = t.shape[-1]
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation {activation!r}: one of {tuple(ACTIVATIONS)}")
+    return ACTIVATIONS[activation], n, k, dt
+
+
+def linear_bwd(dy: torch.Tensor, x: torch.Tensor | None, weight: torch.Tensor | None, kept: torch.Tensor | None = None,
                activation: str | None = None, gate: torch.Tensor | None = None, dropout: float = 0.0,
                state: torch.Tensor | None = None, need: tuple[bool, bool, bool, bool] = (True, True, True, True),
                weight_dtype: torch.dtype | None = None, param_dtype: torch.dtype | None = None):
     """Gradients (dx, dweight, dbias, dgate) of ``linear_fwd`` (``saf3r_linear_bwd``) from ``dy``, fp32 or of x's type, of
     y's shape (it is the residual's gradient itself). ``kept`` is the forward pass's, read for an activation or the
     gate's gradient; the other arguments are those of that call. ``need``: which of the four are computed, the others are
-    None (dgate also without a gate). dweight is of ``weight_dtype`` (the weight's type or fp32), dbias and dgate of gate's
-    type, without one of ``param_dtype`` (default x's). Equal inputs give equal bits."""
-    act, n, k = _linear_args(x, weight, activation)
-    dev, dt = x.get_device(), x.dtype
-    shape = (*x.shape[:-1], n)
-    if dy.shape != shape or dy.get_device() != dev or (dy.dtype != torch.float32 and dy.dtype != dt):
-        raise ValueError(f"dy must be float32 or {dt} {shape} on {x.device}, got {dy.dtype} {tuple(dy.shape)} on {dy.device}")
+    None (dgate also without a gate); x may be None where dweight is not needed, the weight where dx is not. dweight is of
+    ``weight_dtype`` (the weight's type or fp32), dbias and dgate of gate's type, without one of ``param_dtype`` (default x's).
+    Equal inputs give equal bits."""
     need_dx, need_dw, need_db, need_dg = need
     need_dg = need_dg and gate is not None
+    if x is None or weight is None:
+        if (need_dw and x is None) or (need_dx and weight is None):
+            raise ValueError("dx reads the weight, dweight reads x")
+        act, n, k, dt = _some_linear_args(dy, x, weight, kept, activation)
+        dev, shape = dy.get_device(), dy.shape
+    else:
+        act, n, k = _linear_args(x, weight, activation)
+        dev, dt = x.get_device(), x.dtype
+        shape = (*x.shape[:-1], n)
+    if dy.shape != shape or dy.get_device() != dev or (dy.dtype != torch.float32 and dy.dtype != dt):
+        raise ValueError(f"dy must be float32 or {dt} {tuple(shape)} on cuda:{dev}, got {dy.dtype} {tuple(dy.shape)} on "
+                         f"{dy.device}")
     zrows, zstride = None, 0
     if kept is not None:
         if kept.shape != shape or kept.dtype != dt or kept.get_device() != dev:
-            raise ValueError(f"kept must be {dt} {shape} on {x.device}, got {kept.dtype} {tuple(kept.shape)} on {kept.device}")
+            raise ValueError(f"kept must be {dt} {tuple(shape)} on {dy.device}, got {kept.dtype} {tuple(kept.shape)} on "
+                             f"{kept.device}")
         zrows, zstride = _flat_rows(kept)
     elif act or need_dg:
         raise ValueError("the gradients of an activation and of a gate need what the forward pass kept (keep=True)")
@@ -1474,21 +1505,21 @@ def linear_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, kept: to
         read = torch.float32
     limit, drop_state = _drop(dropout, state, dev) if dropout else (0, None)
     if dev != _here():
-        with torch.cuda.device(x.device):
+        with torch.cuda.device(dy.device):
             return linear_bwd(dy, x, weight, kept, activation, gate, dropout, state, need, weight_dtype, kind)
     drows, dstride = _flat_rows(dy)
-    rows, stride = _flat_rows(x)
-    w, wstride = _flat_rows(weight)
-    dx = x.new_empty(x.shape) if need_dx else None
+    rows, stride = _flat_rows(x) if need_dw else (None, 0)
+    w, wstride = _flat_rows(weight) if need_dx else (None, 0)
+    dx = weight.new_empty((*shape[:-1], k)) if need_dx else None
     dw = None if not need_dw else x.new_empty((n, k)) if weight_dtype == dt else x.new_empty((n, k), dtype=weight_dtype)
-    db = x.new_empty(n, dtype=read) if need_db else None
-    dg = x.new_empty(n, dtype=read) if need_dg else None
-    dp, xp, wp, count = drows.data_ptr(), rows.data_ptr(), w.data_ptr(), dy.numel() // n
+    db = dy.new_empty(n, dtype=read) if need_db else None
+    dg = dy.new_empty(n, dtype=read) if need_dg else None
+    dp, xp, wp, count = drows.data_ptr(), _ptr(rows), _ptr(w), dy.numel() // n
     own_dz = act or g is not None or limit or dy.dtype != dt or _copied(dp, dstride, n)
     copies = (need_dw and _copied(xp, stride, k)) | (need_dx and _copied(wp, wstride, k)) << 1 | (
         4 if own_dz and (need_dx or need_dw) else 0)
     nbytes = _linear_bwd_bytes(count, k, n, copies)
-    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    ws = dy.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _mark("linear_bwd", "start")
     _lib.check(_lib.load().saf3r_linear_bwd(dp, dstride, _DTYPES[dy.dtype], xp, stride, wp, wstride, _DTYPES[dt], count, k, n,
                                             _ptr(zrows), zstride, _ptr(g), _DTYPES[read], act, limit, _ptr(drop_state),
