@@ -854,8 +854,9 @@ static double tile_time(int kind, int64_t wgs, int64_t steps, int epilogue) {
 // Cycles of a value's epilogue behind its conversion.
 static int epilogue_cycles(int act, int drop) { return (act != SAF3R_NO_ACTIVATION ? 80 : 0) + (drop ? 70 : 0); }
 
-// Tiles and splits of the least such time. Splits have two steps at least; their join is a launch more, and writes and reads
-// the partial sums once (5.5 TB/s). Against one kind and split for all sizes: 4096 x 1024 from 1041 rows 27.6 -> 16.3 us,
+// Tiles and splits of the least such time. There are two steps a split at least, but steps are shared out rounded up: the last
+// split has what is left, which may be one step (19 steps in splits of 3). The join is a launch more, and writes and reads the
+// partial sums once (5.5 TB/s). Against one kind and split for all sizes: 4096 x 1024 from 1041 rows 27.6 -> 16.3 us,
 // 1024 x 1024 from 2748 rows 24 -> 15, 128 x 512 from 20000 rows 24.6 -> 18.9, 10992 x 1024 from 4096 105 -> 93.
 static Plan plan_of(int64_t m, int n, int64_t k, bool rows_kind, int epilogue) {
   Plan r{};
