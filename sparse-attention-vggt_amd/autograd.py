@@ -216,7 +216,7 @@ class _ResidualNorm(torch.autograd.Function):
         if dy is None:
             dy = torch.zeros(h.shape, dtype=y_dtype, device=h.device)
         dx, dbranch, dg, dw, db = ops.residual_norm_bwd(dh, dy, h, mean, rstd, branch, gate, weight, dropout, state,
-                                                        ctx.needs_input_grad[1:5])
+                                                        ctx.needs_input_grad[1:5], bias_dtype)
         return dx, dbranch, dg, dw, db if db is None else db.to(bias_dtype), None, None, None
 
 

@@ -1587,12 +1587,13 @@ def residual_norm_fwd(x: torch.Tensor, branch: torch.Tensor, gate: torch.Tensor 
 def residual_norm_bwd(dh: torch.Tensor | None, dy: torch.Tensor, h: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
                       branch: torch.Tensor | None = None, gate: torch.Tensor | None = None,
                       weight: torch.Tensor | None = None, dropout: float = 0.0, state: torch.Tensor | None = None,
-                      need: tuple[bool, bool, bool, bool] = (True, True, True, True)):
+                      need: tuple[bool, bool, bool, bool] = (True, True, True, True),
+                      param_dtype: torch.dtype | None = None):
     """Gradients (dx, dbranch, dgate, dweight, dbias) of ``residual_norm_fwd`` (``saf3r_residual_norm_bwd``) from ``dh`` (of
     h's type; None: zeros) and ``dy`` (of y's type); ``h``, ``mean`` and ``rstd`` are its results, the other arguments
     those of that call (``branch`` is read for the gate's gradient only). ``need``: whether dbranch, dgate, dweight and
-    dbias are computed; the others are None, dgate also without a gate. The parameters' gradients are of their type
-    (without one of y's). Equal inputs give equal bits."""
+    dbias are computed; the others are None, dgate also without a gate. The parameters' gradients are of gate's or weight's
+    type, without either of ``param_dtype`` (default y's). Equal inputs give equal bits."""
     _need_cuda(h, dy)
     yt = dy.dtype
     _residual_types(h, yt)
@@ -1613,12 +1614,16 @@ def residual_norm_bwd(dh: torch.Tensor | None, dy: torch.Tensor, h: torch.Tensor
     for n, t in (("mean", mean), ("rstd", rstd)):
         if t.shape != stats or t.dtype != torch.float32 or t.get_device() != dev:
             raise ValueError(f"{n} must be float32 {tuple(stats)} on {h.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    kind = gate.dtype if gate is not None else yt if weight is None else weight.dtype
+    kind = gate.dtype if gate is not None else weight.dtype if weight is not None else yt if param_dtype is None else param_dtype
     read, g, w = _column_params(dim, yt, dev, ("gate", "weight"), (gate, weight))
+    if kind not in _DTYPES:
+        raise ValueError(f"gradients of parameters in float32, bfloat16 or float16, not {kind}")
+    if g is None and w is None and kind != yt:
+        read = torch.float32
     limit, drop_state = _drop(dropout, state, dev) if dropout else (0, None)
     if dev != _here():
         with torch.cuda.device(h.device):
-            return residual_norm_bwd(dh, dy, h, mean, rstd, branch, gate, weight, dropout, state, need)
+            return residual_norm_bwd(dh, dy, h, mean, rstd, branch, gate, weight, dropout, state, need, kind)
     lib = _lib.load()
     drows, dstride = _flat_rows(dy)
     hrows, hstride = _flat_rows(h)
