@@ -612,7 +612,8 @@ int64_t saf3r_layer_norm_bwd_workspace_bytes(int64_t rows, int dim);
 /*
  * Linear layer with its epilogue: y = residual + gate drop(act(x w^T + bias)), rows of `out` from rows of `in`.
  *   x [rows][in], w [out][in]: bf16 or fp16 (`type`), any strides and alignment. Of an operand whose rows are not at 16-byte
- *   alignment, or of no multiple of 8 elements, the workspace takes a copy first.
+ *   alignment, are of no multiple of 8 elements, overlap or lie more than 4194304 elements apart, the workspace takes a copy
+ *   first.
  *   bias, gate: [out] of param_type (fp32 or `type`), NULL: none. activation: enum saf3r_activation.
  *   drop: 65536 times the probability of dropping an element, 0 .. 65536 (0: no dropout); state: device int64 [2], the seed
  *   and the stream (its low 32 bits) of the keep mask, a function of them and of the element's row and column: sixteen bits
@@ -630,7 +631,7 @@ int saf3r_linear_fwd(const void* x, int64_t x_stride, const void* w, int64_t w_s
 
 /* Workspace bytes of saf3r_linear_fwd (0 for most sizes), -1 for sizes that it rejects. activation, drop: of that call.
  * copies: 1: of x, 2: of w (their pointer is no multiple of 16 bytes, their stride or `in` none of 8 elements, or the stride
- * is less than `in`). */
+ * is less than `in` or more than 4194304). */
 int64_t saf3r_linear_fwd_workspace_bytes(int64_t rows, int in, int out, int activation, int drop, int copies);
 
 /*
