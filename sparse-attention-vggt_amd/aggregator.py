@@ -65,7 +65,9 @@ class Mlp(nn.Module):
         self.drop = nn.Dropout(drop) if drop else nn.Identity()
 
     def forward(self, x):
-        return self.drop(self.fc2(self.drop(self.act(self.fc1(x)))))
+        h = self.act(self.fc1(x))
+        drop = getattr(self, "drop", None)  # (a model that was saved whole before there was one has none)
+        return self.fc2(h) if drop is None else drop(self.fc2(drop(h)))
 
 
 def frame_local_attention(attn: Attention, x: torch.Tensor, pos, num_special: int) -> torch.Tensor:

@@ -58,6 +58,8 @@ def _flags_but(n: int, on, skip) -> tuple:
 
 
 class BaseHeadwiseSparseAttentionWrapper(nn.Module):
+    linear_kernels = False  # (of a model that was saved whole before it was an option)
+
     def __init__(self, orig_module, num_special_tokens, num_heads, **kwargs):
         super().__init__()
         self.orig_module = orig_module
