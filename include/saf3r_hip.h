@@ -638,7 +638,8 @@ int64_t saf3r_linear_fwd_workspace_bytes(int64_t rows, int in, int out, int acti
  * Gradients of saf3r_linear_fwd from dy (rows of y_type; it is the residual's gradient itself), each may be NULL:
  *   dx (rows of `type`), dw [out][in] (rows of dw_type: fp32 or `type`), dbias and dgate [out] of param_type.
  *   kept: as written by the forward pass, for an activation or dgate. gate, activation, drop and state: of that call.
- *   The sums have a fixed order: equal calls give equal bits.
+ *   The products read dy gate keep / (1 - p) act'(kept) rounded to `type`, dbias its unrounded values. Sums are fp32 and
+ *   have a fixed order: equal calls give equal bits.
  *   workspace: saf3r_linear_bwd_workspace_bytes, 16-byte aligned, for this call alone until it is done on its stream.
  */
 int saf3r_linear_bwd(const void* dy, int64_t dy_stride, int y_type, const void* x, int64_t x_stride, const void* w,

@@ -1,7 +1,7 @@
 // Dropout by itself: y = x keep / (1 - p), the mask of dropout.h. Its gradient is the same function of dy.
 //
-// Bound by HBM: x is read and y written once, and no mask (87936 x 1024 in bf16: 61 to 67 us, 5.4 to 5.9 TB/s). A block of the generator (ten rounds of two 32-bit products, at a
-// quarter of the vector rate) serves a vector of eight elements.
+// Bound by HBM: x is read and y written once, and no mask (87936 x 1024 in bf16: 61 to 67 us, 5.4 to 5.9 TB/s). A block of the
+// generator (ten rounds of two 32-bit products, at a quarter of the vector rate) serves a vector of eight elements.
 #include "dropout.h"
 #include "row_ops.h"
 

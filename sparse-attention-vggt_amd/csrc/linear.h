@@ -53,8 +53,8 @@ __device__ __forceinline__ float tanh_share(float z) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-2.3022082f * z * (1.f + 0.044715f * z * z)));
 }
 
-// z within [low, high], one instruction (fminf makes a NaN quiet first: the gradient of 87936 x 4096 300 us in place of 289). A
-// NaN's is some number.
+// z within [low, high], one instruction (fminf makes a NaN quiet first: sums over rows of the exact GELU's gradient, 87936 x 4096
+// in bf16 without a dz, 300 us in place of 291 to 297; bound by HBM with a dz, the same). A NaN's is some number.
 __device__ __forceinline__ float clamp(float z, float low, float high) { return __builtin_amdgcn_fmed3f(z, low, high); }
 
 __device__ __forceinline__ float gelu_of(float z, float q) { return fmaxf(z, 0.f) - clamp(fabsf(z), 0.f, 15.f) * q; }

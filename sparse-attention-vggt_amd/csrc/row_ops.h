@@ -12,8 +12,8 @@ namespace saf3r {
 template <int N>
 using Int = std::integral_constant<int, N>;
 
-// VE elements of T at p (for VE > 1 aligned to 16 bytes, a shorter vector to its size) as floats. (Eight floats lie at 16 bytes as
-// anything else does: their own type promises 32.)
+// VE elements of T at p (for VE > 1 aligned to 16 bytes, a shorter vector to its size) as floats. (Eight floats lie at 16 bytes
+// as anything else does: their own type promises 32.)
 template <int VE, typename T>
 __device__ __forceinline__ void load_vec(const T* p, float (&x)[VE]) {
   typedef T vec __attribute__((ext_vector_type(VE)));

@@ -1440,8 +1440,8 @@ def linear_fwd(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
 
 
 def _some_linear_args(dy, x, weight, kept, activation):
-    """``_linear_args`` of a backward pass without x, the weight or both, and the rows' type: the one that is there names it (of the
-    sums alone nothing is rounded to it)."""
+    """``_linear_args`` of a backward pass without x, the weight or both, and the rows' type: the one that is there names it (of
+    the sums alone nothing is rounded to it)."""
     if not dy.is_cuda:
         raise ValueError("saf3r kernels take GPU tensors")
     if dy.dim() < 1 or dy.shape[-1] < 1:
@@ -1470,7 +1470,8 @@ def linear_bwd(dy: torch.Tensor, x: torch.Tensor | None, weight: torch.Tensor | 
     gate's gradient; the other arguments are those of that call. ``need``: which of the four are computed, the others are
     None (dgate also without a gate); x may be None where dweight is not needed, the weight where dx is not. dweight is of
     ``weight_dtype`` (the weight's type or fp32), dbias and dgate of gate's type, without one of ``param_dtype`` (default x's).
-    Equal inputs give equal bits."""
+    The products read the gradient behind the epilogue rounded to x's type, also where dy is fp32; the sums take it
+    unrounded. Equal inputs give equal bits."""
     need_dx, need_dw, need_db, need_dg = need
     need_dg = need_dg and gate is not None
     if x is None or weight is None:
@@ -1614,7 +1615,7 @@ def residual_norm_bwd(dh: torch.Tensor | None, dy: torch.Tensor, h: torch.Tensor
     for n, t in (("mean", mean), ("rstd", rstd)):
         if t.shape != stats or t.dtype != torch.float32 or t.get_device() != dev:
             raise ValueError(f"{n} must be float32 {tuple(stats)} on {h.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    kind = gate.dtype if gate is not None else weight.dtype if weight is not None else yt if param_dtype is None else param_dtype
+    kind = next((t.dtype for t in (gate, weight) if t is not None), yt if param_dtype is None else param_dtype)
     read, g, w = _column_params(dim, yt, dev, ("gate", "weight"), (gate, weight))
     if kind not in _DTYPES:
         raise ValueError(f"gradients of parameters in float32, bfloat16 or float16, not {kind}")

@@ -19,8 +19,8 @@ def mods(pkg):
 
 
 @pytest.mark.parametrize("rows,k,n,dt,master,residual,act,p", [
-    (40, 64, 72, BF, False, BF, "gelu", 0.0), (300, 65, 131, FP, False, F32, None, 0.1), (300, 128, 136, BF, True, F32, "gelu", 0.1),
-    (1, 8, 8, BF, True, None, None, 0.0), (0, 24, 16, BF, False, None, "gelu", 0.0)])
+    (40, 64, 72, BF, False, BF, "gelu", 0.0), (300, 65, 131, FP, False, F32, None, 0.1),
+    (300, 128, 136, BF, True, F32, "gelu", 0.1), (1, 8, 8, BF, True, None, None, 0.0), (0, 24, 16, BF, False, None, "gelu", 0.0)])
 def test_any_set_of_gradients(mods, rows, k, n, dt, master, residual, act, p):
     ad = mods[0]
     g = torch.Generator().manual_seed(rows + k)
@@ -72,9 +72,9 @@ def test_operands_that_are_not_there(mods):
                        ((dy[0, 0], None, w), "last dimension")):
         with pytest.raises(ValueError, match=text):
             ops.linear_bwd(*args, need=(True, False, False, False))
-    for args, text in (((dy, x[1:], None), "x must be"), ((dy, x.cpu(), None), "x must be"), ((dy, x.float(), None), "x must be")):
-        with pytest.raises(ValueError, match=text):
-            ops.linear_bwd(*args, need=(False, True, False, False))
+    for other in (x[1:], x.cpu(), x.float()):
+        with pytest.raises(ValueError, match="x must be"):
+            ops.linear_bwd(dy, other, None, need=(False, True, False, False))
 
 
 @pytest.mark.parametrize("act", [None, "gelu"])
